@@ -1,5 +1,6 @@
 """ctypes declarations of the C ABI (include/diskmule_cuda.h, include/diskmule_stack.h,
-include/diskmule_selftest.h, include/diskmule_synth.h, include/diskmule_gguf.h).
+include/diskmule_selftest.h, include/diskmule_synth.h, include/diskmule_gguf.h,
+include/diskmule_attention.h).
 
 The product path is the CUDA library `libdiskmule_cuda.so` built next to this file.
 Nothing here falls back to a CPU implementation: if the library is missing the
@@ -88,6 +89,41 @@ class ExpertCacheStats(C.Structure):
         ("resident_bytes", C.c_uint64), ("h2d_bytes", C.c_uint64), ("fills", C.c_uint64),
     ]
 
+
+class PromptDesc(C.Structure):
+    """dm_attention_prompt_desc."""
+    _fields_ = [
+        ("type", I32), ("heads", I32), ("kv_heads", I32), ("head_dim", I32),
+        ("sequences", I32), ("causal", I32), ("window", I32), ("scale", C.c_float),
+        ("q_tokens", C.c_int64), ("k_tokens", C.c_int64),
+        ("q", P), ("k", P), ("v", P), ("out", P), ("lse", P),
+        ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+        ("out_stride", C.c_int64 * 2), ("q_offsets", P), ("k_offsets", P),
+    ]
+
+
+class KvCacheDesc(C.Structure):
+    """dm_kv_cache_desc."""
+    _fields_ = [
+        ("type", I32), ("layers", I32), ("kv_heads", I32), ("head_dim", I32),
+        ("page_tokens", I32), ("pages", I32), ("max_sequences", I32), ("max_pages", I32),
+        ("memory", P), ("page_table", P), ("lengths", P), ("references", P),
+    ]
+
+
+class DecodeDesc(C.Structure):
+    """dm_attention_decode_desc."""
+    _fields_ = [
+        ("layer", I32), ("heads", I32), ("batch", I32), ("window", I32),
+        ("shared_tokens", I32), ("max_length", I32), ("scale", C.c_float),
+        ("q", P), ("out", P), ("lse", P),
+        ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("sequences", P),
+        ("workspace", P), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+# DM_KV_* status bits
+KV_OUT_OF_PAGES, KV_BAD_SEQUENCE, KV_TOO_LONG, KV_BAD_TOKEN = 1, 2, 4, 8
 
 # int64_t read(void *user, int32_t layer, int32_t expert, int32_t tensor, void *dst, uint64_t n)
 READ_FN = C.CFUNCTYPE(C.c_int64, P, I32, I32, I32, P, C.c_uint64)
@@ -187,6 +223,19 @@ SIGNATURES = {
     "dm_gguf_metadata_array": ([P, C.c_char_p, C.POINTER(C.c_uint32), C.POINTER(C.c_uint64),
                                 C.POINTER(P)], I32),
     "dm_gguf_expert_layout": ([P, C.c_char_p, C.c_char_p, I32, P], I32),
+    "dm_attention_prompt": ([P, C.POINTER(PromptDesc), P], I32),
+    "dm_kv_cache_create": ([P, C.POINTER(KvCacheDesc), C.POINTER(P)], I32),
+    "dm_kv_cache_destroy": ([P], None),
+    "dm_kv_cache_describe": ([P, C.POINTER(KvCacheDesc)], I32),
+    "dm_kv_cache_status": ([P, C.POINTER(I32), P], I32),
+    "dm_kv_cache_extend": ([P, P, P, I32, P], I32),
+    "dm_kv_cache_write": ([P, I32, P, P, P, P, P, P, I32, C.c_int64, P], I32),
+    "dm_kv_cache_fork": ([P, P, P, I32, P], I32),
+    "dm_kv_cache_compact": ([P, P, P, P, I32, C.c_int64, P], I32),
+    "dm_kv_cache_free": ([P, P, I32, P], I32),
+    "dm_kv_cache_copy_pages": ([P, P, P, I32, P], I32),
+    "dm_attention_decode_workspace": ([P, I32, I32, I32, I32, C.POINTER(C.c_uint64)], I32),
+    "dm_attention_decode": ([P, C.POINTER(DecodeDesc), P], I32),
     "dm_synth_fill_host": ([I32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_float,
                             C.c_float, P], I32),
     "dm_synth_fill_device": ([I32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_float,

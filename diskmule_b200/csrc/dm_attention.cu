@@ -1,0 +1,634 @@
+// dm_attention.cu -- attention: argument checks, launches, and the kernels on mma.sync tiles
+// of 16 query rows.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "dm_attention.cuh"
+
+using dmi::fail;
+
+namespace dma {
+
+// ---------------------------------------------------------------------------
+// 16 query rows against a range of keys. The block's four warps take chunks of 16 keys in
+// turn, each with its own ring of shared-memory stages (cp.async) and its own softmax
+// state, so nothing in the loop waits for another warp; the four states join at the end.
+// ---------------------------------------------------------------------------
+
+constexpr int kRows = 16;    // query rows of a block: one mma tile
+constexpr int kChunk = 16;   // keys of a step of one warp; pages are multiples of it
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+
+enum Mode { kPrompt, kOwn, kShared };
+
+template <int DP>
+struct RowsCfg {
+  static constexpr int kStages = DP == 64 ? 4 : 3;
+  static constexpr int kTile = kChunk * DP * 2;   // bytes of a K or V tile
+  static constexpr int kRing = kStages * 2 * kTile;
+  static constexpr int kJoin = kWarps * kRows * DP * 4;
+  static constexpr int kSmem = kWarps * kRing > kJoin ? kWarps * kRing : kJoin;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
+  const int bytes = valid ? 16 : 0;  // 0: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
+}
+__device__ __forceinline__ void ldm4(uint32_t addr, uint32_t *r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldm4t(uint32_t addr, uint32_t *r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct RowsSmem {
+  int64_t q[kRows];     // element offset of the row's query, -1: no row
+  int64_t out[kRows];   // element offset of its output
+  int64_t index[kRows]; // its row in lse and in the parts
+  int low[kRows], high[kRows];  // the keys that it sees
+  float2 ml[kWarps][kRows];
+  TileOf tile;
+};
+
+template <int MODE, int DP, bool BF16>
+__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
+rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
+  using Cfg = RowsCfg<DP>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ RowsSmem sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int dim = MODE == kPrompt ? p.dim : c.head_dim;
+  const int group = MODE == kPrompt ? p.group : d.group;
+
+  // ---- the block's rows, its keys and where they lie
+  int kv_head, first = 0, last, table_row = 0;
+  int64_t k0 = 0;  // prompt: first key row
+  if (MODE == kPrompt) {
+    kv_head = blockIdx.y;
+    if (warp == 0) {
+      const TileOf t = find_tile(p.q_offsets, p.sequences, p.q_tokens, group, kRows, blockIdx.x);
+      if (lane == 0) sh.tile = t;
+    }
+    __syncthreads();
+    const TileOf t = sh.tile;
+    if (t.seq < 0) return;
+    const int64_t k1 = min((int64_t)max(p.k_offsets[t.seq + 1], 0), p.k_tokens);
+    k0 = min((int64_t)max(p.k_offsets[t.seq], 0), p.k_tokens);
+    const int lq = t.q1 - t.q0, lk = (int)max((int64_t)0, k1 - k0);
+    if (tid < kRows) {
+      const int64_t r = (int64_t)t.tile * kRows + tid;
+      const int token = (int)(r / group), head = kv_head * group + (int)(r % group);
+      const int64_t at = t.q0 + token;
+      const bool valid = token < lq;
+      const int place = token + lk - lq;
+      sh.q[tid] = valid ? at * p.q_stride[0] + head * p.q_stride[1] : -1;
+      sh.out[tid] = at * p.out_stride[0] + head * p.out_stride[1];
+      sh.index[tid] = at * p.heads + head;
+      sh.low[tid] = p.window ? max(0, place - p.window + 1) : 0;
+      sh.high[tid] = p.causal ? max(0, min(lk, place + 1)) : lk;
+    }
+  } else {
+    const int rows = MODE == kOwn ? group : d.batch * group;
+    const int blocks = (rows + kRows - 1) / kRows;
+    const int rb = blockIdx.x % blocks;
+    kv_head = (blockIdx.x / blocks) % c.kv_heads;
+    const int entry = MODE == kOwn ? blockIdx.x / blocks / c.kv_heads : 0;
+    int unused;
+    table_row = sequence_of(c, d, entry, &unused);
+    if (tid < kRows) {
+      const int r = rb * kRows + tid;
+      const int b = MODE == kOwn ? entry : r / group;
+      const int head = kv_head * group + r % group;
+      const bool valid = r < rows;
+      int length = 0;
+      if (valid) sequence_of(c, d, b, &length);
+      sh.q[tid] = valid ? b * d.q_stride[0] + head * d.q_stride[1] : -1;
+      sh.out[tid] = b * d.out_stride[0] + head * d.out_stride[1];
+      sh.index[tid] = (int64_t)b * d.heads + head;
+      const int low = d.window ? max(0, length - d.window) : 0;
+      sh.low[tid] = MODE == kOwn ? max(low, d.shared) : low;
+      sh.high[tid] = MODE == kOwn ? length : min(length, d.shared);
+    }
+  }
+  __syncthreads();
+  int low = INT32_MAX, high = 0;
+#pragma unroll
+  for (int r = 0; r < kRows; r++)
+    if (sh.q[r] >= 0) low = min(low, sh.low[r]), high = max(high, sh.high[r]);
+  low = low / kChunk * kChunk;
+  first = low, last = high;
+  if (MODE != kPrompt && high > low) {
+    // this block's part: whole chunks for every warp, and no fewer than 128 keys
+    const int per = max(128, (((high - low) + d.splits - 1) / d.splits + 63) / 64 * 64);
+    first = (int)min((int64_t)high, low + (int64_t)blockIdx.y * per);
+    last = (int)min((int64_t)high, (int64_t)first + per);
+  }
+
+  // ---- this thread's rows (tid % 32 / 4 and + 8) and its query fragments
+  const int ra = lane >> 2, rb8 = ra + 8;
+  const int64_t qa = sh.q[ra], qb = sh.q[rb8];
+  // a row that is not there sees everything: its results are dropped
+  const int low_a = qa < 0 ? 0 : sh.low[ra], high_a = qa < 0 ? INT32_MAX : sh.high[ra];
+  const int low_b = qb < 0 ? 0 : sh.low[rb8], high_b = qb < 0 ? INT32_MAX : sh.high[rb8];
+  const uint16_t *qp = MODE == kPrompt ? p.q : d.q;
+  uint32_t qf[DP / 16][4];
+#pragma unroll
+  for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int col = k * 16 + h * 8 + (lane & 3) * 2;
+      const bool in = col < dim;
+      qf[k][h * 2] = in && qa >= 0 ? *reinterpret_cast<const uint32_t *>(qp + qa + col) : 0u;
+      qf[k][h * 2 + 1] = in && qb >= 0 ? *reinterpret_cast<const uint32_t *>(qp + qb + col) : 0u;
+    }
+
+  // ---- the warp's ring
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * Cfg::kRing;
+  constexpr int kVec = DP / 8;  // 16-byte vectors of a row
+  const int vecs = dim / 8;
+  auto page_of = [&](int key) -> int {
+    if (MODE == kPrompt || key >= last) return -1;
+    return c.table[(int64_t)table_row * c.max_pages + key / c.page_tokens];
+  };
+  auto load = [&](int key, int page, int stage) {
+    const uint32_t kd = ring + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;
+    const uint8_t *kb, *vb;
+    int64_t ks, vs;  // bytes from row to row
+    bool there = true;
+    if (MODE == kPrompt) {
+      kb = reinterpret_cast<const uint8_t *>(p.k + (k0 + key) * p.k_stride[0] + kv_head * p.k_stride[1]);
+      vb = reinterpret_cast<const uint8_t *>(p.v + (k0 + key) * p.v_stride[0] + kv_head * p.v_stride[1]);
+      ks = p.k_stride[0] * 2, vs = p.v_stride[0] * 2;
+    } else {
+      there = (unsigned)page < (unsigned)c.pages;
+      kb = c.memory + (there ? page : 0) * c.page_bytes + d.layer * c.layer_bytes +
+           kv_head * c.head_bytes + (int64_t)(key % c.page_tokens) * dim * 2;
+      vb = kb + c.kv_heads * c.head_bytes;
+      ks = vs = dim * 2;
+    }
+#pragma unroll
+    for (int i = 0; i < kChunk * kVec / 32; i++) {
+      const int at = i * 32 + lane, r = at / kVec, v = at % kVec;
+      const bool valid = there && key + r < last && v < vecs;
+      const uint32_t to = (uint32_t)(r * kVec + (v ^ (r & 7))) * 16;
+      cp16(kd + to, valid ? kb + r * ks + v * 16 : kb, valid);
+      cp16(vd + to, valid ? vb + r * vs + v * 16 : vb, valid);
+    }
+  };
+
+  float o[DP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
+  const float scale = MODE == kPrompt ? p.scale : d.scale;
+
+  constexpr int kStep = kWarps * kChunk;
+  int key_load = first + warp * kChunk;
+  int page = page_of(key_load);
+  auto issue = [&](int stage) {
+    if (key_load < last) {
+      const int next = page_of(key_load + kStep);  // one step ahead of its use
+      load(key_load, page, stage);
+      page = next;
+    }
+    key_load += kStep;
+    asm volatile("cp.async.commit_group;");
+  };
+#pragma unroll
+  for (int s = 0; s < Cfg::kStages - 1; s++) issue(s);
+  int stage = 0;
+  for (int key = first + warp * kChunk; key < last; key += kStep) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kStages - 2));
+    __syncwarp();  // all lanes' copies are there, and all have left the stage that is next
+    issue(stage == 0 ? Cfg::kStages - 1 : stage - 1);
+    const uint32_t kt = ring + stage * 2 * Cfg::kTile, vt = kt + Cfg::kTile;
+    float s[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+    {
+      const int r = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+      for (int k = 0; k < DP / 16; k++) {
+        uint32_t b[4];
+        const int v = 2 * k + ((lane >> 3) & 1);
+        ldm4(kt + (r * kVec + (v ^ (r & 7))) * 16, b);
+        mma16816<BF16>(s[0], qf[k], b[0], b[1]);
+        mma16816<BF16>(s[1], qf[k], b[2], b[3]);
+      }
+    }
+    // scores, masked, and the new maxima
+    float na = ma, nb = mb;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int j = key + t * 8 + (lane & 3) * 2 + e;
+        s[t][e] = j >= low_a && j < high_a ? s[t][e] * scale : -INFINITY;
+        s[t][2 + e] = j >= low_b && j < high_b ? s[t][2 + e] * scale : -INFINITY;
+        na = fmaxf(na, s[t][e]);
+        nb = fmaxf(nb, s[t][2 + e]);
+      }
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, x));
+      nb = fmaxf(nb, __shfl_xor_sync(0xffffffffu, nb, x));
+    }
+    // a row that has seen nothing yet keeps a zero reference
+    const float za = na == -INFINITY ? 0.0f : na, zb = nb == -INFINITY ? 0.0f : nb;
+    const float fa = exp2_fast(ma - za), fb = exp2_fast(mb - zb);
+    ma = na, mb = nb;
+    la *= fa, lb *= fb;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        s[t][e] = exp2_fast(s[t][e] - za);
+        s[t][2 + e] = exp2_fast(s[t][2 + e] - zb);
+        la += s[t][e], lb += s[t][2 + e];
+      }
+#pragma unroll
+    for (int i = 0; i < DP / 8; i++) o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
+    const uint32_t pf[4] = {pack2<BF16>(s[0][0], s[0][1]), pack2<BF16>(s[0][2], s[0][3]),
+                            pack2<BF16>(s[1][0], s[1][1]), pack2<BF16>(s[1][2], s[1][3])};
+    // Where a key is hidden from one row and seen by another, 0 * v must stay 0 for the
+    // first: values that are not finite are left out of the product and added for the rows
+    // that see them.
+    const bool mixed = __any_sync(0xffffffffu, low_a > key || high_a < key + kChunk ||
+                                                   low_b > key || high_b < key + kChunk);
+    bool wild = false;
+    {
+      const int r = (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+      for (int n = 0; n < DP / 16; n++) {
+        uint32_t b[4];
+        const int v = 2 * n + (lane >> 4);
+        ldm4t(vt + (r * kVec + (v ^ (r & 7))) * 16, b);
+        if (mixed)
+#pragma unroll
+          for (int i = 0; i < 4; i++) b[i] = zero_not_finite<BF16>(b[i], wild);
+        mma16816<BF16>(o[2 * n], pf, b[0], b[1]);
+        mma16816<BF16>(o[2 * n + 1], pf, b[2], b[3]);
+      }
+    }
+    if (mixed && __any_sync(0xffffffffu, wild)) {
+      for (int r = 0; r < kChunk; r++) {
+        const bool sees_a = key + r >= low_a && key + r < high_a;
+        const bool sees_b = key + r >= low_b && key + r < high_b;
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++) {
+          uint32_t w;
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w)
+                       : "r"(vt + (r * kVec + (n ^ (r & 7))) * 16 + (lane & 3) * 4));
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const uint16_t x = (uint16_t)(w >> (16 * e));
+            if (!not_finite<BF16>(x)) continue;
+            if (sees_a) o[n][e] += to_float<BF16>(x);
+            if (sees_b) o[n][2 + e] += to_float<BF16>(x);
+          }
+        }
+      }
+    }
+    stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;");
+
+  // ---- join the warps' states in shared memory
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) {
+    la += __shfl_xor_sync(0xffffffffu, la, x);
+    lb += __shfl_xor_sync(0xffffffffu, lb, x);
+  }
+  __syncthreads();
+  float *join = reinterpret_cast<float *>(smem) + warp * kRows * DP;
+#pragma unroll
+  for (int n = 0; n < DP / 8; n++) {
+    const int col = n * 8 + (lane & 3) * 2;
+    *reinterpret_cast<float2 *>(join + ra * DP + col) = make_float2(o[n][0], o[n][1]);
+    *reinterpret_cast<float2 *>(join + rb8 * DP + col) = make_float2(o[n][2], o[n][3]);
+  }
+  if ((lane & 3) == 0) {
+    sh.ml[warp][ra] = make_float2(ma, la);
+    sh.ml[warp][rb8] = make_float2(mb, lb);
+  }
+  __syncthreads();
+  const bool final = MODE == kPrompt || d.part.parts == 1;
+  constexpr int kLanes = DP / 4;  // threads along a row, four columns each
+  const float *all = reinterpret_cast<const float *>(smem);
+  for (int r = tid / kLanes; r < kRows; r += kThreads / kLanes) {
+    if (sh.q[r] < 0) continue;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) m = fmaxf(m, sh.ml[w][r].x);
+    const float z = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int col = (tid % kLanes) * 4;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+      const float f = exp2_fast(sh.ml[w][r].x - z);
+      const float4 u = *reinterpret_cast<const float4 *>(all + (w * kRows + r) * DP + col);
+      l += sh.ml[w][r].y * f;
+      v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
+    }
+    if (final) {
+      float *lse = MODE == kPrompt ? p.lse : d.lse;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      if (col < dim) {
+        uint16_t *out = (MODE == kPrompt ? p.out : d.out) + sh.out[r] + col;
+        *reinterpret_cast<uint2 *>(out) =
+            make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
+      }
+      if (lse && col == 0) lse[sh.index[r]] = l == 0.0f ? -INFINITY : (m + log2_fast(l)) * kLn2;
+    } else {
+      const int64_t at = (int64_t)(d.first_part + blockIdx.y) * d.part.rows + sh.index[r];
+      if (col < dim && l != 0.0f) *reinterpret_cast<float4 *>(d.part.o + at * dim + col) = v;
+      if (col == 0) d.part.ml[at] = make_float2(m, l);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Join the parts of each row: one block per row, four slices of the parts side by side.
+// ---------------------------------------------------------------------------
+
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads) join_kernel(DecodeArgs d, int dim) {
+  __shared__ float top[kThreads], sum[kWarps];
+  __shared__ float4 acc[kWarps][64];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float m = -INFINITY;
+  for (int i = tid; i < d.part.parts; i += kThreads) m = fmaxf(m, d.part.ml[i * d.part.rows + row].x);
+  top[tid] = m;
+  __syncthreads();
+  for (int i = 0; i < kThreads; i++) m = fmaxf(m, top[i]);
+  const float z = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  float4 v[2] = {};
+  for (int i = warp; i < d.part.parts; i += kWarps) {
+    const float2 ml = d.part.ml[i * d.part.rows + row];
+    if (ml.y == 0.0f) continue;
+    const float f = exp2_fast(ml.x - z);
+    l += ml.y * f;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int col = (h * 32 + lane) * 4;
+      if (col >= dim) continue;
+      const float4 u = *reinterpret_cast<const float4 *>(d.part.o + (i * d.part.rows + row) * dim + col);
+      v[h].x += u.x * f, v[h].y += u.y * f, v[h].z += u.z * f, v[h].w += u.w * f;
+    }
+  }
+  acc[warp][lane] = v[0];
+  acc[warp][32 + lane] = v[1];
+  if (lane == 0) sum[warp] = l;
+  __syncthreads();
+  l = sum[0] + sum[1] + sum[2] + sum[3];
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (tid < 64 && tid * 4 < dim) {
+    float4 s = acc[0][tid];
+    for (int w = 1; w < kWarps; w++) {
+      const float4 u = acc[w][tid];
+      s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
+    }
+    const int64_t b = row / d.heads, head = row % d.heads;
+    uint16_t *out = d.out + b * d.out_stride[0] + head * d.out_stride[1] + tid * 4;
+    *reinterpret_cast<uint2 *>(out) =
+        make_uint2(pack2<BF16>(s.x * inv, s.y * inv), pack2<BF16>(s.z * inv, s.w * inv));
+  }
+  if (tid == 0 && d.lse) d.lse[row] = l == 0.0f ? -INFINITY : (m + log2_fast(l)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+
+template <int MODE, int DP, bool BF16>
+int32_t launch_rows(dim3 grid, const PromptArgs &p, const DecodeArgs &d, const KvView &c,
+                    cudaStream_t s) {
+  auto fn = rows_kernel<MODE, DP, BF16>;
+  static bool set = false;  // per instantiation; setting it twice is harmless
+  if (!set) {
+    DM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsCfg<DP>::kSmem),
+            "attention shared memory");
+    set = true;
+  }
+  fn<<<grid, kThreads, RowsCfg<DP>::kSmem, s>>>(p, d, c);
+  DM_CUDA(cudaGetLastError(), "attention launch");
+  return DM_OK;
+}
+
+template <int MODE>
+int32_t launch_rows(int type, int dim, dim3 grid, const PromptArgs &p, const DecodeArgs &d,
+                    const KvView &c, cudaStream_t s) {
+  const bool bf = type == DM_BF16;
+  if (dim <= 64)
+    return bf ? launch_rows<MODE, 64, true>(grid, p, d, c, s) : launch_rows<MODE, 64, false>(grid, p, d, c, s);
+  if (dim <= 128)
+    return bf ? launch_rows<MODE, 128, true>(grid, p, d, c, s) : launch_rows<MODE, 128, false>(grid, p, d, c, s);
+  return bf ? launch_rows<MODE, 256, true>(grid, p, d, c, s) : launch_rows<MODE, 256, false>(grid, p, d, c, s);
+}
+
+// How a decode call is cut into parts. The workspace holds one state per part and row.
+struct DecodePlan {
+  int shared_splits = 0, own_splits = 0;
+  int parts() const { return shared_splits + own_splits; }
+};
+
+constexpr int kTargetBlocks = 296;  // two blocks of four warps on each of 148 SMs
+
+DecodePlan decode_plan(int kv_heads, int heads, int batch, int shared, int max_length) {
+  DecodePlan plan;
+  if (batch == 0) return plan;
+  const int group = heads / kv_heads;
+  if (shared > 0) {
+    const int64_t items = (int64_t)kv_heads * (((int64_t)batch * group + kRows - 1) / kRows);
+    plan.shared_splits = (int)std::max<int64_t>(
+        1, std::min<int64_t>((kTargetBlocks + items - 1) / items, (shared + 255) / 256));
+  }
+  if (max_length > shared || shared == 0) {
+    const int64_t items = (int64_t)batch * kv_heads * ((group + kRows - 1) / kRows);
+    const int own = std::max(1, max_length - shared);
+    plan.own_splits = (int)std::max<int64_t>(
+        1, std::min<int64_t>((kTargetBlocks + items - 1) / items, (own + 255) / 256));
+  }
+  return plan;
+}
+
+uint64_t decode_workspace(const DecodePlan &plan, int64_t rows, int dim) {
+  return plan.parts() > 1 ? (uint64_t)plan.parts() * rows * (dim * 4 + 8) : 0;
+}
+
+}  // namespace dma
+
+using namespace dma;
+
+static int32_t check_strides(const int64_t *given, int64_t heads, int dim, int64_t *use, const char *what) {
+  const bool none = given[0] == 0 && given[1] == 0;
+  use[0] = none ? heads * dim : given[0];
+  use[1] = none ? dim : given[1];
+  if (use[0] % 8 || use[1] % 8)
+    return fail(DM_ERR_INVALID_ARGUMENT, "%s strides must be multiples of 8 elements", what);
+  if (use[0] < 0 || use[1] < 0) return fail(DM_ERR_INVALID_ARGUMENT, "%s strides are negative", what);
+  return DM_OK;
+}
+
+static int32_t check_scale(float given, int dim, float *use) {
+  if (!std::isfinite(given) || given < 0.0f)
+    return fail(DM_ERR_POSITIVE_PARAMETER, "attention needs a finite scale that is not negative");
+  *use = (given == 0.0f ? 1.0f / std::sqrt((float)dim) : given) * kLog2e;
+  return DM_OK;
+}
+
+extern "C" {
+
+int32_t dm_attention_prompt(dm_cuda_context *ctx, const dm_attention_prompt_desc *in, void *stream) {
+  if (!ctx || !in) return fail(DM_ERR_INVALID_ARGUMENT, "null argument");
+  if (in->type != DM_BF16 && in->type != DM_F16)
+    return fail(DM_ERR_UNSUPPORTED_TENSOR_TYPE, "attention takes bf16 or f16");
+  if (in->heads <= 0 || in->kv_heads <= 0 || in->heads % in->kv_heads || in->heads / in->kv_heads > 128)
+    return fail(DM_ERR_ELEMENT_COUNT, "%d query heads over %d key/value heads", in->heads, in->kv_heads);
+  if (in->kv_heads > 65535) return fail(DM_ERR_ELEMENT_COUNT, "%d key/value heads", in->kv_heads);
+  if (in->head_dim <= 0 || in->head_dim % 8 || in->head_dim > 256)
+    return fail(DM_ERR_ELEMENT_COUNT, "head_dim %d is not a multiple of 8 up to 256", in->head_dim);
+  if (in->sequences < 0 || in->window < 0)
+    return fail(DM_ERR_ELEMENT_COUNT, "%d sequences, window %d", in->sequences, in->window);
+  if (in->q_tokens < 0 || in->k_tokens < 0 || in->q_tokens > INT32_MAX || in->k_tokens > INT32_MAX)
+    return fail(DM_ERR_ELEMENT_COUNT, "a bad number of tokens");
+  if (in->sequences == 0 || in->q_tokens == 0) return DM_OK;
+  if (!in->q || !in->out || !in->q_offsets || (in->k_tokens && (!in->k || !in->v)))
+    return fail(DM_ERR_INVALID_ARGUMENT, "null tensor");
+  if (((uintptr_t)in->q | (uintptr_t)in->k | (uintptr_t)in->v | (uintptr_t)in->out) & 15)
+    return fail(DM_ERR_INVALID_ARGUMENT, "attention tensors must be 16-byte aligned");
+  PromptArgs a{};
+  a.q = (const uint16_t *)in->q;
+  a.k = (const uint16_t *)in->k;
+  a.v = (const uint16_t *)in->v;
+  a.out = (uint16_t *)in->out;
+  a.lse = in->lse;
+  if (int32_t rc = check_strides(in->q_stride, in->heads, in->head_dim, a.q_stride, "query")) return rc;
+  if (int32_t rc = check_strides(in->k_stride, in->kv_heads, in->head_dim, a.k_stride, "key")) return rc;
+  if (int32_t rc = check_strides(in->v_stride, in->kv_heads, in->head_dim, a.v_stride, "value")) return rc;
+  if (int32_t rc = check_strides(in->out_stride, in->heads, in->head_dim, a.out_stride, "output")) return rc;
+  if (int32_t rc = check_scale(in->scale, in->head_dim, &a.scale)) return rc;
+  a.q_offsets = in->q_offsets;
+  a.k_offsets = in->k_offsets ? in->k_offsets : in->q_offsets;
+  a.q_tokens = in->q_tokens;
+  a.k_tokens = in->k_tokens;
+  a.heads = in->heads;
+  a.kv_heads = in->kv_heads;
+  a.group = in->heads / in->kv_heads;
+  a.dim = in->head_dim;
+  a.sequences = in->sequences;
+  a.causal = in->causal;
+  a.window = in->window;
+  cudaSetDevice(ctx->device);
+  const int64_t tiles = in->q_tokens * a.group / kRows + in->sequences;
+  if (tiles > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
+  return launch_rows<kPrompt>(in->type, in->head_dim, dim3((unsigned)tiles, in->kv_heads), a,
+                              DecodeArgs{}, KvView{}, (cudaStream_t)stream);
+}
+
+int32_t dm_attention_decode_workspace(const dm_kv_cache *cache, int32_t heads, int32_t batch,
+                                      int32_t shared_tokens, int32_t max_length, uint64_t *bytes) {
+  if (!cache || !bytes) return fail(DM_ERR_INVALID_ARGUMENT, "null argument");
+  const dm_kv_cache_desc &d = cache->desc;
+  if (heads <= 0 || heads % d.kv_heads)
+    return fail(DM_ERR_ELEMENT_COUNT, "%d query heads over %d key/value heads", heads, d.kv_heads);
+  if (batch < 0 || (int64_t)batch * heads > (1 << 24))
+    return fail(DM_ERR_ELEMENT_COUNT, "a batch of %d", batch);
+  if (shared_tokens < 0 || shared_tokens % d.page_tokens || shared_tokens > (int64_t)d.max_pages * d.page_tokens)
+    return fail(DM_ERR_ELEMENT_COUNT, "%d shared tokens are no whole pages of the table", shared_tokens);
+  if (max_length < 0) return fail(DM_ERR_ELEMENT_COUNT, "max_length %d", max_length);
+  *bytes = decode_workspace(decode_plan(d.kv_heads, heads, batch, shared_tokens, max_length),
+                            (int64_t)batch * heads, d.head_dim);
+  return DM_OK;
+}
+
+int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *in, void *stream) {
+  if (!cache || !in) return fail(DM_ERR_INVALID_ARGUMENT, "null argument");
+  const dm_kv_cache_desc &kd = cache->desc;
+  uint64_t need = 0;
+  if (int32_t rc = dm_attention_decode_workspace(cache, in->heads, in->batch, in->shared_tokens,
+                                                 in->max_length, &need))
+    return rc;
+  if (in->layer < 0 || in->layer >= kd.layers)
+    return fail(DM_ERR_INVALID_LAYER, "layer %d of %d", in->layer, kd.layers);
+  if (in->window < 0) return fail(DM_ERR_ELEMENT_COUNT, "window %d", in->window);
+  if (in->batch == 0) return DM_OK;
+  if (!in->q || !in->out) return fail(DM_ERR_INVALID_ARGUMENT, "null tensor");
+  if (((uintptr_t)in->q | (uintptr_t)in->out) & 15)
+    return fail(DM_ERR_INVALID_ARGUMENT, "attention tensors must be 16-byte aligned");
+  if (need && (!in->workspace || ((uintptr_t)in->workspace & 15)))
+    return fail(DM_ERR_INVALID_ARGUMENT, "decode needs a 16-byte aligned workspace");
+  if (in->workspace_bytes < need)
+    return fail(DM_ERR_BYTE_LENGTH, "a workspace of %llu bytes, %llu are needed",
+                (unsigned long long)in->workspace_bytes, (unsigned long long)need);
+  DecodeArgs a{};
+  a.q = (const uint16_t *)in->q;
+  a.out = (uint16_t *)in->out;
+  a.lse = in->lse;
+  if (int32_t rc = check_strides(in->q_stride, in->heads, kd.head_dim, a.q_stride, "query")) return rc;
+  if (int32_t rc = check_strides(in->out_stride, in->heads, kd.head_dim, a.out_stride, "output")) return rc;
+  if (int32_t rc = check_scale(in->scale, kd.head_dim, &a.scale)) return rc;
+  a.sequences = in->sequences;
+  a.heads = in->heads;
+  a.group = in->heads / kd.kv_heads;
+  a.batch = in->batch;
+  a.layer = in->layer;
+  a.window = in->window;
+  a.shared = in->shared_tokens;
+  a.max_length = in->max_length;
+  const DecodePlan plan = decode_plan(kd.kv_heads, in->heads, in->batch, in->shared_tokens, in->max_length);
+  a.part.parts = plan.parts();
+  a.part.rows = (int64_t)in->batch * in->heads;
+  a.part.o = (float *)in->workspace;
+  a.part.ml = (float2 *)(a.part.o + (int64_t)a.part.parts * a.part.rows * kd.head_dim);
+  cudaSetDevice(cache->ctx->device);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (plan.shared_splits) {
+    const int64_t items = (int64_t)kd.kv_heads * (((int64_t)in->batch * a.group + kRows - 1) / kRows);
+    a.first_part = 0;
+    a.splits = plan.shared_splits;
+    if (int32_t rc = launch_rows<kShared>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
+                                          PromptArgs{}, a, cache->view, s))
+      return rc;
+  }
+  if (plan.own_splits) {
+    const int64_t items = (int64_t)in->batch * kd.kv_heads * ((a.group + kRows - 1) / kRows);
+    a.first_part = plan.shared_splits;
+    a.splits = plan.own_splits;
+    if (int32_t rc = launch_rows<kOwn>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
+                                       PromptArgs{}, a, cache->view, s))
+      return rc;
+  }
+  if (plan.parts() > 1) {
+    if (kd.type == DM_BF16) join_kernel<true><<<(unsigned)a.part.rows, kThreads, 0, s>>>(a, kd.head_dim);
+    else join_kernel<false><<<(unsigned)a.part.rows, kThreads, 0, s>>>(a, kd.head_dim);
+    DM_CUDA(cudaGetLastError(), "attention join launch");
+  }
+  return DM_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,142 @@
+// dm_attention.cuh -- shared parts of the attention kernels (include/diskmule_attention.h).
+//
+// All of them keep, per query row, the running maximum m of the scores (times log2 e), the
+// running sum l of 2^(score - m) and the output sum o of 2^(score - m) v, in f32. Two such
+// states over disjoint keys join as m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), o
+// likewise; the result is o / l and lse = (m + log2 l) ln 2.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "dm_kvcache.cuh"
+
+namespace dma {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct PromptArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t *out;
+  float *lse;
+  int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2];
+  const int32_t *q_offsets, *k_offsets;
+  int64_t q_tokens, k_tokens;
+  int32_t heads, kv_heads, group, dim, sequences, causal, window;
+  float scale;  // times log2 e
+};
+
+// States of parts of the keys: o [part][row][dim], ml [part][row] = (m, l), with row =
+// batch * heads + head. o is undefined where l is zero.
+struct PartArgs {
+  float *o;
+  float2 *ml;
+  int32_t parts;
+  int64_t rows;
+};
+
+struct DecodeArgs {
+  const uint16_t *q;
+  uint16_t *out;
+  float *lse;
+  int64_t q_stride[2], out_stride[2];
+  const int32_t *sequences;
+  int32_t heads, group, batch, layer, window, shared, max_length;
+  float scale;
+  PartArgs part;       // part.parts == 1: results go straight to out and lse
+  int32_t first_part;  // of this launch
+  int32_t splits;      // parts of this launch
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// two f32 -> two 16-bit values, `low` in the low half
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float low, float high) {
+  uint32_t r;
+  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+  return r;
+}
+
+// 16-bit patterns whose exponent is all ones are infinities and NaN
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint16_t x) {
+  constexpr uint16_t e = BF16 ? 0x7f80 : 0x7c00;
+  return (x & e) == e;
+}
+template <bool BF16>
+__device__ __forceinline__ float to_float(uint16_t x) {
+  if (BF16) return __uint_as_float((uint32_t)x << 16);
+  return __half2float(__ushort_as_half(x));
+}
+// x with its non-finite halves zeroed; `any` is set where there are some
+template <bool BF16>
+__device__ __forceinline__ uint32_t zero_not_finite(uint32_t x, bool &any) {
+  if (not_finite<BF16>((uint16_t)x)) x &= 0xffff0000u, any = true;
+  if (not_finite<BF16>((uint16_t)(x >> 16))) x &= 0xffffu, any = true;
+  return x;
+}
+
+// Packed prompts: sequence and place of tile `tile` when a sequence of L tokens has
+// ceil(L * per_token / rows) tiles. One warp; seq = -1 behind the last tile.
+struct TileOf {
+  int seq, tile, q0, q1;
+};
+__device__ __forceinline__ TileOf find_tile(const int32_t *offsets, int sequences, int64_t tokens,
+                                            int per_token, int rows, int64_t tile) {
+  const int lane = threadIdx.x & 31;
+  TileOf r{-1, 0, 0, 0};
+  for (int s0 = 0; s0 < sequences; s0 += 32) {
+    const int s = s0 + lane;
+    int q0 = 0, q1 = 0;
+    if (s < sequences) {
+      q0 = (int)min((int64_t)max(offsets[s], 0), tokens);
+      q1 = (int)max((int64_t)q0, min((int64_t)offsets[s + 1], tokens));
+    }
+    const int64_t n = ((int64_t)(q1 - q0) * per_token + rows - 1) / rows;
+    int64_t upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, tile < upto);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      r.seq = s0 + src;
+      r.tile = (int)__shfl_sync(0xffffffffu, tile - (upto - n), src);
+      r.q0 = __shfl_sync(0xffffffffu, q0, src);
+      r.q1 = __shfl_sync(0xffffffffu, q1, src);
+      return r;
+    }
+    tile -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return r;
+}
+
+// Row of the page table and tokens of batch entry b; an entry that is out of range is empty.
+__device__ __forceinline__ int sequence_of(const KvView &c, const DecodeArgs &a, int b, int *length) {
+  const int row = a.sequences ? a.sequences[b] : b;
+  if (row < 0 || row >= c.max_sequences) {
+    *length = 0;
+    return 0;
+  }
+  *length = min(max(c.lengths[row], 0), min(a.max_length, c.max_pages * c.page_tokens));
+  return row;
+}
+
+}  // namespace dma
