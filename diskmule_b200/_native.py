@@ -224,6 +224,7 @@ SIGNATURES = {
                                 C.POINTER(P)], I32),
     "dm_gguf_expert_layout": ([P, C.c_char_p, C.c_char_p, I32, P], I32),
     "dm_attention_prompt": ([P, C.POINTER(PromptDesc), P], I32),
+    "dm_attention_status": ([P, P], I32),
     "dm_kv_cache_create": ([P, C.POINTER(KvCacheDesc), C.POINTER(P)], I32),
     "dm_kv_cache_destroy": ([P], None),
     "dm_kv_cache_describe": ([P, C.POINTER(KvCacheDesc)], I32),

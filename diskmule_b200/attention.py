@@ -38,6 +38,11 @@ def prompt_attention(ctx: CudaContext, *, type: int, heads: int, kv_heads: int, 
     check(N.lib().dm_attention_prompt(ctx.handle, C.byref(d), _stream(stream)))
 
 
+def attention_status(ctx: CudaContext, stream: int = 0):
+    """Wait for `stream`; raises if a bounded wait inside an attention kernel ran out."""
+    check(N.lib().dm_attention_status(ctx.handle, _stream(stream)))
+
+
 class KvCache:
     """A paged key/value cache (dm_kv_cache). `memory`, `page_table`, `lengths` and
     `references` are device pointers that the caller keeps alive, or 0 to let the cache

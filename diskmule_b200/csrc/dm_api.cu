@@ -97,6 +97,7 @@ int32_t dm_cuda_create(int32_t device_ordinal, dm_cuda_context **out) {
     snprintf(ctx->name, sizeof ctx->name, "%s", prop.name);
   cudaError_t err = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
   if (err == cudaSuccess) err = cudaMalloc(&ctx->status, 256);
+  if (err == cudaSuccess) err = cudaMemset(ctx->status, 0, 256);
   if (err != cudaSuccess) {
     delete ctx;
     return cuda_fail(err, "context set-up");

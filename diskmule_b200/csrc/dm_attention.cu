@@ -7,6 +7,7 @@
 #include <cstdint>
 
 #include "dm_attention.cuh"
+#include "dm_attention_tc.cuh"
 
 using dmi::fail;
 
@@ -544,6 +545,7 @@ int32_t dm_attention_prompt(dm_cuda_context *ctx, const dm_attention_prompt_desc
   a.causal = in->causal;
   a.window = in->window;
   cudaSetDevice(ctx->device);
+  if (tile_prompt_fits(a)) return launch_tile_prompt(in->type, a, ctx->status, (cudaStream_t)stream);
   const int64_t tiles = in->q_tokens * a.group / kRows + in->sequences;
   if (tiles > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
   return launch_rows<kPrompt>(in->type, in->head_dim, dim3((unsigned)tiles, in->kv_heads), a,

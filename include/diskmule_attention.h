@@ -57,6 +57,9 @@ typedef struct {
 
 DM_API int32_t dm_attention_prompt(dm_cuda_context *ctx, const dm_attention_prompt_desc *desc,
                                    void *stream);
+/* Waits for `stream`; DM_ERR_TIMEOUT if a bounded wait inside an attention kernel of this
+ * context has run out since the last call (its output is then undefined). */
+DM_API int32_t dm_attention_status(dm_cuda_context *ctx, void *stream);
 
 /* ---- the paged cache ---------------------------------------------------------------- */
 
