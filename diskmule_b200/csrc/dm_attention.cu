@@ -453,20 +453,30 @@ int32_t launch_rows(int type, int dim, dim3 grid, const PromptArgs &p, const Dec
 
 // How a decode call is cut into parts. The workspace holds one state per part and row.
 struct DecodePlan {
-  int shared_splits = 0, own_splits = 0;
-  int parts() const { return shared_splits + own_splits; }
+  bool tiles = false;  // the shared part runs on tcgen05 tiles
+  int shared_splits = 0, shared_parts = 0, own_splits = 0;
+  int parts() const { return shared_parts + own_splits; }
 };
 
 constexpr int kTargetBlocks = 296;  // two blocks of four warps on each of 148 SMs
+constexpr int kTileBlocks = 148;    // one block of tiles on each
+constexpr int kMinTileRows = 16;
 
-DecodePlan decode_plan(int kv_heads, int heads, int batch, int shared, int max_length) {
+DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, int max_length) {
   DecodePlan plan;
   if (batch == 0) return plan;
   const int group = heads / kv_heads;
-  if (shared > 0) {
+  plan.tiles = shared > 0 && batch * group > kMinTileRows && group <= 128;
+  if (plan.tiles) {
+    const int units = tile_shared_alternates(dim, group, batch) ? 2 : 1;
+    const int tiles = (shared + 127) / 128;
+    plan.shared_splits = std::max(1, std::min(kTileBlocks / tile_shared_items(dim, kv_heads, group, batch), tiles / units));
+    plan.shared_parts = plan.shared_splits * units;
+  } else if (shared > 0) {
     const int64_t items = (int64_t)kv_heads * (((int64_t)batch * group + kRows - 1) / kRows);
     plan.shared_splits = (int)std::max<int64_t>(
         1, std::min<int64_t>((kTargetBlocks + items - 1) / items, (shared + 255) / 256));
+    plan.shared_parts = plan.shared_splits;
   }
   if (max_length > shared || shared == 0) {
     const int64_t items = (int64_t)batch * kv_heads * ((group + kRows - 1) / kRows);
@@ -563,7 +573,7 @@ int32_t dm_attention_decode_workspace(const dm_kv_cache *cache, int32_t heads, i
   if (shared_tokens < 0 || shared_tokens % d.page_tokens || shared_tokens > (int64_t)d.max_pages * d.page_tokens)
     return fail(DM_ERR_ELEMENT_COUNT, "%d shared tokens are no whole pages of the table", shared_tokens);
   if (max_length < 0) return fail(DM_ERR_ELEMENT_COUNT, "max_length %d", max_length);
-  *bytes = decode_workspace(decode_plan(d.kv_heads, heads, batch, shared_tokens, max_length),
+  *bytes = decode_workspace(decode_plan(d.kv_heads, heads, d.head_dim, batch, shared_tokens, max_length),
                             (int64_t)batch * heads, d.head_dim);
   return DM_OK;
 }
@@ -602,7 +612,7 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
   a.window = in->window;
   a.shared = in->shared_tokens;
   a.max_length = in->max_length;
-  const DecodePlan plan = decode_plan(kd.kv_heads, in->heads, in->batch, in->shared_tokens, in->max_length);
+  const DecodePlan plan = decode_plan(kd.kv_heads, in->heads, kd.head_dim, in->batch, in->shared_tokens, in->max_length);
   a.part.parts = plan.parts();
   a.part.rows = (int64_t)in->batch * in->heads;
   a.part.o = (float *)in->workspace;
@@ -613,13 +623,14 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
     const int64_t items = (int64_t)kd.kv_heads * (((int64_t)in->batch * a.group + kRows - 1) / kRows);
     a.first_part = 0;
     a.splits = plan.shared_splits;
-    if (int32_t rc = launch_rows<kShared>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
+    if (int32_t rc = plan.tiles ? launch_tile_shared(kd.type, a, cache->view, cache->ctx->status, s)
+                                : launch_rows<kShared>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
                                           PromptArgs{}, a, cache->view, s))
       return rc;
   }
   if (plan.own_splits) {
     const int64_t items = (int64_t)in->batch * kd.kv_heads * ((a.group + kRows - 1) / kRows);
-    a.first_part = plan.shared_splits;
+    a.first_part = plan.shared_parts;
     a.splits = plan.own_splits;
     if (int32_t rc = launch_rows<kOwn>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
                                        PromptArgs{}, a, cache->view, s))
