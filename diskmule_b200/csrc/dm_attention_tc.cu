@@ -124,6 +124,16 @@ struct Work {
   }
 };
 
+// One lane of a converged warp. What it decides is uniform, so the operands of the
+// instructions under it can stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(yes));
+  return yes != 0;
+}
+
 // Bounded wait that also ends when another role has given up.
 __device__ __forceinline__ bool wait(TcSmem &sh, uint64_t &bar, uint32_t parity) {
   const uint32_t b = smem_u32(&bar);
@@ -139,6 +149,16 @@ __device__ __forceinline__ bool wait(TcSmem &sh, uint64_t &bar, uint32_t parity)
 // The same for a whole warp: one answer for all lanes.
 __device__ __forceinline__ bool wait_warp(TcSmem &sh, uint64_t &bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait(sh, bar, parity));
+}
+
+// Two units: the 168 registers a thread that 384 threads start with, split anew (256 x 208 +
+// 128 x 88 = 384 x 168), so that a row's 128 scores and the weights made from them stay in
+// registers. Every warp of a group of four calls the same one.
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+}
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 }
 
 template <int MODE, int DP, bool BF16>
@@ -285,6 +305,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
 
   if (warp == Cfg::kSoftWarps) {
     // ---- TMA
+    if (kUnits == 2) give_registers();
     if (w.tiles > 0) {
       if (lane == 0) {
         for (int u = 0; u < kUnits; u++) {
@@ -343,7 +364,9 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     }
   } else if (warp == Cfg::kSoftWarps + 1) {
     // ---- MMA issue
-    if (lane == 0 && w.tiles > 0) {
+    if (kUnits == 2) give_registers();
+    // the whole warp follows the schedule, one lane issues
+    if (w.tiles > 0) {
       constexpr uint32_t kQk = idesc(BF16, kTileKeys, false), kPv = idesc(BF16, DP, true);
       uint32_t full = 0, clean = 0;  // parity of the next V tile in a slot, by its barrier
       bool ok = true;
@@ -351,23 +374,29 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       auto products_s = [&](int u, int t, int buffer) {
         const uint64_t qd = q_desc + ((u * Cfg::kTile) >> 4);
         const uint64_t kd = sw128_desc(ring + ((2 * t) % Cfg::kSlots) * Cfg::kTile);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < DP / 16; k++) {
-          const uint64_t at = (k / 4) * (Cfg::kSlab >> 4) + (k % 4) * 2;
-          mma_ss(tmem + buffer * 128, qd + at, kd + at, kQk, k > 0);
+          for (int k = 0; k < DP / 16; k++) {
+            const uint64_t at = (k / 4) * (Cfg::kSlab >> 4) + (k % 4) * 2;
+            mma_ss(tmem + buffer * 128, qd + at, kd + at, kQk, k > 0);
+          }
+          mma_commit(smem_u32(&sh.s_full[buffer]));
         }
-        mma_commit(smem_u32(&sh.s_full[buffer]));
+        __syncwarp();
       };
       auto products_o = [&](int u, int t, int buffer, bool add) {
         const uint64_t vd = v_desc(ring + ((2 * t + 1) % Cfg::kSlots) * Cfg::kTile, Cfg::kSlab);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kTileKeys / 16; k++)
-          mma_ts(tmem + Cfg::kOutCol + u * DP, tmem + buffer * 128 + k * 8, vd + k * (2048 >> 4), kPv,
-                 add || k > 0);
-        mma_commit(smem_u32(&sh.pv_done[u]));
+          for (int k = 0; k < kTileKeys / 16; k++)
+            mma_ts(tmem + Cfg::kOutCol + u * DP, tmem + buffer * 128 + k * 8, vd + k * (2048 >> 4), kPv,
+                   add || k > 0);
+          mma_commit(smem_u32(&sh.pv_done[u]));
+        }
+        __syncwarp();
       };
       auto k_there = [&](int t) {
-        return wait(sh, sh.full[(2 * t) % Cfg::kSlots], (2 * t / Cfg::kSlots) & 1);
+        return wait_warp(sh, sh.full[(2 * t) % Cfg::kSlots], (2 * t / Cfg::kSlots) & 1);
       };
       // first of the units that use V tile t waits for it, in its clean form where mixed
       auto v_there = [&](int t, bool first_use) {
@@ -377,9 +406,12 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         uint32_t &parity = mixed ? clean : full;
         const uint32_t now = (parity >> slot) & 1;
         parity ^= 1u << slot;
-        return wait(sh, mixed ? sh.clean[slot] : sh.full[slot], now);
+        return wait_warp(sh, mixed ? sh.clean[slot] : sh.full[slot], now);
       };
-      auto release = [&](int i) { mma_commit(smem_u32(&sh.empty[i % Cfg::kSlots])); };
+      auto release = [&](int i) {
+        if (elect_one()) mma_commit(smem_u32(&sh.empty[i % Cfg::kSlots]));
+        __syncwarp();
+      };
       if (kUnits == 2) {
         const int n[2] = {n0, n1};
         const int most = max(n0, n1);
@@ -387,7 +419,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         for (int u = 0; u < 2; u++) {
           if (n[u] == 0 || !ok) continue;
           const int t = tile_of(u, 0);
-          ok = wait(sh, sh.q_full[u], 0) && k_there(t);
+          ok = wait_warp(sh, sh.q_full[u], 0) && k_there(t);
           if (!ok) break;
           fence_after();
           products_s(u, t, u);
@@ -399,7 +431,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             if (i >= n[u] || !ok) continue;
             const int t = tile_of(u, i);
             const bool first_use = alternate || u == 0 || i >= n0;
-            ok = wait(sh, sh.p_full[u], i & 1) && v_there(t, first_use);
+            ok = wait_warp(sh, sh.p_full[u], i & 1) && v_there(t, first_use);
             if (!ok) break;
             fence_after();
             products_o(u, t, u, i > 0);
@@ -415,7 +447,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           }
         }
       } else {
-        ok = wait(sh, sh.q_full[0], 0) && k_there(0);
+        ok = wait_warp(sh, sh.q_full[0], 0) && k_there(0);
         if (ok) {
           fence_after();
           products_s(0, 0, 0);
@@ -429,7 +461,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             products_s(0, t + 1, (t + 1) & 1);
             release(2 * t + 2);
           }
-          ok = wait(sh, sh.p_full[t & 1], (t >> 1) & 1) && v_there(t, true);
+          ok = wait_warp(sh, sh.p_full[t & 1], (t >> 1) & 1) && v_there(t, true);
           if (!ok) break;
           fence_after();
           products_o(0, t, t & 1, t > 0);
@@ -437,13 +469,14 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         }
       }
       if (!ok) {  // products in flight end before tensor memory is given back
-        mma_commit(smem_u32(&sh.drain));
+        if (elect_one()) mma_commit(smem_u32(&sh.drain));
         mbar_wait(smem_u32(&sh.drain), 0);
       }
     }
     __syncwarp();
   } else if (warp >= Cfg::kSoftWarps + 2) {
     // ---- values that are not finite leave mixed tiles
+    if (kUnits == 2) give_registers();
     const int who = tid - (Cfg::kSoftWarps + 2) * 32;
     uint32_t dirty = 0;  // parity of the next mixed tile in a slot
     for (int t = 0; t < w.tiles; t++) {
@@ -476,6 +509,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     }
   } else {
     // ---- softmax: one thread per row
+    if (kUnits == 2) take_registers();
     const int n = unit ? n1 : n0;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
     const uint32_t o_at = tmem + lanes + Cfg::kOutCol + unit * DP;
