@@ -49,6 +49,13 @@ Plan plan_of(const dm_kv_cache *c) {
   return p;
 }
 
+// The next kernel on the stream may be scheduled now; this one waits until the one before it
+// has ended and its writes are seen.
+__device__ __forceinline__ void chain() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Inclusive sum over the block; `total` gets the block's. Every thread of the block calls it.
 __device__ int block_scan(int v, int *total) {
   __shared__ int sums[kPlanThreads / 32];
@@ -109,6 +116,12 @@ template <int OP>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, PlanArgs a) {
   __shared__ int bad;
   const int tid = threadIdx.x;
+  chain();
+  // the first pages' references come in beside the list (most calls need no others)
+  int refs[kFreeBatch];
+#pragma unroll
+  for (int k = 0; k < kFreeBatch; k++)
+    refs[k] = tid * kFreeBatch + k < c.pages ? c.references[tid * kFreeBatch + k] : 1;
   if (tid == 0) bad = 0;
   __syncthreads();
   for (int i = tid; i < a.n; i += kPlanThreads) {
@@ -186,10 +199,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
   int found = 0;
   if (!bad && total <= c.pages) {
     for (int p0 = 0; p0 < c.pages && found < total; p0 += kPlanThreads * kFreeBatch) {
-      int refs[kFreeBatch], mine = 0;
+      int mine = 0;
       const int at = p0 + tid * kFreeBatch;
+      if (p0 > 0)
 #pragma unroll
-      for (int k = 0; k < kFreeBatch; k++) refs[k] = at + k < c.pages ? c.references[at + k] : 1;
+        for (int k = 0; k < kFreeBatch; k++) refs[k] = at + k < c.pages ? c.references[at + k] : 1;
 #pragma unroll
       for (int k = 0; k < kFreeBatch; k++) mine += refs[k] == 0;
       int sum;
@@ -222,10 +236,55 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
   }
 }
 
+// `rows` rows of `vec` 16-byte vectors in each of a page's parts (layer, K or V, head): a
+// thread keeps its place in a part and walks over the parts, kDepth loads in flight, so the
+// loop has no division. Parts blockIdx.x, + gridDim.x, ... of the page are this block's
+// share (several at once where a part has fewer vectors than the block threads). from(r) is
+// the source row's address in part 0, null for none. ONCE: nobody reads the source again.
+constexpr int kDepth = 4;
+
+template <bool ONCE>
+__device__ __forceinline__ uint4 load16(const uint8_t *p) {
+  const uint4 *v = reinterpret_cast<const uint4 *>(p);
+  return ONCE ? __ldcs(v) : *v;
+}
+
+template <bool ONCE, typename From>
+__device__ __forceinline__ void copy_parts(const KvView &c, uint8_t *to, int rows, From from) {
+  const int vec = c.head_dim / 8, chunk = rows * vec;
+  const int parts = c.layers * 2 * c.kv_heads;
+  const int wide = chunk < kCopyThreads ? kCopyThreads / chunk : 1;  // parts side by side
+  const int place = wide > 1 ? threadIdx.x / chunk : 0;
+  if (place >= wide) return;
+  const int step = gridDim.x * wide;
+  for (int in = wide > 1 ? threadIdx.x % chunk : threadIdx.x; in < chunk; in += kCopyThreads) {
+    const uint8_t *src = from(in / vec);
+    if (src) {
+      src += (in % vec) * 16;
+      uint8_t *dst = to + (int64_t)in * 16;
+      int part = blockIdx.x * wide + place;
+      for (; part + (kDepth - 1) * step < parts; part += kDepth * step) {
+        uint4 r[kDepth];
+#pragma unroll
+        for (int k = 0; k < kDepth; k++)
+          r[k] = load16<ONCE>(src + (part + k * step) * c.head_bytes);
+#pragma unroll
+        for (int k = 0; k < kDepth; k++)
+          *reinterpret_cast<uint4 *>(dst + (part + k * step) * c.head_bytes) = r[k];
+      }
+      for (; part < parts; part += step)
+        *reinterpret_cast<uint4 *>(dst + part * c.head_bytes) =
+            load16<ONCE>(src + part * c.head_bytes);
+    }
+    if (wide > 1) break;
+  }
+}
+
 // Fork: block (x, i) copies its part of entry i's partial page; block (0, i) also writes the
 // child's row and counts the shared pages.
 __global__ void __launch_bounds__(kCopyThreads)
 fork_kernel(KvView c, Plan p, const int32_t *parents, const int32_t *children) {
+  chain();
   if (!*p.ok) return;
   const int i = blockIdx.y;
   const int parent = parents[i], child = children[i];
@@ -252,36 +311,16 @@ fork_kernel(KvView c, Plan p, const int32_t *parents, const int32_t *children) {
   if ((unsigned)old >= (unsigned)c.pages) return;
   const uint8_t *src = c.memory + old * c.page_bytes;
   uint8_t *dst = c.memory + p.fresh[p.first[i]] * c.page_bytes;
-  // the used rows of every (layer, K or V, head): `rest` rows that lie together
-  const uint32_t chunk = (uint32_t)(rest * c.head_dim / 8);  // 16-byte vectors
-  const uint32_t total = chunk * (uint32_t)(c.layers * 2 * c.kv_heads);
-  const uint32_t stride = gridDim.x * kCopyThreads;
-  for (uint32_t v0 = blockIdx.x * kCopyThreads + threadIdx.x; v0 < total; v0 += 4 * stride) {
-    uint4 r[4];
-    int64_t at[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const uint32_t v = v0 + k * stride;
-      if (v >= total) continue;
-      at[k] = (v / chunk) * c.head_bytes + (int64_t)(v % chunk) * 16;
-      r[k] = *reinterpret_cast<const uint4 *>(src + at[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const uint32_t v = v0 + k * stride;
-      if (v >= total) continue;
-      *reinterpret_cast<uint4 *>(dst + at[k]) = r[k];
-    }
-  }
+  const int64_t row_bytes = c.head_dim * 2;
+  copy_parts<false>(c, dst, rest, [&](int r) { return src + r * row_bytes; });
 }
 
 // Compact: block (x, f) gathers its part of fresh page f (f strides over the plan's).
 __global__ void __launch_bounds__(kCopyThreads)
 gather_kernel(KvView c, Plan p, PlanArgs a) {
+  chain();
   if (!*p.ok) return;
   const int total = *p.total;
-  const int vec = c.head_dim / 8;
-  const uint32_t chunks = (uint32_t)(c.layers * 2 * c.kv_heads);
   __shared__ int64_t source[256];  // of each row of the page, -1 where it has none
   for (int f = blockIdx.y; f < total; f += gridDim.y) {
     const int i = p.owner[f], row = a.rows[i];
@@ -297,38 +336,21 @@ gather_kernel(KvView c, Plan p, PlanArgs a) {
       } else {
         const int page = c.table[(int64_t)row * c.max_pages + token / c.page_tokens];
         if ((unsigned)page < (unsigned)c.pages)
-          at = page * c.page_bytes + (int64_t)(token % c.page_tokens) * vec * 16;
+          at = page * c.page_bytes + (int64_t)(token % c.page_tokens) * c.head_dim * 2;
       }
       source[r] = at;
     }
     __syncthreads();
     uint8_t *dst = c.memory + p.fresh[f] * c.page_bytes;
-    const uint32_t chunk = (uint32_t)(used * vec), all = chunk * chunks;
-    const uint32_t stride = gridDim.x * kCopyThreads;
-    for (uint32_t v0 = blockIdx.x * kCopyThreads + threadIdx.x; v0 < all; v0 += 4 * stride) {
-      uint4 r[4];
-      int64_t to[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const uint32_t v = v0 + k * stride;
-        to[k] = -1;
-        if (v >= all) continue;
-        const uint32_t part = v / chunk, in = v % chunk;
-        const int64_t from = source[in / vec];
-        if (from < 0) continue;
-        to[k] = part * c.head_bytes + (int64_t)in * 16;
-        r[k] = *reinterpret_cast<const uint4 *>(c.memory + from + part * c.head_bytes +
-                                                (in % vec) * 16);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (to[k] >= 0) *reinterpret_cast<uint4 *>(dst + to[k]) = r[k];
-    }
+    copy_parts<true>(c, dst, used, [&](int r) -> const uint8_t * {
+      return source[r] < 0 ? nullptr : c.memory + source[r];
+    });
   }
 }
 
 // Compact, after the rows have moved: block i lets go of the old pages and writes the row.
 __global__ void __launch_bounds__(kCopyThreads) settle_kernel(KvView c, Plan p, PlanArgs a) {
+  chain();
   if (!*p.ok) return;
   const int i = blockIdx.x, row = a.rows[i];
   const int count = a.other[i + 1] - a.other[i];
@@ -351,6 +373,7 @@ __global__ void __launch_bounds__(kCopyThreads) settle_kernel(KvView c, Plan p, 
 // Free: block i takes the length of its sequence (a repeat finds zero) and lets go.
 __global__ void __launch_bounds__(kCopyThreads) free_kernel(KvView c, const int32_t *rows) {
   __shared__ int held;
+  chain();
   const int row = rows[blockIdx.x];
   if (row < 0 || row >= c.max_sequences) {
     if (threadIdx.x == 0) atomicOr(c.status, DM_KV_BAD_SEQUENCE);
@@ -374,11 +397,14 @@ struct WriteArgs {
   int64_t tokens;
 };
 
-// Write: one warp per token; lanes over its heads' 16-byte vectors, K then V.
+// Write: one thread per 16-byte vector of a token's keys and values.
 __global__ void __launch_bounds__(kCopyThreads) write_kernel(KvView c, WriteArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5);
+  chain();
+  const int vec = c.head_dim / 8, half = c.kv_heads * vec;
+  const int64_t at = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
+  const int64_t t = at / (2 * half);
   if (t >= a.tokens) return;
-  const int lane = threadIdx.x & 31;
+  const int i = (int)(at - t * 2 * half);
   // the sequence whose rows hold t: the last offset that is not above it
   int low = 0, high = a.n;
   while (high - low > 1) {
@@ -386,33 +412,31 @@ __global__ void __launch_bounds__(kCopyThreads) write_kernel(KvView c, WriteArgs
     if (a.offsets[mid] <= t) low = mid;
     else high = mid;
   }
-  const int row = a.rows[low];
+  const int row = a.rows[low], o0 = a.offsets[low], o1 = a.offsets[low + 1];
   int64_t place = -1;
   int page = -1;
-  if (row >= 0 && row < c.max_sequences && t >= a.offsets[low] && t < a.offsets[low + 1]) {
+  if (row >= 0 && row < c.max_sequences && t >= o0 && t < o1) {
     const int length = c.lengths[row];
-    place = length - ((int64_t)a.offsets[low + 1] - t);
+    place = length - ((int64_t)o1 - t);
     if (place >= 0 && place < length && place / c.page_tokens < c.max_pages)
       page = c.table[(int64_t)row * c.max_pages + place / c.page_tokens];
   }
   if ((unsigned)page >= (unsigned)c.pages) {
-    if (lane == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
+    if (i == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
     return;
   }
+  const int which = i >= half, head = (i - which * half) / vec, in = (i - which * half) % vec;
+  const uint8_t *src = (which ? a.v : a.k) +
+                       (t * a.stride[which][0] + head * a.stride[which][1]) * 2 + in * 16;
   uint8_t *dst = c.memory + page * c.page_bytes + a.layer * c.layer_bytes +
-                 (place % c.page_tokens) * c.head_dim * 2;
-  const int vec = c.head_dim / 8, half = c.kv_heads * vec;
-  for (int i = lane; i < 2 * half; i += 32) {
-    const int which = i >= half, head = (i - which * half) / vec, in = (i - which * half) % vec;
-    const uint8_t *src = (which ? a.v : a.k) +
-                         (t * a.stride[which][0] + head * a.stride[which][1]) * 2 + in * 16;
-    *reinterpret_cast<uint4 *>(dst + (which * c.kv_heads + head) * c.head_bytes + in * 16) =
-        *reinterpret_cast<const uint4 *>(src);
-  }
+                 (which * c.kv_heads + head) * c.head_bytes +
+                 (place % c.page_tokens) * c.head_dim * 2 + in * 16;
+  *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
 }
 
 __global__ void __launch_bounds__(kCopyThreads)
 copy_pages_kernel(KvView c, const int32_t *source, const int32_t *target) {
+  chain();
   const int from = source[blockIdx.y], to = target[blockIdx.y];
   if ((unsigned)from >= (unsigned)c.pages || (unsigned)to >= (unsigned)c.pages) {
     if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
@@ -439,6 +463,22 @@ int blocks_along(int64_t vectors, int64_t items, int64_t blocks) {
   return (int)std::max<int64_t>(1, std::min(fit, blocks / std::max<int64_t>(1, items)));
 }
 constexpr int kGridBlocks = 148 * 8;
+
+// A launch that may be scheduled while the kernel before it still runs (see chain).
+template <typename... Params, typename... Args>
+int32_t launch(void (*kernel)(Params...), dim3 grid, int threads, void *stream, Args... args) {
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = threads;
+  config.stream = (cudaStream_t)stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  DM_CUDA(cudaLaunchKernelEx(&config, kernel, Params(args)...), "cache launch");
+  return DM_OK;
+}
 
 int32_t check_list(const dm_kv_cache *cache, const void *list, int32_t n) {
   if (!cache) return fail(DM_ERR_INVALID_ARGUMENT, "null cache");
@@ -572,10 +612,8 @@ int32_t dm_kv_cache_extend(dm_kv_cache *c, const int32_t *sequences, const int32
   if (n == 0) return DM_OK;
   if (!counts) return fail(DM_ERR_INVALID_ARGUMENT, "null counts");
   cudaSetDevice(c->ctx->device);
-  plan_kernel<kExtend><<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(
-      c->view, plan_of(c), PlanArgs{sequences, counts, nullptr, 0, n});
-  DM_CUDA(cudaGetLastError(), "cache extend launch");
-  return DM_OK;
+  return launch(plan_kernel<kExtend>, 1, kPlanThreads, stream, c->view, plan_of(c),
+                PlanArgs{sequences, counts, nullptr, 0, n});
 }
 
 int32_t dm_kv_cache_write(dm_kv_cache *c, int32_t layer, const void *k, const void *v,
@@ -600,11 +638,10 @@ int32_t dm_kv_cache_write(dm_kv_cache *c, int32_t layer, const void *k, const vo
   if (((uintptr_t)k | (uintptr_t)v) & 15)
     return fail(DM_ERR_INVALID_ARGUMENT, "keys and values must be 16-byte aligned");
   cudaSetDevice(c->ctx->device);
-  const int warps = kCopyThreads / 32;
-  write_kernel<<<(unsigned)((tokens + warps - 1) / warps), kCopyThreads, 0, (cudaStream_t)stream>>>(
-      c->view, a);
-  DM_CUDA(cudaGetLastError(), "cache write launch");
-  return DM_OK;
+  const int64_t vectors = tokens * c->desc.kv_heads * c->desc.head_dim / 4;  // K and V
+  const int64_t blocks = (vectors + kCopyThreads - 1) / kCopyThreads;
+  if (blocks > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many tokens in one write");
+  return launch(write_kernel, (unsigned)blocks, kCopyThreads, stream, c->view, a);
 }
 
 int32_t dm_kv_cache_fork(dm_kv_cache *c, const int32_t *parents, const int32_t *children,
@@ -614,14 +651,12 @@ int32_t dm_kv_cache_fork(dm_kv_cache *c, const int32_t *parents, const int32_t *
   if (!parents) return fail(DM_ERR_INVALID_ARGUMENT, "null parents");
   if (n > 65535) return fail(DM_ERR_ELEMENT_COUNT, "%d forks in one call", n);
   cudaSetDevice(c->ctx->device);
-  cudaStream_t s = (cudaStream_t)stream;
-  plan_kernel<kFork><<<1, kPlanThreads, 0, s>>>(c->view, plan_of(c),
-                                                PlanArgs{children, parents, nullptr, 0, n});
+  if (int32_t rc = launch(plan_kernel<kFork>, 1, kPlanThreads, stream, c->view, plan_of(c),
+                          PlanArgs{children, parents, nullptr, 0, n}))
+    return rc;
   // half a page is copied on average
   const dim3 grid(blocks_along(c->view.page_bytes / 32, n, kGridBlocks), n);
-  fork_kernel<<<grid, kCopyThreads, 0, s>>>(c->view, plan_of(c), parents, children);
-  DM_CUDA(cudaGetLastError(), "cache fork launch");
-  return DM_OK;
+  return launch(fork_kernel, grid, kCopyThreads, stream, c->view, plan_of(c), parents, children);
 }
 
 int32_t dm_kv_cache_compact(dm_kv_cache *c, const int32_t *sequences, const int32_t *keep_offsets,
@@ -631,26 +666,22 @@ int32_t dm_kv_cache_compact(dm_kv_cache *c, const int32_t *sequences, const int3
   if (n == 0) return DM_OK;
   if (!keep_offsets || (kept && !keep)) return fail(DM_ERR_INVALID_ARGUMENT, "null keep list");
   cudaSetDevice(c->ctx->device);
-  cudaStream_t s = (cudaStream_t)stream;
   const PlanArgs a{sequences, keep_offsets, keep, kept, n};
-  plan_kernel<kCompact><<<1, kPlanThreads, 0, s>>>(c->view, plan_of(c), a);
+  if (int32_t rc = launch(plan_kernel<kCompact>, 1, kPlanThreads, stream, c->view, plan_of(c), a))
+    return rc;
   // at most this many fresh pages
   const int64_t fresh = std::min<int64_t>(c->desc.pages, kept / c->desc.page_tokens + n);
   const dim3 grid(blocks_along(c->view.page_bytes / 16, fresh, kGridBlocks),
-                  (unsigned)std::min<int64_t>(fresh, kGridBlocks));
-  gather_kernel<<<grid, kCopyThreads, 0, s>>>(c->view, plan_of(c), a);
-  settle_kernel<<<n, kCopyThreads, 0, s>>>(c->view, plan_of(c), a);
-  DM_CUDA(cudaGetLastError(), "cache compact launch");
-  return DM_OK;
+                  (unsigned)std::min<int64_t>(fresh, 65535));
+  if (int32_t rc = launch(gather_kernel, grid, kCopyThreads, stream, c->view, plan_of(c), a)) return rc;
+  return launch(settle_kernel, n, kCopyThreads, stream, c->view, plan_of(c), a);
 }
 
 int32_t dm_kv_cache_free(dm_kv_cache *c, const int32_t *sequences, int32_t n, void *stream) {
   if (int32_t rc = check_list(c, sequences, n)) return rc;
   if (n == 0) return DM_OK;
   cudaSetDevice(c->ctx->device);
-  free_kernel<<<n, kCopyThreads, 0, (cudaStream_t)stream>>>(c->view, sequences);
-  DM_CUDA(cudaGetLastError(), "cache free launch");
-  return DM_OK;
+  return launch(free_kernel, n, kCopyThreads, stream, c->view, sequences);
 }
 
 int32_t dm_kv_cache_copy_pages(dm_kv_cache *c, const int32_t *source, const int32_t *target,
@@ -662,9 +693,7 @@ int32_t dm_kv_cache_copy_pages(dm_kv_cache *c, const int32_t *source, const int3
   if (!source || !target) return fail(DM_ERR_INVALID_ARGUMENT, "null list");
   cudaSetDevice(c->ctx->device);
   const dim3 grid(blocks_along(c->view.page_bytes / 16, n, kGridBlocks), n);
-  copy_pages_kernel<<<grid, kCopyThreads, 0, (cudaStream_t)stream>>>(c->view, source, target);
-  DM_CUDA(cudaGetLastError(), "page copy launch");
-  return DM_OK;
+  return launch(copy_pages_kernel, grid, kCopyThreads, stream, c->view, source, target);
 }
 
 }  // extern "C"
