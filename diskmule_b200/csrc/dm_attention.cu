@@ -469,7 +469,7 @@ DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, 
   plan.tiles = shared > 0 && batch * group > kMinTileRows && group <= 128;
   if (plan.tiles) {
     const int units = tile_shared_alternates(dim, group, batch) ? 2 : 1;
-    const int tiles = (shared + 127) / 128;
+    const int tiles = (shared + tile_keys(dim) - 1) / tile_keys(dim);
     plan.shared_splits = std::max(1, std::min(kTileBlocks / tile_shared_items(dim, kv_heads, group, batch), tiles / units));
     plan.shared_parts = plan.shared_splits * units;
   } else if (shared > 0) {

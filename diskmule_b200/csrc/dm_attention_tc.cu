@@ -1,8 +1,8 @@
-// dm_attention_tc.cu -- attention on tcgen05 tiles: 128 query rows against 128 keys.
+// dm_attention_tc.cu -- attention on tcgen05 tiles: 128 query rows against a tile of keys.
 //
 // A block holds one or two units. A unit is 128 query rows (whole groups of query heads of
-// one key/value head: row = token * group + head) with its own scores S [128 x 128 f32],
-// weights P (16-bit, over S in tensor memory) and output sum O [128 x dim f32]. Per tile:
+// one key/value head: row = token * group + head) with its own scores S [128 x keys f32],
+// weights P (16-bit) and output sum O [128 x dim f32], all in tensor memory. Per tile:
 //   S = Q K^T       tcgen05.mma, both operands in shared memory (128-byte swizzle, TMA)
 //   P = 2^(S - m)   one thread per row: maximum, exponentials, sum, all f32
 //   O += P V        tcgen05.mma, P in tensor memory, V as it lies (keys down, dim across)
@@ -10,14 +10,21 @@
 // by more than 2^8 since m was taken; until then the weights of newer keys may reach 2^8,
 // which changes no relative rounding, and the common factor leaves in o / l.
 //
-// Up to dim 128 two units alternate on the tensor pipe: while one computes its exponentials
-// the other's products run, and both read the same K and V tiles. For dim 256, O takes half
-// of tensor memory, so one unit runs with two S buffers and the products of the next tile
-// run under the exponentials of this one.
+// The threads of a unit should never wait for products. So S of the next tile is computed
+// while the weights of this one are: P has columns of its own beside S, and tensor memory
+// (512 columns) sets the tile's keys. dim 64: 2 units of S 128 + P 64 + O 64. dim 128: 2 of
+// S 80 + P 40 + O 128. dim 256, where O takes 256: one unit with two S of 128, each turned
+// into P in place. Both units read the same K and V tiles.
 //
-// Warps: 4 per unit softmax and output; then TMA, MMA issue, and two that keep values that
-// are not finite out of tiles in which some key is hidden from some row (0 * NaN): they
-// zero them in shared memory, and the output step adds them for the rows that see them.
+// A block works through several items (prompt: 256 or 128 query rows; it takes over blocks
+// that have not started yet), so that loads, first products and output of different items
+// overlap. Every wait and every product costs its warp 100 cycles or more, so each job has
+// warps of its own with a short loop: 4 per unit for softmax and output, one each for the
+// products S and O of a unit, for the loads of K and of V, for the choice of items, and one
+// that keeps values that are not finite out of tiles in which some key is hidden from some
+// row (0 * NaN): it zeroes them in shared memory, and the output step adds them for the rows
+// that see them. (One warp for all products of both units: 3600 cycles for 128 keys at dim
+// 128, where the tensor pipe needs 2048; one per unit: 4100.)
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -34,32 +41,63 @@ using namespace dm::tc;
 
 namespace {
 
-constexpr int kUnitRows = 128, kTileKeys = 128;
+constexpr int kUnitRows = 128;
 constexpr int kStatusWord = 32;  // of the context's status buffer: a bounded wait ran out
+constexpr int kItems = 4;        // items between the first role and the last
+constexpr int kMostSlots = 5;
 
 template <int DP>
 struct TcCfg {
   static constexpr int kUnits = DP == 256 ? 1 : 2;
   static constexpr int kBuffers = DP == 256 ? 2 : 1;         // S buffers of a unit
+  static constexpr int kKeys = DP == 128 ? 80 : 128;         // of a tile
+  // warps
   static constexpr int kSoftWarps = 4 * kUnits;
-  static constexpr int kThreads = (kSoftWarps + 4) * 32;
-  static constexpr int kSlab = 128 * 128;                    // 128 rows x 64 values
-  static constexpr int kTile = DP / 64 * kSlab;              // a Q, K or V tile
-  static constexpr int kSlots = DP == 64 ? 8 : DP == 128 ? 4 : 2;  // ring of K and V tiles
-  static constexpr int kSmem = 1024 + (kUnits + kSlots) * kTile;
-  static constexpr int kOutCol = 256;                        // O in tensor memory; S before it
+  static constexpr int kItemWarp = kSoftWarps, kKWarp = kItemWarp + 1, kVWarp = kItemWarp + 2;
+  static constexpr int kScrubWarp = kItemWarp + 3;
+  static constexpr int kSWarp = kItemWarp + 4;               // products S, one warp per unit
+  static constexpr int kOWarp = kSWarp + kUnits;             // products O
+  static constexpr int kConsumers = kSoftWarps + 3 + 2 * kUnits;  // of an item
+  static constexpr int kThreads = DP == 256 ? 384 : 512;     // whole groups of four warps
+  // K and V move in chunks, each in a ring of its own: whole tiles, or for dim 256 quarters
+  // (64 values of all keys of K, 32 keys of V), so that a chunk's place is free again soon.
+  static constexpr int kChunks = DP == 256 ? 4 : 1;          // of a tile
+  static constexpr int kChunkBytes = kKeys * DP * 2 / kChunks;
+  static constexpr int kVKeys = kKeys / kChunks;             // keys of a V chunk
+  static constexpr int kKSlabs = DP / 64 / kChunks;          // 64-value slabs of a K chunk
+  static constexpr int kSlots = DP == 128 ? 4 : 5;           // of a ring
+  static constexpr int kQBytes = kUnitRows * DP * 2;
+  static constexpr int kSmem = 1024 + kUnits * kQBytes + 2 * kSlots * kChunkBytes;
+  // columns of tensor memory
+  static constexpr int kUnitCols = DP == 64 ? 192 : 128;     // from unit to unit (buffer to buffer)
+  static constexpr int kPCol = DP == 256 ? 0 : kKeys;        // P from S; 0: in its place
+  static constexpr int kOCol = DP == 64 ? 384 : 256;
+  // Registers: the launch's share (128 or 168 a thread) split anew, so that a row's scores and
+  // the weights made from them stay in registers: 256 x 192 + 256 x 64 = 512 x 128, and
+  // 128 x 216 + 256 x 144 = 384 x 168.
+  static constexpr int kSoftRegs = DP == 256 ? 216 : 192, kOtherRegs = DP == 256 ? 144 : 64;
+};
+
+// What the roles know of an item.
+struct Item {
+  int stop, kv_head, first, tiles;  // first key, number of key tiles
+  int n[2];                         // tiles of each unit
+  int max_low, min_high;            // every row sees the keys [max_low, min_high)
+  int token0, lq, lk, q0, k0;       // first token of the item and of its sequence
+  int table_row, wild;              // wild: values that are not finite were found
 };
 
 struct TcSmem {
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
-  // K and V tiles: loaded; a V tile that is mixed has `dirty` in place of `full` for loaded,
-  // and `clean` for fit to use; `empty` when its last product is done. K takes the even slots.
-  uint64_t full[8], empty[8], dirty[8], clean[8], drain;
+  uint64_t item_full[kItems], item_empty[kItems], next_block;
+  uint64_t want;  // the keys of an item have been asked for: time for the next item
+  uint64_t q_full, q_empty, s_full[2], s_free[2], p_full[2], pv_done[2];
+  // chunks: loaded; fit to use (V, by the scrub warp); all products done
+  uint64_t k_full[kMostSlots], k_empty[kMostSlots];
+  uint64_t v_full[kMostSlots], v_clean[kMostSlots], v_empty[kMostSlots], drain[4];
+  uint4 answer;  // which block was taken over
+  Item item[kItems];
   uint32_t tmem;
   volatile int abort;
-  int wild;      // a hidden-somewhere tile held values that are not finite
-  int max_low, min_high, keys;
-  TileOf tile;
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1,
@@ -72,6 +110,29 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Ask for a block of this grid that has not started; the answer lands in shared memory.
+__device__ __forceinline__ void take_block(uint32_t answer, uint32_t bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          answer),
+      "r"(bar)
+      : "memory");
+}
+// The taken block's x index, or -1 when none was left.
+__device__ __forceinline__ int taken_block(uint32_t answer) {
+  uint32_t yes, x, y, z, w;
+  asm volatile(
+      "{\n .reg .b128 h;\n .reg .pred p;\n"
+      " ld.shared.b128 h, [%5];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      " selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n mov.u32 %3, 0;\n mov.u32 %4, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, %4}, h;\n}\n"
+      : "=r"(yes), "=r"(x), "=r"(y), "=r"(z), "=r"(w)
+      : "r"(answer)
+      : "memory");
+  return yes ? (int)x : -1;
 }
 
 // 32 consecutive f32 columns of this warp's 32 lanes
@@ -88,6 +149,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r) {
         "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(taddr));
 }
+// 8 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
 // V [keys][64 values] slabs as the second operand with the values along N: 8-key groups lie
 // 1024 bytes apart, 64-value slabs one slab apart.
 __device__ __forceinline__ uint64_t v_desc(uint32_t addr, uint32_t slab) {
@@ -107,21 +176,10 @@ struct TcArgs {
   DecodeArgs d;
   KvView c;
   int tokens;     // of a unit: 128 / group
-  int tiles;      // prompt: upper bound of the number of tiles
+  int tiles;      // prompt: upper bound of the number of items per key/value head
   int alternate;  // shared: one unit's rows hold them all; the units take tiles in turn
+  int k_box, v_box;  // shared: rows of a TMA box
   int32_t *timeout;
-};
-
-// What the roles of a block agree on.
-struct Work {
-  int kv_head, first, tiles;  // first key, number of key tiles
-  int max_low, min_high, keys;
-  int64_t k0;
-  int table_row;
-  __device__ bool mixed(int t) const {  // some row does not see some key of tile t
-    const int key = first + t * kTileKeys;
-    return key < max_low || key + kTileKeys > min_high;
-  }
 };
 
 // One lane of a converged warp. What it decides is uniform, so the operands of the
@@ -134,31 +192,150 @@ __device__ __forceinline__ bool elect_one() {
   return yes != 0;
 }
 
-// Bounded wait that also ends when another role has given up.
+// The products with the issuing lane as a predicate: no branch around them, so the addresses
+// are computed for the whole warp, in uniform registers, where the instruction wants them.
+__device__ __forceinline__ void mma_ss_if(uint32_t lead, uint32_t d, uint64_t adesc, uint64_t bdesc,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_if(uint32_t lead, uint32_t d, uint32_t a, uint64_t bdesc,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t lead, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+      "r"(lead)
+      : "memory");
+}
+// A value that is the same in all lanes, in a uniform register.
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
+
+// Bounded wait that also ends when another role has given up; one answer for the warp. A
+// warp that waits sleeps in try_wait: one that polls takes issue slots from the softmax warps
+// beside it (measured: a third of the prompt rate).
+__device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ bool wait(TcSmem &sh, uint64_t &bar, uint32_t parity) {
   const uint32_t b = smem_u32(&bar);
-  if (mbar_try(b, parity)) return true;
+  if (__all_sync(0xffffffffu, mbar_look(b, parity))) return true;
   const long long start = clock64();
-  while (!sh.abort) {
-    if (mbar_try(b, parity)) return true;
-    if (clock64() - start > kWaitCycles) break;
+  bool done = false;
+  while (!done && !sh.abort) {
+    done = __all_sync(0xffffffffu, mbar_look(b, parity));
+    if (!done && clock64() - start > kWaitCycles) break;
   }
-  sh.abort = 1;
-  return false;
-}
-// The same for a whole warp: one answer for all lanes.
-__device__ __forceinline__ bool wait_warp(TcSmem &sh, uint64_t &bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait(sh, bar, parity));
+  done = __all_sync(0xffffffffu, done);
+  if (!done) sh.abort = 1;
+  return done;
 }
 
-// Two units: the 168 registers a thread that 384 threads start with, split anew (256 x 208 +
-// 128 x 88 = 384 x 168), so that a row's 128 scores and the weights made from them stay in
-// registers. Every warp of a group of four calls the same one.
-__device__ __forceinline__ void take_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
+
+// The keys [low, high) that token i of an item's sequence sees.
+__device__ __forceinline__ int low_of(const PromptArgs &p, int lq, int lk, int i) {
+  return p.window ? max(0, i + lk - lq - p.window + 1) : 0;
+}
+__device__ __forceinline__ int high_of(const PromptArgs &p, int lq, int lk, int i) {
+  return p.causal ? max(0, min(lk, i + lk - lq + 1)) : lk;
+}
+
+// Whether some row does not see some key of tile t.
+template <int KEYS>
+__device__ __forceinline__ bool mixed(const Item &w, int t) {
+  const int key = w.first + t * KEYS;
+  return key < w.max_low || key + KEYS > w.min_high;
+}
+
+template <int REGS>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
 __device__ __forceinline__ void give_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+// A place in a ring: slot and how often the ring has been gone round.
+template <int SLOTS>
+struct Place {
+  int slot = 0;
+  uint32_t round = 0;
+  __device__ void next() {
+    if (++slot == SLOTS) slot = 0, round++;
+  }
+  __device__ uint32_t parity() const { return round & 1; }
+  // the same slot, one round earlier
+  __device__ void back(int n) {
+    for (; n > 0; n--)
+      if (--slot < 0) slot = SLOTS - 1, round--;
+  }
+};
+
+// Load the K or V tiles of an item into the ring, chunk by chunk.
+template <int MODE, int DP, bool V>
+__device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles, const TcArgs &a,
+                                           const CUtensorMap *map, uint32_t ring, uint32_t lead,
+                                           Place<TcCfg<DP>::kSlots> &place) {
+  using Cfg = TcCfg<DP>;
+  constexpr int kRows = V ? Cfg::kVKeys : Cfg::kKeys;     // keys of a chunk
+  constexpr int kSlabs = V ? DP / 64 : Cfg::kKSlabs;      // its slabs of 64 values
+  const int lane = threadIdx.x & 31;
+  const int kv_head = w.kv_head, k0 = w.k0, table_row = w.table_row;
+  int key = w.first;
+  for (int t = 0; t < tiles; t++, key += Cfg::kKeys) {
+#pragma unroll 1
+    for (int c = 0; c < Cfg::kChunks; c++, place.next()) {
+      const int from = V ? key + c * kRows : key, x0 = V ? 0 : c * kSlabs * 64;
+      const uint32_t bar = smem_u32(V ? &sh.v_full[place.slot] : &sh.k_full[place.slot]);
+      const uint32_t dst = ring + place.slot * Cfg::kChunkBytes;
+      int page = 0, boxes = 1, box = kRows;
+      if (MODE == kTcShared) {  // pages of the chunk: one lane each
+        box = V ? a.v_box : a.k_box;
+        boxes = max(0, min(kRows, a.d.shared - from)) / box;
+        if (lane < boxes) {
+          const int p = a.c.table[(int64_t)table_row * a.c.max_pages + (from + lane * box) / a.c.page_tokens];
+          page = (unsigned)p < (unsigned)a.c.pages ? p : a.c.pages;  // behind the map: zeros
+        }
+      }
+      if (place.round > 0 && !wait(sh, V ? sh.v_empty[place.slot] : sh.k_empty[place.slot], place.parity() ^ 1))
+        return false;
+      if (lead) mbar_expect_tx(bar, kSlabs * boxes * box * 128);
+      if (MODE == kTcPrompt) {
+        if (lead)
+          for (int s = 0; s < kSlabs; s++) tma_load_3d(dst + s * kRows * 128, map, x0 + s * 64, kv_head, k0 + from, bar);
+      } else {
+        __syncwarp();
+        if (lane < boxes)
+          for (int s = 0; s < kSlabs; s++)
+            tma_load_4d(dst + s * kRows * 128 + lane * box * 128, map, x0 + s * 64,
+                        (from + lane * box) % a.c.page_tokens, kv_head, page, bar);
+      }
+      __syncwarp();
+    }
+  }
+  return true;
 }
 
 template <int MODE, int DP, bool BF16>
@@ -166,432 +343,414 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
 tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
             const __grid_constant__ CUtensorMap v_map, const __grid_constant__ TcArgs a) {
   using Cfg = TcCfg<DP>;
-  constexpr int kUnits = Cfg::kUnits;
+  constexpr int kUnits = Cfg::kUnits, kKeys = Cfg::kKeys, kChunks = Cfg::kChunks, kSlots = Cfg::kSlots;
+  using Ring = Place<kSlots>;
   extern __shared__ uint8_t raw[];
   __shared__ TcSmem sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-  const uint32_t ring = base + kUnits * Cfg::kTile;
+  const uint32_t k_ring = base + kUnits * Cfg::kQBytes, v_ring = k_ring + kSlots * Cfg::kChunkBytes;
   const int group = MODE == kTcPrompt ? a.p.group : a.d.group;
   const int per_unit = a.tokens * group;  // rows in use of a unit's 128
-
-  // ---- which rows, which keys
-  Work w{};
-  int token0 = 0;  // first token (batch entry) of the block
-  int lq = 0, lk = 0, split = 0;
   const int alternate = MODE == kTcShared && a.alternate;
-  if (MODE == kTcPrompt) {
-    // key/value heads side by side, the last (longest, if causal) tiles of the batch first
-    w.kv_head = blockIdx.x % a.p.kv_heads;
-    const int tile = a.tiles - 1 - blockIdx.x / a.p.kv_heads;
-    if (warp == 0) {
-      const TileOf t = find_tile(a.p.q_offsets, a.p.sequences, a.p.q_tokens, 1, kUnits * a.tokens, tile);
-      if (lane == 0) sh.tile = t;
-    }
-  }
+  const int split = MODE == kTcShared ? blockIdx.y : 0;
+  auto tile_of = [&](int u, int i) -> int { return alternate ? 2 * i + u : i; };
+  // whether tile t of an item is one of the n of unit u
+  auto is_mine = [&](int u, int t, int n) -> bool { return alternate ? (t & 1) == u : t < n; };
+
   if (tid == 0) {
     sh.abort = 0;
-    sh.wild = 0;
-    sh.max_low = 0, sh.min_high = INT32_MAX, sh.keys = 0;
+    for (int i = 0; i < kItems; i++) {
+      mbar_init(smem_u32(&sh.item_full[i]), 1);
+      mbar_init(smem_u32(&sh.item_empty[i]), Cfg::kConsumers);
+    }
     for (int i = 0; i < 2; i++) {
-      mbar_init(smem_u32(&sh.q_full[i]), 1);
       mbar_init(smem_u32(&sh.s_full[i]), 1);
+      mbar_init(smem_u32(&sh.s_free[i]), 4);
       mbar_init(smem_u32(&sh.p_full[i]), 4);
       mbar_init(smem_u32(&sh.pv_done[i]), 1);
     }
-    for (int i = 0; i < Cfg::kSlots; i++) {
-      mbar_init(smem_u32(&sh.full[i]), 1);
-      mbar_init(smem_u32(&sh.empty[i]), 1);
-      mbar_init(smem_u32(&sh.dirty[i]), 1);
-      mbar_init(smem_u32(&sh.clean[i]), 2);
+    for (int i = 0; i < kSlots; i++) {
+      mbar_init(smem_u32(&sh.k_full[i]), 1);
+      mbar_init(smem_u32(&sh.k_empty[i]), kUnits);
+      mbar_init(smem_u32(&sh.v_full[i]), 1);
+      mbar_init(smem_u32(&sh.v_clean[i]), 1);
+      mbar_init(smem_u32(&sh.v_empty[i]), kUnits);
     }
-    mbar_init(smem_u32(&sh.drain), 1);
+    mbar_init(smem_u32(&sh.q_full), 1);
+    mbar_init(smem_u32(&sh.q_empty), kUnits);
+    mbar_init(smem_u32(&sh.next_block), 1);
+    mbar_init(smem_u32(&sh.want), 1);
+    for (int i = 0; i < 4; i++) mbar_init(smem_u32(&sh.drain[i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-
-  // this thread's row, if it is a softmax thread
-  const int unit = warp >> 2, row = tid & 127;
-  const bool softmax = warp < Cfg::kSoftWarps;
-  int low = 0, high = INT32_MAX;
-  bool valid = false;
-  int64_t out_at = 0, index = 0;
-  if (MODE == kTcPrompt) {
-    const TileOf t = sh.tile;
-    if (t.seq < 0) return;
-    w.k0 = min((int64_t)max(a.p.k_offsets[t.seq], 0), a.p.k_tokens);
-    const int64_t k1 = min((int64_t)max(a.p.k_offsets[t.seq + 1], 0), a.p.k_tokens);
-    lq = t.q1 - t.q0;
-    lk = (int)max((int64_t)0, k1 - w.k0);
-    token0 = t.tile * kUnits * a.tokens;
-    const int last = min(lq, token0 + kUnits * a.tokens) - 1;
-    // limits of the first and last token bound the others'
-    auto low_of = [&](int i) { return a.p.window ? max(0, i + lk - lq - a.p.window + 1) : 0; };
-    auto high_of = [&](int i) { return a.p.causal ? max(0, min(lk, i + lk - lq + 1)) : lk; };
-    w.max_low = low_of(last);
-    w.min_high = high_of(token0);
-    w.keys = lk;
-    w.first = low_of(token0) / kTileKeys * kTileKeys;
-    const int end = high_of(last);
-    w.tiles = end > w.first ? (end - w.first + kTileKeys - 1) / kTileKeys : 0;
-    if (softmax) {
-      const int token = token0 + unit * a.tokens + row / group;
-      const int head = w.kv_head * group + row % group;
-      valid = row < per_unit && token < lq;
-      if (valid) {
-        low = low_of(token), high = high_of(token);
-        out_at = (t.q0 + (int64_t)token) * a.p.out_stride[0] + head * a.p.out_stride[1];
-        index = (t.q0 + (int64_t)token) * a.p.heads + head;
-      }
-    }
-    token0 += t.q0;
-  } else {
-    const int blocks = (a.d.batch + (alternate ? 1 : kUnits) * a.tokens - 1) / ((alternate ? 1 : kUnits) * a.tokens);
-    const int rb = blockIdx.x % blocks;
-    w.kv_head = blockIdx.x / blocks;
-    split = blockIdx.y;
-    token0 = rb * (alternate ? 1 : kUnits) * a.tokens;
-    int unused;
-    w.table_row = sequence_of(a.c, a.d, 0, &unused);
-    if (softmax) {
-      const int b = token0 + (alternate ? 0 : unit * a.tokens) + row / group;
-      const int head = w.kv_head * group + row % group;
-      valid = row < per_unit && b < a.d.batch;
-      if (valid) {
-        int length;
-        sequence_of(a.c, a.d, b, &length);
-        low = a.d.window ? max(0, length - a.d.window) : 0;
-        high = min(length, a.d.shared);
-        out_at = b * a.d.out_stride[0] + head * a.d.out_stride[1];
-        index = (int64_t)b * a.d.heads + head;
-      }
-      const int top = __reduce_max_sync(0xffffffffu, valid ? low : 0);
-      const int bottom = __reduce_min_sync(0xffffffffu, high);
-      const int most = __reduce_max_sync(0xffffffffu, valid ? high : 0);
-      if (lane == 0) {
-        atomicMax(&sh.max_low, top);
-        atomicMin(&sh.min_high, bottom);
-        atomicMax(&sh.keys, most);
-      }
-    }
-    __syncthreads();
-    w.max_low = sh.max_low, w.min_high = sh.min_high, w.keys = sh.keys;
-    const int all = (a.d.shared + kTileKeys - 1) / kTileKeys;
-    const int per = (all + a.d.splits - 1) / a.d.splits;
-    const int t0 = min(all, split * per), t1 = min((w.keys + kTileKeys - 1) / kTileKeys, t0 + per);
-    w.first = t0 * kTileKeys;
-    w.tiles = max(0, t1 - t0);
-  }
-
-  // tiles of unit u; its i-th is tile i, or 2 i + u when the units alternate
-  auto count = [&](int u) -> int {
-    if (alternate) return (w.tiles + 1 - u) / 2;
-    if (MODE == kTcPrompt && kUnits == 2 && u == 0 && a.p.causal) {  // may need fewer
-      const TileOf t = sh.tile;
-      const int end = max(0, min(lk, min(lq, token0 - t.q0 + a.tokens) + lk - lq));
-      return max(0, min(w.tiles, (end - w.first + kTileKeys - 1) / kTileKeys));
-    }
-    if (MODE == kTcPrompt && u == 1 && token0 - sh.tile.q0 + a.tokens >= lq) return 0;
-    return w.tiles;
-  };
-  auto tile_of = [&](int u, int i) -> int { return alternate ? 2 * i + u : i; };
-  const int n0 = count(0), n1 = kUnits == 2 ? count(1) : 0;
-
-  if (warp == Cfg::kSoftWarps) tmem_alloc(smem_u32(&sh.tmem), 512);
+  if (warp == Cfg::kItemWarp) tmem_alloc(smem_u32(&sh.tmem), 512);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
+  bool ok = true;  // of the role: no wait has run out
 
-  if (warp == Cfg::kSoftWarps) {
-    // ---- TMA
-    if (kUnits == 2) give_registers();
-    if (w.tiles > 0) {
-      if (lane == 0) {
-        for (int u = 0; u < kUnits; u++) {
-          if ((u ? n1 : n0) == 0) continue;
-          const uint32_t bar = smem_u32(&sh.q_full[u]);
-          mbar_expect_tx(bar, DP / 64 * per_unit * 128);
-          for (int s = 0; s < DP / 64; s++)
-            tma_load_4d(base + u * Cfg::kTile + s * Cfg::kSlab, &q_map, s * 64, 0, w.kv_head,
-                        token0 + (alternate ? 0 : u * a.tokens), bar);
-        }
-      }
-      int issued = 0;
-      uint32_t parity = 0, dirty = 0;  // of the next load into a slot, by its barrier
-      const int box = MODE == kTcShared ? min(a.c.page_tokens, kTileKeys) : kTileKeys;
-      for (int i = 0; i < 2 * w.tiles; i++) {  // K and V of tile i / 2
-        const int slot = i % Cfg::kSlots;
-        const int key = w.first + (i >> 1) * kTileKeys;
-        // pages of a tile: one lane each
-        int page = 0, boxes = 1;
-        if (MODE == kTcShared) {
-          boxes = min(kTileKeys, a.d.shared - key) / box;
-          if (lane < boxes) {
-            const int p = a.c.table[(int64_t)w.table_row * a.c.max_pages + (key + lane * box) / a.c.page_tokens];
-            page = (unsigned)p < (unsigned)a.c.pages ? p : a.c.pages;  // behind the map: zeros
+  if (warp >= Cfg::kSoftWarps) {
+    give_registers<Cfg::kOtherRegs>();
+    if (warp == Cfg::kItemWarp) {
+      // ---- choice of items
+      int block = blockIdx.x, items = 0, asks = 0;
+      while (ok) {
+      Item w{};
+      if (MODE == kTcPrompt) {
+        if (block < 0) {
+          w.stop = 1;
+        } else {
+          // key/value heads side by side, the last (longest, if causal) tiles of the batch first
+          w.kv_head = block % a.p.kv_heads;
+          const TileOf t = find_tile(a.p.q_offsets, a.p.sequences, a.p.q_tokens, 1, kUnits * a.tokens,
+                                     a.tiles - 1 - block / a.p.kv_heads);
+          if (t.seq < 0) {
+            w.stop = -1;  // behind the last tile
+          } else {
+            w.q0 = t.q0;
+            w.k0 = (int)min((int64_t)max(a.p.k_offsets[t.seq], 0), a.p.k_tokens);
+            const int k1 = (int)min((int64_t)max(a.p.k_offsets[t.seq + 1], 0), a.p.k_tokens);
+            const int lq = w.lq = t.q1 - t.q0, lk = w.lk = max(0, k1 - w.k0);
+            w.token0 = t.tile * kUnits * a.tokens;
+            const int last = min(lq, w.token0 + kUnits * a.tokens) - 1;
+            // limits of the first and last token bound the others'
+            w.max_low = low_of(a.p, lq, lk, last);
+            w.min_high = high_of(a.p, lq, lk, w.token0);
+            w.first = low_of(a.p, lq, lk, w.token0) / 16 * 16;
+            auto tiles_to = [&](int end) { return max(0, (end - w.first + kKeys - 1) / kKeys); };
+            w.tiles = tiles_to(high_of(a.p, lq, lk, last));
+            w.n[0] = tiles_to(high_of(a.p, lq, lk, min(last, w.token0 + a.tokens - 1)));
+            w.n[1] = kUnits == 2 && w.token0 + a.tokens < lq ? w.tiles : 0;
           }
         }
-        if (i >= Cfg::kSlots && !wait_warp(sh, sh.empty[slot], (i / Cfg::kSlots - 1) & 1)) break;
-        const bool mixed = (i & 1) && w.mixed(i >> 1);
-        const uint32_t bar = smem_u32(mixed ? &sh.dirty[slot] : &sh.full[slot]);
-        (mixed ? dirty : parity) ^= 1u << slot;
-        const CUtensorMap *map = i & 1 ? &v_map : &k_map;
-        const uint32_t dst = ring + slot * Cfg::kTile;
-        if (lane == 0) mbar_expect_tx(bar, DP / 64 * boxes * box * 128);
-        __syncwarp();
-        if (lane < boxes) {
-          for (int s = 0; s < DP / 64; s++) {
-            if (MODE == kTcPrompt)
-              tma_load_3d(dst + s * Cfg::kSlab, map, s * 64, w.kv_head, (int)w.k0 + key, bar);
-            else
-              tma_load_4d(dst + s * Cfg::kSlab + lane * box * 128, map, s * 64,
-                          (key + lane * box) % a.c.page_tokens, w.kv_head, page, bar);
-          }
+      } else if (items > 0) {
+        w.stop = 1;
+      } else {
+        const int units = alternate ? 1 : kUnits;
+        const int blocks = (a.d.batch + units * a.tokens - 1) / (units * a.tokens);
+        w.kv_head = block / blocks;
+        w.token0 = block % blocks * units * a.tokens;
+        int length;
+        w.table_row = sequence_of(a.c, a.d, 0, &length);
+        int top = 0, bottom = INT32_MAX, most = 0;
+        for (int b = w.token0 + lane; b < min(a.d.batch, w.token0 + units * a.tokens); b += 32) {
+          sequence_of(a.c, a.d, b, &length);
+          top = max(top, a.d.window ? max(0, length - a.d.window) : 0);
+          bottom = min(bottom, min(length, a.d.shared));
+          most = max(most, min(length, a.d.shared));
         }
-        issued = i + 1;
+        w.max_low = __reduce_max_sync(0xffffffffu, top);
+        w.min_high = __reduce_min_sync(0xffffffffu, bottom);
+        most = __reduce_max_sync(0xffffffffu, most);
+        const int all = (a.d.shared + kKeys - 1) / kKeys;
+        const int per = (all + a.d.splits - 1) / a.d.splits;
+        const int t0 = min(all, split * per), t1 = min((most + kKeys - 1) / kKeys, t0 + per);
+        w.first = t0 * kKeys;
+        w.tiles = max(0, t1 - t0);
+        w.n[0] = alternate ? (w.tiles + 1) / 2 : w.tiles;
+        w.n[1] = kUnits == 1 ? 0 : alternate ? w.tiles / 2 : w.tiles;
       }
-      if (sh.abort) {  // the copies in flight land before the block ends
-        for (int i = max(0, issued - Cfg::kSlots); i < issued; i++) {
-          const int slot = i % Cfg::kSlots;
-          const bool mixed = (i & 1) && w.mixed(i >> 1);
-          mbar_wait(smem_u32(mixed ? &sh.dirty[slot] : &sh.full[slot]),
-                    (((mixed ? dirty : parity) >> slot) & 1) ^ 1);
+      if (w.stop >= 0) {
+        const int at = items % kItems;
+        if (items >= kItems && !(ok = wait(sh, sh.item_empty[at], (items / kItems - 1) & 1))) break;
+        if (lane == 0) {
+          sh.item[at] = w;
+          mbar_arrive(smem_u32(&sh.item_full[at]));
         }
-        for (int u = 0; u < kUnits; u++)
-          if ((u ? n1 : n0) > 0) mbar_wait(smem_u32(&sh.q_full[u]), 0);
+        __syncwarp();
+        items++;
+        if (w.stop) break;
       }
-    }
-  } else if (warp == Cfg::kSoftWarps + 1) {
-    // ---- MMA issue
-    if (kUnits == 2) give_registers();
-    // the whole warp follows the schedule, one lane issues
-    if (w.tiles > 0) {
-      constexpr uint32_t kQk = idesc(BF16, kTileKeys, false), kPv = idesc(BF16, DP, true);
-      uint32_t full = 0, clean = 0;  // parity of the next V tile in a slot, by its barrier
-      bool ok = true;
-      const uint64_t q_desc = sw128_desc(base);
-      auto products_s = [&](int u, int t, int buffer) {
-        const uint64_t qd = q_desc + ((u * Cfg::kTile) >> 4);
-        const uint64_t kd = sw128_desc(ring + ((2 * t) % Cfg::kSlots) * Cfg::kTile);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < DP / 16; k++) {
-            const uint64_t at = (k / 4) * (Cfg::kSlab >> 4) + (k % 4) * 2;
-            mma_ss(tmem + buffer * 128, qd + at, kd + at, kQk, k > 0);
+      if (MODE == kTcPrompt) {
+        // No sooner than it is needed: blocks that have not started are for whoever is done
+        // first. (The loads are a few tiles ahead of the products.)
+        if (w.stop == 0 && !(ok = wait(sh, sh.want, (items - 1) & 1))) break;
+        if (lane == 0) {
+          fence_async_smem();  // the last answer has been read
+          mbar_expect_tx(smem_u32(&sh.next_block), 16);
+          take_block(smem_u32(&sh.answer), smem_u32(&sh.next_block));
+        }
+        asks++;
+        if (!(ok = wait(sh, sh.next_block, (asks - 1) & 1))) break;
+        block = taken_block(smem_u32(&sh.answer));
+        __syncwarp();
+      }
+      }
+      if (!ok && asks > 0) mbar_wait(smem_u32(&sh.next_block), (asks - 1) & 1);
+    } else if (warp <= Cfg::kOWarp + kUnits - 1) {
+      // ---- loads, products and clean-up go through the tiles of every item
+      const uint32_t lead = elect_one();
+      const uint32_t columns = uniform(tmem);
+      const int unit = warp >= Cfg::kOWarp ? warp - Cfg::kOWarp : warp - Cfg::kSWarp;  // of products
+      Ring place;
+      int q_uses = 0, number = 0;  // items with tiles; products of this warp
+      for (int items = 0; ok; items++) {
+        const int at = items % kItems;
+        if (!(ok = wait(sh, sh.item_full[at], (items / kItems) & 1))) break;
+        const Item &w = sh.item[at];
+        if (uniform(w.stop)) break;
+        const int tiles = uniform(w.tiles);
+        if (warp == Cfg::kKWarp) {
+          // ---- queries and keys
+          if (tiles > 0) {
+            if (q_uses > 0 && !(ok = wait(sh, sh.q_empty, (q_uses - 1) & 1))) break;
+            if (lead) {
+              const uint32_t bar = smem_u32(&sh.q_full);
+              const int units = alternate ? 1 : kUnits;
+              mbar_expect_tx(bar, units * DP / 64 * per_unit * 128);
+              for (int u = 0; u < units; u++)
+                for (int s = 0; s < DP / 64; s++)
+                  tma_load_4d(base + u * Cfg::kQBytes + s * kUnitRows * 128, &q_map, s * 64, 0, w.kv_head,
+                              w.q0 + w.token0 + u * a.tokens, bar);
+            }
+            __syncwarp();
+            q_uses++;
           }
-          mma_commit(smem_u32(&sh.s_full[buffer]));
-        }
-        __syncwarp();
-      };
-      auto products_o = [&](int u, int t, int buffer, bool add) {
-        const uint64_t vd = v_desc(ring + ((2 * t + 1) % Cfg::kSlots) * Cfg::kTile, Cfg::kSlab);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kTileKeys / 16; k++)
-            mma_ts(tmem + Cfg::kOutCol + u * DP, tmem + buffer * 128 + k * 8, vd + k * (2048 >> 4), kPv,
-                   add || k > 0);
-          mma_commit(smem_u32(&sh.pv_done[u]));
-        }
-        __syncwarp();
-      };
-      auto k_there = [&](int t) {
-        return wait_warp(sh, sh.full[(2 * t) % Cfg::kSlots], (2 * t / Cfg::kSlots) & 1);
-      };
-      // first of the units that use V tile t waits for it, in its clean form where mixed
-      auto v_there = [&](int t, bool first_use) {
-        if (!first_use) return true;
-        const int slot = (2 * t + 1) % Cfg::kSlots;
-        const bool mixed = w.mixed(t);
-        uint32_t &parity = mixed ? clean : full;
-        const uint32_t now = (parity >> slot) & 1;
-        parity ^= 1u << slot;
-        return wait_warp(sh, mixed ? sh.clean[slot] : sh.full[slot], now);
-      };
-      auto release = [&](int i) {
-        if (elect_one()) mma_commit(smem_u32(&sh.empty[i % Cfg::kSlots]));
-        __syncwarp();
-      };
-      if (kUnits == 2) {
-        const int n[2] = {n0, n1};
-        const int most = max(n0, n1);
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          if (n[u] == 0 || !ok) continue;
-          const int t = tile_of(u, 0);
-          ok = wait_warp(sh, sh.q_full[u], 0) && k_there(t);
-          if (!ok) break;
-          fence_after();
-          products_s(u, t, u);
-          if (alternate || u == 1 || n1 == 0) release(2 * t);
-        }
-        for (int i = 0; i < most && ok; i++) {
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            if (i >= n[u] || !ok) continue;
-            const int t = tile_of(u, i);
-            const bool first_use = alternate || u == 0 || i >= n0;
-            ok = wait_warp(sh, sh.p_full[u], i & 1) && v_there(t, first_use);
-            if (!ok) break;
-            fence_after();
-            products_o(u, t, u, i > 0);
-            if (alternate || u == 1 || i >= n1) release(2 * t + 1);
-            if (i + 1 < n[u]) {
-              const int s = tile_of(u, i + 1);
-              ok = k_there(s);
-              if (!ok) break;
-              fence_after();
-              products_s(u, s, u);
-              if (alternate || u == 1 || i + 1 >= n1) release(2 * s);
+          ok = load_tiles<MODE, DP, false>(sh, w, tiles, a, &k_map, k_ring, lead, place);
+          if (ok && lead) mbar_arrive(smem_u32(&sh.want));
+        } else if (warp == Cfg::kVWarp) {
+          // ---- values
+          ok = load_tiles<MODE, DP, true>(sh, w, tiles, a, &v_map, v_ring, lead, place);
+        } else if (warp == Cfg::kScrubWarp) {
+          // ---- values that are not finite leave mixed tiles; the others are passed on
+          // rows behind the last key are no one's: other sequences, or what the ring held before
+          const int keys = MODE == kTcPrompt ? w.lk : a.d.shared;
+          bool found = false;
+          for (int t = 0; t < tiles && ok; t++) {
+            const bool mix = mixed<kKeys>(w, t);
+            for (int c = 0; c < kChunks; c++, place.next()) {
+              if (!(ok = wait(sh, sh.v_full[place.slot], place.parity()))) break;
+              if (mix) {
+                const uint32_t v = v_ring + place.slot * Cfg::kChunkBytes;
+                constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
+#pragma unroll 4
+                for (int j = lane; j < Cfg::kChunkBytes / 16; j += 32) {
+                  const uint4 x = lds16(v + j * 16);
+                  const uint32_t bad[4] = {__vcmpeq2(x.x & kExp, kExp), __vcmpeq2(x.y & kExp, kExp),
+                                           __vcmpeq2(x.z & kExp, kExp), __vcmpeq2(x.w & kExp, kExp)};
+                  if (bad[0] | bad[1] | bad[2] | bad[3]) {
+                    found |= w.first + t * kKeys + c * Cfg::kVKeys + j / 8 % Cfg::kVKeys < keys;
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v + j * 16),
+                                 "r"(x.x & ~bad[0]), "r"(x.y & ~bad[1]), "r"(x.z & ~bad[2]), "r"(x.w & ~bad[3])
+                                 : "memory");
+                  }
+                }
+                if (found) sh.item[at].wild = 1;
+                fence_async_smem();
+                __syncwarp();
+              }
+              if (lead) mbar_arrive(smem_u32(&sh.v_clean[place.slot]));
             }
           }
-        }
-      } else {
-        ok = wait_warp(sh, sh.q_full[0], 0) && k_there(0);
-        if (ok) {
-          fence_after();
-          products_s(0, 0, 0);
-          release(0);
-        }
-        for (int t = 0; t < n0 && ok; t++) {
-          if (t + 1 < n0) {
-            ok = k_there(t + 1);
-            if (!ok) break;
-            fence_after();
-            products_s(0, t + 1, (t + 1) & 1);
-            release(2 * t + 2);
+        } else if (warp < Cfg::kOWarp) {
+          // ---- products S of one unit. Tiles that are not its own are given back at once.
+          constexpr uint32_t kQk = idesc(BF16, kKeys, false);
+          constexpr int kQSlab = kUnitRows * 128, kKSlab = kKeys * 128;
+          const uint64_t qd = sw128_desc(base + (alternate ? 0 : unit) * Cfg::kQBytes);
+          const int n = uniform(w.n[unit]);
+          if (tiles > 0 && !(ok = wait(sh, sh.q_full, q_uses++ & 1))) break;
+          if (tiles > 0 && n == 0 && lead) mbar_arrive(smem_u32(&sh.q_empty));
+          for (int t = 0, left = n; t < tiles && ok; t++) {
+            const bool mine = is_mine(unit, t, n);
+            const int buffer = Cfg::kBuffers == 2 ? number & 1 : unit;
+            if (Cfg::kPCol && mine && number > 0 && !(ok = wait(sh, sh.s_free[unit], (number - 1) & 1)))
+              break;  // S has been read
+#pragma unroll
+            for (int c = 0; c < kChunks; c++, place.next()) {
+              if (!(ok = wait(sh, sh.k_full[place.slot], place.parity()))) break;
+              const uint32_t empty = smem_u32(&sh.k_empty[place.slot]);
+              if (!mine) {
+                if (lead) mbar_arrive(empty);
+                continue;
+              }
+              fence_after();
+              const uint64_t kd = sw128_desc(k_ring + place.slot * Cfg::kChunkBytes);
+#pragma unroll
+              for (int k = 0; k < 4 * Cfg::kKSlabs; k++)
+                mma_ss_if(lead, columns + buffer * Cfg::kUnitCols,
+                          qd + ((c * Cfg::kKSlabs + k / 4) * kQSlab >> 4) + (k % 4) * 2,
+                          kd + ((k / 4) * kKSlab >> 4) + (k % 4) * 2, kQk, c > 0 || k > 0);
+              if (c == kChunks - 1) commit_if(lead, smem_u32(&sh.s_full[buffer]));
+              commit_if(lead, empty);
+            }
+            if (!mine || !ok) continue;
+            if (--left == 0) commit_if(lead, smem_u32(&sh.q_empty));  // the queries have been read
+            // Where weights take the place of S, the next S goes to where those of the tile before
+            // are: their product has to be done. (Waited for here, where this tile's cannot be.)
+            if (!Cfg::kPCol && number > 0) ok = wait(sh, sh.pv_done[unit], (number - 1) & 1);
+            number++;
           }
-          ok = wait_warp(sh, sh.p_full[t & 1], (t >> 1) & 1) && v_there(t, true);
-          if (!ok) break;
-          fence_after();
-          products_o(0, t, t & 1, t > 0);
-          release(2 * t + 1);
+        } else {
+          // ---- products O of one unit
+          constexpr uint32_t kPv = idesc(BF16, DP, true);
+          constexpr int kVSlab = Cfg::kVKeys * 128;
+          const int n = uniform(w.n[unit]);
+          const uint32_t d = columns + Cfg::kOCol + unit * DP;
+          for (int t = 0, own = 0; t < tiles && ok; t++) {
+            const bool mine = is_mine(unit, t, n);
+            const int buffer = Cfg::kBuffers == 2 ? number & 1 : unit;
+            const uint32_t p = columns + buffer * Cfg::kUnitCols + Cfg::kPCol;
+            if (mine && !(ok = wait(sh, sh.p_full[buffer], (Cfg::kBuffers == 2 ? number >> 1 : number) & 1)))
+              break;
+#pragma unroll
+            for (int c = 0; c < kChunks; c++, place.next()) {
+              if (!(ok = wait(sh, sh.v_clean[place.slot], place.parity()))) break;
+              const uint32_t empty = smem_u32(&sh.v_empty[place.slot]);
+              if (!mine) {
+                if (lead) mbar_arrive(empty);
+                continue;
+              }
+              fence_after();
+              const uint64_t vd = v_desc(v_ring + place.slot * Cfg::kChunkBytes, kVSlab);
+#pragma unroll
+              for (int k = 0; k < Cfg::kVKeys / 16; k++)
+                mma_ts_if(lead, d, p + (c * Cfg::kVKeys / 16 + k) * 8, vd + k * (2048 >> 4), kPv,
+                          own > 0 || c > 0 || k > 0);
+              if (c == kChunks - 1) commit_if(lead, smem_u32(&sh.pv_done[unit]));
+              commit_if(lead, empty);
+            }
+            if (mine) number++, own++;
+          }
+        }
+        __syncwarp();
+        if (ok && lead) mbar_arrive(smem_u32(&sh.item_empty[at]));
+      }
+      if (!ok) {  // copies and products in flight end before the block does
+        if (warp >= Cfg::kSWarp) {
+          uint64_t &bar = sh.drain[warp - Cfg::kSWarp];
+          commit_if(lead, smem_u32(&bar));
+          mbar_wait(smem_u32(&bar), 0);
+        } else if (warp != Cfg::kScrubWarp) {
+          const int issued = (int)min((uint32_t)kSlots, place.round * kSlots + place.slot);
+          place.back(issued);
+          for (int i = 0; i < issued; i++, place.next())
+            mbar_wait(smem_u32(warp == Cfg::kKWarp ? &sh.k_full[place.slot] : &sh.v_full[place.slot]), place.parity());
+          if (warp == Cfg::kKWarp && q_uses > 0) mbar_wait(smem_u32(&sh.q_full), (q_uses - 1) & 1);
         }
       }
-      if (!ok) {  // products in flight end before tensor memory is given back
-        if (elect_one()) mma_commit(smem_u32(&sh.drain));
-        mbar_wait(smem_u32(&sh.drain), 0);
-      }
-    }
-    __syncwarp();
-  } else if (warp >= Cfg::kSoftWarps + 2) {
-    // ---- values that are not finite leave mixed tiles
-    if (kUnits == 2) give_registers();
-    const int who = tid - (Cfg::kSoftWarps + 2) * 32;
-    uint32_t dirty = 0;  // parity of the next mixed tile in a slot
-    for (int t = 0; t < w.tiles; t++) {
-      if (!w.mixed(t)) continue;
-      const int slot = (2 * t + 1) % Cfg::kSlots;
-      const uint32_t parity = (dirty >> slot) & 1;
-      dirty ^= 1u << slot;
-      if (!wait_warp(sh, sh.dirty[slot], parity)) break;
-      const uint32_t v = ring + slot * Cfg::kTile;
-      constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
-      bool found = false;
-#pragma unroll 4
-      for (int i = who; i < Cfg::kTile / 16; i += 64) {
-        const uint4 x = lds16(v + i * 16);
-        const uint32_t hit = __vcmpeq2(x.x & kExp, kExp) | __vcmpeq2(x.y & kExp, kExp) |
-                             __vcmpeq2(x.z & kExp, kExp) | __vcmpeq2(x.w & kExp, kExp);
-        if (hit) {
-          found = true;
-          const uint32_t e[4] = {x.x & ~__vcmpeq2(x.x & kExp, kExp), x.y & ~__vcmpeq2(x.y & kExp, kExp),
-                                 x.z & ~__vcmpeq2(x.z & kExp, kExp), x.w & ~__vcmpeq2(x.w & kExp, kExp)};
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v + i * 16), "r"(e[0]),
-                       "r"(e[1]), "r"(e[2]), "r"(e[3])
-                       : "memory");
-        }
-      }
-      if (found) sh.wild = 1;
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.clean[slot]));
     }
   } else {
     // ---- softmax: one thread per row
-    if (kUnits == 2) take_registers();
-    const int n = unit ? n1 : n0;
+    take_registers<Cfg::kSoftRegs>();
+    const int unit = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
-    const uint32_t o_at = tmem + lanes + Cfg::kOutCol + unit * DP;
+    const uint32_t o_at = tmem + lanes + Cfg::kOCol + unit * DP;
     const float c = MODE == kTcPrompt ? a.p.scale : a.d.scale;
-    float m = -INFINITY, l = 0.0f;  // m in units of the raw score
-    bool ok = true;
-    for (int i = 0; i < n; i++) {
-      const int buffer = kUnits == 2 ? unit : i & 1;
-      const int phase = kUnits == 2 ? i : i >> 1;
-      if (!(ok = wait_warp(sh, sh.s_full[buffer], phase & 1))) break;
-      fence_after();
-      const uint32_t s_at = tmem + lanes + buffer * 128;
-      const int key = w.first + tile_of(unit, i) * kTileKeys;
-      float x[128];
-#pragma unroll
-      for (int j = 0; j < 4; j++) tmem_ld32(s_at + 32 * j, x + 32 * j);
-      tmem_wait_ld();
-      const int from = low - key, to = high - key;  // columns [from, to) are visible
-      if (__any_sync(0xffffffffu, from > 0 || to < kTileKeys)) {
-#pragma unroll
-        for (int j = 0; j < 128; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
+    const uint64_t cc = pair(c, c);
+    const int dim = MODE == kTcPrompt ? a.p.dim : a.c.head_dim;
+    int number = 0;  // tiles of this unit so far
+    for (int items = 0; ok; items++) {
+      const int at = items % kItems;
+      if (!(ok = wait(sh, sh.item_full[at], (items / kItems) & 1))) break;
+      const Item &w = sh.item[at];
+      if (w.stop) break;
+      const int n = w.n[unit];
+      int low = 0, high = INT32_MAX;  // the keys that the row sees; all, if it is not in use
+      int64_t out_at = 0, index = 0;
+      const int token = w.token0 + (alternate ? 0 : unit * a.tokens) + row / group;
+      const int head = w.kv_head * group + row % group;
+      const bool valid = row < per_unit && token < (MODE == kTcPrompt ? w.lq : a.d.batch);
+      if (valid) {
+        const int64_t r = w.q0 + (int64_t)token;
+        if (MODE == kTcPrompt) {
+          low = low_of(a.p, w.lq, w.lk, token), high = high_of(a.p, w.lq, w.lk, token);
+          out_at = r * a.p.out_stride[0] + head * a.p.out_stride[1];
+          index = r * a.p.heads + head;
+        } else {
+          int length;
+          sequence_of(a.c, a.d, token, &length);
+          low = a.d.window ? max(0, length - a.d.window) : 0;
+          high = min(length, a.d.shared);
+          out_at = r * a.d.out_stride[0] + head * a.d.out_stride[1];
+          index = r * a.d.heads + head;
+        }
       }
-      float top[4] = {x[0], x[1], x[2], x[3]};
+      float m = -INFINITY, l = 0.0f;  // m in units of the raw score
+      for (int i = 0; i < n; i++, number++) {
+        const int buffer = Cfg::kBuffers == 2 ? number & 1 : unit;
+        if (!(ok = wait(sh, sh.s_full[buffer], (Cfg::kBuffers == 2 ? number >> 1 : number) & 1))) break;
+        fence_after();
+        const uint32_t s_at = tmem + lanes + buffer * Cfg::kUnitCols;
+        const int key = w.first + tile_of(unit, i) * kKeys;
+        float x[kKeys];
 #pragma unroll
-      for (int j = 4; j < 128; j += 8)
+        for (int j = 0; j + 32 <= kKeys; j += 32) tmem_ld32(s_at + j, x + j);
+        if (kKeys % 32) tmem_ld16(s_at + kKeys / 32 * 32, reinterpret_cast<uint32_t *>(x + kKeys / 32 * 32));
+        tmem_wait_ld();
+        if (Cfg::kPCol) {
+          fence_before();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[unit]));
+        }
+        const int from = low - key, to = high - key;  // columns [from, to) are visible
+        if (__any_sync(0xffffffffu, from > 0 || to < kKeys)) {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          top[k] = j + 4 + k < 128 ? fmaxf(fmaxf(top[k], x[j + k]), x[j + 4 + k]) : fmaxf(top[k], x[j + k]);
-      const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-      // 2^8: the slack of the running maximum. Each row goes by its own scores alone.
-      const bool grows = (now - m) * c > 8.0f;
-      if (__any_sync(0xffffffffu, grows)) {
-        const float f = grows ? exp2_fast((m - now) * c) : 1.0f;
-        if (i > 0) {
-          if (!(ok = wait_warp(sh, sh.pv_done[unit], (i - 1) & 1))) break;
-          fence_after();
+          for (int j = 0; j < kKeys; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
+        }
+        float top[4] = {m, m, m, m};
+#pragma unroll
+        for (int j = 0; j < kKeys; j += 8)
+#pragma unroll
+          for (int k = 0; k < 4; k++) top[k] = max3(top[k], x[j + 2 * k], x[j + 2 * k + 1]);
+        const float now = max3(top[0], top[1], fmaxf(top[2], top[3]));
+        // 2^8: the slack of the running maximum. Each row goes by its own scores alone.
+        const bool grows = (now - m) * c > 8.0f;
+        if (__any_sync(0xffffffffu, grows)) {
+          const float f = grows ? exp2_fast((m - now) * c) : 1.0f;
+          if (i > 0) {
+            if (!(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
+            fence_after();
 #pragma unroll 1
-          for (int j = 0; j < DP; j += 16) {
-            uint32_t o[16];
-            tmem_ld16(o_at + j, o);
-            tmem_wait_ld();
+            for (int j = 0; j < DP; j += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_at + j, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st16(o_at + j, o);
+              for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(o_at + j, o);
+            }
           }
+          l *= f;
+          if (grows) m = now;
         }
-        l *= f;
-        if (grows) m = now;
-      }
-      const float z = m == -INFINITY ? 0.0f : -m * c;
-      const uint64_t cc = pair(c, c), zz = pair(z, z);
-      uint64_t sum[2] = {0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        uint32_t p[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++) {
-          const uint64_t e = fma2(pair(x[32 * j + 2 * k], x[32 * j + 2 * k + 1]), cc, zz);
-          const float e0 = exp2_fast(__uint_as_float((uint32_t)e));
-          const float e1 = exp2_fast(__uint_as_float((uint32_t)(e >> 32)));
-          sum[k & 1] = add2(sum[k & 1], pair(e0, e1));
-          p[k] = pack2<BF16>(e0, e1);
+        const float z = m == -INFINITY ? 0.0f : -m * c;
+        const uint64_t zz = pair(z, z);
+        // where P has its own columns, the last product has to have read them
+        if (Cfg::kPCol && number > 0) {
+          if (!(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
+          fence_after();
         }
-        tmem_st16(s_at + 16 * j, p);
+        uint64_t sum[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < kKeys; j += 16) {
+          uint32_t p[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            const uint64_t e = fma2(pair(x[j + 2 * k], x[j + 2 * k + 1]), cc, zz);
+            const float e0 = exp2_fast(__uint_as_float((uint32_t)e));
+            const float e1 = exp2_fast(__uint_as_float((uint32_t)(e >> 32)));
+            sum[k & 1] = add2(sum[k & 1], pair(e0, e1));
+            p[k] = pack2<BF16>(e0, e1);
+          }
+          tmem_st8(s_at + Cfg::kPCol + j / 2, p);
+        }
+        sum[0] = add2(sum[0], sum[1]);
+        l += __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
+        // With two S the last product may still run: its barrier is not to get two phases ahead
+        // of this warp.
+        if (Cfg::kBuffers == 2 && number > 0 && !(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buffer]));
       }
-      sum[0] = add2(sum[0], sum[1]);
-      l += __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
-      tmem_wait_st();
-      // With two S buffers the product of step i - 1 may still run. Its barrier must not get
-      // two phases ahead of this warp, so it is waited for before step i's can start.
-      if (Cfg::kBuffers == 2 && i > 0 && !(ok = wait_warp(sh, sh.pv_done[unit], (i - 1) & 1))) break;
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buffer]));
-    }
-    // ---- result
-    if (ok && n > 0) ok = wait_warp(sh, sh.pv_done[unit], (n - 1) & 1);
-    if (ok) {
+      if (!ok) break;
+      // ---- result
+      if (n > 0 && !(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
       fence_after();
-      const bool wild = n > 0 && sh.wild;
+      const bool wild = n > 0 && *(volatile int *)&sh.item[at].wild;
       const bool final = MODE == kTcPrompt || a.d.part.parts == 1;
-      const int dim = MODE == kTcPrompt ? a.p.dim : a.c.head_dim;
       const float inv = !final ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t part_at =
           MODE == kTcShared
@@ -610,12 +769,12 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         }
         if (wild && valid) {  // rare: what was left out of the products
           for (int i = 0; i < n; i++) {
-            const int t = tile_of(unit, i), key = w.first + t * kTileKeys;
-            if (!w.mixed(t)) continue;
-            for (int r = max(key, low); r < min(key + kTileKeys, high); r++) {
+            const int t = tile_of(unit, i), key = w.first + t * kKeys;
+            if (!mixed<kKeys>(w, t)) continue;
+            for (int r = max(key, low); r < min(key + kKeys, high); r++) {
               const uint16_t *v;
               if (MODE == kTcPrompt) {
-                v = a.p.v + (w.k0 + r) * a.p.v_stride[0] + w.kv_head * a.p.v_stride[1];
+                v = a.p.v + (w.k0 + (int64_t)r) * a.p.v_stride[0] + w.kv_head * a.p.v_stride[1];
               } else {
                 const int page = a.c.table[(int64_t)w.table_row * a.c.max_pages + r / a.c.page_tokens];
                 if ((unsigned)page >= (unsigned)a.c.pages) continue;
@@ -625,8 +784,16 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
                     (int64_t)(r % a.c.page_tokens) * dim;
               }
 #pragma unroll
-              for (int k = 0; k < 32; k++)
-                if (j + k < dim && not_finite<BF16>(v[j + k])) o[k] += to_float<BF16>(v[j + k]);
+              for (int k = 0; k < 32; k += 8) {
+                if (j + k >= dim) break;
+                const uint4 x = *reinterpret_cast<const uint4 *>(v + j + k);
+                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                  const uint16_t h = (uint16_t)(y[e / 2] >> (16 * (e & 1)));
+                  if (not_finite<BF16>(h)) o[k + e] += to_float<BF16>(h);
+                }
+              }
             }
           }
         }
@@ -651,12 +818,15 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       } else if (valid) {
         a.d.part.ml[part_at] = make_float2(m * c, l);
       }
+      fence_before();  // O has been read before the next item's weights are announced
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.item_empty[at]));
     }
   }
   fence_before();
   __syncthreads();
   if (tid == 0 && sh.abort) atomicExch(a.timeout, 1);
-  if (warp == Cfg::kSoftWarps) {
+  if (warp == Cfg::kItemWarp) {
     fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -726,6 +896,9 @@ int32_t launch(bool bf16, int dim, dim3 grid, const CUtensorMap *maps, const TcA
 }
 
 int units_of(int dim) { return dim > 128 ? 1 : 2; }
+// keys of a tile, and of a chunk of V
+int keys_of(int dim) { return dim > 64 && dim <= 128 ? TcCfg<128>::kKeys : TcCfg<64>::kKeys; }
+int v_keys_of(int dim) { return dim > 128 ? TcCfg<256>::kVKeys : keys_of(dim); }
 
 }  // namespace
 
@@ -747,10 +920,10 @@ int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *status, c
   const bool bf16 = type == DM_BF16;
   CUtensorMap maps[3];
   const uint64_t dims[3] = {(uint64_t)p.dim, (uint64_t)p.kv_heads, (uint64_t)p.k_tokens};
-  const uint32_t box[3] = {64, 1, (uint32_t)kTileKeys};
+  const uint32_t k_box[3] = {64, 1, (uint32_t)keys_of(p.dim)}, v_box[3] = {64, 1, (uint32_t)v_keys_of(p.dim)};
   const int64_t ks[2] = {p.k_stride[1] * 2, p.k_stride[0] * 2}, vs[2] = {p.v_stride[1] * 2, p.v_stride[0] * 2};
   if (!encode_q(&maps[0], bf16, p.q, p.q_stride, p.dim, p.group, p.kv_heads, p.q_tokens, a.tokens) ||
-      !encode(&maps[1], bf16, p.k, 3, dims, ks, box) || !encode(&maps[2], bf16, p.v, 3, dims, vs, box))
+      !encode(&maps[1], bf16, p.k, 3, dims, ks, k_box) || !encode(&maps[2], bf16, p.v, 3, dims, vs, v_box))
     return fail(DM_ERR_COMMAND, "could not describe the attention tensors for TMA");
   return launch<kTcPrompt>(bf16, p.dim, dim3((unsigned)(tiles * p.kv_heads)), maps, a, stream);
 }
@@ -758,6 +931,8 @@ int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *status, c
 bool tile_shared_alternates(int dim, int group, int batch) {
   return units_of(dim) == 2 && batch <= kUnitRows / group;
 }
+
+int tile_keys(int dim) { return keys_of(dim); }
 
 int tile_shared_items(int dim, int kv_heads, int group, int batch) {
   const int units = tile_shared_alternates(dim, group, batch) ? 1 : units_of(dim);
@@ -777,10 +952,14 @@ int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, i
   CUtensorMap maps[3];
   const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_tokens, (uint64_t)c.kv_heads, (uint64_t)c.pages};
   const int64_t strides[3] = {c.head_dim * 2, c.head_bytes, c.page_bytes};
-  const uint32_t box[4] = {64, (uint32_t)std::min(c.page_tokens, kTileKeys), 1, 1};
+  // a box lies in one page and divides a chunk: pages are powers of two from 16
+  auto rows = [&](int keys) { return std::min(c.page_tokens, keys & -keys); };
+  a.k_box = rows(keys_of(c.head_dim));
+  a.v_box = rows(v_keys_of(c.head_dim));
+  const uint32_t k_box[4] = {64, (uint32_t)a.k_box, 1, 1}, v_box[4] = {64, (uint32_t)a.v_box, 1, 1};
   const uint8_t *k = c.memory + d.layer * c.layer_bytes, *v = k + c.kv_heads * c.head_bytes;
   if (!encode_q(&maps[0], bf16, d.q, d.q_stride, c.head_dim, d.group, c.kv_heads, d.batch, a.tokens) ||
-      !encode(&maps[1], bf16, k, 4, dims, strides, box) || !encode(&maps[2], bf16, v, 4, dims, strides, box))
+      !encode(&maps[1], bf16, k, 4, dims, strides, k_box) || !encode(&maps[2], bf16, v, 4, dims, strides, v_box))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
   const int items = tile_shared_items(c.head_dim, c.kv_heads, d.group, d.batch);
   return launch<kTcShared>(bf16, c.head_dim, dim3((unsigned)items, (unsigned)d.splits), maps, a, stream);

@@ -11,6 +11,7 @@ int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *status, c
 
 // The shared part of a decode call, in d.splits parts, or twice as many where the two units
 // of a block alternate.
+int tile_keys(int dim);  // keys of a tile
 bool tile_shared_alternates(int dim, int group, int batch);
 int tile_shared_items(int dim, int kv_heads, int group, int batch);
 int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, int32_t *status,
