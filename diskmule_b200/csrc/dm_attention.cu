@@ -82,21 +82,26 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
   const int dim = MODE == kPrompt ? p.dim : c.head_dim;
   const int group = MODE == kPrompt ? p.group : d.group;
 
+  // The own part of a decode call reads nothing that the shared part's kernel before it
+  // writes, and that one has waited for what both read: they run side by side.
+  const bool beside = MODE == kOwn && d.first_part > 0;
+  if (!beside) wait_for_previous();
+  let_next_start();
+
   // ---- the block's rows, its keys and where they lie
   int kv_head, first = 0, last, table_row = 0;
   int64_t k0 = 0;  // prompt: first key row
   if (MODE == kPrompt) {
     kv_head = blockIdx.y;
     if (warp == 0) {
-      const TileOf t = find_tile(p.q_offsets, p.sequences, p.q_tokens, group, kRows, blockIdx.x);
+      const TileOf t = find_tile(p, group, kRows, blockIdx.x);
       if (lane == 0) sh.tile = t;
     }
     __syncthreads();
     const TileOf t = sh.tile;
     if (t.seq < 0) return;
-    const int64_t k1 = min((int64_t)max(p.k_offsets[t.seq + 1], 0), p.k_tokens);
-    k0 = min((int64_t)max(p.k_offsets[t.seq], 0), p.k_tokens);
-    const int lq = t.q1 - t.q0, lk = (int)max((int64_t)0, k1 - k0);
+    k0 = t.k0;
+    const int lq = t.q1 - t.q0, lk = t.k1 - t.k0;
     if (tid < kRows) {
       const int64_t r = (int64_t)t.tile * kRows + tid;
       const int token = (int)(r / group), head = kv_head * group + (int)(r % group);
@@ -334,7 +339,9 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
     sh.ml[warp][rb8] = make_float2(mb, lb);
   }
   __syncthreads();
-  const bool final = MODE == kPrompt || d.part.parts == 1;
+  // All of it is done before the kernel after this one may read the parts of both.
+  if (beside) wait_for_previous();
+  const bool final = MODE == kPrompt || d.part.parts == 1 || d.joins;
   constexpr int kLanes = DP / 4;  // threads along a row, four columns each
   const float *all = reinterpret_cast<const float *>(smem);
   for (int r = tid / kLanes; r < kRows; r += kThreads / kLanes) {
@@ -342,6 +349,9 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; w++) m = fmaxf(m, sh.ml[w][r].x);
+    const float2 *ml = d.part.ml + sh.index[r];
+    if (MODE == kOwn && d.joins)
+      for (int i = 0; i < d.first_part; i++) m = fmaxf(m, ml[i * d.part.rows].x);
     const float z = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -352,6 +362,18 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
       const float4 u = *reinterpret_cast<const float4 *>(all + (w * kRows + r) * DP + col);
       l += sh.ml[w][r].y * f;
       v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
+    }
+    if (MODE == kOwn && d.joins && col < dim) {
+      const float *part = d.part.o + sh.index[r] * dim + col;
+#pragma unroll 4
+      for (int i = 0; i < d.first_part; i++) {
+        const float2 s = ml[i * d.part.rows];
+        const float4 u = *reinterpret_cast<const float4 *>(part + i * d.part.rows * dim);
+        if (s.y == 0.0f) continue;  // nothing was written
+        const float f = exp2_fast(s.x - z);
+        l += s.y * f;
+        v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
+      }
     }
     if (final) {
       float *lse = MODE == kPrompt ? p.lse : d.lse;
@@ -376,15 +398,19 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
 
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads) join_kernel(DecodeArgs d, int dim) {
-  __shared__ float top[kThreads], sum[kWarps];
+  __shared__ float top[kWarps], sum[kWarps];
   __shared__ float4 acc[kWarps][64];
+  let_next_start();
+  wait_for_previous();
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float m = -INFINITY;
   for (int i = tid; i < d.part.parts; i += kThreads) m = fmaxf(m, d.part.ml[i * d.part.rows + row].x);
-  top[tid] = m;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  if (lane == 0) top[warp] = m;
   __syncthreads();
-  for (int i = 0; i < kThreads; i++) m = fmaxf(m, top[i]);
+  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   const float z = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   float4 v[2] = {};
@@ -435,9 +461,7 @@ int32_t launch_rows(dim3 grid, const PromptArgs &p, const DecodeArgs &d, const K
             "attention shared memory");
     set = true;
   }
-  fn<<<grid, kThreads, RowsCfg<DP>::kSmem, s>>>(p, d, c);
-  DM_CUDA(cudaGetLastError(), "attention launch");
-  return DM_OK;
+  return launch_chained("attention launch", fn, grid, kThreads, RowsCfg<DP>::kSmem, s, p, d, c);
 }
 
 template <int MODE>
@@ -461,6 +485,7 @@ struct DecodePlan {
 constexpr int kTargetBlocks = 296;  // two blocks of four warps on each of 148 SMs
 constexpr int kTileBlocks = 148;    // one block of tiles on each
 constexpr int kMinTileRows = 16;
+constexpr int kOneSplitKeys = 1024;
 
 DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, int max_length) {
   DecodePlan plan;
@@ -483,6 +508,9 @@ DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, 
     const int own = std::max(1, max_length - shared);
     plan.own_splits = (int)std::max<int64_t>(
         1, std::min<int64_t>((kTargetBlocks + items - 1) / items, (own + 255) / 256));
+    // One split joins the shared parts itself: no third launch. Up to 1024 keys that is
+    // worth more than more blocks.
+    if (shared > 0 && own <= kOneSplitKeys) plan.own_splits = 1;
   }
   return plan;
 }
@@ -632,15 +660,14 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
     const int64_t items = (int64_t)in->batch * kd.kv_heads * ((a.group + kRows - 1) / kRows);
     a.first_part = plan.shared_parts;
     a.splits = plan.own_splits;
+    a.joins = plan.shared_parts > 0 && plan.own_splits == 1;
     if (int32_t rc = launch_rows<kOwn>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
                                        PromptArgs{}, a, cache->view, s))
       return rc;
   }
-  if (plan.parts() > 1) {
-    if (kd.type == DM_BF16) join_kernel<true><<<(unsigned)a.part.rows, kThreads, 0, s>>>(a, kd.head_dim);
-    else join_kernel<false><<<(unsigned)a.part.rows, kThreads, 0, s>>>(a, kd.head_dim);
-    DM_CUDA(cudaGetLastError(), "attention join launch");
-  }
+  if (plan.parts() > 1 && !a.joins)
+    return launch_chained("attention join launch", kd.type == DM_BF16 ? join_kernel<true> : join_kernel<false>,
+                          dim3((unsigned)a.part.rows), kThreads, 0, s, a, kd.head_dim);
   return DM_OK;
 }
 

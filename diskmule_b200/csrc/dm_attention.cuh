@@ -50,6 +50,7 @@ struct DecodeArgs {
   PartArgs part;       // part.parts == 1: results go straight to out and lse
   int32_t first_part;  // of this launch
   int32_t splits;      // parts of this launch
+  int32_t joins;       // own part: this launch joins the parts before its own
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -70,6 +71,18 @@ __device__ __forceinline__ uint32_t pack2(float low, float high) {
   if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
   return r;
+}
+
+// 32 bytes at once where `wide` (the address is a multiple of 32), else 16
+__device__ __forceinline__ void store32(void *p, const uint32_t *r, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4 *>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    reinterpret_cast<uint4 *>(p)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+  }
 }
 
 // 16-bit patterns whose exponent is all ones are infinities and NaN
@@ -94,18 +107,18 @@ __device__ __forceinline__ uint32_t zero_not_finite(uint32_t x, bool &any) {
 // Packed prompts: sequence and place of tile `tile` when a sequence of L tokens has
 // ceil(L * per_token / rows) tiles. One warp; seq = -1 behind the last tile.
 struct TileOf {
-  int seq, tile, q0, q1;
+  int seq, tile, q0, q1, k0, k1;  // query and key rows of the sequence
 };
-__device__ __forceinline__ TileOf find_tile(const int32_t *offsets, int sequences, int64_t tokens,
-                                            int per_token, int rows, int64_t tile) {
+__device__ __forceinline__ TileOf find_tile(const PromptArgs &p, int per_token, int rows, int64_t tile) {
   const int lane = threadIdx.x & 31;
-  TileOf r{-1, 0, 0, 0};
-  for (int s0 = 0; s0 < sequences; s0 += 32) {
+  TileOf r{-1, 0, 0, 0, 0, 0};
+  for (int s0 = 0; s0 < p.sequences; s0 += 32) {
     const int s = s0 + lane;
-    int q0 = 0, q1 = 0;
-    if (s < sequences) {
-      q0 = (int)min((int64_t)max(offsets[s], 0), tokens);
-      q1 = (int)max((int64_t)q0, min((int64_t)offsets[s + 1], tokens));
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+    if (s < p.sequences) {  // rows outside the tensors are not there
+      q0 = p.q_offsets[s], q1 = p.q_offsets[s + 1], k0 = p.k_offsets[s], k1 = p.k_offsets[s + 1];
+      q0 = (int)min((int64_t)max(q0, 0), p.q_tokens), q1 = max(q0, (int)min((int64_t)q1, p.q_tokens));
+      k0 = (int)min((int64_t)max(k0, 0), p.k_tokens), k1 = max(k0, (int)min((int64_t)k1, p.k_tokens));
     }
     const int64_t n = ((int64_t)(q1 - q0) * per_token + rows - 1) / rows;
     int64_t upto = n;
@@ -121,6 +134,8 @@ __device__ __forceinline__ TileOf find_tile(const int32_t *offsets, int sequence
       r.tile = (int)__shfl_sync(0xffffffffu, tile - (upto - n), src);
       r.q0 = __shfl_sync(0xffffffffu, q0, src);
       r.q1 = __shfl_sync(0xffffffffu, q1, src);
+      r.k0 = __shfl_sync(0xffffffffu, k0, src);
+      r.k1 = __shfl_sync(0xffffffffu, k1, src);
       return r;
     }
     tile -= __shfl_sync(0xffffffffu, upto, 31);

@@ -57,8 +57,10 @@ struct TcCfg {
   static constexpr int kScrubWarp = kItemWarp + 3;
   static constexpr int kSWarp = kItemWarp + 4;               // products S, one warp per unit
   static constexpr int kOWarp = kSWarp + kUnits;             // products O
-  static constexpr int kConsumers = kSoftWarps + 3 + 2 * kUnits;  // of an item
   static constexpr int kThreads = DP == 256 ? 384 : 512;     // whole groups of four warps
+  // the warps behind the last one scrub too
+  static constexpr int kScrubWarps = 1 + kThreads / 32 - (kOWarp + kUnits);
+  static constexpr int kConsumers = kThreads / 32 - 1;       // of an item
   // K and V move in chunks, each in a ring of its own: whole tiles, or for dim 256 quarters
   // (64 values of all keys of K, 32 keys of V), so that a chunk's place is free again soon.
   static constexpr int kChunks = DP == 256 ? 4 : 1;          // of a tile
@@ -179,6 +181,7 @@ struct TcArgs {
   int tiles;      // prompt: upper bound of the number of items per key/value head
   int alternate;  // shared: one unit's rows hold them all; the units take tiles in turn
   int k_box, v_box;  // shared: rows of a TMA box
+  int wide;          // rows of the result (or of the parts) lie on 32-byte boundaries
   int32_t *timeout;
 };
 
@@ -374,7 +377,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       mbar_init(smem_u32(&sh.k_full[i]), 1);
       mbar_init(smem_u32(&sh.k_empty[i]), kUnits);
       mbar_init(smem_u32(&sh.v_full[i]), 1);
-      mbar_init(smem_u32(&sh.v_clean[i]), 1);
+      mbar_init(smem_u32(&sh.v_clean[i]), Cfg::kScrubWarps);
       mbar_init(smem_u32(&sh.v_empty[i]), kUnits);
     }
     mbar_init(smem_u32(&sh.q_full), 1);
@@ -389,6 +392,9 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
+  // What a kernel after this one may read without waiting is older than this one's inputs.
+  wait_for_previous();
+  let_next_start();
   bool ok = true;  // of the role: no wait has run out
 
   if (warp >= Cfg::kSoftWarps) {
@@ -404,15 +410,13 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         } else {
           // key/value heads side by side, the last (longest, if causal) tiles of the batch first
           w.kv_head = block % a.p.kv_heads;
-          const TileOf t = find_tile(a.p.q_offsets, a.p.sequences, a.p.q_tokens, 1, kUnits * a.tokens,
-                                     a.tiles - 1 - block / a.p.kv_heads);
+          const TileOf t = find_tile(a.p, 1, kUnits * a.tokens, a.tiles - 1 - block / a.p.kv_heads);
           if (t.seq < 0) {
             w.stop = -1;  // behind the last tile
           } else {
             w.q0 = t.q0;
-            w.k0 = (int)min((int64_t)max(a.p.k_offsets[t.seq], 0), a.p.k_tokens);
-            const int k1 = (int)min((int64_t)max(a.p.k_offsets[t.seq + 1], 0), a.p.k_tokens);
-            const int lq = w.lq = t.q1 - t.q0, lk = w.lk = max(0, k1 - w.k0);
+            w.k0 = t.k0;
+            const int lq = w.lq = t.q1 - t.q0, lk = w.lk = t.k1 - t.k0;
             w.token0 = t.tile * kUnits * a.tokens;
             const int last = min(lq, w.token0 + kUnits * a.tokens) - 1;
             // limits of the first and last token bound the others'
@@ -479,7 +483,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
       }
       if (!ok && asks > 0) mbar_wait(smem_u32(&sh.next_block), (asks - 1) & 1);
-    } else if (warp <= Cfg::kOWarp + kUnits - 1) {
+    } else {
       // ---- loads, products and clean-up go through the tiles of every item
       const uint32_t lead = elect_one();
       const uint32_t columns = uniform(tmem);
@@ -513,7 +517,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         } else if (warp == Cfg::kVWarp) {
           // ---- values
           ok = load_tiles<MODE, DP, true>(sh, w, tiles, a, &v_map, v_ring, lead, place);
-        } else if (warp == Cfg::kScrubWarp) {
+        } else if (warp == Cfg::kScrubWarp || warp >= Cfg::kOWarp + kUnits) {
           // ---- values that are not finite leave mixed tiles; the others are passed on
           // rows behind the last key are no one's: other sequences, or what the ring held before
           const int keys = MODE == kTcPrompt ? w.lk : a.d.shared;
@@ -524,16 +528,27 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
               if (!(ok = wait(sh, sh.v_full[place.slot], place.parity()))) break;
               if (mix) {
                 const uint32_t v = v_ring + place.slot * Cfg::kChunkBytes;
+                // an exponent of all ones carries into the sign's place
                 constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
-#pragma unroll 4
-                for (int j = lane; j < Cfg::kChunkBytes / 16; j += 32) {
+                constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;
+                const int who = warp == Cfg::kScrubWarp ? 0 : warp - (Cfg::kOWarp + kUnits) + 1;
+                constexpr int kStep = 32 * Cfg::kScrubWarps;
+                uint32_t any = 0;
+#pragma unroll 8
+                for (int j = who * 32 + lane; j < Cfg::kChunkBytes / 16; j += kStep) {
                   const uint4 x = lds16(v + j * 16);
-                  const uint32_t bad[4] = {__vcmpeq2(x.x & kExp, kExp), __vcmpeq2(x.y & kExp, kExp),
-                                           __vcmpeq2(x.z & kExp, kExp), __vcmpeq2(x.w & kExp, kExp)};
-                  if (bad[0] | bad[1] | bad[2] | bad[3]) {
+                  any |= ((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne);
+                }
+                if (any & 0x80008000u) {
+                  for (int j = who * 32 + lane; j < Cfg::kChunkBytes / 16; j += kStep) {
+                    const uint4 x = lds16(v + j * 16);
+                    bool bad = false;
+                    uint32_t y[4] = {x.x, x.y, x.z, x.w};
+                    for (int k = 0; k < 4; k++) y[k] = zero_not_finite<BF16>(y[k], bad);
+                    if (!bad) continue;
                     found |= w.first + t * kKeys + c * Cfg::kVKeys + j / 8 % Cfg::kVKeys < keys;
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v + j * 16),
-                                 "r"(x.x & ~bad[0]), "r"(x.y & ~bad[1]), "r"(x.z & ~bad[2]), "r"(x.w & ~bad[3])
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v + j * 16), "r"(y[0]),
+                                 "r"(y[1]), "r"(y[2]), "r"(y[3])
                                  : "memory");
                   }
                 }
@@ -618,11 +633,11 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (ok && lead) mbar_arrive(smem_u32(&sh.item_empty[at]));
       }
       if (!ok) {  // copies and products in flight end before the block does
-        if (warp >= Cfg::kSWarp) {
+        if (warp >= Cfg::kSWarp && warp < Cfg::kOWarp + kUnits) {
           uint64_t &bar = sh.drain[warp - Cfg::kSWarp];
           commit_if(lead, smem_u32(&bar));
           mbar_wait(smem_u32(&bar), 0);
-        } else if (warp != Cfg::kScrubWarp) {
+        } else if (warp == Cfg::kKWarp || warp == Cfg::kVWarp) {
           const int issued = (int)min((uint32_t)kSlots, place.round * kSlots + place.slot);
           place.back(issued);
           for (int i = 0; i < issued; i++, place.next())
@@ -799,17 +814,20 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         }
         if (valid && final) {
           uint16_t *out = (MODE == kTcPrompt ? a.p.out : a.d.out) + out_at + j;
+          uint32_t h[16];
 #pragma unroll
-          for (int k = 0; k < 32; k += 8)
-            if (j + k < dim)
-              *reinterpret_cast<uint4 *>(out + k) =
-                  make_uint4(pack2<BF16>(o[k] * inv, o[k + 1] * inv), pack2<BF16>(o[k + 2] * inv, o[k + 3] * inv),
-                             pack2<BF16>(o[k + 4] * inv, o[k + 5] * inv), pack2<BF16>(o[k + 6] * inv, o[k + 7] * inv));
+          for (int k = 0; k < 16; k++) h[k] = pack2<BF16>(o[2 * k] * inv, o[2 * k + 1] * inv);
+#pragma unroll
+          for (int k = 0; k < 32; k += 16) {
+            if (j + k + 16 <= dim) store32(out + k, h + k / 2, a.wide);
+            else if (j + k < dim)  // dim is a multiple of 8
+              *reinterpret_cast<uint4 *>(out + k) = make_uint4(h[k / 2], h[k / 2 + 1], h[k / 2 + 2], h[k / 2 + 3]);
+          }
         } else if (valid && l != 0.0f) {
           float *out = a.d.part.o + part_at * dim + j;
 #pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            if (j + k < dim) *reinterpret_cast<float4 *>(out + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          for (int k = 0; k < 32; k += 8)
+            if (j + k < dim) store32(out + k, reinterpret_cast<const uint32_t *>(o + k), a.wide);
         }
       }
       if (valid && final) {
@@ -881,9 +899,8 @@ int32_t launch(dim3 grid, const CUtensorMap *maps, const TcArgs &a, cudaStream_t
             "attention shared memory");
     set = true;
   }
-  fn<<<grid, TcCfg<DP>::kThreads, TcCfg<DP>::kSmem, s>>>(maps[0], maps[1], maps[2], a);
-  DM_CUDA(cudaGetLastError(), "attention launch");
-  return DM_OK;
+  return launch_chained("attention launch", fn, grid, TcCfg<DP>::kThreads, TcCfg<DP>::kSmem, s, maps[0],
+                        maps[1], maps[2], a);
 }
 
 template <int MODE>
@@ -899,6 +916,10 @@ int units_of(int dim) { return dim > 128 ? 1 : 2; }
 // keys of a tile, and of a chunk of V
 int keys_of(int dim) { return dim > 64 && dim <= 128 ? TcCfg<128>::kKeys : TcCfg<64>::kKeys; }
 int v_keys_of(int dim) { return dim > 128 ? TcCfg<256>::kVKeys : keys_of(dim); }
+
+bool aligned32(const uint16_t *p, const int64_t *stride) {
+  return ((uintptr_t)p & 31) == 0 && stride[0] % 16 == 0 && stride[1] % 16 == 0;
+}
 
 }  // namespace
 
@@ -917,6 +938,7 @@ int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *status, c
   const int64_t tiles = p.q_tokens / (units_of(p.dim) * a.tokens) + p.sequences;
   if (tiles * p.kv_heads > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
   a.tiles = (int)tiles;
+  a.wide = aligned32(p.out, p.out_stride);
   const bool bf16 = type == DM_BF16;
   CUtensorMap maps[3];
   const uint64_t dims[3] = {(uint64_t)p.dim, (uint64_t)p.kv_heads, (uint64_t)p.k_tokens};
@@ -948,6 +970,7 @@ int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, i
   a.tokens = kUnitRows / d.group;
   a.alternate = tile_shared_alternates(c.head_dim, d.group, d.batch);
   a.timeout = status + kStatusWord;
+  a.wide = d.part.parts > 1 ? ((uintptr_t)d.part.o & 31) == 0 : aligned32(d.out, d.out_stride);
   const bool bf16 = type == DM_BF16;
   CUtensorMap maps[3];
   const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_tokens, (uint64_t)c.kv_heads, (uint64_t)c.pages};

@@ -49,11 +49,9 @@ Plan plan_of(const dm_kv_cache *c) {
   return p;
 }
 
-// The next kernel on the stream may be scheduled now; this one waits until the one before it
-// has ended and its writes are seen.
 __device__ __forceinline__ void chain() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  dma::let_next_start();
+  dma::wait_for_previous();
 }
 
 // Inclusive sum over the block; `total` gets the block's. Every thread of the block calls it.
@@ -464,20 +462,9 @@ int blocks_along(int64_t vectors, int64_t items, int64_t blocks) {
 }
 constexpr int kGridBlocks = 148 * 8;
 
-// A launch that may be scheduled while the kernel before it still runs (see chain).
 template <typename... Params, typename... Args>
-int32_t launch(void (*kernel)(Params...), dim3 grid, int threads, void *stream, Args... args) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = threads;
-  config.stream = (cudaStream_t)stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  DM_CUDA(cudaLaunchKernelEx(&config, kernel, Params(args)...), "cache launch");
-  return DM_OK;
+int32_t launch(void (*kernel)(Params...), dim3 grid, int threads, void *stream, const Args &...args) {
+  return dma::launch_chained("cache launch", kernel, grid, threads, 0, (cudaStream_t)stream, args...);
 }
 
 int32_t check_list(const dm_kv_cache *cache, const void *list, int32_t n) {
@@ -651,9 +638,8 @@ int32_t dm_kv_cache_fork(dm_kv_cache *c, const int32_t *parents, const int32_t *
   if (!parents) return fail(DM_ERR_INVALID_ARGUMENT, "null parents");
   if (n > 65535) return fail(DM_ERR_ELEMENT_COUNT, "%d forks in one call", n);
   cudaSetDevice(c->ctx->device);
-  if (int32_t rc = launch(plan_kernel<kFork>, 1, kPlanThreads, stream, c->view, plan_of(c),
-                          PlanArgs{children, parents, nullptr, 0, n}))
-    return rc;
+  const PlanArgs a{children, parents, nullptr, 0, n};
+  if (int32_t rc = launch(plan_kernel<kFork>, 1, kPlanThreads, stream, c->view, plan_of(c), a)) return rc;
   // half a page is copied on average
   const dim3 grid(blocks_along(c->view.page_bytes / 32, n, kGridBlocks), n);
   return launch(fork_kernel, grid, kCopyThreads, stream, c->view, plan_of(c), parents, children);

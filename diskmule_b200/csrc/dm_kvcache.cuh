@@ -20,6 +20,34 @@ struct KvView {
   int64_t page_bytes, layer_bytes, head_bytes;  // of a page, of its layer (K and V), of one head
 };
 
+// The next kernel on the stream may be scheduled (it then waits, below).
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// Wait until the kernel before this one on the stream has ended and its writes are seen.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// A launch that may be scheduled while the kernel before it still runs; the kernel calls
+// wait_for_previous before it touches what that one or its predecessors wrote.
+template <typename... Params, typename... Args>
+int32_t launch_chained(const char *what, void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                       cudaStream_t stream, const Args &...args) {
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = threads;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  DM_CUDA(cudaLaunchKernelEx(&config, kernel, args...), what);
+  return DM_OK;
+}
+
 }  // namespace dma
 
 struct dm_kv_cache {
