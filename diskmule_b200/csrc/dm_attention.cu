@@ -8,31 +8,42 @@
 
 #include "dm_attention.cuh"
 #include "dm_attention_tc.cuh"
+#include "dm_tcgen05.cuh"
 
 using dmi::fail;
 
 namespace dma {
 
+using namespace dm::tc;
+
 // ---------------------------------------------------------------------------
-// 16 query rows against a range of keys. The block's four warps take chunks of 16 keys in
-// turn, each with its own ring of shared-memory stages (cp.async) and its own softmax
-// state, so nothing in the loop waits for another warp; the four states join at the end.
+// 16 query rows against a range of keys. The block's warps take chunks of 16 keys in turn,
+// each with its own ring of shared-memory stages and its own softmax state, so nothing in the
+// loop waits for another warp; their states join at the end. Chunks of a cache come by TMA
+// (rows of 64 values, 128-byte swizzle; a few instructions of one lane, where cp.async took a
+// third of the loop's), those of a prompt by cp.async into the same layout.
 // ---------------------------------------------------------------------------
 
 constexpr int kRows = 16;    // query rows of a block: one mma tile
 constexpr int kChunk = 16;   // keys of a step of one warp; pages are multiples of it
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kStages = 3;   // of a warp's ring
+constexpr int kJoinThreads = 128;
+constexpr int kMostJoined = 8;     // shared parts that a block of the own part joins itself
+constexpr int kMostParts = 512;
 
 enum Mode { kPrompt, kOwn, kShared };
 
-template <int DP>
+template <int DP, int WARPS>
 struct RowsCfg {
-  static constexpr int kStages = DP == 64 ? 4 : 3;
+  static constexpr int kThreads = WARPS * 32;
   static constexpr int kTile = kChunk * DP * 2;   // bytes of a K or V tile
+  static constexpr int kSlab = kChunk * 128;      // 64 values of its rows
   static constexpr int kRing = kStages * 2 * kTile;
-  static constexpr int kJoin = kWarps * kRows * DP * 4;
-  static constexpr int kSmem = kWarps * kRing > kJoin ? kWarps * kRing : kJoin;
+  static constexpr int kJoin = WARPS * kRows * DP * 4;
+  // room for the warps' states, too; rings are aligned to 1024 bytes
+  static constexpr int kSmem = 1024 + WARPS * kRing;
+  static_assert(kJoin <= WARPS * kRing, "the states fit the rings");
+  static constexpr int kBlocks = kSmem <= 112 * 1024 ? 2 : 1;  // per SM
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
@@ -63,22 +74,37 @@ __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Add a state (ml, o) to the sums that refer to z.
+__device__ __forceinline__ void add_state(float &l, float4 &v, float2 ml, float4 o, float z) {
+  const float f = exp2_fast(ml.x - z);
+  l += ml.y * f;
+  v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+}
+
+template <int WARPS>
 struct RowsSmem {
   int64_t q[kRows];     // element offset of the row's query, -1: no row
   int64_t out[kRows];   // element offset of its output
   int64_t index[kRows]; // its row in lse and in the parts
   int low[kRows], high[kRows];  // the keys that it sees
-  float2 ml[kWarps][kRows];
+  float2 ml[WARPS][kRows];
+  uint64_t full[WARPS][kStages];  // a chunk of a warp has landed
   TileOf tile;
 };
 
-template <int MODE, int DP, bool BF16>
-__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2)
-rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
-  using Cfg = RowsCfg<DP>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ RowsSmem sh;
+template <int MODE, int DP, int WARPS, bool BF16>
+__global__ void __launch_bounds__(WARPS * 32, (RowsCfg<DP, WARPS>::kBlocks))
+rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+            const __grid_constant__ PromptArgs p, const __grid_constant__ DecodeArgs d,
+            const __grid_constant__ KvView c) {
+  using Cfg = RowsCfg<DP, WARPS>;
+  constexpr int kWarps = WARPS, kThreads = Cfg::kThreads;
+  extern __shared__ uint8_t raw[];
+  uint8_t *smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
+  __shared__ RowsSmem<WARPS> sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (MODE != kPrompt && tid < WARPS * kStages) mbar_init(smem_u32(&sh.full[tid / kStages][tid % kStages]), 1);
+  if (MODE != kPrompt) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   const int dim = MODE == kPrompt ? p.dim : c.head_dim;
   const int group = MODE == kPrompt ? p.group : d.group;
 
@@ -169,37 +195,37 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
       qf[k][h * 2 + 1] = in && qb >= 0 ? *reinterpret_cast<const uint32_t *>(qp + qb + col) : 0u;
     }
 
-  // ---- the warp's ring
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * Cfg::kRing;
+  // ---- the warp's ring: V behind K, slabs of 64 values, 128-byte swizzle
+  const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing;
   constexpr int kVec = DP / 8;  // 16-byte vectors of a row
-  const int vecs = dim / 8;
+  auto at = [](int r, int v) { return (uint32_t)((v >> 3) * Cfg::kSlab + r * 128 + ((v ^ r) & 7) * 16); };
   auto page_of = [&](int key) -> int {
     if (MODE == kPrompt || key >= last) return -1;
-    return c.table[(int64_t)table_row * c.max_pages + key / c.page_tokens];
+    const int page = c.table[(int64_t)table_row * c.max_pages + key / c.page_tokens];
+    return (unsigned)page < (unsigned)c.pages ? page : c.pages;  // behind the map: zeros
   };
   auto load = [&](int key, int page, int stage) {
     const uint32_t kd = ring + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;
-    const uint8_t *kb, *vb;
-    int64_t ks, vs;  // bytes from row to row
-    bool there = true;
     if (MODE == kPrompt) {
-      kb = reinterpret_cast<const uint8_t *>(p.k + (k0 + key) * p.k_stride[0] + kv_head * p.k_stride[1]);
-      vb = reinterpret_cast<const uint8_t *>(p.v + (k0 + key) * p.v_stride[0] + kv_head * p.v_stride[1]);
-      ks = p.k_stride[0] * 2, vs = p.v_stride[0] * 2;
-    } else {
-      there = (unsigned)page < (unsigned)c.pages;
-      kb = c.memory + (there ? page : 0) * c.page_bytes + d.layer * c.layer_bytes +
-           kv_head * c.head_bytes + (int64_t)(key % c.page_tokens) * dim * 2;
-      vb = kb + c.kv_heads * c.head_bytes;
-      ks = vs = dim * 2;
-    }
+      const uint16_t *kb = p.k + (k0 + key) * p.k_stride[0] + kv_head * p.k_stride[1];
+      const uint16_t *vb = p.v + (k0 + key) * p.v_stride[0] + kv_head * p.v_stride[1];
 #pragma unroll
-    for (int i = 0; i < kChunk * kVec / 32; i++) {
-      const int at = i * 32 + lane, r = at / kVec, v = at % kVec;
-      const bool valid = there && key + r < last && v < vecs;
-      const uint32_t to = (uint32_t)(r * kVec + (v ^ (r & 7))) * 16;
-      cp16(kd + to, valid ? kb + r * ks + v * 16 : kb, valid);
-      cp16(vd + to, valid ? vb + r * vs + v * 16 : vb, valid);
+      for (int i = 0; i < kChunk * kVec / 32; i++) {
+        const int n = i * 32 + lane, r = n / kVec, v = n % kVec;
+        const bool valid = key + r < last && v < dim / 8;
+        cp16(kd + at(r, v), valid ? kb + r * p.k_stride[0] + v * 8 : kb, valid);
+        cp16(vd + at(r, v), valid ? vb + r * p.v_stride[0] + v * 8 : vb, valid);
+      }
+    } else {
+      const uint32_t bar = smem_u32(&sh.full[warp][stage]);
+      if (lane == 0) mbar_expect_tx(bar, 2 * Cfg::kTile);
+      __syncwarp();
+      if (lane < 2 * (DP / 64)) {  // one slab each
+        const bool is_v = lane >= DP / 64;
+        const int slab = lane % (DP / 64);
+        tma_load_4d((is_v ? vd : kd) + slab * Cfg::kSlab, is_v ? &v_map : &k_map, slab * 64,
+                    key % c.page_tokens, kv_head, page, bar);
+      }
     }
   };
 
@@ -219,29 +245,37 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
       page = next;
     }
     key_load += kStep;
-    asm volatile("cp.async.commit_group;");
+    if (MODE == kPrompt) asm volatile("cp.async.commit_group;");
   };
 #pragma unroll
-  for (int s = 0; s < Cfg::kStages - 1; s++) issue(s);
+  for (int s = 0; s < kStages - 1; s++) issue(s);
   int stage = 0;
+  uint32_t parity = 0;  // of the ring's round
+  bool late = false;    // a wait has run out
   for (int key = first + warp * kChunk; key < last; key += kStep) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kStages - 2));
+    if (MODE == kPrompt) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2));
+    } else if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.full[warp][stage]), parity))) {
+      late = true;
+      break;
+    }
     __syncwarp();  // all lanes' copies are there, and all have left the stage that is next
-    issue(stage == 0 ? Cfg::kStages - 1 : stage - 1);
+    issue(stage == 0 ? kStages - 1 : stage - 1);
     const uint32_t kt = ring + stage * 2 * Cfg::kTile, vt = kt + Cfg::kTile;
-    float s[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+    // two chains of products per 8 keys: one would be bound by the latency of its links
+    float s[2][4] = {}, s2[2][4] = {};
     {
       const int r = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
       for (int k = 0; k < DP / 16; k++) {
         uint32_t b[4];
         const int v = 2 * k + ((lane >> 3) & 1);
-        ldm4(kt + (r * kVec + (v ^ (r & 7))) * 16, b);
-        mma16816<BF16>(s[0], qf[k], b[0], b[1]);
-        mma16816<BF16>(s[1], qf[k], b[2], b[3]);
+        ldm4(kt + at(r, v), b);
+        mma16816<BF16>(k & 1 ? s2[0] : s[0], qf[k], b[0], b[1]);
+        mma16816<BF16>(k & 1 ? s2[1] : s[1], qf[k], b[2], b[3]);
       }
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[0][i] += s2[0][i], s[1][i] += s2[1][i];
     }
     // scores, masked, and the new maxima
     float na = ma, nb = mb;
@@ -260,11 +294,19 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
       na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, x));
       nb = fmaxf(nb, __shfl_xor_sync(0xffffffffu, nb, x));
     }
+    // The maxima that the sums refer to have slack: they follow only when a score is 2^8 above
+    // (each row by its own scores), so that most chunks rescale nothing.
+    const bool ga = na - ma > 8.0f, gb = nb - mb > 8.0f;
+    if (__any_sync(0xffffffffu, ga || gb)) {
+      const float fa = ga ? exp2_fast(ma - na) : 1.0f, fb = gb ? exp2_fast(mb - nb) : 1.0f;
+      if (ga) ma = na;
+      if (gb) mb = nb;
+      la *= fa, lb *= fb;
+#pragma unroll
+      for (int i = 0; i < DP / 8; i++) o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
+    }
     // a row that has seen nothing yet keeps a zero reference
-    const float za = na == -INFINITY ? 0.0f : na, zb = nb == -INFINITY ? 0.0f : nb;
-    const float fa = exp2_fast(ma - za), fb = exp2_fast(mb - zb);
-    ma = na, mb = nb;
-    la *= fa, lb *= fb;
+    const float za = ma == -INFINITY ? 0.0f : ma, zb = mb == -INFINITY ? 0.0f : mb;
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -273,8 +315,6 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
         s[t][2 + e] = exp2_fast(s[t][2 + e] - zb);
         la += s[t][e], lb += s[t][2 + e];
       }
-#pragma unroll
-    for (int i = 0; i < DP / 8; i++) o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
     const uint32_t pf[4] = {pack2<BF16>(s[0][0], s[0][1]), pack2<BF16>(s[0][2], s[0][3]),
                             pack2<BF16>(s[1][0], s[1][1]), pack2<BF16>(s[1][2], s[1][3])};
     // Where a key is hidden from one row and seen by another, 0 * v must stay 0 for the
@@ -289,7 +329,7 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
       for (int n = 0; n < DP / 16; n++) {
         uint32_t b[4];
         const int v = 2 * n + (lane >> 4);
-        ldm4t(vt + (r * kVec + (v ^ (r & 7))) * 16, b);
+        ldm4t(vt + at(r, v), b);
         if (mixed)
 #pragma unroll
           for (int i = 0; i < 4; i++) b[i] = zero_not_finite<BF16>(b[i], wild);
@@ -305,7 +345,7 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
         for (int n = 0; n < DP / 8; n++) {
           uint32_t w;
           asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w)
-                       : "r"(vt + (r * kVec + (n ^ (r & 7))) * 16 + (lane & 3) * 4));
+                       : "r"(vt + at(r, n) + (lane & 3) * 4));
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const uint16_t x = (uint16_t)(w >> (16 * e));
@@ -316,9 +356,13 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
         }
       }
     }
-    stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+    if (++stage == kStages) stage = 0, parity ^= 1;
   }
-  asm volatile("cp.async.wait_group 0;");
+  if (MODE == kPrompt) asm volatile("cp.async.wait_group 0;");
+  if (late) {  // the copies in flight land before the block's states take their place
+    if (lane == 0) atomicExch(d.timeout, 1);
+    for (int i = 0; i < kStages; i++) mbar_wait(smem_u32(&sh.full[warp][i]), parity);
+  }
 
   // ---- join the warps' states in shared memory
 #pragma unroll
@@ -343,38 +387,42 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
   if (beside) wait_for_previous();
   const bool final = MODE == kPrompt || d.part.parts == 1 || d.joins;
   constexpr int kLanes = DP / 4;  // threads along a row, four columns each
+  const int col = (tid % kLanes) * 4;
   const float *all = reinterpret_cast<const float *>(smem);
+  const int parts = MODE == kOwn && d.joins ? d.first_part : 0;  // of the shared keys
   for (int r = tid / kLanes; r < kRows; r += kThreads / kLanes) {
     if (sh.q[r] < 0) continue;
+    // all loads first: there are few parts, and one after the other costs a microsecond each
+    const float *part = d.part.o + sh.index[r] * dim + col;
+    float2 ml[kMostJoined];
+    float4 u[kMostJoined];
+    if (MODE == kOwn) {
+#pragma unroll
+      for (int i = 0; i < kMostJoined; i++) {
+        ml[i] = make_float2(-INFINITY, 0.0f);
+        u[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i < parts) {
+          ml[i] = d.part.ml[i * d.part.rows + sh.index[r]];
+          if (col < dim) u[i] = *reinterpret_cast<const float4 *>(part + i * d.part.rows * dim);
+        }
+      }
+    }
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; w++) m = fmaxf(m, sh.ml[w][r].x);
-    const float2 *ml = d.part.ml + sh.index[r];
-    if (MODE == kOwn && d.joins)
-      for (int i = 0; i < d.first_part; i++) m = fmaxf(m, ml[i * d.part.rows].x);
+    if (MODE == kOwn)
+#pragma unroll
+      for (int i = 0; i < kMostJoined; i++) m = fmaxf(m, ml[i].x);
     const float z = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const int col = (tid % kLanes) * 4;
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-      const float f = exp2_fast(sh.ml[w][r].x - z);
-      const float4 u = *reinterpret_cast<const float4 *>(all + (w * kRows + r) * DP + col);
-      l += sh.ml[w][r].y * f;
-      v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
-    }
-    if (MODE == kOwn && d.joins && col < dim) {
-      const float *part = d.part.o + sh.index[r] * dim + col;
-#pragma unroll 4
-      for (int i = 0; i < d.first_part; i++) {
-        const float2 s = ml[i * d.part.rows];
-        const float4 u = *reinterpret_cast<const float4 *>(part + i * d.part.rows * dim);
-        if (s.y == 0.0f) continue;  // nothing was written
-        const float f = exp2_fast(s.x - z);
-        l += s.y * f;
-        v.x += u.x * f, v.y += u.y * f, v.z += u.z * f, v.w += u.w * f;
-      }
-    }
+    for (int w = 0; w < kWarps; w++)
+      add_state(l, v, sh.ml[w][r], *reinterpret_cast<const float4 *>(all + (w * kRows + r) * DP + col), z);
+    if (MODE == kOwn)
+#pragma unroll
+      for (int i = 0; i < kMostJoined; i++)
+        if (ml[i].y != 0.0f) add_state(l, v, ml[i], u[i], z);  // else nothing was written
     if (final) {
       float *lse = MODE == kPrompt ? p.lse : d.lse;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -393,19 +441,27 @@ rows_kernel(PromptArgs p, DecodeArgs d, KvView c) {
 }
 
 // ---------------------------------------------------------------------------
-// Join the parts of each row: one block per row, four slices of the parts side by side.
+// Join the parts of each row: one block per row. Bound by the latency of two dependent loads
+// and, with many parts, by their bytes.
 // ---------------------------------------------------------------------------
 
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads) join_kernel(DecodeArgs d, int dim) {
-  __shared__ float top[kWarps], sum[kWarps];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeArgs d, int dim) {
+  constexpr int kWarps = kJoinThreads / 32;
+  __shared__ float top[kWarps], sum[kWarps], factor[kMostParts];
   __shared__ float4 acc[kWarps][64];
-  let_next_start();
-  wait_for_previous();
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = d.part.parts;
+  wait_for_previous();
+  let_next_start();
+  float2 ml[kMostParts / kJoinThreads];
   float m = -INFINITY;
-  for (int i = tid; i < d.part.parts; i += kThreads) m = fmaxf(m, d.part.ml[i * d.part.rows + row].x);
+#pragma unroll
+  for (int k = 0; k < kMostParts / kJoinThreads; k++) {
+    const int i = tid + k * kJoinThreads;
+    ml[k] = i < parts ? d.part.ml[i * d.part.rows + row] : make_float2(-INFINITY, 0.0f);
+    m = fmaxf(m, ml[k].x);
+  }
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
   if (lane == 0) top[warp] = m;
@@ -413,25 +469,34 @@ __global__ void __launch_bounds__(kThreads) join_kernel(DecodeArgs d, int dim) {
   m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   const float z = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kMostParts / kJoinThreads; k++) {
+    // a part that has seen nothing was not written
+    const float f = ml[k].y == 0.0f ? 0.0f : exp2_fast(ml[k].x - z);
+    l += ml[k].y * f;
+    factor[tid + k * kJoinThreads] = f;
+  }
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  if (lane == 0) sum[warp] = l;
+  __syncthreads();
+  l = sum[0] + sum[1] + sum[2] + sum[3];
   float4 v[2] = {};
-  for (int i = warp; i < d.part.parts; i += kWarps) {
-    const float2 ml = d.part.ml[i * d.part.rows + row];
-    if (ml.y == 0.0f) continue;
-    const float f = exp2_fast(ml.x - z);
-    l += ml.y * f;
+  const float *part = d.part.o + row * dim + lane * 4;
+#pragma unroll 4
+  for (int i = warp; i < parts; i += kWarps) {
+    const float f = factor[i];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const int col = (h * 32 + lane) * 4;
-      if (col >= dim) continue;
-      const float4 u = *reinterpret_cast<const float4 *>(d.part.o + (i * d.part.rows + row) * dim + col);
+      float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (f != 0.0f && h * 128 + lane * 4 < dim)
+        u = *reinterpret_cast<const float4 *>(part + i * d.part.rows * dim + h * 128);
       v[h].x += u.x * f, v[h].y += u.y * f, v[h].z += u.z * f, v[h].w += u.w * f;
     }
   }
   acc[warp][lane] = v[0];
   acc[warp][32 + lane] = v[1];
-  if (lane == 0) sum[warp] = l;
   __syncthreads();
-  l = sum[0] + sum[1] + sum[2] + sum[3];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   if (tid < 64 && tid * 4 < dim) {
     float4 s = acc[0][tid];
@@ -451,67 +516,113 @@ __global__ void __launch_bounds__(kThreads) join_kernel(DecodeArgs d, int dim) {
 // launches
 // ---------------------------------------------------------------------------
 
-template <int MODE, int DP, bool BF16>
-int32_t launch_rows(dim3 grid, const PromptArgs &p, const DecodeArgs &d, const KvView &c,
-                    cudaStream_t s) {
-  auto fn = rows_kernel<MODE, DP, BF16>;
+template <int MODE, int DP, int WARPS, bool BF16>
+int32_t launch_rows(dim3 grid, const CUtensorMap *maps, const PromptArgs &p, const DecodeArgs &d,
+                    const KvView &c, cudaStream_t s) {
+  using Cfg = RowsCfg<DP, WARPS>;
+  auto fn = rows_kernel<MODE, DP, WARPS, BF16>;
   static bool set = false;  // per instantiation; setting it twice is harmless
   if (!set) {
-    DM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsCfg<DP>::kSmem),
+    DM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem),
             "attention shared memory");
     set = true;
   }
-  return launch_chained("attention launch", fn, grid, kThreads, RowsCfg<DP>::kSmem, s, p, d, c);
+  return launch_chained("attention launch", fn, grid, Cfg::kThreads, Cfg::kSmem, s, maps[0], maps[1], p, d, c);
 }
 
-template <int MODE>
-int32_t launch_rows(int type, int dim, dim3 grid, const PromptArgs &p, const DecodeArgs &d,
-                    const KvView &c, cudaStream_t s) {
+template <int MODE, int WARPS>
+int32_t launch_rows(int type, int dim, dim3 grid, const CUtensorMap *maps, const PromptArgs &p,
+                    const DecodeArgs &d, const KvView &c, cudaStream_t s) {
   const bool bf = type == DM_BF16;
   if (dim <= 64)
-    return bf ? launch_rows<MODE, 64, true>(grid, p, d, c, s) : launch_rows<MODE, 64, false>(grid, p, d, c, s);
+    return bf ? launch_rows<MODE, 64, WARPS, true>(grid, maps, p, d, c, s)
+              : launch_rows<MODE, 64, WARPS, false>(grid, maps, p, d, c, s);
   if (dim <= 128)
-    return bf ? launch_rows<MODE, 128, true>(grid, p, d, c, s) : launch_rows<MODE, 128, false>(grid, p, d, c, s);
-  return bf ? launch_rows<MODE, 256, true>(grid, p, d, c, s) : launch_rows<MODE, 256, false>(grid, p, d, c, s);
+    return bf ? launch_rows<MODE, 128, WARPS, true>(grid, maps, p, d, c, s)
+              : launch_rows<MODE, 128, WARPS, false>(grid, maps, p, d, c, s);
+  return bf ? launch_rows<MODE, 256, 4, true>(grid, maps, p, d, c, s)
+            : launch_rows<MODE, 256, 4, false>(grid, maps, p, d, c, s);
 }
 
 // How a decode call is cut into parts. The workspace holds one state per part and row.
 struct DecodePlan {
   bool tiles = false;  // the shared part runs on tcgen05 tiles
-  int shared_splits = 0, shared_parts = 0, own_splits = 0;
-  int parts() const { return shared_parts + own_splits; }
+  bool wide = false;   // own keys: eight warps a block
+  bool joins = false;  // the own part joins the shared ones
+  int shared_splits = 0, shared_parts = 0, own_parts = 0;
+  int parts() const { return shared_parts + own_parts; }
 };
 
-constexpr int kTargetBlocks = 296;  // two blocks of four warps on each of 148 SMs
-constexpr int kTileBlocks = 148;    // one block of tiles on each
+constexpr int kSms = 148;
 constexpr int kMinTileRows = 16;
-constexpr int kOneSplitKeys = 1024;
+constexpr int kSplitKeys = 128;  // a block's keys at least, where there are several
+
+// Blocks that cut `items` rows of blocks along `keys`: as many as run at once, no more (a
+// second round costs more than shorter blocks save).
+int splits_of(int64_t items, int keys, int64_t at_once) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(at_once / items, (keys + kSplitKeys - 1) / kSplitKeys));
+}
+
+// Microseconds on one B200, as measured: a block of tiles has 9 besides 1.3 for each step of
+// its units, a block of rows 7 besides 0.9 for each chunk of every warp (beside tiles they get
+// done 0.7 of what they would alone), the join kernel 4 besides 0.45 for each MB of parts.
+constexpr float kTileUs = 9.0f, kTileStepUs = 1.3f, kRowsUs = 7.0f, kRowsStepUs = 0.9f, kBeside = 0.7f,
+                kJoinUs = 4.0f, kJoinMbUs = 0.45f;
 
 DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, int max_length) {
   DecodePlan plan;
   if (batch == 0) return plan;
   const int group = heads / kv_heads;
-  plan.tiles = shared > 0 && batch * group > kMinTileRows && group <= 128;
-  if (plan.tiles) {
+  const bool has_own = max_length > shared || shared == 0;
+  const int own = std::max(1, max_length - shared);
+  const int64_t own_items = (int64_t)batch * kv_heads * ((group + kRows - 1) / kRows);
+  // Blocks of eight warps have an SM to themselves, two of four warps share one: the first
+  // are sooner done, where all of them run at once.
+  plan.wide = dim <= 128 && own_items <= kSms;
+  const int per_sm = plan.wide || dim > 128 ? 1 : 2, warps = plan.wide ? 8 : 4;
+  if (has_own) plan.own_parts = splits_of(own_items, own, kSms * per_sm);
+  plan.tiles = shared > 0 && (int64_t)batch * group > kMinTileRows && group <= 128;
+  if (shared > 0 && !plan.tiles) {
+    const int64_t items = (int64_t)kv_heads * (((int64_t)batch * group + kRows - 1) / kRows);
+    plan.shared_splits = splits_of(items, shared, (dim > 128 ? 1 : 2) * kSms);
+    plan.shared_parts = plan.shared_splits;
+  } else if (plan.tiles) {
+    // More parts: shorter blocks, fewer SMs for the own part beside them, more to join.
     const int units = tile_shared_alternates(dim, group, batch) ? 2 : 1;
     const int tiles = (shared + tile_keys(dim) - 1) / tile_keys(dim);
-    plan.shared_splits = std::max(1, std::min(kTileBlocks / tile_shared_items(dim, kv_heads, group, batch), tiles / units));
-    plan.shared_parts = plan.shared_splits * units;
-  } else if (shared > 0) {
-    const int64_t items = (int64_t)kv_heads * (((int64_t)batch * group + kRows - 1) / kRows);
-    plan.shared_splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>((kTargetBlocks + items - 1) / items, (shared + 255) / 256));
-    plan.shared_parts = plan.shared_splits;
+    const int items = tile_shared_items(dim, kv_heads, group, batch);
+    const int most = std::max(1, std::min(kSms / items, tiles / units));
+    float best = 0.0f;
+    for (int splits = 1, step = 1; splits <= most; splits += step, step = splits / 8 + 1) {
+      DecodePlan at = plan;
+      at.shared_splits = splits;
+      at.shared_parts = splits * units;
+      const int per = (tiles + splits - 1) / splits;
+      float us = kTileUs + kTileStepUs * ((per + units - 1) / units);
+      const int left = kSms - std::min(kSms, items * splits);  // SMs beside the tiles
+      if (has_own) {
+        // own blocks are cut for the SMs that are left, if that leaves enough
+        at.own_parts = splits_of(own_items, own, (int64_t)(left >= kSms / 2 ? left : kSms) * per_sm);
+        const float blocks = (float)own_items * at.own_parts;
+        const float one = kRowsUs + kRowsStepUs * ((own + at.own_parts - 1) / at.own_parts + 16 * warps - 1) / (16 * warps);
+        if (blocks <= left * per_sm) {
+          us = std::max(us, one);
+        } else {  // what the tiles leave time for, then on all SMs
+          const float done = kBeside * left * per_sm * (us / one);
+          us += std::max(0.0f, blocks - done) / (kSms * per_sm) * one;
+          us = std::max(us, one);
+        }
+      }
+      at.joins = has_own && at.own_parts == 1 && at.shared_parts <= kMostJoined;
+      if (!at.joins && at.parts() > 1)
+        us += kJoinUs + kJoinMbUs * at.parts() * ((float)batch * heads * dim * 4e-6f);
+      if (splits == 1 || us < best) {
+        best = us;
+        plan = at;
+      }
+    }
   }
-  if (max_length > shared || shared == 0) {
-    const int64_t items = (int64_t)batch * kv_heads * ((group + kRows - 1) / kRows);
-    const int own = std::max(1, max_length - shared);
-    plan.own_splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>((kTargetBlocks + items - 1) / items, (own + 255) / 256));
-    // One split joins the shared parts itself: no third launch. Up to 1024 keys that is
-    // worth more than more blocks.
-    if (shared > 0 && own <= kOneSplitKeys) plan.own_splits = 1;
-  }
+  plan.joins = plan.shared_parts > 0 && plan.own_parts == 1 && plan.shared_parts <= kMostJoined;
   return plan;
 }
 
@@ -583,11 +694,12 @@ int32_t dm_attention_prompt(dm_cuda_context *ctx, const dm_attention_prompt_desc
   a.causal = in->causal;
   a.window = in->window;
   cudaSetDevice(ctx->device);
-  if (tile_prompt_fits(a)) return launch_tile_prompt(in->type, a, ctx->status, (cudaStream_t)stream);
+  if (tile_prompt_fits(a)) return launch_tile_prompt(in->type, a, ctx->status + kStatusWord, (cudaStream_t)stream);
   const int64_t tiles = in->q_tokens * a.group / kRows + in->sequences;
   if (tiles > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
-  return launch_rows<kPrompt>(in->type, in->head_dim, dim3((unsigned)tiles, in->kv_heads), a,
-                              DecodeArgs{}, KvView{}, (cudaStream_t)stream);
+  const CUtensorMap none[2]{};
+  return launch_rows<kPrompt, 4>(in->type, in->head_dim, dim3((unsigned)tiles, in->kv_heads), none, a,
+                                 DecodeArgs{}, KvView{}, (cudaStream_t)stream);
 }
 
 int32_t dm_attention_decode_workspace(const dm_kv_cache *cache, int32_t heads, int32_t batch,
@@ -647,27 +759,32 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
   a.part.ml = (float2 *)(a.part.o + (int64_t)a.part.parts * a.part.rows * kd.head_dim);
   cudaSetDevice(cache->ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
+  a.timeout = cache->ctx->status + kStatusWord;
+  CUtensorMap maps[2];
+  if ((plan.own_parts || !plan.tiles) && !describe_chunks(kd.type, cache->view, in->layer, kChunk, maps))
+    return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
   if (plan.shared_splits) {
     const int64_t items = (int64_t)kd.kv_heads * (((int64_t)in->batch * a.group + kRows - 1) / kRows);
     a.first_part = 0;
     a.splits = plan.shared_splits;
-    if (int32_t rc = plan.tiles ? launch_tile_shared(kd.type, a, cache->view, cache->ctx->status, s)
-                                : launch_rows<kShared>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
-                                          PromptArgs{}, a, cache->view, s))
+    if (int32_t rc = plan.tiles ? launch_tile_shared(kd.type, a, cache->view, s)
+                                : launch_rows<kShared, 4>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits), maps,
+                                                      PromptArgs{}, a, cache->view, s))
       return rc;
   }
-  if (plan.own_splits) {
+  if (plan.own_parts) {
     const int64_t items = (int64_t)in->batch * kd.kv_heads * ((a.group + kRows - 1) / kRows);
     a.first_part = plan.shared_parts;
-    a.splits = plan.own_splits;
-    a.joins = plan.shared_parts > 0 && plan.own_splits == 1;
-    if (int32_t rc = launch_rows<kOwn>(kd.type, kd.head_dim, dim3((unsigned)items, a.splits),
-                                       PromptArgs{}, a, cache->view, s))
+    a.splits = plan.own_parts;
+    a.joins = plan.joins;
+    const dim3 grid((unsigned)items, a.splits);
+    if (int32_t rc = plan.wide ? launch_rows<kOwn, 8>(kd.type, kd.head_dim, grid, maps, PromptArgs{}, a, cache->view, s)
+                               : launch_rows<kOwn, 4>(kd.type, kd.head_dim, grid, maps, PromptArgs{}, a, cache->view, s))
       return rc;
   }
   if (plan.parts() > 1 && !a.joins)
     return launch_chained("attention join launch", kd.type == DM_BF16 ? join_kernel<true> : join_kernel<false>,
-                          dim3((unsigned)a.part.rows), kThreads, 0, s, a, kd.head_dim);
+                          dim3((unsigned)a.part.rows), kJoinThreads, 0, s, a, kd.head_dim);
   return DM_OK;
 }
 

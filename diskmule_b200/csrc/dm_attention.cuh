@@ -17,6 +17,7 @@
 namespace dma {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kStatusWord = 32;  // of the context's status buffer: a bounded wait ran out
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct PromptArgs {
@@ -51,6 +52,7 @@ struct DecodeArgs {
   int32_t first_part;  // of this launch
   int32_t splits;      // parts of this launch
   int32_t joins;       // own part: this launch joins the parts before its own
+  int32_t *timeout;    // set when a bounded wait runs out
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {

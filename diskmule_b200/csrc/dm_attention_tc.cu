@@ -42,7 +42,6 @@ using namespace dm::tc;
 namespace {
 
 constexpr int kUnitRows = 128;
-constexpr int kStatusWord = 32;  // of the context's status buffer: a bounded wait ran out
 constexpr int kItems = 4;        // items between the first role and the last
 constexpr int kMostSlots = 5;
 
@@ -102,14 +101,6 @@ struct TcSmem {
   volatile int abort;
 };
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1,
-                                            int c2, int c3, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3, %4, %5}], [%6];" ::"r"(dst),
-      "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
-      : "memory");
-}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -890,6 +881,14 @@ bool encode_q(CUtensorMap *map, bool bf16, const void *q, const int64_t *stride,
   return encode(map, bf16, q, 4, dims, strides, box);
 }
 
+// K (which 0) or V (1) of a cache layer as {dim, token of a page, key/value head, page}
+bool encode_cache(CUtensorMap *map, bool bf16, const KvView &c, int layer, int which, int rows) {
+  const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_tokens, (uint64_t)c.kv_heads, (uint64_t)c.pages};
+  const int64_t strides[3] = {c.head_dim * 2, c.head_bytes, c.page_bytes};
+  const uint32_t box[4] = {64, (uint32_t)rows, 1, 1};
+  return encode(map, bf16, c.memory + layer * c.layer_bytes + which * c.kv_heads * c.head_bytes, 4, dims, strides, box);
+}
+
 template <int MODE, int DP, bool BF16>
 int32_t launch(dim3 grid, const CUtensorMap *maps, const TcArgs &a, cudaStream_t s) {
   auto fn = tile_kernel<MODE, DP, BF16>;
@@ -930,11 +929,11 @@ bool tile_prompt_fits(const PromptArgs &p) {
   return p.k_tokens > 0;
 }
 
-int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *status, cudaStream_t stream) {
+int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *timeout, cudaStream_t stream) {
   TcArgs a{};
   a.p = p;
   a.tokens = kUnitRows / p.group;
-  a.timeout = status + kStatusWord;
+  a.timeout = timeout;
   const int64_t tiles = p.q_tokens / (units_of(p.dim) * a.tokens) + p.sequences;
   if (tiles * p.kv_heads > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
   a.tiles = (int)tiles;
@@ -954,6 +953,11 @@ bool tile_shared_alternates(int dim, int group, int batch) {
   return units_of(dim) == 2 && batch <= kUnitRows / group;
 }
 
+bool describe_chunks(int32_t type, const KvView &c, int layer, int rows, CUtensorMap *maps) {
+  return encode_cache(&maps[0], type == DM_BF16, c, layer, 0, rows) &&
+         encode_cache(&maps[1], type == DM_BF16, c, layer, 1, rows);
+}
+
 int tile_keys(int dim) { return keys_of(dim); }
 
 int tile_shared_items(int dim, int kv_heads, int group, int batch) {
@@ -962,27 +966,22 @@ int tile_shared_items(int dim, int kv_heads, int group, int batch) {
   return kv_heads * ((batch + per - 1) / per);
 }
 
-int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, int32_t *status,
-                           cudaStream_t stream) {
+int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, cudaStream_t stream) {
   TcArgs a{};
   a.d = d;
   a.c = c;
   a.tokens = kUnitRows / d.group;
   a.alternate = tile_shared_alternates(c.head_dim, d.group, d.batch);
-  a.timeout = status + kStatusWord;
+  a.timeout = d.timeout;
   a.wide = d.part.parts > 1 ? ((uintptr_t)d.part.o & 31) == 0 : aligned32(d.out, d.out_stride);
   const bool bf16 = type == DM_BF16;
   CUtensorMap maps[3];
-  const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_tokens, (uint64_t)c.kv_heads, (uint64_t)c.pages};
-  const int64_t strides[3] = {c.head_dim * 2, c.head_bytes, c.page_bytes};
   // a box lies in one page and divides a chunk: pages are powers of two from 16
   auto rows = [&](int keys) { return std::min(c.page_tokens, keys & -keys); };
   a.k_box = rows(keys_of(c.head_dim));
   a.v_box = rows(v_keys_of(c.head_dim));
-  const uint32_t k_box[4] = {64, (uint32_t)a.k_box, 1, 1}, v_box[4] = {64, (uint32_t)a.v_box, 1, 1};
-  const uint8_t *k = c.memory + d.layer * c.layer_bytes, *v = k + c.kv_heads * c.head_bytes;
   if (!encode_q(&maps[0], bf16, d.q, d.q_stride, c.head_dim, d.group, c.kv_heads, d.batch, a.tokens) ||
-      !encode(&maps[1], bf16, k, 4, dims, strides, k_box) || !encode(&maps[2], bf16, v, 4, dims, strides, v_box))
+      !encode_cache(&maps[1], bf16, c, d.layer, 0, a.k_box) || !encode_cache(&maps[2], bf16, c, d.layer, 1, a.v_box))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
   const int items = tile_shared_items(c.head_dim, c.kv_heads, d.group, d.batch);
   return launch<kTcShared>(bf16, c.head_dim, dim3((unsigned)items, (unsigned)d.splits), maps, a, stream);
