@@ -16,12 +16,11 @@ from ._native import check
 from .moe import CudaContext
 
 
-def _stream(stream: int):
-    return C.c_void_p(stream) if stream else None
+_CONTIGUOUS = (C.c_int64 * 2)()
 
 
 def _strides(pair):
-    return (C.c_int64 * 2)(*pair) if pair is not None else (C.c_int64 * 2)()
+    return _CONTIGUOUS if pair is None else (C.c_int64 * 2)(*pair)
 
 
 def prompt_attention(ctx: CudaContext, *, type: int, heads: int, kv_heads: int, head_dim: int,
@@ -35,12 +34,12 @@ def prompt_attention(ctx: CudaContext, *, type: int, heads: int, kv_heads: int, 
                      q_tokens, k_tokens, q, k, v, out, lse or None, _strides(q_stride),
                      _strides(k_stride), _strides(v_stride), _strides(out_stride), q_offsets,
                      k_offsets or None)
-    check(N.lib().dm_attention_prompt(ctx.handle, C.byref(d), _stream(stream)))
+    check(N.lib().dm_attention_prompt(ctx.handle, C.byref(d), stream or None))
 
 
 def attention_status(ctx: CudaContext, stream: int = 0):
     """Wait for `stream`; raises if a bounded wait inside an attention kernel ran out."""
-    check(N.lib().dm_attention_status(ctx.handle, _stream(stream)))
+    check(N.lib().dm_attention_status(ctx.handle, stream or None))
 
 
 class KvCache:
@@ -53,6 +52,7 @@ class KvCache:
                  memory: int = 0, page_table: int = 0, lengths: int = 0, references: int = 0):
         self._h = None
         self._ctx = ctx
+        self._lib = N.lib()
         d = N.KvCacheDesc(type, layers, kv_heads, head_dim, page_tokens, pages, max_sequences,
                           max_pages, memory or None, page_table or None, lengths or None,
                           references or None)
@@ -66,43 +66,43 @@ class KvCache:
 
     def describe(self) -> N.KvCacheDesc:
         d = N.KvCacheDesc()
-        check(N.lib().dm_kv_cache_describe(self._h, C.byref(d)))
+        check(self._lib.dm_kv_cache_describe(self._h, C.byref(d)))
         return d
 
     def status(self, stream: int = 0) -> int:
         """Wait for `stream`; the KV_* bits since the last call."""
         bits = C.c_int32(0)
-        check(N.lib().dm_kv_cache_status(self._h, C.byref(bits), _stream(stream)))
+        check(self._lib.dm_kv_cache_status(self._h, C.byref(bits), stream or None))
         return bits.value
 
     def extend(self, sequences: int, counts: int, n: int, stream: int = 0):
-        check(N.lib().dm_kv_cache_extend(self._h, sequences, counts, n, _stream(stream)))
+        check(self._lib.dm_kv_cache_extend(self._h, sequences, counts, n, stream or None))
 
     def write(self, layer: int, k: int, v: int, sequences: int, offsets: int, n: int, tokens: int,
               k_stride=None, v_stride=None, stream: int = 0):
-        check(N.lib().dm_kv_cache_write(
+        check(self._lib.dm_kv_cache_write(
             self._h, layer, k, v, None if k_stride is None else _strides(k_stride),
             None if v_stride is None else _strides(v_stride), sequences, offsets, n, tokens,
-            _stream(stream)))
+            stream or None))
 
     def fork(self, parents: int, children: int, n: int, stream: int = 0):
-        check(N.lib().dm_kv_cache_fork(self._h, parents, children, n, _stream(stream)))
+        check(self._lib.dm_kv_cache_fork(self._h, parents, children, n, stream or None))
 
     def compact(self, sequences: int, keep_offsets: int, keep: int, n: int, kept: int,
                 stream: int = 0):
-        check(N.lib().dm_kv_cache_compact(self._h, sequences, keep_offsets, keep, n, kept,
-                                          _stream(stream)))
+        check(self._lib.dm_kv_cache_compact(self._h, sequences, keep_offsets, keep, n, kept,
+                                          stream or None))
 
     def free(self, sequences: int, n: int, stream: int = 0):
-        check(N.lib().dm_kv_cache_free(self._h, sequences, n, _stream(stream)))
+        check(self._lib.dm_kv_cache_free(self._h, sequences, n, stream or None))
 
     def copy_pages(self, source: int, target: int, n: int, stream: int = 0):
-        check(N.lib().dm_kv_cache_copy_pages(self._h, source, target, n, _stream(stream)))
+        check(self._lib.dm_kv_cache_copy_pages(self._h, source, target, n, stream or None))
 
     def decode_workspace(self, heads: int, batch: int, shared_tokens: int, max_length: int) -> int:
         """Bytes of workspace that decode_attention needs for these numbers."""
         n = C.c_uint64(0)
-        check(N.lib().dm_attention_decode_workspace(self._h, heads, batch, shared_tokens,
+        check(self._lib.dm_attention_decode_workspace(self._h, heads, batch, shared_tokens,
                                                     max_length, C.byref(n)))
         return n.value
 
@@ -114,11 +114,11 @@ class KvCache:
         d = N.DecodeDesc(layer, heads, batch, window, shared_tokens, max_length, scale, q, out,
                          lse or None, _strides(q_stride), _strides(out_stride), sequences or None,
                          workspace or None, workspace_bytes)
-        check(N.lib().dm_attention_decode(self._h, C.byref(d), _stream(stream)))
+        check(self._lib.dm_attention_decode(self._h, C.byref(d), stream or None))
 
     def close(self):
         if self._h:
-            N.lib().dm_kv_cache_destroy(self._h)
+            self._lib.dm_kv_cache_destroy(self._h)
             self._h = None
 
     def __del__(self):

@@ -92,12 +92,21 @@ int32_t dm_cuda_create(int32_t device_ordinal, dm_cuda_context **out) {
   auto *ctx = new (std::nothrow) dm_cuda_context();
   if (!ctx) return fail(DM_ERR_ALLOCATION, "host allocation failed");
   ctx->device = device_ordinal;
-  cudaDeviceProp prop;
-  if (cudaGetDeviceProperties(&prop, device_ordinal) == cudaSuccess)
-    snprintf(ctx->name, sizeof ctx->name, "%s", prop.name);
+  // the properties of a device take a millisecond to read: once per device
+  static std::mutex names_mutex;
+  static char names[64][sizeof ctx->name];
+  {
+    std::lock_guard<std::mutex> lock(names_mutex);
+    char *name = device_ordinal < 64 ? names[device_ordinal] : ctx->name;
+    cudaDeviceProp prop;
+    if (!name[0] && cudaGetDeviceProperties(&prop, device_ordinal) == cudaSuccess)
+      snprintf(name, sizeof ctx->name, "%s", prop.name);
+    if (name != ctx->name) memcpy(ctx->name, name, sizeof ctx->name);
+  }
   cudaError_t err = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
   if (err == cudaSuccess) err = cudaMalloc(&ctx->status, 256);
-  if (err == cudaSuccess) err = cudaMemset(ctx->status, 0, 256);
+  if (err == cudaSuccess) err = cudaMemsetAsync(ctx->status, 0, 256, ctx->stream);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(ctx->stream);
   if (err != cudaSuccess) {
     delete ctx;
     return cuda_fail(err, "context set-up");

@@ -516,3 +516,107 @@ def test_decode_refusals(ctx):
     assert status(scale=-1.0) == N.ERR_POSITIVE_PARAMETER
     assert status(q_stride=(60, 64)) == N.ERR_INVALID_ARGUMENT
     pool.cache.decode_attention(**{**good, "batch": 0})
+
+
+def test_prompt_broadcast_heads(ctx):
+    """Keys and values that all heads share as one row (stride 0): no tensor map describes
+    that, so these run on the 16-row kernel."""
+    gen = generator(31)
+    q = normal(gen, (70, 6, 64), torch.float16, 2.0)
+    k1, v1 = (normal(gen, (70, 1, 64), torch.float16) for _ in range(2))
+    k, v = k1.expand(70, 3, 64), v1.expand(70, 3, 64)
+    out, lse = run_prompt(ctx, q, k, v, [40, 30], [40, 30], k_stride=(64, 0), v_stride=(64, 0))
+    check_prompt(q, k, v, [40, 30], [40, 30], out, lse, tokens=16)
+    for causal, window in ((False, 0), (True, 9)):
+        out, lse = run_prompt(ctx, q, k, v, [40, 30], [40, 30], causal, window, k_stride=(64, 0), v_stride=(64, 0))
+        check_prompt(q, k, v, [40, 30], [40, 30], out, lse, causal, window, tokens=16)
+    k1[20], v1[33] = float("nan"), float("inf")
+    bad, _ = run_prompt(ctx, q, k, v, [40, 30], [40, 30], k_stride=(64, 0), v_stride=(64, 0))
+    good, _ = run_prompt(ctx, q, k1.nan_to_num(0, 0, 0).expand(70, 3, 64), v1.nan_to_num(0, 0, 0).expand(70, 3, 64),
+                         [40, 30], [40, 30], k_stride=(64, 0), v_stride=(64, 0))
+    assert torch.equal(bad[:20], good[:20]) and torch.equal(bad[40:], good[40:])
+
+
+def test_prompt_without_any_keys(ctx):
+    q = normal(generator(33), (5, 2, 128), torch.bfloat16)
+    k = torch.zeros(0, 2, 128, dtype=torch.bfloat16, device="cuda")
+    out, lse = run_prompt(ctx, q, k, k, [2, 3], [0, 0], k_stride=(0, 0), v_stride=(0, 0))
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_prompt_rows_beyond_32_bits(ctx, dim):
+    """Rows that lie more than 2^31 elements into their tensors."""
+    n, stride = 300, 1 << 23
+    big = torch.empty((n - 1) * stride + 2 * dim, dtype=torch.bfloat16, device="cuda")
+    q, k, v = (big.as_strided((n, 1, dim), (stride, dim, 1)) for _ in range(3))
+    gen = generator(37)
+    q.copy_(normal(gen, (n, 1, dim), torch.bfloat16))
+    out = big.as_strided((n, 1, dim), (stride, dim, 1), dim)
+    assert (n - 1) * stride > 2 ** 31
+    out, lse = run_prompt(ctx, q, k, v, [n], [n], out=out, q_stride=(stride, dim), k_stride=(stride, dim),
+                          v_stride=(stride, dim), out_stride=(stride, dim))
+    check_prompt(q, k, v, [n], [n], out, lse, tokens=20)
+
+
+def test_prompts_back_to_back_on_one_stream(ctx):
+    """A call may be scheduled before the one in front of it has ended: it must still read what
+    that one writes."""
+    gen = generator(41)
+    n = 700
+    x = normal(gen, (n, 2, 64), torch.bfloat16)
+    o = ints([0, n])
+
+    def attend(q, out):
+        prompt_attention(ctx, type=N.BF16, heads=2, kv_heads=2, head_dim=64, q=q.data_ptr(), k=q.data_ptr(),
+                         v=q.data_ptr(), out=out.data_ptr(), q_tokens=n, k_tokens=n, sequences=1,
+                         q_offsets=o.data_ptr())
+    bufs = [x] + [torch.zeros_like(x) for _ in range(20)]
+    for _ in range(5):
+        for a, b in zip(bufs, bufs[1:]):
+            attend(a, b)
+    torch.cuda.synchronize()
+    want = x
+    for b in bufs[1:]:
+        out = torch.zeros_like(x)
+        attend(want, out)
+        torch.cuda.synchronize()
+        assert torch.equal(out, b)
+        want = out
+
+
+def test_decode_right_after_its_cache_calls(ctx):
+    """extend, write, fork and decode queued without a wait in between, against the same calls
+    with one after each."""
+    def play(wait):
+        cache = KvCache(ctx, type=N.BF16, layers=1, kv_heads=2, head_dim=64, page_tokens=16, pages=400,
+                        max_sequences=9, max_pages=40)
+        gen = generator(43)
+        k, v = (normal(gen, (500, 2, 64), torch.bfloat16) for _ in range(2))
+        rows, count, off = ints([0]), ints([500]), ints([0, 500])
+        kids, parents, ones, koff = ints(range(1, 9)), ints([0] * 8), ints([1] * 8), ints(range(9))
+        q = normal(gen, (8, 8, 64), torch.bfloat16, 2.0)
+        out = torch.zeros_like(q)
+        size = cache.decode_workspace(8, 8, 496, 520)
+        work = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+        calls = [lambda: cache.extend(rows.data_ptr(), count.data_ptr(), 1),
+                 lambda: cache.write(0, k.data_ptr(), v.data_ptr(), rows.data_ptr(), off.data_ptr(), 1, 500),
+                 lambda: cache.fork(parents.data_ptr(), kids.data_ptr(), 8)]
+        for _ in range(10):
+            calls += [lambda: cache.extend(kids.data_ptr(), ones.data_ptr(), 8),
+                      lambda: cache.write(0, k.data_ptr(), v.data_ptr(), kids.data_ptr(), koff.data_ptr(), 8, 8),
+                      lambda: cache.decode_attention(layer=0, heads=8, q=q.data_ptr(), out=out.data_ptr(), batch=8,
+                                                     max_length=520, shared_tokens=496, sequences=kids.data_ptr(),
+                                                     workspace=work.data_ptr(), workspace_bytes=size)]
+        torch.cuda.synchronize()
+        for c in calls:
+            c()
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        assert cache.status() == 0
+        cache.close()
+        return out
+    want = play(True)
+    for _ in range(3):
+        assert torch.equal(play(False), want)
