@@ -563,11 +563,12 @@ int splits_of(int64_t items, int keys, int64_t at_once) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(at_once / items, (keys + kSplitKeys - 1) / kSplitKeys));
 }
 
-// Microseconds on one B200, as measured: a block of tiles has 9 besides 1.3 for each step of
-// its units, a block of rows 7 besides 0.9 for each chunk of every warp (beside tiles they get
-// done 0.7 of what they would alone), the join kernel 4 besides 0.45 for each MB of parts.
-constexpr float kTileUs = 9.0f, kTileStepUs = 1.3f, kRowsUs = 7.0f, kRowsStepUs = 0.9f, kBeside = 0.7f,
-                kJoinUs = 4.0f, kJoinMbUs = 0.45f;
+// Microseconds on one B200, as measured: a block of tiles has 9 besides 1.2 for each step of
+// its units (dim above 128: 2.6); a block of rows 7 besides 0.9 (1.2) for each chunk of every
+// warp, and beside tiles they get done 0.7 of what they would alone; a join in place 2; the
+// join kernel 4 besides 0.4 for each MB of parts.
+constexpr float kTileUs = 9.0f, kTileStepUs = 1.2f, kTileStepWideUs = 2.6f, kRowsUs = 7.0f, kRowsStepUs = 0.9f,
+                kRowsStepWideUs = 1.2f, kBeside = 0.7f, kInPlaceUs = 2.0f, kJoinUs = 4.0f, kJoinMbUs = 0.4f;
 
 DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, int max_length) {
   DecodePlan plan;
@@ -598,23 +599,26 @@ DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, 
       at.shared_splits = splits;
       at.shared_parts = splits * units;
       const int per = (tiles + splits - 1) / splits;
-      float us = kTileUs + kTileStepUs * ((per + units - 1) / units);
+      float us = kTileUs + (dim > 128 ? kTileStepWideUs : kTileStepUs) * ((per + units - 1) / units);
       const int left = kSms - std::min(kSms, items * splits);  // SMs beside the tiles
       if (has_own) {
         // own blocks are cut for the SMs that are left, if that leaves enough
         at.own_parts = splits_of(own_items, own, (int64_t)(left >= kSms / 2 ? left : kSms) * per_sm);
         const float blocks = (float)own_items * at.own_parts;
-        const float one = kRowsUs + kRowsStepUs * ((own + at.own_parts - 1) / at.own_parts + 16 * warps - 1) / (16 * warps);
+        const float one = kRowsUs + (dim > 128 ? kRowsStepWideUs : kRowsStepUs) * ((own + at.own_parts - 1) / at.own_parts + 16 * warps - 1) / (16 * warps);
+        at.joins = at.own_parts == 1 && at.shared_parts <= kMostJoined;
         if (blocks <= left * per_sm) {
           us = std::max(us, one);
-        } else {  // what the tiles leave time for, then on all SMs
-          const float done = kBeside * left * per_sm * (us / one);
+        } else {  // what the tiles leave time for, then on all SMs; blocks that join wait for them
+          float done = kBeside * left * per_sm * (us / one);
+          if (at.joins) done = std::min(done, (float)left * per_sm);
           us += std::max(0.0f, blocks - done) / (kSms * per_sm) * one;
           us = std::max(us, one);
         }
       }
-      at.joins = has_own && at.own_parts == 1 && at.shared_parts <= kMostJoined;
-      if (!at.joins && at.parts() > 1)
+      if (at.joins)
+        us += kInPlaceUs;
+      else if (at.parts() > 1)
         us += kJoinUs + kJoinMbUs * at.parts() * ((float)batch * heads * dim * 4e-6f);
       if (splits == 1 || us < best) {
         best = us;

@@ -44,6 +44,7 @@ namespace {
 constexpr int kUnitRows = 128;
 constexpr int kItems = 4;        // items between the first role and the last
 constexpr int kMostSlots = 5;
+constexpr int kWantTiles = 6;    // tiles left to load when the next item is chosen; at least 1
 
 template <int DP>
 struct TcCfg {
@@ -90,7 +91,7 @@ struct Item {
 
 struct TcSmem {
   uint64_t item_full[kItems], item_empty[kItems], next_block;
-  uint64_t want;  // the keys of an item have been asked for: time for the next item
+  uint64_t want;  // the item's last tiles are being loaded: time for the next item
   uint64_t q_full, q_empty, s_full[2], s_free[2], p_full[2], pv_done[2];
   // chunks: loaded; fit to use (V, by the scrub warp); all products done
   uint64_t k_full[kMostSlots], k_empty[kMostSlots];
@@ -299,32 +300,33 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   const int kv_head = w.kv_head, k0 = w.k0, table_row = w.table_row;
   int key = w.first;
   for (int t = 0; t < tiles; t++, key += Cfg::kKeys) {
+    // No sooner than it is needed: blocks that have not started are for whoever is done first.
+    if (!V && t == max(0, tiles - kWantTiles) && lead) mbar_arrive(smem_u32(&sh.want));
 #pragma unroll 1
     for (int c = 0; c < Cfg::kChunks; c++, place.next()) {
       const int from = V ? key + c * kRows : key, x0 = V ? 0 : c * kSlabs * 64;
       const uint32_t bar = smem_u32(V ? &sh.v_full[place.slot] : &sh.k_full[place.slot]);
       const uint32_t dst = ring + place.slot * Cfg::kChunkBytes;
+      // shared: the boxes of the chunk's pages, each in kSlabs slabs; one lane for each
       int page = 0, boxes = 1, box = kRows;
-      if (MODE == kTcShared) {  // pages of the chunk: one lane each
+      const int slab = lane % kSlabs, mine = lane / kSlabs;
+      if (MODE == kTcShared) {
         box = V ? a.v_box : a.k_box;
         boxes = max(0, min(kRows, a.d.shared - from)) / box;
-        if (lane < boxes) {
-          const int p = a.c.table[(int64_t)table_row * a.c.max_pages + (from + lane * box) / a.c.page_tokens];
+        if (mine < boxes) {
+          const int p = a.c.table[(int64_t)table_row * a.c.max_pages + (from + mine * box) / a.c.page_tokens];
           page = (unsigned)p < (unsigned)a.c.pages ? p : a.c.pages;  // behind the map: zeros
         }
       }
       if (place.round > 0 && !wait(sh, V ? sh.v_empty[place.slot] : sh.k_empty[place.slot], place.parity() ^ 1))
         return false;
       if (lead) mbar_expect_tx(bar, kSlabs * boxes * box * 128);
+      __syncwarp();
       if (MODE == kTcPrompt) {
-        if (lead)
-          for (int s = 0; s < kSlabs; s++) tma_load_3d(dst + s * kRows * 128, map, x0 + s * 64, kv_head, k0 + from, bar);
-      } else {
-        __syncwarp();
-        if (lane < boxes)
-          for (int s = 0; s < kSlabs; s++)
-            tma_load_4d(dst + s * kRows * 128 + lane * box * 128, map, x0 + s * 64,
-                        (from + lane * box) % a.c.page_tokens, kv_head, page, bar);
+        if (lane < kSlabs) tma_load_3d(dst + slab * kRows * 128, map, x0 + slab * 64, kv_head, k0 + from, bar);
+      } else if (mine < boxes) {
+        tma_load_4d(dst + slab * kRows * 128 + mine * box * 128, map, x0 + slab * 64,
+                    (from + mine * box) % a.c.page_tokens, kv_head, page, bar);
       }
       __syncwarp();
     }
@@ -459,8 +461,6 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (w.stop) break;
       }
       if (MODE == kTcPrompt) {
-        // No sooner than it is needed: blocks that have not started are for whoever is done
-        // first. (The loads are a few tiles ahead of the products.)
         if (w.stop == 0 && !(ok = wait(sh, sh.want, (items - 1) & 1))) break;
         if (lane == 0) {
           fence_async_smem();  // the last answer has been read
@@ -504,7 +504,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             q_uses++;
           }
           ok = load_tiles<MODE, DP, false>(sh, w, tiles, a, &k_map, k_ring, lead, place);
-          if (ok && lead) mbar_arrive(smem_u32(&sh.want));
+          if (tiles == 0 && lead) mbar_arrive(smem_u32(&sh.want));
         } else if (warp == Cfg::kVWarp) {
           // ---- values
           ok = load_tiles<MODE, DP, true>(sh, w, tiles, a, &v_map, v_ring, lead, place);
@@ -678,6 +678,9 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         const int buffer = Cfg::kBuffers == 2 ? number & 1 : unit;
         if (!(ok = wait(sh, sh.s_full[buffer], (Cfg::kBuffers == 2 ? number >> 1 : number) & 1))) break;
         fence_after();
+        // Two units whose exponentials run at the same time share the exponential unit and both
+        // leave it idle afterwards; half a tile apart they do not. (Packed prompts: 4%.)
+        if (kUnits == 2 && unit == 1 && i == 0 && n > 1) __nanosleep(300);
         const uint32_t s_at = tmem + lanes + buffer * Cfg::kUnitCols;
         const int key = w.first + tile_of(unit, i) * kKeys;
         float x[kKeys];
