@@ -13,8 +13,9 @@
 // The threads of a unit should never wait for products. So S of the next tile is computed
 // while the weights of this one are: P has columns of its own beside S, and tensor memory
 // (512 columns) sets the tile's keys. dim 64: 2 units of S 128 + P 64 + O 64. dim 128: 2 of
-// S 80 + P 40 + O 128. dim 256, where O takes 256: one unit with two S of 128, each turned
-// into P in place. Both units read the same K and V tiles.
+// S 80 + P 40 + O 128. dim 256: one of S 128 + two P of 64 + O 256 (the threads of a single
+// unit are not to wait for its product either; with P in the place of two S in turn 8192 x
+// 9472 tokens took 10% longer). Both units read the same K and V tiles.
 //
 // A block works through several items (prompt: 256 or 128 query rows; it takes over blocks
 // that have not started yet), so that loads, first products and output of different items
@@ -49,7 +50,6 @@ constexpr int kWantTiles = 6;    // tiles left to load when the next item is cho
 template <int DP>
 struct TcCfg {
   static constexpr int kUnits = DP == 256 ? 1 : 2;
-  static constexpr int kBuffers = DP == 256 ? 2 : 1;         // S buffers of a unit
   static constexpr int kKeys = DP == 128 ? 80 : 128;         // of a tile
   // warps
   static constexpr int kSoftWarps = 4 * kUnits;
@@ -71,8 +71,8 @@ struct TcCfg {
   static constexpr int kQBytes = kUnitRows * DP * 2;
   static constexpr int kSmem = 1024 + kUnits * kQBytes + 2 * kSlots * kChunkBytes;
   // columns of tensor memory
-  static constexpr int kUnitCols = DP == 64 ? 192 : 128;     // from unit to unit (buffer to buffer)
-  static constexpr int kPCol = DP == 256 ? 0 : kKeys;        // P from S; 0: in its place
+  static constexpr int kUnitCols = DP == 64 ? 192 : 128;     // S from unit to unit
+  static constexpr int kPCol = kKeys;                        // P from S
   static constexpr int kOCol = DP == 64 ? 384 : 256;
   // Registers: the launch's share (128 or 168 a thread) split anew, so that a row's scores and
   // the weights made from them stay in registers: 256 x 192 + 256 x 64 = 512 x 128, and
@@ -92,7 +92,8 @@ struct Item {
 struct TcSmem {
   uint64_t item_full[kItems], item_empty[kItems], next_block;
   uint64_t want;  // the item's last tiles are being loaded: time for the next item
-  uint64_t q_full, q_empty, s_full[2], s_free[2], p_full[2], pv_done[2];
+  uint64_t q_full, q_empty, s_full[2], s_free[2];  // S by unit
+  uint64_t p_full[2], pv_done[2];                  // weights: by unit, or the two of one unit
   // chunks: loaded; fit to use (V, by the scrub warp); all products done
   uint64_t k_full[kMostSlots], k_empty[kMostSlots];
   uint64_t v_full[kMostSlots], v_clean[kMostSlots], v_empty[kMostSlots], drain[4];
@@ -350,6 +351,9 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
   const int per_unit = a.tokens * group;  // rows in use of a unit's 128
   const int alternate = MODE == kTcShared && a.alternate;
   const int split = MODE == kTcShared ? blockIdx.y : 0;
+  // P of a unit's product `number`: which, and how often it has been used before
+  auto p_of = [&](int u, int number) -> int { return kUnits == 2 ? u : number & 1; };
+  auto p_round = [&](int number) -> int { return kUnits == 2 ? number : number >> 1; };
   auto tile_of = [&](int u, int i) -> int { return alternate ? 2 * i + u : i; };
   // whether tile t of an item is one of the n of unit u
   auto is_mine = [&](int u, int t, int n) -> bool { return alternate ? (t & 1) == u : t < n; };
@@ -560,8 +564,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           if (tiles > 0 && n == 0 && lead) mbar_arrive(smem_u32(&sh.q_empty));
           for (int t = 0, left = n; t < tiles && ok; t++) {
             const bool mine = is_mine(unit, t, n);
-            const int buffer = Cfg::kBuffers == 2 ? number & 1 : unit;
-            if (Cfg::kPCol && mine && number > 0 && !(ok = wait(sh, sh.s_free[unit], (number - 1) & 1)))
+            if (mine && number > 0 && !(ok = wait(sh, sh.s_free[unit], (number - 1) & 1)))
               break;  // S has been read
 #pragma unroll
             for (int c = 0; c < kChunks; c++, place.next()) {
@@ -575,17 +578,14 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
               const uint64_t kd = sw128_desc(k_ring + place.slot * Cfg::kChunkBytes);
 #pragma unroll
               for (int k = 0; k < 4 * Cfg::kKSlabs; k++)
-                mma_ss_if(lead, columns + buffer * Cfg::kUnitCols,
+                mma_ss_if(lead, columns + unit * Cfg::kUnitCols,
                           qd + ((c * Cfg::kKSlabs + k / 4) * kQSlab >> 4) + (k % 4) * 2,
                           kd + ((k / 4) * kKSlab >> 4) + (k % 4) * 2, kQk, c > 0 || k > 0);
-              if (c == kChunks - 1) commit_if(lead, smem_u32(&sh.s_full[buffer]));
+              if (c == kChunks - 1) commit_if(lead, smem_u32(&sh.s_full[unit]));
               commit_if(lead, empty);
             }
             if (!mine || !ok) continue;
             if (--left == 0) commit_if(lead, smem_u32(&sh.q_empty));  // the queries have been read
-            // Where weights take the place of S, the next S goes to where those of the tile before
-            // are: their product has to be done. (Waited for here, where this tile's cannot be.)
-            if (!Cfg::kPCol && number > 0) ok = wait(sh, sh.pv_done[unit], (number - 1) & 1);
             number++;
           }
         } else {
@@ -596,10 +596,9 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           const uint32_t d = columns + Cfg::kOCol + unit * DP;
           for (int t = 0, own = 0; t < tiles && ok; t++) {
             const bool mine = is_mine(unit, t, n);
-            const int buffer = Cfg::kBuffers == 2 ? number & 1 : unit;
-            const uint32_t p = columns + buffer * Cfg::kUnitCols + Cfg::kPCol;
-            if (mine && !(ok = wait(sh, sh.p_full[buffer], (Cfg::kBuffers == 2 ? number >> 1 : number) & 1)))
-              break;
+            const int which = p_of(unit, number);
+            const uint32_t p = columns + unit * Cfg::kUnitCols + Cfg::kPCol + (which - unit) * kKeys / 2;
+            if (mine && !(ok = wait(sh, sh.p_full[which], p_round(number) & 1))) break;
 #pragma unroll
             for (int c = 0; c < kChunks; c++, place.next()) {
               if (!(ok = wait(sh, sh.v_clean[place.slot], place.parity()))) break;
@@ -614,7 +613,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
               for (int k = 0; k < Cfg::kVKeys / 16; k++)
                 mma_ts_if(lead, d, p + (c * Cfg::kVKeys / 16 + k) * 8, vd + k * (2048 >> 4), kPv,
                           own > 0 || c > 0 || k > 0);
-              if (c == kChunks - 1) commit_if(lead, smem_u32(&sh.pv_done[unit]));
+              if (c == kChunks - 1) commit_if(lead, smem_u32(&sh.pv_done[which]));
               commit_if(lead, empty);
             }
             if (mine) number++, own++;
@@ -675,23 +674,17 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
       float m = -INFINITY, l = 0.0f;  // m in units of the raw score
       for (int i = 0; i < n; i++, number++) {
-        const int buffer = Cfg::kBuffers == 2 ? number & 1 : unit;
-        if (!(ok = wait(sh, sh.s_full[buffer], (Cfg::kBuffers == 2 ? number >> 1 : number) & 1))) break;
+        if (!(ok = wait(sh, sh.s_full[unit], number & 1))) break;
         fence_after();
-        // Two units whose exponentials run at the same time share the exponential unit and both
-        // leave it idle afterwards; half a tile apart they do not. (Packed prompts: 4%.)
-        if (kUnits == 2 && unit == 1 && i == 0 && n > 1) __nanosleep(300);
-        const uint32_t s_at = tmem + lanes + buffer * Cfg::kUnitCols;
+        const uint32_t s_at = tmem + lanes + unit * Cfg::kUnitCols;
         const int key = w.first + tile_of(unit, i) * kKeys;
         float x[kKeys];
 #pragma unroll
         for (int j = 0; j + 32 <= kKeys; j += 32) tmem_ld32(s_at + j, x + j);
         if (kKeys % 32) tmem_ld16(s_at + kKeys / 32 * 32, reinterpret_cast<uint32_t *>(x + kKeys / 32 * 32));
         tmem_wait_ld();
-        if (Cfg::kPCol) {
-          fence_before();
-          if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[unit]));
-        }
+        fence_before();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[unit]));
         const int from = low - key, to = high - key;  // columns [from, to) are visible
         if (__any_sync(0xffffffffu, from > 0 || to < kKeys)) {
 #pragma unroll
@@ -708,7 +701,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? exp2_fast((m - now) * c) : 1.0f;
           if (i > 0) {
-            if (!(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
+            if (!(ok = wait(sh, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
             fence_after();
 #pragma unroll 1
             for (int j = 0; j < DP; j += 16) {
@@ -725,9 +718,11 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         }
         const float z = m == -INFINITY ? 0.0f : -m * c;
         const uint64_t zz = pair(z, z);
-        // where P has its own columns, the last product has to have read them
-        if (Cfg::kPCol && number > 0) {
-          if (!(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
+        // the last product that reads these columns is done
+        const int which = p_of(unit, number), round = p_round(number);
+        const uint32_t p_at = s_at + Cfg::kPCol + (which - unit) * kKeys / 2;
+        if (round > 0) {
+          if (!(ok = wait(sh, sh.pv_done[which], (round - 1) & 1))) break;
           fence_after();
         }
         uint64_t sum[2] = {0, 0};
@@ -742,21 +737,18 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             sum[k & 1] = add2(sum[k & 1], pair(e0, e1));
             p[k] = pack2<BF16>(e0, e1);
           }
-          tmem_st8(s_at + Cfg::kPCol + j / 2, p);
+          tmem_st8(p_at + j / 2, p);
         }
         sum[0] = add2(sum[0], sum[1]);
         l += __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
-        // With two S the last product may still run: its barrier is not to get two phases ahead
-        // of this warp.
-        if (Cfg::kBuffers == 2 && number > 0 && !(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
         tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[buffer]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[which]));
       }
       if (!ok) break;
       // ---- result
-      if (n > 0 && !(ok = wait(sh, sh.pv_done[unit], (number - 1) & 1))) break;
+      if (n > 0 && !(ok = wait(sh, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
       fence_after();
       const bool wild = n > 0 && *(volatile int *)&sh.item[at].wild;
       const bool final = MODE == kTcPrompt || a.d.part.parts == 1;
