@@ -294,9 +294,9 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, x));
       nb = fmaxf(nb, __shfl_xor_sync(0xffffffffu, nb, x));
     }
-    // The maxima that the sums refer to have slack: they follow only when a score is 2^8 above
-    // (each row by its own scores), so that most chunks rescale nothing.
-    const bool ga = na - ma > 8.0f, gb = nb - mb > 8.0f;
+    // The sums refer to the exact maxima: the largest weight, which has the most say, is then 1
+    // and rounds to 16 bits without an error. Once the maxima have settled nothing is rescaled.
+    const bool ga = na > ma, gb = nb > mb;
     if (__any_sync(0xffffffffu, ga || gb)) {
       const float fa = ga ? exp2_fast(ma - na) : 1.0f, fb = gb ? exp2_fast(mb - nb) : 1.0f;
       if (ga) ma = na;
