@@ -521,12 +521,7 @@ int32_t launch_rows(dim3 grid, const CUtensorMap *maps, const PromptArgs &p, con
                     const KvView &c, cudaStream_t s) {
   using Cfg = RowsCfg<DP, WARPS>;
   auto fn = rows_kernel<MODE, DP, WARPS, BF16>;
-  static bool set = false;  // per instantiation; setting it twice is harmless
-  if (!set) {
-    DM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem),
-            "attention shared memory");
-    set = true;
-  }
+  DM_CUDA(dm::ensure_smem_limit((const void *)fn), "attention shared memory");
   return launch_chained("attention launch", fn, grid, Cfg::kThreads, Cfg::kSmem, s, maps[0], maps[1], p, d, c);
 }
 

@@ -887,12 +887,7 @@ bool encode_cache(CUtensorMap *map, bool bf16, const KvView &c, int layer, int w
 template <int MODE, int DP, bool BF16>
 int32_t launch(dim3 grid, const CUtensorMap *maps, const TcArgs &a, cudaStream_t s) {
   auto fn = tile_kernel<MODE, DP, BF16>;
-  static bool set = false;  // per instantiation; setting it twice is harmless
-  if (!set) {
-    DM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<DP>::kSmem),
-            "attention shared memory");
-    set = true;
-  }
+  DM_CUDA(dm::ensure_smem_limit((const void *)fn), "attention shared memory");
   return launch_chained("attention launch", fn, grid, TcCfg<DP>::kThreads, TcCfg<DP>::kSmem, s, maps[0],
                         maps[1], maps[2], a);
 }
