@@ -549,7 +549,13 @@ struct DecodePlan {
 };
 
 constexpr int kSms = 148;
-constexpr int kMinTileRows = 16;
+// The shared part runs on tiles where its rows fill more than one block of 16 and those blocks
+// would read more than 12 MB of keys and values (each reads them all). 8 key/value heads of
+// dim 128, us of 16-row blocks and of tiles: 24 to 192 rows a head on 256 tokens (2 to 13 MB)
+// 12 to 21 and 14 to 27; 24 to 96 rows on 1216 (20 to 60 MB) 21 to 24 and 17 to 21; 128 rows
+// on 9728 (319 MB) 61 and 41. One block of rows reads what tiles would: 16 rows on 32768
+// tokens take 48 and 52.
+constexpr int64_t kMostRowsBytes = 12 << 20;
 constexpr int kSplitKeys = 128;  // a block's keys at least, where there are several
 
 // Blocks that cut `items` rows of blocks along `keys`: as many as run at once, no more (a
@@ -577,10 +583,10 @@ DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, 
   plan.wide = dim <= 128 && own_items <= kSms;
   const int per_sm = plan.wide || dim > 128 ? 1 : 2, warps = plan.wide ? 8 : 4;
   if (has_own) plan.own_parts = splits_of(own_items, own, kSms * per_sm);
-  plan.tiles = shared > 0 && (int64_t)batch * group > kMinTileRows && group <= 128;
+  const int64_t row_blocks = ((int64_t)batch * group + kRows - 1) / kRows;
+  plan.tiles = row_blocks > 1 && group <= 128 && kv_heads * row_blocks * shared * dim * 4 > kMostRowsBytes;
   if (shared > 0 && !plan.tiles) {
-    const int64_t items = (int64_t)kv_heads * (((int64_t)batch * group + kRows - 1) / kRows);
-    plan.shared_splits = splits_of(items, shared, (dim > 128 ? 1 : 2) * kSms);
+    plan.shared_splits = splits_of(kv_heads * row_blocks, shared, (dim > 128 ? 1 : 2) * kSms);
     plan.shared_parts = plan.shared_splits;
   } else if (plan.tiles) {
     // More parts: shorter blocks, fewer SMs for the own part beside them, more to join.

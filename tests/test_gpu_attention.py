@@ -357,6 +357,78 @@ def test_decode_long(ctx, shared, lens, kv, heads):
     check_decode(pool, q, 0, out, lse)
 
 
+# Shared parts of more rows and tokens than blocks of 16 rows take: tiles of 128 rows.
+DECODES_ON_TILES = [
+    # heads, kv heads, dim, page, shared, lengths
+    (64, 2, 64, 16, 4224, [4224 + 31 * i for i in range(7)]),
+    (40, 4, 128, 32, 1056, [1056 + 9 * i for i in range(20)]),
+    (24, 8, 128, 16, 640, [641 + 40 * i for i in range(22)]),
+    (5, 1, 80, 16, 4000, [4001 + i for i in range(33)]),
+    (12, 2, 200, 16, 1600, [1600 + 3 * i for i in range(20)]),
+    (24, 1, 256, 64, 1280, [1281 + 100 * (i % 5) for i in range(12)]),
+    (8, 1, 256, 128, 4096, [4100 + i for i in range(16)]),     # one tile's rows
+    (128, 1, 64, 256, 8192, [8192, 8200, 8500]),
+    (4, 1, 8, 16, 49984, [49984 + 2 * i for i in range(33)]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv,dim,page,shared,lens", DECODES_ON_TILES)
+def test_decode_on_tiles(ctx, heads, kv, dim, page, shared, lens, dtype):
+    pool = Pool(ctx, dtype, kv, dim, page, shared, lens, seed=heads + dim, junk=float("nan"))
+    q = normal(generator(1), (len(lens), heads, dim), dtype, 2.0)
+    out, lse = run_decode(pool, q, 1, shared, max(lens))
+    check_decode(pool, q, 1, out, lse)
+
+
+@pytest.mark.parametrize("dim,shared", [(64, 8192), (128, 4096), (256, 2048)])
+@pytest.mark.parametrize("window", [0, 1, 30, 700, 100000])
+def test_decode_on_tiles_empty_short_and_reordered_sequences(ctx, dim, shared, window):
+    """Lengths of zero, inside the shared tokens, at their end and behind it, in any order;
+    windows that end before, in and behind the shared tokens."""
+    lens = [shared + 70, shared, 0, 50, shared + 9, shared + 300, shared - 1, 1] + [shared + 20] * 8
+    pool = Pool(ctx, torch.bfloat16, 2, dim, 16, shared, lens, seed=9)
+    order = [5, 0, 2, 4, 4, 3, 1, 6, 7, 9, 8, 10, 11, 12, 13, 14]
+    q = normal(generator(4), (len(order), 8, dim), torch.bfloat16, 2.0)
+    out, lse = run_decode(pool, q, 1, shared, max(lens), sequences=order, window=window)
+    check_decode(pool, q, 1, out, lse, sequences=order, window=window)
+    assert (out[2] == 0).all() and torch.isinf(lse[2]).all()
+
+
+@pytest.mark.parametrize("dim,shared", [(64, 8192), (128, 4096), (256, 2048)])
+@pytest.mark.parametrize("wild", [float("nan"), float("inf"), None])
+def test_decode_on_tiles_hidden_values_have_no_influence(ctx, dim, shared, wild):
+    """Shared tokens that a shorter sequence or a window does not see, and what those see
+    that do."""
+    wild = torch.finfo(torch.bfloat16).min if wild is None else wild
+    lens = [shared + 30, 100, shared + 5, shared] + [shared] * 12
+    pool = Pool(ctx, torch.bfloat16, 2, dim, 16, shared, lens, seed=18)
+    pool.lengths[1] = 100
+    q = normal(generator(10), (16, 8, dim), torch.bfloat16, 2.0)
+    for window in (0, 150):
+        want, want_lse = run_decode(pool, q, 0, shared, max(lens), window=window)
+        saved = pool.memory.clone()
+        for key in (100, 104, shared - 1):
+            page = int(pool.table[0, key // 16])
+            pool.memory[page, 0, :, :, key % 16] = wild
+        out, lse = run_decode(pool, q, 0, shared, max(lens), window=window)
+        assert torch.equal(out[1], want[1]) and torch.equal(lse[1], want_lse[1])
+        assert not torch.equal(out[3], want[3])
+        if not math.isfinite(wild):
+            assert not torch.isfinite(out[3]).any()
+        pool.memory.copy_(saved)
+        # a value alone, seen by all but the short sequence: its column, no other
+        page = int(pool.table[0, (shared - 20) // 16])
+        pool.memory[page, 0, 1, 1, (shared - 20) % 16, 5] = float("inf")
+        out, lse = run_decode(pool, q, 0, shared, max(lens), window=window)
+        assert torch.equal(lse, want_lse) and torch.equal(out[1], want[1])
+        other = torch.ones_like(out, dtype=torch.bool)
+        other[:, 4:, 5] = False
+        assert torch.equal(out[other], want[other])
+        assert (out[[0, 2, 3] + list(range(4, 16)), 4:, 5] == float("inf")).all()
+        pool.memory.copy_(saved)
+
+
 def test_decode_empty_short_and_reordered_sequences(ctx):
     """Rows picked out of order, one of them twice; a length of zero and one below the
     shared tokens; a row number outside the table is an empty sequence."""
