@@ -544,6 +544,7 @@ struct DecodePlan {
   bool tiles = false;  // the shared part runs on tcgen05 tiles
   bool wide = false;   // own keys: eight warps a block
   bool joins = false;  // the own part joins the shared ones
+  int shared = 0;      // tokens that are read once for all; the rest is each sequence's own
   int shared_splits = 0, shared_parts = 0, own_parts = 0;
   int parts() const { return shared_parts + own_parts; }
 };
@@ -569,7 +570,8 @@ int splits_of(int64_t items, int keys, int64_t at_once) {
 // warp, and beside tiles they get done 0.7 of what they would alone; a join in place 2; the
 // join kernel 4 besides 0.4 for each MB of parts.
 constexpr float kTileUs = 9.0f, kTileStepUs = 1.2f, kTileStepWideUs = 2.6f, kRowsUs = 7.0f, kRowsStepUs = 0.9f,
-                kRowsStepWideUs = 1.2f, kBeside = 0.7f, kInPlaceUs = 2.0f, kJoinUs = 4.0f, kJoinMbUs = 0.4f;
+                kRowsStepWideUs = 1.2f, kBeside = 0.7f, kInPlaceUs = 2.0f, kJoinUs = 4.0f, kJoinMbUs = 0.4f,
+                kThirdUs = 2.0f;
 
 DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, int max_length) {
   DecodePlan plan;
@@ -581,22 +583,57 @@ DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, 
   // Blocks of eight warps have an SM to themselves, two of four warps share one: the first
   // are sooner done, where all of them run at once.
   plan.wide = dim <= 128 && own_items <= kSms;
-  const int per_sm = plan.wide || dim > 128 ? 1 : 2, warps = plan.wide ? 8 : 4;
-  if (has_own) plan.own_parts = splits_of(own_items, own, kSms * per_sm);
+  const int per_sm = plan.wide || dim > 128 ? 1 : 2, warps = plan.wide ? 8 : 4, at_once = kSms * per_sm;
+  const float step = dim > 128 ? kRowsStepWideUs : kRowsStepUs;
+  auto rows_us = [&](int keys, int warps) { return kRowsUs + step * ((keys + 16 * warps - 1) / (16 * warps)); };
+  auto join_us = [&](int parts) { return kJoinUs + kJoinMbUs * parts * ((float)batch * heads * dim * 4e-6f); };
+
+  // Each sequence reads all of its tokens: one launch, or two. With 32 and 8 heads of dim 128
+  // and 64 shared tokens 13 us instead of 17 for 16 sequences, 21 instead of 24 for 64 (one
+  // launch less; the caller's side 15.8 instead of 17.8), with 1056 for one 15 and 15 (20 and
+  // 17.8); but 49 instead of 32 for 16 sequences with 4128.
+  DecodePlan alone = plan;
+  float alone_us = 0.0f;
+  const int most_parts = splits_of(own_items, std::max(1, max_length), at_once);
+  for (int parts : {1, most_parts}) {
+    const float us = std::max(1.0f, (float)own_items / at_once) * rows_us((max_length + parts - 1) / parts, warps) +
+                     (parts > 1 ? join_us(parts) : 0.0f);
+    if (parts == 1 || us < alone_us) {
+      alone_us = us;
+      alone.own_parts = parts;
+    }
+  }
+  if (shared == 0) return alone;
+
+  // The shared tokens once for all, then what is left: two launches, or three.
+  plan.shared = shared;
+  if (has_own) plan.own_parts = splits_of(own_items, own, at_once);
   const int64_t row_blocks = ((int64_t)batch * group + kRows - 1) / kRows;
   plan.tiles = row_blocks > 1 && group <= 128 && kv_heads * row_blocks * shared * dim * 4 > kMostRowsBytes;
-  if (shared > 0 && !plan.tiles) {
-    plan.shared_splits = splits_of(kv_heads * row_blocks, shared, (dim > 128 ? 1 : 2) * kSms);
-    plan.shared_parts = plan.shared_splits;
-  } else if (plan.tiles) {
+  float best = 0.0f;
+  if (!plan.tiles) {
+    const int64_t items = kv_heads * row_blocks;
+    plan.shared_parts = plan.shared_splits = splits_of(items, shared, (dim > 128 ? 1 : 2) * kSms);
+    plan.joins = plan.own_parts == 1 && plan.shared_parts <= kMostJoined;
+    const float blocks = (float)items * plan.shared_splits;
+    best = std::max(1.0f, blocks / ((dim > 128 ? 1 : 2) * kSms)) *
+           rows_us((shared + plan.shared_splits - 1) / plan.shared_splits, 4);
+    if (has_own) {
+      const float one = rows_us((own + plan.own_parts - 1) / plan.own_parts, warps);
+      // beside the shared blocks, if they leave room, else behind them
+      const float left = plan.wide || dim > 128 ? kSms - blocks : at_once - blocks;
+      best = (float)own_items * plan.own_parts <= left ? std::max(best, one)
+                                                      : best + one * std::max(1.0f, (float)own_items / at_once);
+    }
+    best += plan.joins ? kInPlaceUs : plan.parts() > 1 ? join_us(plan.parts()) : 0.0f;
+  } else {
     // More parts: shorter blocks, fewer SMs for the own part beside them, more to join.
     const int units = tile_shared_alternates(dim, group, batch) ? 2 : 1;
     const int tiles = (shared + tile_keys(dim) - 1) / tile_keys(dim);
     const int items = tile_shared_items(dim, kv_heads, group, batch);
     const int most = std::max(1, std::min(kSms / items, tiles / units));
-    float best = 0.0f;
-    for (int splits = 1, step = 1; splits <= most; splits += step, step = splits / 8 + 1) {
-      DecodePlan at = plan;
+    DecodePlan at = plan;
+    for (int splits = 1, next = 1; splits <= most; splits += next, next = splits / 8 + 1) {
       at.shared_splits = splits;
       at.shared_parts = splits * units;
       const int per = (tiles + splits - 1) / splits;
@@ -606,29 +643,26 @@ DecodePlan decode_plan(int kv_heads, int heads, int dim, int batch, int shared, 
         // own blocks are cut for the SMs that are left, if that leaves enough
         at.own_parts = splits_of(own_items, own, (int64_t)(left >= kSms / 2 ? left : kSms) * per_sm);
         const float blocks = (float)own_items * at.own_parts;
-        const float one = kRowsUs + (dim > 128 ? kRowsStepWideUs : kRowsStepUs) * ((own + at.own_parts - 1) / at.own_parts + 16 * warps - 1) / (16 * warps);
+        const float one = rows_us((own + at.own_parts - 1) / at.own_parts, warps);
         at.joins = at.own_parts == 1 && at.shared_parts <= kMostJoined;
         if (blocks <= left * per_sm) {
           us = std::max(us, one);
         } else {  // what the tiles leave time for, then on all SMs; blocks that join wait for them
           float done = kBeside * left * per_sm * (us / one);
           if (at.joins) done = std::min(done, (float)left * per_sm);
-          us += std::max(0.0f, blocks - done) / (kSms * per_sm) * one;
+          us += std::max(0.0f, blocks - done) / at_once * one;
           us = std::max(us, one);
         }
       }
-      if (at.joins)
-        us += kInPlaceUs;
-      else if (at.parts() > 1)
-        us += kJoinUs + kJoinMbUs * at.parts() * ((float)batch * heads * dim * 4e-6f);
+      us += at.joins ? kInPlaceUs : at.parts() > 1 ? join_us(at.parts()) : 0.0f;
       if (splits == 1 || us < best) {
         best = us;
         plan = at;
       }
     }
   }
-  plan.joins = plan.shared_parts > 0 && plan.own_parts == 1 && plan.shared_parts <= kMostJoined;
-  return plan;
+  if (has_own && !plan.joins) best += kThirdUs;
+  return alone_us < best ? alone : plan;
 }
 
 uint64_t decode_workspace(const DecodePlan &plan, int64_t rows, int dim) {
@@ -755,9 +789,9 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
   a.batch = in->batch;
   a.layer = in->layer;
   a.window = in->window;
-  a.shared = in->shared_tokens;
   a.max_length = in->max_length;
   const DecodePlan plan = decode_plan(kd.kv_heads, in->heads, kd.head_dim, in->batch, in->shared_tokens, in->max_length);
+  a.shared = plan.shared;
   a.part.parts = plan.parts();
   a.part.rows = (int64_t)in->batch * in->heads;
   a.part.o = (float *)in->workspace;

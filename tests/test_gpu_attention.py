@@ -429,6 +429,66 @@ def test_decode_on_tiles_hidden_values_have_no_influence(ctx, dim, shared, wild)
         pool.memory.copy_(saved)
 
 
+# Shared parts on blocks of 16 rows: joined by the blocks of the own part, or behind them.
+DECODES_ON_ROWS = [
+    # heads, kv heads, dim, page, shared, lengths
+    (4, 2, 64, 16, 1056, [1057 + 3 * i for i in range(32)]),
+    (8, 2, 80, 32, 512, [512 + i % 9 for i in range(20)]),
+    (8, 1, 128, 64, 512, [513 + i for i in range(33)]),
+    (16, 4, 128, 128, 512, [560, 513, 530, 540, 512, 520]),
+    (40, 1, 128, 16, 640, [641 + 9 * i for i in range(6)]),
+    (8, 1, 200, 64, 320, [321 + i % 20 for i in range(24)]),
+    (16, 2, 256, 16, 480, [481, 500, 490, 485]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv,dim,page,shared,lens", DECODES_ON_ROWS)
+def test_decode_on_rows(ctx, heads, kv, dim, page, shared, lens, dtype):
+    pool = Pool(ctx, dtype, kv, dim, page, shared, lens, seed=heads + dim, junk=float("nan"))
+    q = normal(generator(1), (len(lens), heads, dim), dtype, 2.0)
+    for layer in (0, 1):
+        out, lse = run_decode(pool, q, layer, shared, max(lens))
+        check_decode(pool, q, layer, out, lse)
+
+
+ROWS = [(4, 2, 64, 32, 1056, 90), (8, 1, 128, 33, 512, 40), (16, 2, 256, 4, 480, 20)]
+
+
+@pytest.mark.parametrize("heads,kv,dim,batch,shared,own", ROWS)
+@pytest.mark.parametrize("window", [0, 1, 30, 300, 100000])
+def test_decode_on_rows_empty_short_and_reordered_sequences(ctx, heads, kv, dim, batch, shared, own, window):
+    lens = [shared + own, 0, shared, 50] + [shared - 1, shared + 9, 1, shared + own] * 8
+    lens = lens[:batch]
+    pool = Pool(ctx, torch.bfloat16, kv, dim, 16, shared, lens, seed=9)
+    order = [(i * 5 + 3) % batch if batch % 5 else i for i in range(batch)]
+    order[1] = order[0]
+    q = normal(generator(4), (batch, heads, dim), torch.bfloat16, 2.0)
+    out, lse = run_decode(pool, q, 1, shared, max(lens), sequences=order, window=window)
+    check_decode(pool, q, 1, out, lse, sequences=order, window=window)
+
+
+@pytest.mark.parametrize("heads,kv,dim,batch,shared,own", ROWS)
+@pytest.mark.parametrize("wild", [float("nan"), float("inf"), None])
+def test_decode_on_rows_hidden_values_have_no_influence(ctx, heads, kv, dim, batch, shared, own, wild):
+    wild = torch.finfo(torch.bfloat16).min if wild is None else wild
+    lens = [shared + own, 100, shared + 5, shared] + [shared] * (batch - 4)
+    pool = Pool(ctx, torch.bfloat16, kv, dim, 16, shared, lens, seed=18)
+    pool.lengths[1] = 100
+    q = normal(generator(10), (batch, heads, dim), torch.bfloat16, 2.0)
+    for window in (0, 150):
+        want, want_lse = run_decode(pool, q, 0, shared, max(lens), window=window)
+        for key in (100, 104, shared - 1):
+            page = int(pool.table[0, key // 16])
+            saved = pool.memory[page].clone()
+            pool.memory[page, 0, :, :, key % 16] = wild
+            out, lse = run_decode(pool, q, 0, shared, max(lens), window=window)
+            assert torch.equal(out[1], want[1]) and torch.equal(lse[1], want_lse[1])
+            hidden = window > 0 and key < shared - window
+            assert torch.equal(out[3], want[3]) == hidden
+            pool.memory[page] = saved
+
+
 def test_decode_empty_short_and_reordered_sequences(ctx):
     """Rows picked out of order, one of them twice; a length of zero and one below the
     shared tokens; a row number outside the table is an empty sequence."""
