@@ -16,11 +16,8 @@ from ._native import check
 from .moe import CudaContext
 
 
-_CONTIGUOUS = (C.c_int64 * 2)()
-
-
-def _strides(pair):
-    return _CONTIGUOUS if pair is None else (C.c_int64 * 2)(*pair)
+def _strides(pair):  # zeros: contiguous
+    return (C.c_int64 * 2)() if pair is None else (C.c_int64 * 2)(*pair)
 
 
 def prompt_attention(ctx: CudaContext, *, type: int, heads: int, kv_heads: int, head_dim: int,
@@ -31,9 +28,12 @@ def prompt_attention(ctx: CudaContext, *, type: int, heads: int, kv_heads: int, 
     """Packed attention of `sequences` prompts (dm_attention_prompt). `*_stride` are
     (token, head) pairs, None for contiguous tensors; scale 0 is 1 / sqrt(head_dim)."""
     d = N.PromptDesc(type, heads, kv_heads, head_dim, sequences, int(causal), window, scale,
-                     q_tokens, k_tokens, q, k, v, out, lse or None, _strides(q_stride),
-                     _strides(k_stride), _strides(v_stride), _strides(out_stride), q_offsets,
-                     k_offsets or None)
+                     q_tokens, k_tokens, q, k, v, out, lse or None)
+    d.q_offsets = q_offsets
+    d.k_offsets = k_offsets or None
+    if q_stride or k_stride or v_stride or out_stride:
+        d.q_stride, d.k_stride = _strides(q_stride), _strides(k_stride)
+        d.v_stride, d.out_stride = _strides(v_stride), _strides(out_stride)
     check(N.lib().dm_attention_prompt(ctx.handle, C.byref(d), stream or None))
 
 
@@ -112,8 +112,12 @@ class KvCache:
                          workspace: int = 0, workspace_bytes: int = 0, stream: int = 0):
         """One query token per sequence over the cache (dm_attention_decode)."""
         d = N.DecodeDesc(layer, heads, batch, window, shared_tokens, max_length, scale, q, out,
-                         lse or None, _strides(q_stride), _strides(out_stride), sequences or None,
-                         workspace or None, workspace_bytes)
+                         lse or None)
+        d.sequences = sequences or None
+        d.workspace = workspace or None
+        d.workspace_bytes = workspace_bytes
+        if q_stride or out_stride:
+            d.q_stride, d.out_stride = _strides(q_stride), _strides(out_stride)
         check(self._lib.dm_attention_decode(self._h, C.byref(d), stream or None))
 
     def close(self):
