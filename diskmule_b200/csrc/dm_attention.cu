@@ -237,12 +237,12 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 
   constexpr int kStep = kWarps * kChunk;
   int key_load = first + warp * kChunk;
-  int page = page_of(key_load);
+  int page = page_of(key_load), page2 = page_of(key_load + kStep);
   auto issue = [&](int stage) {
     if (key_load < last) {
-      const int next = page_of(key_load + kStep);  // one step ahead of its use
+      const int next = page_of(key_load + 2 * kStep);  // two steps ahead of its use
       load(key_load, page, stage);
-      page = next;
+      page = page2, page2 = next;
     }
     key_load += kStep;
     if (MODE == kPrompt) asm volatile("cp.async.commit_group;");

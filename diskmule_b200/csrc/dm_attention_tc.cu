@@ -300,7 +300,19 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   const int lane = threadIdx.x & 31;
   const int kv_head = w.kv_head, k0 = w.k0, table_row = w.table_row;
   int key = w.first;
+  // shared: a box lies in one page; lane i looks the tile's i-th up, a tile ahead. Boxes and
+  // pages are powers of two or whole chunks.
+  const int box = MODE == kTcPrompt ? kRows : V ? a.v_box : a.k_box;
+  const int most = kRows / box, page_bits = 31 - __clz(a.c.page_tokens);
+  auto page_at = [&](int at) -> int {
+    if (lane * box >= Cfg::kKeys || at + lane * box >= a.d.shared) return 0;
+    const int p = a.c.table[(int64_t)table_row * a.c.max_pages + ((at + lane * box) >> page_bits)];
+    return (unsigned)p < (unsigned)a.c.pages ? p : a.c.pages;  // behind the map: zeros
+  };
+  int next_pages = MODE == kTcShared && tiles > 0 ? page_at(key) : 0;
   for (int t = 0; t < tiles; t++, key += Cfg::kKeys) {
+    const int pages = next_pages;
+    if (MODE == kTcShared && t + 1 < tiles) next_pages = page_at(key + Cfg::kKeys);
     // No sooner than it is needed: blocks that have not started are for whoever is done first.
     if (!V && t == max(0, tiles - kWantTiles) && lead) mbar_arrive(smem_u32(&sh.want));
 #pragma unroll 1
@@ -308,17 +320,10 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
       const int from = V ? key + c * kRows : key, x0 = V ? 0 : c * kSlabs * 64;
       const uint32_t bar = smem_u32(V ? &sh.v_full[place.slot] : &sh.k_full[place.slot]);
       const uint32_t dst = ring + place.slot * Cfg::kChunkBytes;
-      // shared: the boxes of the chunk's pages, each in kSlabs slabs; one lane for each
-      int page = 0, boxes = 1, box = kRows;
+      // shared: the chunk's boxes, each in kSlabs slabs; one lane for each
       const int slab = lane % kSlabs, mine = lane / kSlabs;
-      if (MODE == kTcShared) {
-        box = V ? a.v_box : a.k_box;
-        boxes = max(0, min(kRows, a.d.shared - from)) / box;
-        if (mine < boxes) {
-          const int p = a.c.table[(int64_t)table_row * a.c.max_pages + (from + mine * box) / a.c.page_tokens];
-          page = (unsigned)p < (unsigned)a.c.pages ? p : a.c.pages;  // behind the map: zeros
-        }
-      }
+      const int boxes = MODE == kTcPrompt ? 1 : from + kRows <= a.d.shared ? most : max(0, a.d.shared - from) / box;
+      const int page = MODE == kTcShared ? __shfl_sync(0xffffffffu, pages, (V ? c * most : 0) + mine) : 0;
       if (place.round > 0 && !wait(sh, V ? sh.v_empty[place.slot] : sh.k_empty[place.slot], place.parity() ^ 1))
         return false;
       if (lead) mbar_expect_tx(bar, kSlabs * boxes * box * 128);
@@ -327,7 +332,7 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
         if (lane < kSlabs) tma_load_3d(dst + slab * kRows * 128, map, x0 + slab * 64, kv_head, k0 + from, bar);
       } else if (mine < boxes) {
         tma_load_4d(dst + slab * kRows * 128 + mine * box * 128, map, x0 + slab * 64,
-                    (from + mine * box) % a.c.page_tokens, kv_head, page, bar);
+                    (from + mine * box) & (a.c.page_tokens - 1), kv_head, page, bar);
       }
       __syncwarp();
     }
