@@ -199,9 +199,10 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   const uint32_t ring = smem_u32(smem) + warp * Cfg::kRing;
   constexpr int kVec = DP / 8;  // 16-byte vectors of a row
   auto at = [](int r, int v) { return (uint32_t)((v >> 3) * Cfg::kSlab + r * 128 + ((v ^ r) & 7) * 16); };
+  const int page_bits = MODE == kPrompt ? 0 : 31 - __clz(c.page_tokens);  // pages are powers of two
   auto page_of = [&](int key) -> int {
     if (MODE == kPrompt || key >= last) return -1;
-    const int page = c.table[(int64_t)table_row * c.max_pages + key / c.page_tokens];
+    const int page = c.table[(int64_t)table_row * c.max_pages + (key >> page_bits)];
     return (unsigned)page < (unsigned)c.pages ? page : c.pages;  // behind the map: zeros
   };
   auto load = [&](int key, int page, int stage) {
@@ -224,7 +225,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         const bool is_v = lane >= DP / 64;
         const int slab = lane % (DP / 64);
         tma_load_4d((is_v ? vd : kd) + slab * Cfg::kSlab, is_v ? &v_map : &k_map, slab * 64,
-                    key % c.page_tokens, kv_head, page, bar);
+                    key & (c.page_tokens - 1), kv_head, page, bar);
       }
     }
   };
