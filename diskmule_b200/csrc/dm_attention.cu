@@ -93,6 +93,7 @@ struct RowsSmem {
   int64_t out[kRows];   // element offset of its output
   int64_t index[kRows]; // its row in lse and in the parts
   int low[kRows], high[kRows];  // the keys that it sees
+  int table[kRows];             // its sequence's row of the page table
   float2 ml[WARPS][kRows];
   uint64_t full[WARPS][kStages];  // a chunk of a warp has landed
   TileOf tile;
@@ -152,15 +153,13 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     const int rb = blockIdx.x % blocks;
     kv_head = (blockIdx.x / blocks) % c.kv_heads;
     const int entry = MODE == kOwn ? blockIdx.x / blocks / c.kv_heads : 0;
-    int unused;
-    table_row = sequence_of(c, d, entry, &unused);
     if (tid < kRows) {
       const int r = rb * kRows + tid;
       const int b = MODE == kOwn ? entry : r / group;
       const int head = kv_head * group + r % group;
       const bool valid = r < rows;
       int length = 0;
-      if (valid) sequence_of(c, d, b, &length);
+      sh.table[tid] = valid ? sequence_of(c, d, b, &length) : 0;
       sh.q[tid] = valid ? b * d.q_stride[0] + head * d.q_stride[1] : -1;
       sh.out[tid] = b * d.out_stride[0] + head * d.out_stride[1];
       sh.index[tid] = (int64_t)b * d.heads + head;
@@ -171,9 +170,14 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   }
   __syncthreads();
   int low = INT32_MAX, high = 0;
+  // Pages are looked up for the row that sees the most keys: the others, which may be shorter
+  // or empty, have the same pages as far as they reach and no entries behind that.
 #pragma unroll
   for (int r = 0; r < kRows; r++)
-    if (sh.q[r] >= 0) low = min(low, sh.low[r]), high = max(high, sh.high[r]);
+    if (sh.q[r] >= 0) {
+      if (MODE != kPrompt && sh.high[r] > high) table_row = sh.table[r];
+      low = min(low, sh.low[r]), high = max(high, sh.high[r]);
+    }
   low = low / kChunk * kChunk;
   first = low, last = high;
   if (MODE != kPrompt && high > low) {

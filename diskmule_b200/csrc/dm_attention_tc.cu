@@ -99,7 +99,8 @@ struct Item {
   int n[2];                         // tiles of each unit
   int max_low, min_high;            // every row sees the keys [max_low, min_high)
   int token0, lq, lk, q0, k0;       // first token of the item and of its sequence
-  int table_row, wild;              // wild: values that are not finite were found
+  int table_row, end;               // shared: where its pages are looked up; no row sees keys from `end` on
+  int wild;                         // values that are not finite were found
 };
 
 struct TcSmem {
@@ -311,14 +312,14 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   constexpr int kRows = V ? Cfg::kVKeys : Cfg::kKeys;     // keys of a chunk
   constexpr int kSlabs = V ? DP / 64 : Cfg::kKSlabs;      // its slabs of 64 values
   const int lane = threadIdx.x & 31;
-  const int kv_head = w.kv_head, k0 = w.k0, table_row = w.table_row;
+  const int kv_head = w.kv_head, k0 = w.k0, table_row = w.table_row, end = w.end;
   int key = w.first;
   // shared: a box lies in one page; lane i looks the tile's i-th up, a tile ahead. Boxes and
   // pages are powers of two or whole chunks.
   const int box = MODE == kTcPrompt ? kRows : V ? a.v_box : a.k_box;
   const int most = kRows / box, page_bits = 31 - __clz(a.c.page_tokens);
   auto page_at = [&](int at) -> int {
-    if (lane * box >= Cfg::kKeys || at + lane * box >= a.d.shared) return 0;
+    if (lane * box >= Cfg::kKeys || at + lane * box >= end) return a.c.pages;
     const int p = a.c.table[(int64_t)table_row * a.c.max_pages + ((at + lane * box) >> page_bits)];
     return (unsigned)p < (unsigned)a.c.pages ? p : a.c.pages;  // behind the map: zeros
   };
@@ -451,18 +452,21 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         const int blocks = (a.d.batch + units * a.tokens - 1) / (units * a.tokens);
         w.kv_head = block / blocks;
         w.token0 = block % blocks * units * a.tokens;
-        int length;
-        w.table_row = sequence_of(a.c, a.d, 0, &length);
-        int top = 0, bottom = INT32_MAX, most = 0;
+        // Pages are looked up for the sequence that has most of the shared tokens: the others,
+        // which may be shorter or empty, have the same pages as far as they reach and no
+        // entries behind that.
+        int top = 0, bottom = INT32_MAX, mine = 0, table_row = 0;
         for (int b = w.token0 + lane; b < min(a.d.batch, w.token0 + units * a.tokens); b += 32) {
-          sequence_of(a.c, a.d, b, &length);
+          int length;
+          const int row = sequence_of(a.c, a.d, b, &length), sees = min(length, a.d.shared);
           top = max(top, a.d.window ? max(0, length - a.d.window) : 0);
-          bottom = min(bottom, min(length, a.d.shared));
-          most = max(most, min(length, a.d.shared));
+          bottom = min(bottom, sees);
+          if (sees > mine) mine = sees, table_row = row;
         }
         w.max_low = __reduce_max_sync(0xffffffffu, top);
         w.min_high = __reduce_min_sync(0xffffffffu, bottom);
-        most = __reduce_max_sync(0xffffffffu, most);
+        const int most = w.end = __reduce_max_sync(0xffffffffu, mine);
+        w.table_row = __shfl_sync(0xffffffffu, table_row, __ffs(__ballot_sync(0xffffffffu, mine == most)) - 1);
         const int all = (a.d.shared + kKeys - 1) / kKeys;
         const int per = (all + a.d.splits - 1) / a.d.splits;
         const int t0 = min(all, split * per), t1 = min((most + kKeys - 1) / kKeys, t0 + per);

@@ -132,11 +132,11 @@ DM_API int32_t dm_kv_cache_copy_pages(dm_kv_cache *cache, const int32_t *source,
 /* q and out [batch, heads, head_dim] (strides as above), lse [batch, heads]. Query row b is
  * the last token of sequences[b] (NULL = row b of the table) and sees all of its tokens, or
  * with window > 0 the last `window`. The first shared_tokens (a multiple of page_tokens, may
- * be 0) of every sequence in the batch lie in the same pages, those of sequences[0]; they
- * are read once, or by each sequence where that is sooner done. A sequence shorter than that
- * sees what it has. max_length bounds every lengths[sequences[b]]; tokens beyond it are not
- * read. workspace is 16-byte aligned scratch of at least dm_attention_decode_workspace bytes
- * for the same numbers; two calls in flight need two. */
+ * be 0) of every sequence in the batch lie in the same pages; they are read once, or by each
+ * sequence where that is sooner done. A sequence shorter than that sees what it has, wherever
+ * it stands in the batch; a row number outside the table is an empty sequence. max_length
+ * bounds every lengths[sequences[b]]; tokens beyond it are not read. workspace is 16-byte
+ * aligned scratch of at least dm_attention_decode_workspace bytes for the same numbers; two calls in flight need two. */
 typedef struct {
   int32_t layer, heads, batch, window;
   int32_t shared_tokens, max_length;

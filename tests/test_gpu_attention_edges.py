@@ -1,0 +1,110 @@
+"""Attention and its cache at their edges: what a finished or short sequence leaves in the page
+table, bounds and sizes near their limits, values near the types' limits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from diskmule_b200 import CudaContext
+from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = CudaContext(0)
+    yield c
+    c.close()
+
+
+def as_left_behind(pool):
+    """-1 behind every sequence's pages, as extend, fork, compact and free leave a table row."""
+    table = pool.table.cpu().numpy()
+    for s, n in enumerate(pool.lengths.cpu().numpy()):
+        table[s, -(-int(n) // pool.page):] = -1
+    pool.table.copy_(ints(table))
+    return pool
+
+
+# Sizes whose shared tokens go to blocks of 16 rows, to tiles, and to each sequence itself.
+SHORT_FIRST = [
+    # heads, kv heads, dim, page, batch, shared
+    (4, 2, 64, 16, 32, 1056),
+    (8, 1, 128, 64, 33, 512),
+    (16, 2, 256, 16, 5, 480),
+    (8, 2, 64, 16, 16, 8192),
+    (40, 4, 128, 32, 20, 1056),
+    (8, 2, 128, 16, 40, 4096),
+    (8, 2, 256, 16, 16, 2048),
+    (8, 2, 128, 16, 3, 128),
+]
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,batch,shared", SHORT_FIRST)
+@pytest.mark.parametrize("first", ["empty", "short", "outside", "half"])
+@pytest.mark.parametrize("window", [0, 100])
+def test_decode_first_sequence_without_the_shared_tokens(ctx, heads, kv, dim, page, batch, shared, first, window):
+    """The shared pages come from a sequence that has them, whichever row of the batch that is:
+    a first sequence that is empty, short or outside the table changes no other row."""
+    lens = [shared + 7 * i % 40 for i in range(batch)]
+    lens[0] = {"empty": 0, "short": 20, "outside": shared, "half": shared // 2}[first]
+    lens[-1] = shared + 90
+    pool = as_left_behind(Pool(ctx, torch.bfloat16, kv, dim, page, shared, lens, seed=batch))
+    q = normal(generator(3), (batch, heads, dim), torch.bfloat16, 2.0)
+    order = list(range(batch))
+    if first == "outside":
+        order[0] = batch + 5
+        out, lse = run_decode(pool, q, 1, shared, max(lens), sequences=order, window=window)
+        check_decode(pool, q[1:], 1, out[1:], lse[1:], sequences=order[1:], window=window)
+        assert (out[0] == 0).all() and (lse[0] == -math.inf).all()
+    else:
+        out, lse = run_decode(pool, q, 1, shared, max(lens), window=window)
+        check_decode(pool, q, 1, out, lse, window=window)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,batch,shared", SHORT_FIRST)
+def test_decode_shared_tokens_that_no_sequence_has_in_full(ctx, heads, kv, dim, page, batch, shared):
+    """Every sequence ends inside the shared tokens, the longest of them in the middle of the
+    batch; the last page of none is mapped."""
+    lens = [(shared * (i + 1)) // (batch + 3) for i in range(batch)]
+    lens[batch // 2] = shared - page - 3
+    lens[0] = 0
+    pool = as_left_behind(Pool(ctx, torch.bfloat16, kv, dim, page, shared, lens, seed=batch + 1))
+    q = normal(generator(5), (batch, heads, dim), torch.bfloat16, 2.0)
+    out, lse = run_decode(pool, q, 0, shared, shared)
+    check_decode(pool, q, 0, out, lse)
+
+
+def test_decode_after_a_row_of_the_batch_is_freed(ctx):
+    """A finished sample keeps its place in the batch: its freed row gives zeros, the others
+    what they gave before."""
+    from diskmule_b200 import _native as N
+    from diskmule_b200.attention import KvCache, offsets
+    n, kv, dim, batch = 1060, 8, 128, 24
+    cache = KvCache(ctx, type=N.BF16, layers=1, kv_heads=kv, head_dim=dim, page_tokens=16, pages=200,
+                    max_sequences=batch + 1, max_pages=80)
+    gen = generator(47)
+    k, v = (normal(gen, (n, kv, dim), torch.bfloat16) for _ in range(2))
+    row, count, off = ints([0]), ints([n]), ints(offsets([n]))
+    cache.extend(row.data_ptr(), count.data_ptr(), 1)
+    cache.write(0, k.data_ptr(), v.data_ptr(), row.data_ptr(), off.data_ptr(), 1, n)
+    rows, parents = ints(range(1, batch + 1)), ints([0] * batch)
+    cache.fork(parents.data_ptr(), rows.data_ptr(), batch)
+    q = normal(gen, (batch, 32, dim), torch.bfloat16, 2.0)
+    shared = n // 16 * 16
+    size = cache.decode_workspace(32, batch, shared, n)
+    work = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    results = []
+    for step in range(2):
+        out = torch.full_like(q, float("nan"))
+        cache.decode_attention(layer=0, heads=32, q=q.data_ptr(), out=out.data_ptr(), batch=batch, max_length=n,
+                               shared_tokens=shared, sequences=rows.data_ptr(), workspace=work.data_ptr(),
+                               workspace_bytes=size)
+        results.append(out)
+        cache.free(rows.data_ptr(), 1)  # the first of the batch
+    torch.cuda.synchronize()
+    assert cache.status() == 0
+    assert torch.equal(results[0][1:], results[1][1:]) and (results[1][0] == 0).all()
+    cache.close()
