@@ -213,7 +213,9 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   auto page_of = [&](int key) -> int {
     if (MODE == kPrompt || key >= last) return -1;
     const int page = c.table[(int64_t)table_row * c.max_pages + (key >> page_bits)];
-    return (unsigned)page < (unsigned)c.pages ? page : c.pages;  // behind the map: zeros
+    if ((unsigned)page < (unsigned)c.pages) return page;
+    if (lane == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
+    return c.pages;  // behind the map: zeros
   };
   auto load = [&](int key, int page, int stage) {
     const uint32_t kd = ring + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;

@@ -321,7 +321,9 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   auto page_at = [&](int at) -> int {
     if (lane * box >= Cfg::kKeys || at + lane * box >= end) return a.c.pages;
     const int p = a.c.table[(int64_t)table_row * a.c.max_pages + ((at + lane * box) >> page_bits)];
-    return (unsigned)p < (unsigned)a.c.pages ? p : a.c.pages;  // behind the map: zeros
+    if ((unsigned)p < (unsigned)a.c.pages) return p;
+    if (!V) atomicOr(a.c.status, DM_KV_BAD_TOKEN);
+    return a.c.pages;  // behind the map: zeros
   };
   int next_pages = MODE == kTcShared && tiles > 0 ? page_at(key) : 0;
   for (int t = 0; t < tiles; t++, key += Cfg::kKeys) {

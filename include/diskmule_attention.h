@@ -16,8 +16,9 @@
  *     sees no key gets zeros and -infinity;
  *   - what a mask hides has no influence, whatever it holds (NaN and infinities included);
  *   - calls are stream-ordered, allocate nothing and may be captured into a CUDA graph;
- *   - arguments are checked before any launch; what only the device can see (page tables,
- *     lengths, lists) is range-checked there and reported through a status word.
+ *   - arguments are checked before any launch; what only the device can see is range-checked
+ *     there. Cache calls and decode report lists, positions and pages out of range through
+ *     the cache's status word (dm_kv_cache_status); prompt offsets are limited to the tensors.
  */
 #ifndef DISKMULE_ATTENTION_H
 #define DISKMULE_ATTENTION_H
@@ -136,7 +137,9 @@ DM_API int32_t dm_kv_cache_copy_pages(dm_kv_cache *cache, const int32_t *source,
  * sequence where that is sooner done. A sequence shorter than that sees what it has, wherever
  * it stands in the batch; a row number outside the table is an empty sequence. max_length
  * bounds every lengths[sequences[b]]; tokens beyond it are not read. workspace is 16-byte
- * aligned scratch of at least dm_attention_decode_workspace bytes for the same numbers; two calls in flight need two. */
+ * aligned scratch of at least dm_attention_decode_workspace bytes for the same numbers; two
+ * calls in flight need two. A page number outside the pool reads as keys and values of zero
+ * and sets DM_KV_BAD_TOKEN. */
 typedef struct {
   int32_t layer, heads, batch, window;
   int32_t shared_tokens, max_length;

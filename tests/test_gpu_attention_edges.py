@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from diskmule_b200 import CudaContext
+from diskmule_b200 import CudaContext, _native as N
+from diskmule_b200.attention import KvCache, offsets
 from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode
 
 pytestmark = pytest.mark.gpu
@@ -80,8 +81,6 @@ def test_decode_shared_tokens_that_no_sequence_has_in_full(ctx, heads, kv, dim, 
 def test_decode_after_a_row_of_the_batch_is_freed(ctx):
     """A finished sample keeps its place in the batch: its freed row gives zeros, the others
     what they gave before."""
-    from diskmule_b200 import _native as N
-    from diskmule_b200.attention import KvCache, offsets
     n, kv, dim, batch = 1060, 8, 128, 24
     cache = KvCache(ctx, type=N.BF16, layers=1, kv_heads=kv, head_dim=dim, page_tokens=16, pages=200,
                     max_sequences=batch + 1, max_pages=80)
@@ -108,3 +107,46 @@ def test_decode_after_a_row_of_the_batch_is_freed(ctx):
     assert cache.status() == 0
     assert torch.equal(results[0][1:], results[1][1:]) and (results[1][0] == 0).all()
     cache.close()
+
+
+def decode(pool, q, layer, shared, longest, **kw):
+    """As run_decode, with the cache's status bits beside the results."""
+    out, lse = torch.full_like(q, float("nan")), torch.full(q.shape[:2], float("nan"), device="cuda")
+    n = pool.cache.decode_workspace(q.shape[1], q.shape[0], shared, longest)
+    work = torch.full((max(n, 16),), 0xff, dtype=torch.uint8, device="cuda")
+    args = dict(layer=layer, heads=q.shape[1], q=q.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
+                batch=q.shape[0], max_length=longest, shared_tokens=shared, workspace=work.data_ptr(),
+                workspace_bytes=n)
+    pool.cache.decode_attention(**{**args, **kw})
+    torch.cuda.synchronize()
+    return out, lse, pool.cache.status()
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,batch,shared", SHORT_FIRST)
+@pytest.mark.parametrize("number", [-1, 1 << 30])
+def test_decode_reports_pages_outside_the_pool(ctx, heads, kv, dim, page, batch, shared, number):
+    lens = [shared + 3 + 11 * i % 70 for i in range(batch)]
+    pool = as_left_behind(Pool(ctx, torch.float16, kv, dim, page, shared, lens, seed=batch + 2))
+    q = normal(generator(7), (batch, heads, dim), torch.float16, 2.0)
+    want, want_lse, status = decode(pool, q, 0, shared, max(lens))
+    assert status == 0
+    # a page of one sequence's own tokens: its row is told of, the others stay
+    last = (lens[1] - 1) // page
+    mapped = int(pool.table[1, last])
+    pool.table[1, last] = number
+    out, lse, status = decode(pool, q, 0, shared, max(lens))
+    assert status == N.KV_BAD_TOKEN
+    rest = [0] + list(range(2, batch))
+    assert torch.equal(out[rest], want[rest]) and torch.equal(lse[rest], want_lse[rest])
+    assert torch.isfinite(out[1]).all()
+    pool.table[1, last] = mapped
+    # a page of the shared tokens
+    saved = pool.table.clone()
+    pool.table[:, shared // page // 2] = number
+    out, lse, status = decode(pool, q, 0, shared, max(lens))
+    assert status == N.KV_BAD_TOKEN and torch.isfinite(out).all()
+    # behind the end of every sequence: nobody asks
+    pool.table.copy_(saved)
+    pool.table[:, -1] = number
+    out, lse, status = decode(pool, q, 0, shared, max(lens))
+    assert status == 0 and torch.equal(out, want) and torch.equal(lse, want_lse)
