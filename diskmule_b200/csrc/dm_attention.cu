@@ -247,6 +247,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   float ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
   const float scale = MODE == kPrompt ? p.scale : d.scale;
+  constexpr float kRoom = kRowsHeadroom<BF16>;
 
   constexpr int kStep = kWarps * kChunk;
   int key_load = first + warp * kChunk;
@@ -307,8 +308,8 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, x));
       nb = fmaxf(nb, __shfl_xor_sync(0xffffffffu, nb, x));
     }
-    // The sums refer to the exact maxima: the largest weight, which has the most say, is then 1
-    // and rounds to 16 bits without an error. Once the maxima have settled nothing is rescaled.
+    // The sums refer to the exact maxima: the largest weight, which has the most say, is then a
+    // power of two and rounds to 16 bits without an error. Once the maxima have settled nothing is rescaled.
     const bool ga = na > ma, gb = nb > mb;
     if (__any_sync(0xffffffffu, ga || gb)) {
       const float fa = ga ? exp2_fast(ma - na) : 1.0f, fb = gb ? exp2_fast(mb - nb) : 1.0f;
@@ -319,7 +320,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       for (int i = 0; i < DP / 8; i++) o[i][0] *= fa, o[i][1] *= fa, o[i][2] *= fb, o[i][3] *= fb;
     }
     // a row that has seen nothing yet keeps a zero reference
-    const float za = ma == -INFINITY ? 0.0f : ma, zb = mb == -INFINITY ? 0.0f : mb;
+    const float za = ma == -INFINITY ? 0.0f : ma - kRoom, zb = mb == -INFINITY ? 0.0f : mb - kRoom;
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -392,8 +393,8 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     *reinterpret_cast<float2 *>(join + rb8 * DP + col) = make_float2(o[n][2], o[n][3]);
   }
   if ((lane & 3) == 0) {
-    sh.ml[warp][ra] = make_float2(ma, la);
-    sh.ml[warp][rb8] = make_float2(mb, lb);
+    sh.ml[warp][ra] = make_float2(ma - kRoom, la);
+    sh.ml[warp][rb8] = make_float2(mb - kRoom, lb);
   }
   __syncthreads();
   // All of it is done before the kernel after this one may read the parts of both.

@@ -1,9 +1,10 @@
 // dm_attention.cuh -- shared parts of the attention kernels (include/diskmule_attention.h).
 //
-// All of them keep, per query row, the running maximum m of the scores (times log2 e), the
-// running sum l of 2^(score - m) and the output sum o of 2^(score - m) v, in f32. Two such
-// states over disjoint keys join as m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), o
-// likewise; the result is o / l and lse = (m + log2 l) ln 2.
+// All of them keep, per query row, a reference m (the running maximum of the scores times
+// log2 e, less a constant for f16), the sum l of 2^(score - m) and the output sum o of
+// 2^(score - m) v, in f32. Two such states over disjoint keys join as m = max(m1, m2),
+// l = l1 2^(m1 - m) + l2 2^(m2 - m), o likewise, whatever their references are; the result is
+// o / l and lse = (m + log2 l) ln 2.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -65,6 +66,16 @@ __device__ __forceinline__ float log2_fast(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Weights are rounded to 16 bits for the product with V. f16 has its full precision from 2^-14
+// to 2^16 only: with the largest weight at 1, keys whose weights lie below 2^-14 would lose
+// bits and those below 2^-25 be gone, however many they are. So f16 weights are 2^(score -
+// maximum + headroom), as large as the type takes: 2^15, and 2^7 on tiles, whose reference may
+// lie 2^8 below the maximum. bf16 has the range of f32.
+template <bool BF16>
+constexpr float kRowsHeadroom = BF16 ? 0.0f : 15.0f;
+template <bool BF16>
+constexpr float kTileHeadroom = BF16 ? 0.0f : 7.0f;
 
 // two f32 -> two 16-bit values, `low` in the low half
 template <bool BF16>

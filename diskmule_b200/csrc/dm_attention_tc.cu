@@ -7,8 +7,8 @@
 //   P = 2^(S - m)   one thread per row: maximum, exponentials, sum, all f32
 //   O += P V        tcgen05.mma, P in tensor memory, V as it lies (keys down, dim across)
 // m is the running maximum with slack: O and l are rescaled only where the maximum has grown
-// by more than 2^8 since m was taken; until then the weights of newer keys may reach 2^8,
-// which changes no relative rounding, and the common factor leaves in o / l.
+// by more than 2^8 since m was taken; until then the weights of newer keys may reach 2^8 (f16:
+// 2^15, see kTileHeadroom), and the common factor leaves in o / l.
 //
 // The threads of a unit should never wait for products. So S of the next tile is computed
 // while the weights of this one are: P has columns of its own beside S, and tensor memory
@@ -28,9 +28,10 @@
 // keys, one per unit 4100; so it is 1750 for 80, 2800 for 128.)
 //
 // Weights are rounded to 16 bits, once, because both operands of a product have one type; the
-// sum l takes them unrounded. Weights of the largest scores lie between 2^-8 and 2^8, so each is
-// off by half a unit in its last place: an error of the result that is no larger than its own
-// rounding where one key has most of the weight, and averages out where many have.
+// sum l takes them unrounded. They lie where the type has all its bits (f16: down to 2^-21 of the
+// reference's), so each is off by half a unit in its last place: an error of the result that is
+// no larger than its own rounding where one key has most of the weight, and averages out where
+// many have.
 //
 // Measured, causal 16384 tokens, 16 heads of dim 128: 807 us, 1.36 PFLOP/s; without a mask 8192
 // keys, dim 256 1.47, dim 64 0.74. What bounds it: dim 128, 1750 cycles a
@@ -668,6 +669,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     const uint32_t o_at = tmem + lanes + Cfg::kOCol + unit * DP;
     const float c = MODE == kTcPrompt ? a.p.scale : a.d.scale;
     const uint64_t cc = pair(c, c);
+    constexpr float kRoom = kTileHeadroom<BF16>;
     const int dim = MODE == kTcPrompt ? a.p.dim : a.c.head_dim;
     int number = 0;  // tiles of this unit so far
     for (int items = 0; ok; items++) {
@@ -740,7 +742,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           l *= f;
           if (grows) m = now;
         }
-        const float z = m == -INFINITY ? 0.0f : -m * c;
+        const float z = m == -INFINITY ? 0.0f : kRoom - m * c;
         const uint64_t zz = pair(z, z);
         // the last product that reads these columns is done
         const int which = p_of(unit, number), round = p_round(number);
@@ -842,9 +844,9 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
       if (valid && final) {
         float *lse = MODE == kTcPrompt ? a.p.lse : a.d.lse;
-        if (lse) lse[index] = l == 0.0f ? -INFINITY : (m * c + log2_fast(l)) * kLn2;
+        if (lse) lse[index] = l == 0.0f ? -INFINITY : (m * c - kRoom + log2_fast(l)) * kLn2;
       } else if (valid) {
-        a.d.part.ml[part_at] = make_float2(m * c, l);
+        a.d.part.ml[part_at] = make_float2(m * c - kRoom, l);
       }
       fence_before();  // O has been read before the next item's weights are announced
       __syncwarp();

@@ -6,9 +6,10 @@ import numpy as np
 import pytest
 import torch
 
+from attention_plain import EPS, check_rows, row, to64
 from diskmule_b200 import CudaContext, _native as N
 from diskmule_b200.attention import KvCache, offsets
-from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode
+from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode, run_prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +151,60 @@ def test_decode_reports_pages_outside_the_pool(ctx, heads, kv, dim, page, batch,
     pool.table[:, -1] = number
     out, lse, status = decode(pool, q, 0, shared, max(lens))
     assert status == 0 and torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+# One key has nearly all the weight and a value of zero (an attention sink): the result is what
+# the many others bring, each of a weight that f16 can hold only next to a larger reference.
+# Weights are off by half of f16's last subnormal place at most, 2^-25, where the largest is 2^7
+# (tiles) or 2^15: 2^-32 of the largest.
+def sink_row(q, k, v, dtype):
+    out, lse, bound, lse_bound = row(q, k, v, 1.0, EPS[dtype])
+    s = k @ q
+    places = len(s) * np.abs(v).max() / math.exp(lse - s.max())
+    assert np.abs(out).min() > 100 * 2.0 ** -32 * places / len(s)
+    return out, lse, bound + (2.0 ** -32 - 2.0 ** -25) * places, lse_bound
+
+
+def sink_values(gen, n, gap, place, dim, dtype):
+    """Keys whose scores under q = (4, 0, ...) are 0 for the sink and -gap to -gap - 1 else."""
+    k, v = torch.zeros(n, dim, device="cuda"), 20 + 20 * torch.rand(n, dim, generator=gen, device="cuda")
+    k[:, 0] = -(gap + torch.rand(n, generator=gen, device="cuda")) / 4
+    k[place, 0], v[place] = 0.0, 0.0
+    return k.to(dtype), v.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("gap,place", [(16, 0), (16, 9000), (19, 0), (19, 16383)])
+def test_prompt_beside_a_sink(ctx, dtype, dim, gap, place):
+    n, lq = 16384, 40
+    k, v = sink_values(generator(dim), n, gap, place, dim, dtype)
+    q = torch.zeros(lq, 2, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 4.0
+    for heads_stride in (dim, 0):  # tiles, and blocks of 16 rows
+        out, lse = run_prompt(ctx, q, k[:, None], v[:, None], [lq], [n], causal=False, scale=1.0,
+                              k_stride=(dim, heads_stride), v_stride=(dim, heads_stride))
+        want = sink_row(to64(q[0, 0]), to64(k), to64(v), dtype)
+        check_rows(out, lse, [((i, h), want) for i in range(lq) for h in range(2)], "sink")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("batch,heads,shared", [(16, 8, 12288), (2, 4, 12288), (1, 4, 0)])
+def test_decode_beside_a_sink(ctx, dtype, dim, batch, heads, shared):
+    n, page = 16384, 64
+    pool = Pool(ctx, dtype, 1, dim, page, shared, [n] * batch, layers=1, seed=51)
+    keys = []
+    for b in range(batch):
+        k, v = sink_values(generator(b), n, 17, 0, dim, dtype)
+        if b and shared:
+            k[:shared], v[:shared] = keys[0][0][:shared], keys[0][1][:shared]
+        keys.append((k, v))
+        ids = pool.table[b, :n // page].long()
+        pool.memory[ids, 0, 0, 0], pool.memory[ids, 0, 1, 0] = k.view(-1, page, dim), v.view(-1, page, dim)
+    q = torch.zeros(batch, heads, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = 4.0
+    out, lse = run_decode(pool, q, 0, shared, n, scale=1.0)
+    for b, (k, v) in enumerate(keys):
+        want = sink_row(to64(q[b, 0]), to64(k), to64(v), dtype)
+        check_rows(out, lse, [((b, h), want) for h in range(heads)], "sink")
