@@ -25,9 +25,9 @@ using namespace dm::tc;
 //
 // Bound by memory where there is enough to read: 64 sequences of 1500 own tokens, 8 key/value
 // heads of dim 128, 67 us, 5.9 TB/s; 256 of them 236 us, 6.7. Small calls are latency (table,
-// queries, keys, join of the warps): 2 sequences of 200 tokens 5 us. Weights are rounded to 16 bits before the product (its operands have
-// one type), the sums are not. A tensor without a tensor map (a stride of zero) takes this
-// kernel for prompts, too.
+// queries, keys, join of the warps): 2 sequences of 200 tokens 5 us. Weights are rounded to 16
+// bits before the product (its operands have one type), the sums are not. Prompts whose tensors
+// are broadcast (a stride of zero) take this kernel, too.
 // ---------------------------------------------------------------------------
 
 constexpr int kRows = 16;    // query rows of a block: one mma tile

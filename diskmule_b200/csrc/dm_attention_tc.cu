@@ -939,7 +939,7 @@ bool aligned32(const uint16_t *p, const int64_t *stride) {
 }  // namespace
 
 bool tile_prompt_fits(const PromptArgs &p) {
-  // a broadcast tensor (stride 0) has no tensor map
+  // broadcast tensors (stride 0) go to blocks of 16 rows, as strides that no map holds
   for (const int64_t *s : {p.q_stride, p.k_stride, p.v_stride})
     if (s[0] <= 0 || s[1] <= 0 || s[0] >= (int64_t)1 << 37 || s[1] * p.group >= (int64_t)1 << 37) return false;
   return p.k_tokens > 0;

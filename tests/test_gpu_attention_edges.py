@@ -112,7 +112,8 @@ def test_decode_after_a_row_of_the_batch_is_freed(ctx):
 
 def decode(pool, q, layer, shared, longest, **kw):
     """As run_decode, with the cache's status bits beside the results."""
-    out, lse = torch.full_like(q, float("nan")), torch.full(q.shape[:2], float("nan"), device="cuda")
+    out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
+    lse = torch.full(q.shape[:2], float("nan"), device="cuda")
     n = pool.cache.decode_workspace(q.shape[1], q.shape[0], shared, longest)
     work = torch.full((max(n, 16),), 0xff, dtype=torch.uint8, device="cuda")
     args = dict(layer=layer, heads=q.shape[1], q=q.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
@@ -208,3 +209,26 @@ def test_decode_beside_a_sink(ctx, dtype, dim, batch, heads, shared):
     for b, (k, v) in enumerate(keys):
         want = sink_row(to64(q[b, 0]), to64(k), to64(v), dtype)
         check_rows(out, lse, [((b, h), want) for h in range(heads)], "sink")
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,batch,shared", SHORT_FIRST)
+@pytest.mark.parametrize("broadcast", ["rows", "heads", "no"])
+def test_decode_broadcast_queries(ctx, heads, kv, dim, page, batch, shared, broadcast):
+    """One query row for the whole batch, one for all heads: whatever the sizes, the call runs
+    (and gives what it gives for rows and heads apart)."""
+    lens = [shared + 1 + 9 * i % 50 for i in range(batch)]
+    pool = as_left_behind(Pool(ctx, torch.bfloat16, kv, dim, page, shared, lens, seed=batch + 3))
+    gen = generator(9)
+    if broadcast == "rows":
+        q = normal(gen, (1, heads, dim), torch.bfloat16, 2.0).expand(batch, heads, dim)
+        stride = (0, dim)
+    elif broadcast == "heads":
+        q = normal(gen, (batch, 1, dim), torch.bfloat16, 2.0).expand(batch, heads, dim)
+        stride = (dim, 0)
+    else:
+        q = normal(gen, (batch, heads, dim), torch.bfloat16, 2.0)
+        q = torch.empty(batch, heads, 2, dim, dtype=q.dtype, device="cuda")[:, :, 1].copy_(q)
+        stride = q.stride()[:2]
+    out, lse, status = decode(pool, q, 1, shared, max(lens), q_stride=stride, out_stride=(heads * dim, dim))
+    assert status == 0
+    check_decode(pool, q, 1, out, lse)
