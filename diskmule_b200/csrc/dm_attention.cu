@@ -688,6 +688,11 @@ uint64_t decode_workspace(const DecodePlan &plan, int64_t rows, int dim) {
 
 using namespace dma;
 
+// A caller's bound on lengths, and what a row of the page table holds.
+static int32_t bounded_length(const dm_kv_cache_desc &d, int32_t max_length) {
+  return (int32_t)std::min<int64_t>(max_length, (int64_t)d.max_pages * d.page_tokens);
+}
+
 static int32_t check_strides(const int64_t *given, int64_t heads, int dim, int64_t *use, const char *what) {
   const bool none = given[0] == 0 && given[1] == 0;
   use[0] = none ? heads * dim : given[0];
@@ -767,7 +772,8 @@ int32_t dm_attention_decode_workspace(const dm_kv_cache *cache, int32_t heads, i
   if (shared_tokens < 0 || shared_tokens % d.page_tokens || shared_tokens > (int64_t)d.max_pages * d.page_tokens)
     return fail(DM_ERR_ELEMENT_COUNT, "%d shared tokens are no whole pages of the table", shared_tokens);
   if (max_length < 0) return fail(DM_ERR_ELEMENT_COUNT, "max_length %d", max_length);
-  *bytes = decode_workspace(decode_plan(d.kv_heads, heads, d.head_dim, batch, shared_tokens, max_length),
+  *bytes = decode_workspace(decode_plan(d.kv_heads, heads, d.head_dim, batch, shared_tokens,
+                                        bounded_length(d, max_length)),
                             (int64_t)batch * heads, d.head_dim);
   return DM_OK;
 }
@@ -804,8 +810,8 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
   a.batch = in->batch;
   a.layer = in->layer;
   a.window = in->window;
-  a.max_length = in->max_length;
-  const DecodePlan plan = decode_plan(kd.kv_heads, in->heads, kd.head_dim, in->batch, in->shared_tokens, in->max_length);
+  a.max_length = bounded_length(kd, in->max_length);
+  const DecodePlan plan = decode_plan(kd.kv_heads, in->heads, kd.head_dim, in->batch, in->shared_tokens, a.max_length);
   a.shared = plan.shared;
   a.part.parts = plan.parts();
   a.part.rows = (int64_t)in->batch * in->heads;

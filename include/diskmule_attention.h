@@ -136,9 +136,10 @@ DM_API int32_t dm_kv_cache_copy_pages(dm_kv_cache *cache, const int32_t *source,
  * be 0) of every sequence in the batch lie in the same pages; they are read once, or by each
  * sequence where that is sooner done. A sequence shorter than that sees what it has, wherever
  * it stands in the batch; a row number outside the table is an empty sequence. max_length
- * bounds every lengths[sequences[b]]; tokens beyond it are not read. workspace is 16-byte
- * aligned scratch of at least dm_attention_decode_workspace bytes for the same numbers; two
- * calls in flight need two. A page number outside the pool reads as keys and values of zero
+ * bounds every lengths[sequences[b]]; tokens beyond it are not read. (The closer it is, the
+ * better the work can be cut; what the page table holds is a bound in any case.) workspace is
+ * 16-byte aligned scratch of at least dm_attention_decode_workspace bytes for the same numbers;
+ * two calls in flight need two. A page number outside the pool reads as keys and values of zero
  * and sets DM_KV_BAD_TOKEN. */
 typedef struct {
   int32_t layer, heads, batch, window;

@@ -232,3 +232,20 @@ def test_decode_broadcast_queries(ctx, heads, kv, dim, page, batch, shared, broa
     out, lse, status = decode(pool, q, 1, shared, max(lens), q_stride=stride, out_stride=(heads * dim, dim))
     assert status == 0
     check_decode(pool, q, 1, out, lse)
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,batch,shared", SHORT_FIRST + [(8, 2, 128, 16, 3, 0), (64, 8, 128, 64, 9, 0)])
+def test_decode_without_a_bound_on_lengths(ctx, heads, kv, dim, page, batch, shared):
+    """A max_length beyond the table is the table's: the same workspace and the same result."""
+    lens = [shared + 1 + 9 * i % 50 for i in range(batch)]
+    pool = as_left_behind(Pool(ctx, torch.bfloat16, kv, dim, page, shared, lens, seed=batch + 4))
+    most = pool.columns * page
+    need = pool.cache.decode_workspace(heads, batch, shared, most)
+    q = normal(generator(11), (batch, heads, dim), torch.bfloat16, 2.0)
+    want, want_lse, status = decode(pool, q, 0, shared, most)
+    assert status == 0
+    check_decode(pool, q, 0, want, want_lse)
+    for bound in (most + 1, 1 << 20, 2 ** 31 - 100, 2 ** 31 - 1):
+        assert pool.cache.decode_workspace(heads, batch, shared, bound) == need
+        out, lse, status = decode(pool, q, 0, shared, bound)
+        assert status == 0 and torch.equal(out, want) and torch.equal(lse, want_lse)
