@@ -140,12 +140,11 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       const int token = (int)(r / group), head = kv_head * group + (int)(r % group);
       const int64_t at = t.q0 + token;
       const bool valid = token < lq;
-      const int place = token + lk - lq;
       sh.q[tid] = valid ? at * p.q_stride[0] + head * p.q_stride[1] : -1;
       sh.out[tid] = at * p.out_stride[0] + head * p.out_stride[1];
       sh.index[tid] = at * p.heads + head;
-      sh.low[tid] = p.window ? max(0, place - p.window + 1) : 0;
-      sh.high[tid] = p.causal ? max(0, min(lk, place + 1)) : lk;
+      sh.low[tid] = low_of(p, lq, lk, token);
+      sh.high[tid] = high_of(p, lq, lk, token);
     }
   } else {
     const int rows = MODE == kOwn ? group : d.batch * group;

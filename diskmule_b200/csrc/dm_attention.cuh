@@ -41,6 +41,16 @@ struct PartArgs {
   int64_t rows;
 };
 
+// Token i of lq stands at key place_of(); it sees the keys [low_of(), high_of()). Lengths and
+// window may be anything up to 2^31, so no sum may exceed the larger of its terms.
+__device__ __forceinline__ int place_of(int lq, int lk, int i) { return i - lq + lk; }
+__device__ __forceinline__ int low_of(const PromptArgs &p, int lq, int lk, int i) {
+  return p.window ? max(0, max(0, place_of(lq, lk, i)) - (p.window - 1)) : 0;
+}
+__device__ __forceinline__ int high_of(const PromptArgs &p, int lq, int lk, int i) {
+  return p.causal ? max(0, min(lk, place_of(lq, lk, i) + 1)) : lk;
+}
+
 struct DecodeArgs {
   const uint16_t *q;
   uint16_t *out;

@@ -264,14 +264,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// The keys [low, high) that token i of an item's sequence sees.
-__device__ __forceinline__ int low_of(const PromptArgs &p, int lq, int lk, int i) {
-  return p.window ? max(0, i + lk - lq - p.window + 1) : 0;
-}
-__device__ __forceinline__ int high_of(const PromptArgs &p, int lq, int lk, int i) {
-  return p.causal ? max(0, min(lk, i + lk - lq + 1)) : lk;
-}
-
 // Whether some row does not see some key of tile t.
 template <int KEYS>
 __device__ __forceinline__ bool mixed(const Item &w, int t) {

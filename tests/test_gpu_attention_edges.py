@@ -249,3 +249,19 @@ def test_decode_without_a_bound_on_lengths(ctx, heads, kv, dim, page, batch, sha
         assert pool.cache.decode_workspace(heads, batch, shared, bound) == need
         out, lse, status = decode(pool, q, 0, shared, bound)
         assert status == 0 and torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lq,lk", [([300], [20]), ([50, 9], [20, 0]), ([40], [400]), ([129, 1], [129, 1])])
+def test_prompt_window_that_hides_nothing(ctx, dim, causal, lq, lk):
+    """However wide the window, also where queries stand before the first key."""
+    gen = generator(dim)
+    q = normal(gen, (sum(lq), 4, dim), torch.bfloat16, 2.0)
+    k, v = (normal(gen, (max(1, sum(lk)), 1, dim), torch.bfloat16) for _ in range(2))
+    for heads_stride in (dim, 0):  # tiles, and blocks of 16 rows
+        strides = dict(k_stride=(dim, heads_stride), v_stride=(dim, heads_stride))
+        want, want_lse = run_prompt(ctx, q, k, v, lq, lk, causal, 0, **strides)
+        for window in (sum(lk) + sum(lq) + 1, 2 ** 31 - 300, 2 ** 31 - 10, 2 ** 31 - 1):
+            out, lse = run_prompt(ctx, q, k, v, lq, lk, causal, window, **strides)
+            assert torch.equal(out, want) and torch.equal(lse, want_lse)
