@@ -722,7 +722,7 @@ int32_t dm_attention_prompt(dm_cuda_context *ctx, const dm_attention_prompt_desc
     return fail(DM_ERR_ELEMENT_COUNT, "head_dim %d is not a multiple of 8 up to 256", in->head_dim);
   if (in->sequences < 0 || in->window < 0)
     return fail(DM_ERR_ELEMENT_COUNT, "%d sequences, window %d", in->sequences, in->window);
-  if (in->q_tokens < 0 || in->k_tokens < 0 || in->q_tokens > INT32_MAX || in->k_tokens > INT32_MAX)
+  if (in->q_tokens < 0 || in->k_tokens < 0 || in->q_tokens > kMostTokens || in->k_tokens > kMostTokens)
     return fail(DM_ERR_ELEMENT_COUNT, "a bad number of tokens");
   if (in->sequences == 0 || in->q_tokens == 0) return DM_OK;
   if (!in->q || !in->out || !in->q_offsets || (in->k_tokens && (!in->k || !in->v)))

@@ -545,8 +545,8 @@ int32_t dm_kv_cache_create(dm_cuda_context *ctx, const dm_kv_cache_desc *d, dm_k
   // rows of a page are counted in 32 bits, and a table row's tokens fit a length
   if (layer_bytes > ((int64_t)1 << 32) / d->layers || (int64_t)d->layers * 2 * d->kv_heads > INT32_MAX)
     return fail(DM_ERR_OVERFLOW, "a page of more than 4 GB");
-  if ((int64_t)d->max_pages * d->page_tokens > INT32_MAX)
-    return fail(DM_ERR_OVERFLOW, "a sequence of more than 2^31 tokens");
+  if ((int64_t)d->max_pages * d->page_tokens > dma::kMostTokens)
+    return fail(DM_ERR_OVERFLOW, "a sequence of more than %d tokens", dma::kMostTokens);
   if ((uintptr_t)d->memory & 15)
     return fail(DM_ERR_INVALID_ARGUMENT, "cache memory must be 16-byte aligned");
   dm_kv_cache *c = new (std::nothrow) dm_kv_cache;

@@ -11,6 +11,10 @@
 
 namespace dma {
 
+// Tokens of a sequence or a packed tensor at most: kernels step past the last one by up to a few
+// hundred, in 32 bits.
+constexpr int32_t kMostTokens = INT32_MAX - 4096;
+
 // What kernels see of a cache. Byte strides; every row of head_dim values is 16-byte aligned.
 struct KvView {
   uint8_t *memory;

@@ -14,6 +14,7 @@
  *   - query head h reads key/value head h / (heads / kv_heads);
  *   - lse (optional) is the natural logarithm of a row's sum of exp(score), f32; a row that
  *     sees no key gets zeros and -infinity;
+ *   - a sequence, and a packed tensor, has at most 2^31 - 4097 tokens;
  *   - what a mask hides has no influence, whatever it holds (NaN and infinities included);
  *   - calls are stream-ordered, allocate nothing and may be captured into a CUDA graph;
  *   - arguments are checked before any launch; what only the device can see is range-checked

@@ -7,8 +7,8 @@ import pytest
 import torch
 
 from attention_plain import EPS, check_rows, row, to64
-from diskmule_b200 import CudaContext, _native as N
-from diskmule_b200.attention import KvCache, offsets
+from diskmule_b200 import CudaContext, DmError, _native as N
+from diskmule_b200.attention import KvCache, offsets, prompt_attention
 from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode, run_prompt
 
 pytestmark = pytest.mark.gpu
@@ -265,3 +265,18 @@ def test_prompt_window_that_hides_nothing(ctx, dim, causal, lq, lk):
         for window in (sum(lk) + sum(lq) + 1, 2 ** 31 - 300, 2 ** 31 - 10, 2 ** 31 - 1):
             out, lse = run_prompt(ctx, q, k, v, lq, lk, causal, window, **strides)
             assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_more_tokens_than_kernels_can_count_are_refused(ctx):
+    """Kernels step past the last token in 32 bits; the limit leaves them room."""
+    with pytest.raises(DmError) as e:
+        KvCache(ctx, type=N.BF16, layers=1, kv_heads=1, head_dim=8, page_tokens=16, pages=4, max_sequences=1,
+                max_pages=(1 << 27) - 1)
+    assert e.value.status == N.ERR_OVERFLOW
+    t, o = torch.zeros(16, 8, dtype=torch.bfloat16, device="cuda"), ints([0, 1])
+    p = t.data_ptr()
+    for q_tokens, k_tokens in ((2 ** 31 - 4096, 16), (16, 2 ** 31 - 1)):
+        with pytest.raises(DmError) as e:
+            prompt_attention(ctx, type=N.BF16, heads=1, kv_heads=1, head_dim=8, q=p, k=p, v=p, out=p,
+                             q_tokens=q_tokens, k_tokens=k_tokens, sequences=1, q_offsets=o.data_ptr())
+        assert e.value.status == N.ERR_ELEMENT_COUNT
