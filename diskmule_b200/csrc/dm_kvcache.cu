@@ -199,6 +199,17 @@ __device__ int leading_same(const int32_t *keep, int count) {
   return low;
 }
 
+// Whether keep[j] opens an entry's list; offsets that do not ascend give any answer.
+__device__ bool opens_entry(const int32_t *offsets, int n, int64_t j) {
+  int low = 0, high = n;  // offsets[low] <= j
+  while (low < high) {
+    const int mid = (low + high + 1) >> 1;
+    if (offsets[mid] <= j) low = mid;
+    else high = mid - 1;
+  }
+  return offsets[low] == j;
+}
+
 // One block. ok = 1 and the plan where the whole call can be done, else 0 and a status bit.
 // Extend has no rows to move and is done here.
 template <int OP>
@@ -228,7 +239,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
         const int row = a.rows[i];
         const int k0 = a.other[i], count = a.other[i + 1] - k0;
         if (k0 < 0 || count < 0 || (int64_t)k0 + count > a.kept || count > c.lengths[row] ||
-            c.lengths[row] > c.max_pages * (int64_t)c.page_tokens) {
+            c.lengths[row] > c.max_pages * (int64_t)c.page_tokens ||
+            (count > 0 && (a.keep[k0] < 0 || a.keep[k0 + count - 1] >= c.lengths[row]))) {
           if ((tid & 31) == 0) atomicOr(&bad, DM_KV_BAD_TOKEN);
           continue;
         }
@@ -244,6 +256,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
         }
         if ((tid & 31) == 0) p.stay[i] = stay, p.moved[i] = 0;
       }
+      // Between its first and last token, which are in range, an entry's list ascends. All
+      // lists in one pass: a step down is rare where no new entry begins.
+      const int64_t end = min((int64_t)a.other[a.n], a.kept) - 1;
+      bool down = false;
+#pragma unroll 4
+      for (int64_t j = max(a.other[0], 0) + tid; j < end; j += kPlanThreads)
+        if (a.keep[j] >= a.keep[j + 1]) down |= !opens_entry(a.other, a.n, j + 1);
+      if (down) atomicOr(&bad, DM_KV_BAD_TOKEN);
       __syncthreads();
     }
     for (int i0 = 0; i0 < a.n; i0 += kPlanThreads) {
@@ -368,18 +388,11 @@ gather_kernel(KvView c, Plan p, PlanArgs a) {
     const int k0 = a.other[i], count = a.other[i + 1] - k0;
     const int j0 = (p.stay[i] + f - p.first[i]) * c.page_tokens;
     const int used = min(c.page_tokens, count - j0);
-    const int length = c.lengths[row];
     for (int r = threadIdx.x; r < used; r += kCopyThreads) {
       const int token = a.keep[k0 + j0 + r];
-      int64_t at = -1;
-      if (token < 0 || token >= length) {
-        atomicOr(c.status, DM_KV_BAD_TOKEN);
-      } else {
-        const int page = c.table[(int64_t)row * c.max_pages + token / c.page_tokens];
-        if ((unsigned)page < (unsigned)c.pages)
-          at = page * c.page_bytes + (int64_t)(token % c.page_tokens) * c.head_dim * 2;
-      }
-      source[r] = at;
+      const int page = c.table[(int64_t)row * c.max_pages + token / c.page_tokens];
+      source[r] = (unsigned)page < (unsigned)c.pages
+                      ? page * c.page_bytes + (int64_t)(token % c.page_tokens) * c.head_dim * 2 : -1;
     }
     __syncthreads();
     uint8_t *dst = c.memory + p.fresh[f] * c.page_bytes;

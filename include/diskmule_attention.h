@@ -74,9 +74,9 @@ DM_API int32_t dm_attention_status(dm_cuda_context *ctx, void *stream);
  * caller's and are taken as they are. page_tokens is a power of two from 16 to 256.
  *
  * The calls below take device int32 lists and update the tables on the device. Pages are
- * handed out in list order, the lowest free page first. A call that needs more pages than
- * are free, or whose list holds a bad or repeated sequence, changes nothing and sets a bit
- * of the status word. Calls on one cache are ordered by the caller (one stream, or events).
+ * handed out in list order, the lowest free page first. Extend, fork and compact change
+ * nothing and set a bit of the status word where they need more pages than are free, or where
+ * a list holds a bad or repeated sequence, a bad count or a token out of range or order. Calls on one cache are ordered by the caller (one stream, or events).
  * A last page that is only partly filled belongs to one sequence alone. */
 typedef struct {
   int32_t type, layers, kv_heads, head_dim, page_tokens, pages, max_sequences, max_pages;
@@ -88,7 +88,7 @@ enum {
   DM_KV_OUT_OF_PAGES = 1,  /* not enough free pages */
   DM_KV_BAD_SEQUENCE = 2,  /* out of range, named twice, or a fork target that is not empty */
   DM_KV_TOO_LONG = 4,      /* a sequence would outgrow its row of the page table */
-  DM_KV_BAD_TOKEN = 8,     /* a token position, count, offset or page outside its range */
+  DM_KV_BAD_TOKEN = 8,     /* a token position, count, offset or page out of range or order */
 };
 
 DM_API int32_t dm_kv_cache_create(dm_cuda_context *ctx, const dm_kv_cache_desc *desc,

@@ -9,6 +9,7 @@ import torch
 from attention_plain import EPS, check_rows, row, to64
 from diskmule_b200 import CudaContext, DmError, _native as N
 from diskmule_b200.attention import KvCache, offsets, prompt_attention
+from test_gpu_kv_cache import Pair
 from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode, run_prompt
 
 pytestmark = pytest.mark.gpu
@@ -280,3 +281,63 @@ def test_more_tokens_than_kernels_can_count_are_refused(ctx):
             prompt_attention(ctx, type=N.BF16, heads=1, kv_heads=1, head_dim=8, q=p, k=p, v=p, out=p,
                              q_tokens=q_tokens, k_tokens=k_tokens, sequences=1, q_offsets=o.data_ptr())
         assert e.value.status == N.ERR_ELEMENT_COUNT
+
+
+# ---------------------------------------------------------------------------
+# the cache
+# ---------------------------------------------------------------------------
+
+BAD_KEEPS = {
+    "behind the end": lambda n: list(range(1, n - 1)) + [n],
+    "far behind the end": lambda n: list(range(0, 20)) + [2 ** 31 - 1],
+    "negative": lambda n: [-1] + list(range(1, 30)),
+    "twice": lambda n: list(range(0, 33)) + [32] + list(range(40, n)),
+    "down": lambda n: list(range(0, 17)) + [20, 19] + list(range(25, n)),
+    "first two": lambda n: [1, 0] + list(range(2, n)),
+    "last two": lambda n: list(range(0, n - 2)) + [n - 1, n - 2],
+    "out of range between": lambda n: list(range(0, 17)) + [n + 5] + list(range(18, n)),
+    "negative between": lambda n: list(range(0, 17)) + [-7] + list(range(18, n)),
+}
+
+
+@pytest.mark.parametrize("case", BAD_KEEPS)
+@pytest.mark.parametrize("others", [0, 1, 2, 40])
+def test_compact_refuses_tokens_out_of_range_or_order(ctx, case, others):
+    """Nothing of the call is done, whichever of its lists is wrong."""
+    t = Pair(ctx, layers=1, kv=1, dim=8, pages=900, seqs=48, max_pages=12)
+    n = 150
+    assert t.extend(list(range(41)), [n] * 41)
+    t.check()
+    good = [list(range(3, n, 2)) for _ in range(others)]
+    for place in sorted({0, others // 2, others}):
+        keeps = good[:place] + [BAD_KEEPS[case](n)] + good[place:]
+        s, o, k = ints(range(len(keeps))), ints(offsets([len(x) for x in keeps])), ints(np.concatenate(keeps))
+        t.cache.compact(s.data_ptr(), o.data_ptr(), k.data_ptr(), len(keeps), k.numel())
+        t.check(status=N.KV_BAD_TOKEN)
+
+
+def test_compact_of_lists_that_meet_in_any_way(ctx):
+    """What one list ends with says nothing about the next: empty lists between, at both ends,
+    equal tokens on both sides."""
+    t = Pair(ctx, layers=1, kv=1, dim=8, pages=200, seqs=12, max_pages=12)
+    assert t.extend(list(range(12)), [100] * 12)
+    keeps = [[], [99], [99], [0], [], [], list(range(50, 100)), list(range(50, 100)), [0, 99], [99], list(range(100)), []]
+    assert t.compact(list(range(12)), keeps)
+    t.check()
+
+
+def test_compact_long_lists(ctx):
+    """More kept tokens than one step of the check takes; a fault in each of its last places."""
+    t = Pair(ctx, layers=1, kv=1, dim=8, page=256, pages=300, seqs=3, max_pages=60)
+    n = 14000
+    assert t.extend([0, 1], [n, n])
+    keep = list(range(5, n))
+    s, o = ints([0, 1]), ints(offsets([len(keep)] * 2))
+    for at in (1, 1023, 4096, 5 * 1024, len(keep) - 2):
+        bad = list(keep)
+        bad[at] = bad[at - 1]
+        k = ints(keep + bad)
+        t.cache.compact(s.data_ptr(), o.data_ptr(), k.data_ptr(), 2, k.numel())
+        t.check(status=N.KV_BAD_TOKEN)
+    assert t.compact([0, 1], [keep, keep])
+    t.check()
