@@ -76,8 +76,10 @@ DM_API int32_t dm_attention_status(dm_cuda_context *ctx, void *stream);
  * The calls below take device int32 lists and update the tables on the device. Pages are
  * handed out in list order, the lowest free page first. Extend, fork and compact change
  * nothing and set a bit of the status word where they need more pages than are free, or where
- * a list holds a bad or repeated sequence, a bad count or a token out of range or order. Calls on one cache are ordered by the caller (one stream, or events).
- * A last page that is only partly filled belongs to one sequence alone. */
+ * a list holds a bad or repeated sequence, a bad count or a token out of range or order.
+ * Free, write and copy_pages do what can be done and set the bit for the rest; a sequence that
+ * is named twice is freed once. Calls on one cache are ordered by the caller (one stream, or
+ * events). A last page that is only partly filled belongs to one sequence alone. */
 typedef struct {
   int32_t type, layers, kv_heads, head_dim, page_tokens, pages, max_sequences, max_pages;
   void *memory;

@@ -341,3 +341,23 @@ def test_compact_long_lists(ctx):
         t.check(status=N.KV_BAD_TOKEN)
     assert t.compact([0, 1], [keep, keep])
     t.check()
+
+
+def test_calls_that_do_what_can_be_done(ctx):
+    """Free, write and copy_pages pass over what is out of range."""
+    t = Pair(ctx, seqs=6)
+    assert t.extend([0, 1, 2], [20, 20, 20])
+    rows = [torch.randint(-30000, 30000, (9, 2, 64), dtype=torch.int16, device="cuda") for _ in range(2)]
+    s, o = ints([1, 9, 0]), ints([0, 3, 6, 9])
+    t.cache.write(1, rows[0].data_ptr(), rows[1].data_ptr(), s.data_ptr(), o.data_ptr(), 3, 9)
+    kept = [torch.cat([x[:3], x[6:]]).cpu().numpy().view(np.uint16) for x in rows]
+    t.plain.write(1, *kept, [1, 0], [0, 3, 6])
+    t.check(status=N.KV_BAD_TOKEN)
+    src, dst = ints([0, 40, 1, -1]), ints([30, 31, 32, 33])
+    t.cache.copy_pages(src.data_ptr(), dst.data_ptr(), 4)
+    t.plain.pool[[30, 32]] = t.plain.pool[[0, 1]]
+    t.check(status=N.KV_BAD_TOKEN)
+    s = ints([0, 6, 2, 0])
+    t.cache.free(s.data_ptr(), 4)
+    t.plain.free([0, 2])
+    t.check(status=N.KV_BAD_SEQUENCE)
