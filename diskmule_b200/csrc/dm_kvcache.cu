@@ -57,14 +57,20 @@ __device__ __forceinline__ void chain() {
   dma::wait_for_previous();
 }
 
+// a + b of numbers that are not negative, at most INT32_MAX
+__device__ __forceinline__ int add_upto(int a, int b) {
+  return (int)min((unsigned)a + (unsigned)b, (unsigned)INT32_MAX);
+}
+
 // Inclusive sum over the block; `total` gets the block's. Every thread of the block calls it.
+// A sum beyond INT32_MAX stays there (entries may ask for more pages than that together).
 __device__ int block_scan(int v, int *total) {
   __shared__ int sums[kPlanThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    if (lane >= o) v = add_upto(v, u);
   }
   if (lane == 31) sums[warp] = v;
   __syncthreads();
@@ -72,12 +78,12 @@ __device__ int block_scan(int v, int *total) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
+    if (lane >= o) s = add_upto(s, u);
   }
   const int before = __shfl_sync(0xffffffffu, s, warp ? warp - 1 : 0);
   *total = __shfl_sync(0xffffffffu, s, 31);
   __syncthreads();
-  return v + (warp ? before : 0);
+  return warp ? add_upto(v, before) : v;
 }
 
 __device__ __forceinline__ int pages_for(const KvView &c, int tokens) {
@@ -295,12 +301,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
         if (wrong) atomicOr(&bad, wrong);
       }
       int sum;
-      const int upto = block_scan(need, &sum);
-      if (i < a.n) p.first[i] = total + upto - need;
-      if (total + sum <= c.pages)
-        for (int r = 0; r < need; r++) p.owner[total + upto - need + r] = i;
-      total += sum;
+      const int upto = block_scan(need, &sum), before = total;
+      total = add_upto(total, sum);
       if (total > c.pages) break;
+      if (i < a.n) p.first[i] = before + upto - need;
+      for (int r = 0; r < need; r++) p.owner[before + upto - need + r] = i;
     }
   }
   __syncthreads();
@@ -555,7 +560,8 @@ int32_t dm_kv_cache_create(dm_cuda_context *ctx, const dm_kv_cache_desc *d, dm_k
                 d->page_tokens);
   const int64_t head_bytes = (int64_t)d->page_tokens * d->head_dim * 2;
   const int64_t layer_bytes = head_bytes * 2 * d->kv_heads;
-  // rows of a page are counted in 32 bits, and a table row's tokens fit a length
+  // pages, rows of a page and a table row's tokens are counted in 32 bits
+  if (d->pages > 1 << 30) return fail(DM_ERR_OVERFLOW, "more than 2^30 pages");
   if (layer_bytes > ((int64_t)1 << 32) / d->layers || (int64_t)d->layers * 2 * d->kv_heads > INT32_MAX)
     return fail(DM_ERR_OVERFLOW, "a page of more than 4 GB");
   if ((int64_t)d->max_pages * d->page_tokens > dma::kMostTokens)

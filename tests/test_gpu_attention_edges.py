@@ -361,3 +361,23 @@ def test_calls_that_do_what_can_be_done(ctx):
     t.cache.free(s.data_ptr(), 4)
     t.plain.free([0, 2])
     t.check(status=N.KV_BAD_SEQUENCE)
+
+
+def test_more_pages_asked_for_than_32_bits_count(ctx):
+    """Entries that each fit their row of the table and together ask for more than 2^31 pages."""
+    rows, most, pages = 17, 134217471, 40
+    with pytest.raises(DmError) as e:
+        KvCache(ctx, type=N.BF16, layers=1, kv_heads=1, head_dim=8, page_tokens=16, pages=(1 << 30) + 1,
+                max_sequences=1, max_pages=1)
+    assert e.value.status == N.ERR_OVERFLOW
+    cache = KvCache(ctx, type=N.BF16, layers=1, kv_heads=1, head_dim=8, page_tokens=16, pages=pages,
+                    max_sequences=rows, max_pages=most)  # a table of 9 GB
+    s, c = ints(range(rows)), ints([most * 16] * rows)
+    assert rows * most > 2 ** 31
+    for n in range(1, rows + 1):
+        cache.extend(s.data_ptr(), c.data_ptr(), n)
+        assert cache.status() == N.KV_OUT_OF_PAGES
+    c = ints([16] * rows)
+    cache.extend(s.data_ptr(), c.data_ptr(), rows)
+    assert cache.status() == 0
+    cache.close()
