@@ -116,6 +116,7 @@ struct TcSmem {
   Item item[kItems];
   uint32_t tmem;
   volatile int abort;
+  volatile uint32_t loaded;  // chunks of K asked for
 };
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -245,17 +246,36 @@ __device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 __device__ __forceinline__ bool wait(TcSmem &sh, uint64_t &bar, uint32_t parity) {
+  constexpr unsigned kAll = 0xffffffffu;
   const uint32_t b = smem_u32(&bar);
-  if (__all_sync(0xffffffffu, mbar_look(b, parity))) return true;
+  if (__all_sync(kAll, mbar_look(b, parity))) return true;
   const long long start = clock64();
-  bool done = false;
-  while (!done && !sh.abort) {
-    done = __all_sync(0xffffffffu, mbar_look(b, parity));
-    if (!done && clock64() - start > kWaitCycles) break;
+  bool done = false, stop = false;
+  while (!done && !stop) {
+    done = __all_sync(kAll, mbar_look(b, parity));
+    stop = __any_sync(kAll, sh.abort || clock64() - start > kWaitCycles);
   }
-  done = __all_sync(0xffffffffu, done);
   if (!done) sh.abort = 1;
   return done;
+}
+// The same for what comes once in an item: the limit holds for a tile, and an item has any
+// number of them, so this goes on as long as the item's keys come in.
+__device__ __forceinline__ bool wait_item(TcSmem &sh, uint64_t &bar, uint32_t parity) {
+  constexpr unsigned kAll = 0xffffffffu;
+  const uint32_t b = smem_u32(&bar);
+  long long start = clock64();
+  uint32_t loaded = kAll;
+  while (!__all_sync(kAll, mbar_look(b, parity))) {
+    if (!__any_sync(kAll, sh.abort || clock64() - start > kWaitCycles)) continue;
+    const uint32_t now = __shfl_sync(kAll, sh.loaded, 0);
+    if (__any_sync(kAll, sh.abort) || now == loaded) {
+      sh.abort = 1;
+      return false;
+    }
+    loaded = now;
+    start = clock64();
+  }
+  return true;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -324,6 +344,7 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
     if (MODE == kTcShared && t + 1 < tiles) next_pages = page_at(key + Cfg::kKeys);
     // No sooner than it is needed: blocks that have not started are for whoever is done first.
     if (!V && t == max(0, tiles - kWantTiles) && lead) mbar_arrive(smem_u32(&sh.want));
+    if (!V && lead) sh.loaded = place.round * TcCfg<DP>::kSlots + place.slot;
 #pragma unroll 1
     for (int c = 0; c < Cfg::kChunks; c++, place.next()) {
       const int from = V ? key + c * kRows : key, x0 = V ? 0 : c * kSlabs * 64;
@@ -374,6 +395,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
 
   if (tid == 0) {
     sh.abort = 0;
+    sh.loaded = 0;
     for (int i = 0; i < kItems; i++) {
       mbar_init(smem_u32(&sh.item_full[i]), 1);
       mbar_init(smem_u32(&sh.item_empty[i]), Cfg::kConsumers);
@@ -482,7 +504,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (w.stop) break;
       }
       if (MODE == kTcPrompt) {
-        if (w.stop == 0 && !(ok = wait(sh, sh.want, (items - 1) & 1))) break;
+        if (w.stop == 0 && !(ok = wait_item(sh, sh.want, (items - 1) & 1))) break;
         if (lane == 0) {
           fence_async_smem();  // the last answer has been read
           mbar_expect_tx(smem_u32(&sh.next_block), 16);
@@ -504,7 +526,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       int q_uses = 0, number = 0;  // items with tiles; products of this warp
       for (int items = 0; ok; items++) {
         const int at = items % kItems;
-        if (!(ok = wait(sh, sh.item_full[at], (items / kItems) & 1))) break;
+        if (!(ok = wait_item(sh, sh.item_full[at], (items / kItems) & 1))) break;
         const Item &w = sh.item[at];
         if (uniform(w.stop)) break;
         const int tiles = uniform(w.tiles);
@@ -666,7 +688,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     int number = 0;  // tiles of this unit so far
     for (int items = 0; ok; items++) {
       const int at = items % kItems;
-      if (!(ok = wait(sh, sh.item_full[at], (items / kItems) & 1))) break;
+      if (!(ok = wait_item(sh, sh.item_full[at], (items / kItems) & 1))) break;
       const Item &w = sh.item[at];
       if (w.stop) break;
       const int n = w.n[unit];

@@ -8,7 +8,7 @@ import torch
 
 from attention_plain import EPS, check_rows, row, to64
 from diskmule_b200 import CudaContext, DmError, _native as N
-from diskmule_b200.attention import KvCache, offsets, prompt_attention
+from diskmule_b200.attention import KvCache, attention_status, offsets, prompt_attention
 from test_gpu_kv_cache import Pair
 from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode, run_prompt
 
@@ -281,6 +281,24 @@ def test_more_tokens_than_kernels_can_count_are_refused(ctx):
             prompt_attention(ctx, type=N.BF16, heads=1, kv_heads=1, head_dim=8, q=p, k=p, v=p, out=p,
                              q_tokens=q_tokens, k_tokens=k_tokens, sequences=1, q_offsets=o.data_ptr())
         assert e.value.status == N.ERR_ELEMENT_COUNT
+
+
+@pytest.mark.parametrize("lq", [1, 130])
+def test_prompt_over_more_keys_than_a_wait_lasts(ctx, lq):
+    """40 million keys, a quarter of a second: a role that waits for the whole item is not to
+    give up (a limit of 0.1 s holds for a tile). All scores are 0 and values whole numbers that
+    16 keys share, so every sum is exact: partial sums are multiples of 16 below 2^28."""
+    n, dim = 40_000_000, 8
+    k = torch.zeros(n, 1, dim, dtype=torch.bfloat16, device="cuda")
+    gen = generator(lq)
+    v = torch.randint(0, 4, (n // 16, 1, dim), generator=gen, device="cuda").to(torch.bfloat16)
+    v = v.repeat_interleave(16, 0)
+    q = normal(gen, (lq, 1, dim), torch.bfloat16)
+    out, lse = run_prompt(ctx, q, k, v, [lq], [n], causal=False)
+    attention_status(ctx)
+    want = v[:, 0].double().mean(0)
+    assert ((out[:, 0].double() - want).abs() <= 1.01 * EPS[torch.bfloat16] * want).all()
+    assert (lse - math.log(n)).abs().max() <= 2.0 ** -19 * math.log(n)
 
 
 # ---------------------------------------------------------------------------
