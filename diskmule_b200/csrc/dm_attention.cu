@@ -209,12 +209,11 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   constexpr int kVec = DP / 8;  // 16-byte vectors of a row
   auto at = [](int r, int v) { return (uint32_t)((v >> 3) * Cfg::kSlab + r * 128 + ((v ^ r) & 7) * 16); };
   const int page_bits = MODE == kPrompt ? 0 : 31 - __clz(c.page_tokens);  // pages are powers of two
+  // As the table has it: a number outside the pool is outside the map, too, and reads as zeros.
+  // It is looked at when it is used, so that nothing waits for it here, and reported at the end.
+  uint32_t largest = 0;
   auto page_of = [&](int key) -> int {
-    if (MODE == kPrompt || key >= last) return -1;
-    const int page = c.table[(int64_t)table_row * c.max_pages + (key >> page_bits)];
-    if ((unsigned)page < (unsigned)c.pages) return page;
-    if (lane == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
-    return c.pages;  // behind the map: zeros
+    return MODE == kPrompt || key >= last ? -1 : c.table[(int64_t)table_row * c.max_pages + (key >> page_bits)];
   };
   auto load = [&](int key, int page, int stage) {
     const uint32_t kd = ring + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;
@@ -232,6 +231,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       const uint32_t bar = smem_u32(&sh.full[warp][stage]);
       if (lane == 0) mbar_expect_tx(bar, 2 * Cfg::kTile);
       __syncwarp();
+      largest = max(largest, (uint32_t)page);
       if (lane < 2 * (DP / 64)) {  // one slab each
         const bool is_v = lane >= DP / 64;
         const int slab = lane % (DP / 64);
@@ -372,6 +372,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     if (++stage == kStages) stage = 0, parity ^= 1;
   }
   if (MODE == kPrompt) asm volatile("cp.async.wait_group 0;");
+  if (MODE != kPrompt && largest >= (uint32_t)c.pages && lane == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
   if (late) {  // the copies in flight land before the block's states take their place
     if (lane == 0) atomicExch(d.timeout, 1);
     for (int i = 0; i < kStages; i++) mbar_wait(smem_u32(&sh.full[warp][i]), parity);

@@ -331,16 +331,17 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   // pages are powers of two or whole chunks.
   const int box = MODE == kTcPrompt ? kRows : V ? a.v_box : a.k_box;
   const int most = kRows / box, page_bits = 31 - __clz(a.c.page_tokens);
+  auto looks = [&](int at) -> bool { return lane * box < Cfg::kKeys && at + lane * box < end; };
+  // As the table has it: a number outside the pool is outside the map, too, and reads as zeros.
+  // It is looked at a tile later, so that nothing waits for it, and reported at the end.
+  uint32_t largest = 0;
   auto page_at = [&](int at) -> int {
-    if (lane * box >= Cfg::kKeys || at + lane * box >= end) return a.c.pages;
-    const int p = a.c.table[(int64_t)table_row * a.c.max_pages + ((at + lane * box) >> page_bits)];
-    if ((unsigned)p < (unsigned)a.c.pages) return p;
-    if (!V) atomicOr(a.c.status, DM_KV_BAD_TOKEN);
-    return a.c.pages;  // behind the map: zeros
+    return looks(at) ? a.c.table[(int64_t)table_row * a.c.max_pages + ((at + lane * box) >> page_bits)] : -1;
   };
   int next_pages = MODE == kTcShared && tiles > 0 ? page_at(key) : 0;
   for (int t = 0; t < tiles; t++, key += Cfg::kKeys) {
     const int pages = next_pages;
+    if (MODE == kTcShared && !V && looks(key)) largest = max(largest, (uint32_t)pages);
     if (MODE == kTcShared && t + 1 < tiles) next_pages = page_at(key + Cfg::kKeys);
     // No sooner than it is needed: blocks that have not started are for whoever is done first.
     if (!V && t == max(0, tiles - kWantTiles) && lead) mbar_arrive(smem_u32(&sh.want));
@@ -367,6 +368,7 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
       __syncwarp();
     }
   }
+  if (MODE == kTcShared && !V && largest >= (uint32_t)a.c.pages) atomicOr(a.c.status, DM_KV_BAD_TOKEN);
   return true;
 }
 
