@@ -245,12 +245,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
         const int row = a.rows[i];
         const int k0 = a.other[i], count = a.other[i + 1] - k0;
         if (k0 < 0 || count < 0 || (int64_t)k0 + count > a.kept || count > c.lengths[row] ||
-            c.lengths[row] > c.max_pages * (int64_t)c.page_tokens ||
-            (count > 0 && (a.keep[k0] < 0 || a.keep[k0 + count - 1] >= c.lengths[row]))) {
+            c.lengths[row] > c.max_pages * (int64_t)c.page_tokens) {
           if ((tid & 31) == 0) atomicOr(&bad, DM_KV_BAD_TOKEN);
           continue;
         }
+        // the ends of the list come in beside the search, which reads nothing outside it
+        const int head = count ? a.keep[k0] : 0, tail = count ? a.keep[k0 + count - 1] : -1;
         const int same = leading_same(a.keep + k0, count);
+        if ((tid & 31) == 0 && (head < 0 || tail >= c.lengths[row])) atomicOr(&bad, DM_KV_BAD_TOKEN);
         int stay = same / c.page_tokens;
         if (same == count) {  // only the tail goes
           stay = pages_for(c, count);
@@ -263,13 +265,20 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
         if ((tid & 31) == 0) p.stay[i] = stay, p.moved[i] = 0;
       }
       // Between its first and last token, which are in range, an entry's list ascends. All
-      // lists in one pass: a step down is rare where no new entry begins.
+      // lists in one pass, kSteps loads of a thread in flight: a step down is rare where no new
+      // entry begins.
+      constexpr int kSteps = 8;
       const int64_t end = min((int64_t)a.other[a.n], a.kept) - 1;
-      bool down = false;
-#pragma unroll 4
-      for (int64_t j = max(a.other[0], 0) + tid; j < end; j += kPlanThreads)
-        if (a.keep[j] >= a.keep[j + 1]) down |= !opens_entry(a.other, a.n, j + 1);
-      if (down) atomicOr(&bad, DM_KV_BAD_TOKEN);
+      for (int64_t j0 = (int64_t)max(a.other[0], 0) + tid; j0 < end; j0 += kSteps * kPlanThreads) {
+        unsigned down = 0;
+#pragma unroll
+        for (int k = 0; k < kSteps; k++) {
+          const int64_t j = j0 + k * kPlanThreads;
+          if (j < end && a.keep[j] >= a.keep[j + 1]) down |= 1u << k;
+        }
+        for (; down; down &= down - 1)
+          if (!opens_entry(a.other, a.n, j0 + (__ffs(down) - 1) * kPlanThreads + 1)) atomicOr(&bad, DM_KV_BAD_TOKEN);
+      }
       __syncthreads();
     }
     for (int i0 = 0; i0 < a.n; i0 += kPlanThreads) {
