@@ -18,7 +18,7 @@
 namespace dma {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kStatusWord = 32;  // of the context's status buffer: a bounded wait ran out
+constexpr int kStatusWord = 48;  // of the context's status buffer: a bounded wait ran out
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct PromptArgs {

@@ -85,6 +85,7 @@ struct dm_cuda_context {
   // operator scratch (grown on demand)
   void *scratch = nullptr;
   size_t scratch_bytes = 0;
+  // 64 words: 0 the operators', 16 the stack's, 32 the self-tests', 48 the attention kernels'
   int32_t *status = nullptr;
 
   int32_t ensure_scratch(size_t bytes) {

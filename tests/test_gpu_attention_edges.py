@@ -301,6 +301,12 @@ def test_prompt_over_more_keys_than_a_wait_lasts(ctx, lq):
     assert (lse - math.log(n)).abs().max() <= 2.0 ** -19 * math.log(n)
 
 
+def test_a_wait_elsewhere_on_the_context_is_not_attentions(ctx):
+    """The self-test of bounded waits runs one out: the attention status does not tell of it."""
+    assert N.lib().dm_selftest_device_wait(ctx.handle, 100_000) == N.ERR_TIMEOUT
+    attention_status(ctx)
+
+
 # ---------------------------------------------------------------------------
 # the cache
 # ---------------------------------------------------------------------------
