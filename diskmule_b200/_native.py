@@ -205,6 +205,7 @@ SIGNATURES = {
     "dm_stack_add_rms_norm": ([P, P, P, P, I32, C.c_float, P, P, P], I32),
     "dm_stack_lm_head_argmax": ([P, P, I32, I32, I32, P, P, P, P, P], I32),
     "dm_selftest_device_wait": ([P, C.c_int64], I32),
+    "dm_selftest_attention_wait": ([P, C.c_int64], I32),
     "dm_gguf_open": ([C.c_char_p, C.c_char_p, C.POINTER(P)], I32),
     "dm_gguf_parse": ([P, C.c_uint64, C.c_char_p, C.POINTER(P)], I32),
     "dm_gguf_close": ([P], None),

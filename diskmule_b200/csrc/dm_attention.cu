@@ -80,6 +80,23 @@ __device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Wait for a copy; false after `limit` clocks (looked at before the warp goes to sleep).
+__device__ __forceinline__ bool copy_landed(uint32_t bar, uint32_t parity, int64_t limit) {
+  const long long start = clock64();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (clock64() - start >= limit) return false;
+    if (mbar_try(bar, parity)) return true;
+  }
+}
+
 // Add a state (ml, o) to the sums that refer to z.
 __device__ __forceinline__ void add_state(float &l, float4 &v, float2 ml, float4 o, float z) {
   const float f = exp2_fast(ml.x - z);
@@ -264,12 +281,16 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   for (int s = 0; s < kStages - 1; s++) issue(s);
   int stage = 0;
   uint32_t parity = 0;  // of the ring's round
-  bool late = false;    // a wait has run out
   for (int key = first + warp * kChunk; key < last; key += kStep) {
     if (MODE == kPrompt) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2));
-    } else if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.full[warp][stage]), parity))) {
-      late = true;
+    } else if (!__all_sync(0xffffffffu, copy_landed(smem_u32(&sh.full[warp][stage]), parity, d.wait_limit))) {
+      // the copies in flight land before the block's states take their place
+      if (lane == 0) atomicExch(d.timeout, 1);
+      for (; key < min(key_load, last); key += kStep) {
+        mbar_wait(smem_u32(&sh.full[warp][stage]), parity);
+        if (++stage == kStages) stage = 0, parity ^= 1;
+      }
       break;
     }
     __syncwarp();  // all lanes' copies are there, and all have left the stage that is next
@@ -373,10 +394,6 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   }
   if (MODE == kPrompt) asm volatile("cp.async.wait_group 0;");
   if (MODE != kPrompt && largest >= (uint32_t)c.pages && lane == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
-  if (late) {  // the copies in flight land before the block's states take their place
-    if (lane == 0) atomicExch(d.timeout, 1);
-    for (int i = 0; i < kStages; i++) mbar_wait(smem_u32(&sh.full[warp][i]), parity);
-  }
 
   // ---- join the warps' states in shared memory
 #pragma unroll
@@ -753,7 +770,7 @@ int32_t dm_attention_prompt(dm_cuda_context *ctx, const dm_attention_prompt_desc
   a.causal = in->causal;
   a.window = in->window;
   cudaSetDevice(ctx->device);
-  if (tile_prompt_fits(a)) return launch_tile_prompt(in->type, a, ctx->status + kStatusWord, (cudaStream_t)stream);
+  if (tile_prompt_fits(a)) return launch_tile_prompt(in->type, a, ctx, (cudaStream_t)stream);
   const int64_t tiles = in->q_tokens * a.group / kRows + in->sequences;
   if (tiles > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
   const CUtensorMap none[2]{};
@@ -820,6 +837,7 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
   cudaSetDevice(cache->ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   a.timeout = cache->ctx->status + kStatusWord;
+  a.wait_limit = wait_limit(cache->ctx);
   CUtensorMap maps[2];
   if ((plan.own_parts || !plan.tiles) && !describe_chunks(kd.type, cache->view, in->layer, kChunk, maps))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");

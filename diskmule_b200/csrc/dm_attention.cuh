@@ -64,6 +64,7 @@ struct DecodeArgs {
   int32_t splits;      // parts of this launch
   int32_t joins;       // own part: this launch joins the parts before its own
   int32_t *timeout;    // set when a bounded wait runs out
+  int64_t wait_limit;  // clocks
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -44,6 +44,7 @@
 
 #include <algorithm>
 
+#include "../../include/diskmule_selftest.h"
 #include "dm_attention.cuh"
 #include "dm_attention_tc.cuh"
 #include "dm_tcgen05.cuh"
@@ -192,6 +193,7 @@ struct TcArgs {
   int k_box, v_box;  // shared: rows of a TMA box
   int wide;          // rows of the result (or of the parts) lie on 32-byte boundaries
   int32_t *timeout;
+  int64_t wait_limit;
 };
 
 // One lane of a converged warp. What it decides is uniform, so the operands of the
@@ -245,7 +247,7 @@ __device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-__device__ __forceinline__ bool wait(TcSmem &sh, uint64_t &bar, uint32_t parity) {
+__device__ __forceinline__ bool wait(TcSmem &sh, int64_t limit, uint64_t &bar, uint32_t parity) {
   constexpr unsigned kAll = 0xffffffffu;
   const uint32_t b = smem_u32(&bar);
   if (__all_sync(kAll, mbar_look(b, parity))) return true;
@@ -253,20 +255,20 @@ __device__ __forceinline__ bool wait(TcSmem &sh, uint64_t &bar, uint32_t parity)
   bool done = false, stop = false;
   while (!done && !stop) {
     done = __all_sync(kAll, mbar_look(b, parity));
-    stop = __any_sync(kAll, sh.abort || clock64() - start > kWaitCycles);
+    stop = __any_sync(kAll, sh.abort || clock64() - start > limit);
   }
   if (!done) sh.abort = 1;
   return done;
 }
 // The same for what comes once in an item: the limit holds for a tile, and an item has any
 // number of them, so this goes on as long as the item's keys come in.
-__device__ __forceinline__ bool wait_item(TcSmem &sh, uint64_t &bar, uint32_t parity) {
+__device__ __forceinline__ bool wait_item(TcSmem &sh, int64_t limit, uint64_t &bar, uint32_t parity) {
   constexpr unsigned kAll = 0xffffffffu;
   const uint32_t b = smem_u32(&bar);
   long long start = clock64();
   uint32_t loaded = kAll;
   while (!__all_sync(kAll, mbar_look(b, parity))) {
-    if (!__any_sync(kAll, sh.abort || clock64() - start > kWaitCycles)) continue;
+    if (!__any_sync(kAll, sh.abort || clock64() - start > limit)) continue;
     const uint32_t now = __shfl_sync(kAll, sh.loaded, 0);
     if (__any_sync(kAll, sh.abort) || now == loaded) {
       sh.abort = 1;
@@ -355,8 +357,8 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
       const int slab = lane % kSlabs, mine = lane / kSlabs;
       const int boxes = MODE == kTcPrompt ? 1 : from + kRows <= a.d.shared ? most : max(0, a.d.shared - from) / box;
       const int page = MODE == kTcShared ? __shfl_sync(0xffffffffu, pages, (V ? c * most : 0) + mine) : 0;
-      if (place.round > 0 && !wait(sh, V ? sh.v_empty[place.slot] : sh.k_empty[place.slot], place.parity() ^ 1))
-        return false;
+      uint64_t &empty = V ? sh.v_empty[place.slot] : sh.k_empty[place.slot];
+      if (place.round > 0 && !wait(sh, a.wait_limit, empty, place.parity() ^ 1)) return false;
       if (lead) mbar_expect_tx(bar, kSlabs * boxes * box * 128);
       __syncwarp();
       if (MODE == kTcPrompt) {
@@ -496,7 +498,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
       if (w.stop >= 0) {
         const int at = items % kItems;
-        if (items >= kItems && !(ok = wait(sh, sh.item_empty[at], (items / kItems - 1) & 1))) break;
+        if (items >= kItems && !(ok = wait(sh, a.wait_limit, sh.item_empty[at], (items / kItems - 1) & 1))) break;
         if (lane == 0) {
           sh.item[at] = w;
           mbar_arrive(smem_u32(&sh.item_full[at]));
@@ -506,14 +508,14 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (w.stop) break;
       }
       if (MODE == kTcPrompt) {
-        if (w.stop == 0 && !(ok = wait_item(sh, sh.want, (items - 1) & 1))) break;
+        if (w.stop == 0 && !(ok = wait_item(sh, a.wait_limit, sh.want, (items - 1) & 1))) break;
         if (lane == 0) {
           fence_async_smem();  // the last answer has been read
           mbar_expect_tx(smem_u32(&sh.next_block), 16);
           take_block(smem_u32(&sh.answer), smem_u32(&sh.next_block));
         }
         asks++;
-        if (!(ok = wait(sh, sh.next_block, (asks - 1) & 1))) break;
+        if (!(ok = wait(sh, a.wait_limit, sh.next_block, (asks - 1) & 1))) break;
         block = taken_block(smem_u32(&sh.answer));
         __syncwarp();
       }
@@ -528,14 +530,14 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       int q_uses = 0, number = 0;  // items with tiles; products of this warp
       for (int items = 0; ok; items++) {
         const int at = items % kItems;
-        if (!(ok = wait_item(sh, sh.item_full[at], (items / kItems) & 1))) break;
+        if (!(ok = wait_item(sh, a.wait_limit, sh.item_full[at], (items / kItems) & 1))) break;
         const Item &w = sh.item[at];
         if (uniform(w.stop)) break;
         const int tiles = uniform(w.tiles);
         if (warp == Cfg::kKWarp) {
           // ---- queries and keys
           if (tiles > 0) {
-            if (q_uses > 0 && !(ok = wait(sh, sh.q_empty, (q_uses - 1) & 1))) break;
+            if (q_uses > 0 && !(ok = wait(sh, a.wait_limit, sh.q_empty, (q_uses - 1) & 1))) break;
             if (lead) {
               const uint32_t bar = smem_u32(&sh.q_full);
               const int units = alternate ? 1 : kUnits;
@@ -561,7 +563,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           for (int t = 0; t < tiles && ok; t++) {
             const bool mix = mixed<kKeys>(w, t);
             for (int c = 0; c < kChunks; c++, place.next()) {
-              if (!(ok = wait(sh, sh.v_full[place.slot], place.parity()))) break;
+              if (!(ok = wait(sh, a.wait_limit, sh.v_full[place.slot], place.parity()))) break;
               if (mix) {
                 const uint32_t v = v_ring + place.slot * Cfg::kChunkBytes;
                 // an exponent of all ones carries into the sign's place
@@ -601,15 +603,15 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           constexpr int kQSlab = kUnitRows * 128, kKSlab = kKeys * 128;
           const uint64_t qd = sw128_desc(base + (alternate ? 0 : unit) * Cfg::kQBytes);
           const int n = uniform(w.n[unit]);
-          if (tiles > 0 && !(ok = wait(sh, sh.q_full, q_uses++ & 1))) break;
+          if (tiles > 0 && !(ok = wait(sh, a.wait_limit, sh.q_full, q_uses++ & 1))) break;
           if (tiles > 0 && n == 0 && lead) mbar_arrive(smem_u32(&sh.q_empty));
           for (int t = 0, left = n; t < tiles && ok; t++) {
             const bool mine = is_mine(unit, t, n);
-            if (mine && number > 0 && !(ok = wait(sh, sh.s_free[unit], (number - 1) & 1)))
+            if (mine && number > 0 && !(ok = wait(sh, a.wait_limit, sh.s_free[unit], (number - 1) & 1)))
               break;  // S has been read
 #pragma unroll
             for (int c = 0; c < kChunks; c++, place.next()) {
-              if (!(ok = wait(sh, sh.k_full[place.slot], place.parity()))) break;
+              if (!(ok = wait(sh, a.wait_limit, sh.k_full[place.slot], place.parity()))) break;
               const uint32_t empty = smem_u32(&sh.k_empty[place.slot]);
               if (!mine) {
                 if (lead) mbar_arrive(empty);
@@ -639,10 +641,10 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             const bool mine = is_mine(unit, t, n);
             const int which = p_of(unit, number);
             const uint32_t p = columns + unit * Cfg::kUnitCols + Cfg::kPCol + (which - unit) * kKeys / 2;
-            if (mine && !(ok = wait(sh, sh.p_full[which], p_round(number) & 1))) break;
+            if (mine && !(ok = wait(sh, a.wait_limit, sh.p_full[which], p_round(number) & 1))) break;
 #pragma unroll
             for (int c = 0; c < kChunks; c++, place.next()) {
-              if (!(ok = wait(sh, sh.v_clean[place.slot], place.parity()))) break;
+              if (!(ok = wait(sh, a.wait_limit, sh.v_clean[place.slot], place.parity()))) break;
               const uint32_t empty = smem_u32(&sh.v_empty[place.slot]);
               if (!mine) {
                 if (lead) mbar_arrive(empty);
@@ -690,7 +692,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     int number = 0;  // tiles of this unit so far
     for (int items = 0; ok; items++) {
       const int at = items % kItems;
-      if (!(ok = wait_item(sh, sh.item_full[at], (items / kItems) & 1))) break;
+      if (!(ok = wait_item(sh, a.wait_limit, sh.item_full[at], (items / kItems) & 1))) break;
       const Item &w = sh.item[at];
       if (w.stop) break;
       const int n = w.n[unit];
@@ -716,7 +718,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
       float m = -INFINITY, l = 0.0f;  // m in units of the raw score
       for (int i = 0; i < n; i++, number++) {
-        if (!(ok = wait(sh, sh.s_full[unit], number & 1))) break;
+        if (!(ok = wait(sh, a.wait_limit, sh.s_full[unit], number & 1))) break;
         fence_after();
         const uint32_t s_at = tmem + lanes + unit * Cfg::kUnitCols;
         const int key = w.first + tile_of(unit, i) * kKeys;
@@ -743,7 +745,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? exp2_fast((m - now) * c) : 1.0f;
           if (i > 0) {
-            if (!(ok = wait(sh, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
+            if (!(ok = wait(sh, a.wait_limit, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
             fence_after();
 #pragma unroll 1
             for (int j = 0; j < DP; j += 16) {
@@ -764,7 +766,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         const int which = p_of(unit, number), round = p_round(number);
         const uint32_t p_at = s_at + Cfg::kPCol + (which - unit) * kKeys / 2;
         if (round > 0) {
-          if (!(ok = wait(sh, sh.pv_done[which], (round - 1) & 1))) break;
+          if (!(ok = wait(sh, a.wait_limit, sh.pv_done[which], (round - 1) & 1))) break;
           fence_after();
         }
         uint64_t sum[2] = {0, 0};
@@ -790,7 +792,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
       if (!ok) break;
       // ---- result
-      if (n > 0 && !(ok = wait(sh, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
+      if (n > 0 && !(ok = wait(sh, a.wait_limit, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
       fence_after();
       const bool wild = n > 0 && *(volatile int *)&sh.item[at].wild;
       const bool final = MODE == kTcPrompt || a.d.part.parts == 1;
@@ -867,6 +869,10 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       fence_before();  // O has been read before the next item's weights are announced
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.item_empty[at]));
+    }
+    if (!ok) {  // stores to tensor memory end before it is freed
+      __syncwarp();
+      tmem_wait_st();
     }
   }
   fence_before();
@@ -961,11 +967,14 @@ bool tile_prompt_fits(const PromptArgs &p) {
   return p.k_tokens > 0;
 }
 
-int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *timeout, cudaStream_t stream) {
+int64_t wait_limit(const dm_cuda_context *ctx) { return ctx->attention_wait ? ctx->attention_wait : kWaitCycles; }
+
+int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, dm_cuda_context *ctx, cudaStream_t stream) {
   TcArgs a{};
   a.p = p;
   a.tokens = kUnitRows / p.group;
-  a.timeout = timeout;
+  a.timeout = ctx->status + kStatusWord;
+  a.wait_limit = wait_limit(ctx);
   const int64_t tiles = p.q_tokens / (units_of(p.dim) * a.tokens) + p.sequences;
   if (tiles * p.kv_heads > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
   a.tiles = (int)tiles;
@@ -1005,6 +1014,7 @@ int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, c
   a.tokens = kUnitRows / d.group;
   a.alternate = tile_shared_alternates(c.head_dim, d.group, d.batch);
   a.timeout = d.timeout;
+  a.wait_limit = d.wait_limit;
   a.wide = d.part.parts > 1 ? ((uintptr_t)d.part.o & 31) == 0 : aligned32(d.out, d.out_stride);
   const bool bf16 = type == DM_BF16;
   CUtensorMap maps[3];
@@ -1020,6 +1030,14 @@ int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, c
 }
 
 }  // namespace dma
+
+extern "C" int32_t dm_selftest_attention_wait(dm_cuda_context *ctx, int64_t cycles) {
+  if (!ctx) return fail(DM_ERR_INVALID_ARGUMENT, "null context");
+  if (cycles < 0 || cycles > dm::tc::kWaitCycles)
+    return fail(DM_ERR_INVALID_ARGUMENT, "the wait limit must be 1..%lld cycles, or 0", dm::tc::kWaitCycles);
+  ctx->attention_wait = cycles;
+  return DM_OK;
+}
 
 extern "C" int32_t dm_attention_status(dm_cuda_context *ctx, void *stream) {
   if (!ctx) return fail(DM_ERR_INVALID_ARGUMENT, "null context");

@@ -9,7 +9,8 @@ namespace dma {
 
 // Whole prompts. The tensors need strides that a tensor map can hold.
 bool tile_prompt_fits(const PromptArgs &p);
-int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, int32_t *timeout, cudaStream_t stream);
+int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, dm_cuda_context *ctx, cudaStream_t stream);
+int64_t wait_limit(const dm_cuda_context *ctx);  // of a bounded wait, clocks
 
 // The shared part of a decode call, in d.splits parts, or twice as many where the two units
 // of a block alternate.

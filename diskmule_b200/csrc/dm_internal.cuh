@@ -87,6 +87,8 @@ struct dm_cuda_context {
   size_t scratch_bytes = 0;
   // 64 words: 0 the operators', 16 the stack's, 32 the self-tests', 48 the attention kernels'
   int32_t *status = nullptr;
+  // clocks after which attention kernels give up a wait; 0: as built
+  int64_t attention_wait = 0;
 
   int32_t ensure_scratch(size_t bytes) {
     if (bytes <= scratch_bytes) return DM_OK;

@@ -7,6 +7,12 @@
  * wait gives up, the kernel records a timeout status and returns, and the call returns
  * DM_ERR_TIMEOUT with the context still usable -- the path a stuck copy or MMA would
  * take, exercised without a stuck copy or MMA.
+ *
+ * dm_selftest_attention_wait sets the limit of the waits in attention kernels that are
+ * launched on the context from then on (0: as built). With a limit of a few thousand
+ * clocks ordinary waits run out, so that the kernels' own way out is taken: copies and
+ * products in flight end, tensor memory is freed, the call's output is undefined and
+ * dm_attention_status returns DM_ERR_TIMEOUT.
  */
 #ifndef DISKMULE_SELFTEST_H
 #define DISKMULE_SELFTEST_H
@@ -20,6 +26,7 @@ extern "C" {
 #endif
 
 DM_API int32_t dm_selftest_device_wait(dm_cuda_context *ctx, int64_t cycles);
+DM_API int32_t dm_selftest_attention_wait(dm_cuda_context *ctx, int64_t cycles);
 
 #ifdef __cplusplus
 }

@@ -307,6 +307,60 @@ def test_a_wait_elsewhere_on_the_context_is_not_attentions(ctx):
     attention_status(ctx)
 
 
+# Limits in clocks: from waits that all run out to a few that do.
+LIMITS = (1, 300, 1000, 2000, 3000, 5000, 8000, 12000, 20000, 50000, 200000)
+
+
+def out_of_time(ctx, run, want):
+    """`run` at every limit: a call whose waits held gives `want`, another says so, and the one
+    after it, with the limit as built, is right again. The calls that ran out of time."""
+    late = 0
+    try:
+        for limit in LIMITS:
+            N.check(N.lib().dm_selftest_attention_wait(ctx.handle, limit))
+            got = run()
+            try:
+                attention_status(ctx)
+            except DmError as e:
+                assert e.status == N.ERR_TIMEOUT
+                late += 1
+            else:
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+            N.check(N.lib().dm_selftest_attention_wait(ctx.handle, 0))
+            assert all(torch.equal(a, b) for a, b in zip(run(), want))
+            attention_status(ctx)
+    finally:
+        N.check(N.lib().dm_selftest_attention_wait(ctx.handle, 0))
+    return late
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[1], [700, 3, 260], [2500] * 12])
+def test_prompt_out_of_time(ctx, dim, lens):
+    gen = generator(dim)
+    q = normal(gen, (sum(lens), 8, dim), torch.bfloat16, 2.0)
+    k, v = (normal(gen, (sum(lens), 2, dim), torch.bfloat16) for _ in range(2))
+    late = out_of_time(ctx, lambda: run_prompt(ctx, q, k, v, lens, lens), run_prompt(ctx, q, k, v, lens, lens))
+    # a warp sleeps before it looks at the clock: shorter calls are done by then
+    assert late > 0 or sum(lens) < 10000
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,batch,shared", SHORT_FIRST)
+def test_decode_out_of_time(ctx, heads, kv, dim, page, batch, shared):
+    lens = [shared + 1 + 37 * i % 900 for i in range(batch)]
+    pool = Pool(ctx, torch.float16, kv, dim, page, shared, lens, seed=batch)
+    q = normal(generator(13), (batch, heads, dim), torch.float16, 2.0)
+    late = out_of_time(ctx, lambda: run_decode(pool, q, 0, shared, max(lens)), run_decode(pool, q, 0, shared, max(lens)))
+    # where a warp has two copies to wait for, both may be there before it asks
+    assert late > 0 or shared == 480
+
+
+def test_limits_of_a_wait_are_checked(ctx):
+    assert N.lib().dm_selftest_attention_wait(None, 10) == N.ERR_INVALID_ARGUMENT
+    assert N.lib().dm_selftest_attention_wait(ctx.handle, -1) == N.ERR_INVALID_ARGUMENT
+    assert N.lib().dm_selftest_attention_wait(ctx.handle, 1 << 40) == N.ERR_INVALID_ARGUMENT
+
+
 # ---------------------------------------------------------------------------
 # the cache
 # ---------------------------------------------------------------------------
