@@ -78,8 +78,9 @@ DM_API int32_t dm_attention_status(dm_cuda_context *ctx, void *stream);
  * nothing and set a bit of the status word where they need more pages than are free, or where
  * a list holds a bad or repeated sequence, a bad count or a token out of range or order.
  * Free, write and copy_pages do what can be done and set the bit for the rest; a sequence that
- * is named twice is freed once. Calls on one cache are ordered by the caller (one stream, or
- * events). A last page that is only partly filled belongs to one sequence alone. */
+ * is named twice is freed once. Fork and copy_pages take at most 65535 entries. Calls on one
+ * cache are ordered by the caller (one stream, or events). A last page that is only partly
+ * filled belongs to one sequence alone. */
 typedef struct {
   int32_t type, layers, kv_heads, head_dim, page_tokens, pages, max_sequences, max_pages;
   void *memory;

@@ -10,7 +10,7 @@ from attention_plain import EPS, check_rows, row, to64
 from diskmule_b200 import CudaContext, DmError, _native as N
 from diskmule_b200.attention import KvCache, attention_status, offsets, prompt_attention
 from test_gpu_kv_cache import Pair
-from test_gpu_attention import Pool, check_decode, generator, ints, normal, run_decode, run_prompt
+from test_gpu_attention import Pool, check_decode, check_prompt, generator, ints, normal, run_decode, run_prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -305,6 +305,22 @@ def test_a_wait_elsewhere_on_the_context_is_not_attentions(ctx):
     """The self-test of bounded waits runs one out: the attention status does not tell of it."""
     assert N.lib().dm_selftest_device_wait(ctx.handle, 100_000) == N.ERR_TIMEOUT
     attention_status(ctx)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (7, 1, 96), (6, 2, 128), (4, 2, 256)])
+def test_prompt_heads_first(ctx, heads, kv, dim, dtype):
+    """q, k, v and out as [heads, tokens, dim], and with rows that are part of wider ones."""
+    gen = generator(61)
+    lens, n = [140, 1, 333], 474
+    q = normal(gen, (heads, n, dim), dtype, 2.0).transpose(0, 1)
+    k, v = (normal(gen, (kv, n, dim + 8), dtype)[:, :, 8:].transpose(0, 1) for _ in range(2))
+    out = torch.full((heads, n, dim + 24), float("nan"), dtype=dtype, device="cuda")[:, :, 16:16 + dim].transpose(0, 1)
+    for causal, window in ((True, 0), (False, 0), (True, 50)):
+        got, lse = run_prompt(ctx, q, k, v, lens, lens, causal, window, out=out)
+        check_prompt(q, k, v, lens, lens, got, lse, causal, window, tokens=16)
+        flat, flat_lse = run_prompt(ctx, q.contiguous(), k.contiguous(), v.contiguous(), lens, lens, causal, window)
+        assert torch.equal(got, flat) and torch.equal(lse, flat_lse)
 
 
 # Limits in clocks: from waits that all run out to a few that do.
