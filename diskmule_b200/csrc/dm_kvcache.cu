@@ -519,7 +519,8 @@ int blocks_along(int64_t vectors, int64_t items, int64_t blocks) {
   return (int)std::max<int64_t>(1, std::min(fit, blocks / std::max<int64_t>(1, items)));
 }
 constexpr int kGridBlocks = 148 * 8;
-constexpr int64_t kSmallCopy = 512 * 1024;
+constexpr int kSmallForks = 16;
+constexpr int64_t kSmallCopy = 512 * 1024, kSmallRows = 16384;  // bytes of pages, table entries
 
 template <typename... Params, typename... Args>
 int32_t launch(void (*kernel)(Params...), dim3 grid, int threads, void *stream, const Args &...args) {
@@ -699,10 +700,13 @@ int32_t dm_kv_cache_fork(dm_kv_cache *c, const int32_t *parents, const int32_t *
   if (n > 65535) return fail(DM_ERR_ELEMENT_COUNT, "%d forks in one call", n);
   cudaSetDevice(c->ctx->device);
   const PlanArgs a{children, parents, nullptr, 0, n};
-  // Up to half a megabyte the plan's block copies (free and fork of 8 beams with 32 KB pages:
-  // 13.3 us with a kernel for the rows, 10.8 without; 8 pages of 131 KB take longer in one
-  // block than the launch).
-  if (n * c->view.page_bytes <= kSmallCopy)
+  // A few small forks are done by the plan's block: a launch less, where the caller's side bounds
+  // a call (free and fork of 8 entries with 32 KB pages 10.8 us instead of 13.4). On the GPU it
+  // gains nothing and loses by size. Free and fork there, us, and with a kernel for the rows: 8
+  // entries with 32 KB pages 9.5 (9.4), with table rows of 2048 entries 10.3 (9.7), of 16384
+  // 17.4 (12.0); 16 entries with 4 KB pages 9.9 (9.4), 64 of them 19.2 (9.8); 2 with 256 KB pages
+  // 10.6 (9.6).
+  if (n <= kSmallForks && n * c->view.page_bytes <= kSmallCopy && (int64_t)n * c->desc.max_pages <= kSmallRows)
     return launch(plan_kernel<kForkSmall>, 1, kPlanThreads, stream, c->view, plan_of(c), a);
   if (int32_t rc = launch(plan_kernel<kFork>, 1, kPlanThreads, stream, c->view, plan_of(c), a)) return rc;
   // half a page is copied on average

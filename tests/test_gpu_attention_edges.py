@@ -475,3 +475,15 @@ def test_more_pages_asked_for_than_32_bits_count(ctx):
     cache.extend(s.data_ptr(), c.data_ptr(), rows)
     assert cache.status() == 0
     cache.close()
+
+
+@pytest.mark.parametrize("n,max_pages,dim", [(1, 16384, 8), (1, 16385, 8), (16, 1024, 8), (16, 1025, 8), (17, 4, 8),
+                                             (16, 4, 256), (9, 40, 80), (70, 300, 64)])
+def test_forks_on_both_sides_of_the_small_ones(ctx, n, max_pages, dim):
+    """Done by the plan's block, or by a kernel behind it: the same tables and rows."""
+    t = Pair(ctx, layers=2, kv=1, dim=dim, pages=10 * n + 9, seqs=2 * n, max_pages=max_pages)
+    assert t.extend(list(range(n)), [int(x) for x in t.r.randint(0, 49, n)])
+    t.write(1, list(range(n)), [int(x) for x in t.plain.lengths[:n]])
+    order = [int(x) for x in t.r.randint(0, n, n)]
+    assert t.fork(order, list(range(2 * n - 1, n - 1, -1)))
+    t.check()
