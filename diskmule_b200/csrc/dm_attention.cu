@@ -710,6 +710,9 @@ static int32_t bounded_length(const dm_kv_cache_desc &d, int32_t max_length) {
   return (int32_t)std::min<int64_t>(max_length, (int64_t)d.max_pages * d.page_tokens);
 }
 
+// Every tile looks for its sequence among all, 32 at a time: half a microsecond for each.
+constexpr int32_t kMostSequences = 1 << 20;
+
 static int32_t check_strides(const int64_t *given, int64_t heads, int dim, int64_t *use, const char *what) {
   const bool none = given[0] == 0 && given[1] == 0;
   use[0] = none ? heads * dim : given[0];
@@ -738,7 +741,7 @@ int32_t dm_attention_prompt(dm_cuda_context *ctx, const dm_attention_prompt_desc
   if (in->kv_heads > 65535) return fail(DM_ERR_ELEMENT_COUNT, "%d key/value heads", in->kv_heads);
   if (in->head_dim <= 0 || in->head_dim % 8 || in->head_dim > 256)
     return fail(DM_ERR_ELEMENT_COUNT, "head_dim %d is not a multiple of 8 up to 256", in->head_dim);
-  if (in->sequences < 0 || in->window < 0)
+  if (in->sequences < 0 || in->sequences > kMostSequences || in->window < 0)
     return fail(DM_ERR_ELEMENT_COUNT, "%d sequences, window %d", in->sequences, in->window);
   if (in->q_tokens < 0 || in->k_tokens < 0 || in->q_tokens > kMostTokens || in->k_tokens > kMostTokens)
     return fail(DM_ERR_ELEMENT_COUNT, "a bad number of tokens");

@@ -129,13 +129,15 @@ __device__ __forceinline__ uint32_t zero_not_finite(uint32_t x, bool &any) {
 }
 
 // Packed prompts: sequence and place of tile `tile` when a sequence of L tokens has
-// ceil(L * per_token / rows) tiles. One warp; seq = -1 behind the last tile.
+// ceil(L * per_token / rows) tiles. One warp; seq = -1 behind the last tile, and then `behind`
+// is how far.
 struct TileOf {
   int seq, tile, q0, q1, k0, k1;  // query and key rows of the sequence
+  int64_t behind;
 };
 __device__ __forceinline__ TileOf find_tile(const PromptArgs &p, int per_token, int rows, int64_t tile) {
   const int lane = threadIdx.x & 31;
-  TileOf r{-1, 0, 0, 0, 0, 0};
+  TileOf r{-1, 0, 0, 0, 0, 0, 0};
   for (int s0 = 0; s0 < p.sequences; s0 += 32) {
     const int s = s0 + lane;
     int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
@@ -164,6 +166,7 @@ __device__ __forceinline__ TileOf find_tile(const PromptArgs &p, int per_token, 
     }
     tile -= __shfl_sync(0xffffffffu, upto, 31);
   }
+  r.behind = tile;
   return r;
 }
 

@@ -117,7 +117,7 @@ struct TcSmem {
   Item item[kItems];
   uint32_t tmem;
   volatile int abort;
-  volatile uint32_t loaded;  // chunks of K asked for
+  volatile uint32_t loaded, asked;  // signs of life: chunks of K, and blocks, asked for
 };
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -261,7 +261,8 @@ __device__ __forceinline__ bool wait(TcSmem &sh, int64_t limit, uint64_t &bar, u
   return done;
 }
 // The same for what comes once in an item: the limit holds for a tile, and an item has any
-// number of them, so this goes on as long as the item's keys come in.
+// number of them, and so have the blocks without an item before it. So this goes on as long as
+// the item's keys come in, or blocks are gone through.
 __device__ __forceinline__ bool wait_item(TcSmem &sh, int64_t limit, uint64_t &bar, uint32_t parity) {
   constexpr unsigned kAll = 0xffffffffu;
   const uint32_t b = smem_u32(&bar);
@@ -269,7 +270,7 @@ __device__ __forceinline__ bool wait_item(TcSmem &sh, int64_t limit, uint64_t &b
   uint32_t loaded = kAll;
   while (!__all_sync(kAll, mbar_look(b, parity))) {
     if (!__any_sync(kAll, sh.abort || clock64() - start > limit)) continue;
-    const uint32_t now = __shfl_sync(kAll, sh.loaded, 0);
+    const uint32_t now = __shfl_sync(kAll, sh.loaded + sh.asked, 0);
     if (__any_sync(kAll, sh.abort) || now == loaded) {
       sh.abort = 1;
       return false;
@@ -399,7 +400,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
 
   if (tid == 0) {
     sh.abort = 0;
-    sh.loaded = 0;
+    sh.loaded = sh.asked = 0;
     for (int i = 0; i < kItems; i++) {
       mbar_init(smem_u32(&sh.item_full[i]), 1);
       mbar_init(smem_u32(&sh.item_empty[i]), Cfg::kConsumers);
@@ -439,6 +440,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     if (warp == Cfg::kItemWarp) {
       // ---- choice of items
       int block = blockIdx.x, items = 0, asks = 0;
+      int64_t all = INT64_MAX;  // tiles of the batch, once a block has been behind them
       while (ok) {
       Item w{};
       if (MODE == kTcPrompt) {
@@ -447,7 +449,12 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         } else {
           // key/value heads side by side, the last (longest, if causal) tiles of the batch first
           w.kv_head = block % a.p.kv_heads;
-          const TileOf t = find_tile(a.p, 1, kUnits * a.tokens, a.tiles - 1 - block / a.p.kv_heads);
+          const int tile = a.tiles - 1 - block / a.p.kv_heads;
+          TileOf t{-1};
+          if (tile < all) {
+            t = find_tile(a.p, 1, kUnits * a.tokens, tile);
+            if (t.seq < 0) all = tile - t.behind;
+          }
           if (t.seq < 0) {
             w.stop = -1;  // behind the last tile
           } else {
@@ -513,6 +520,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           fence_async_smem();  // the last answer has been read
           mbar_expect_tx(smem_u32(&sh.next_block), 16);
           take_block(smem_u32(&sh.answer), smem_u32(&sh.next_block));
+          sh.asked = asks + 1;
         }
         asks++;
         if (!(ok = wait(sh, a.wait_limit, sh.next_block, (asks - 1) & 1))) break;

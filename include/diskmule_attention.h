@@ -39,7 +39,7 @@ typedef struct dm_kv_cache dm_kv_cache;
 /* q [q_tokens, heads, head_dim], k and v [k_tokens, kv_heads, head_dim], out like q, lse
  * [q_tokens, heads]. Strides are in elements, {token, head}; {0, 0} means contiguous.
  * Pointers are 16-byte aligned and strides multiples of 8 elements; head_dim is a multiple
- * of 8 up to 256; at most 128 query heads per key/value head.
+ * of 8 up to 256; at most 128 query heads per key/value head and 2^20 sequences.
  * Sequence s owns query rows [q_offsets[s], q_offsets[s + 1]) and key rows
  * [k_offsets[s], k_offsets[s + 1]) (device int32, [sequences + 1], ascending from >= 0;
  * k_offsets NULL = q_offsets). The last query row is aligned with the last key: query row

@@ -276,6 +276,10 @@ def test_more_tokens_than_kernels_can_count_are_refused(ctx):
     assert e.value.status == N.ERR_OVERFLOW
     t, o = torch.zeros(16, 8, dtype=torch.bfloat16, device="cuda"), ints([0, 1])
     p = t.data_ptr()
+    with pytest.raises(DmError) as e:
+        prompt_attention(ctx, type=N.BF16, heads=1, kv_heads=1, head_dim=8, q=p, k=p, v=p, out=p, q_tokens=16,
+                         k_tokens=16, sequences=(1 << 20) + 1, q_offsets=o.data_ptr())
+    assert e.value.status == N.ERR_ELEMENT_COUNT
     for q_tokens, k_tokens in ((2 ** 31 - 4096, 16), (16, 2 ** 31 - 1)):
         with pytest.raises(DmError) as e:
             prompt_attention(ctx, type=N.BF16, heads=1, kv_heads=1, head_dim=8, q=p, k=p, v=p, out=p,
@@ -321,6 +325,18 @@ def test_prompt_heads_first(ctx, heads, kv, dim, dtype):
         check_prompt(q, k, v, lens, lens, got, lse, causal, window, tokens=16)
         flat, flat_lse = run_prompt(ctx, q.contiguous(), k.contiguous(), v.contiguous(), lens, lens, causal, window)
         assert torch.equal(got, flat) and torch.equal(lse, flat_lse)
+
+
+@pytest.mark.parametrize("at", [0, 30000, 79999])
+def test_prompt_among_very_many_empty_sequences(ctx, at):
+    """Finding the one sequence that has tokens takes longer than a wait may last."""
+    lens = [0] * 80000
+    lens[at] = 200
+    gen = generator(67)
+    q, k, v = (normal(gen, (200, 1, 64), torch.bfloat16) for _ in range(3))
+    out, lse = run_prompt(ctx, q, k, v, lens, lens)
+    attention_status(ctx)
+    check_prompt(q, k, v, [200], [200], out, lse)
 
 
 # Limits in clocks: from waits that all run out to a few that do.
