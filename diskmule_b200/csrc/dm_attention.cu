@@ -598,9 +598,9 @@ int splits_of(int64_t items, int keys, int64_t at_once) {
 
 // Microseconds on one B200, as measured: a block of tiles has 9 besides 1.2 for each step of
 // its units beside blocks of rows (alone 0.95; dim above 128: 1.1 with pages of 64 tokens, 2.0
-// with 16); a block of rows 7 besides 0.9 (1.2) for each chunk of every warp, and beside tiles
-// they get done 0.7 of what they would alone; a join in place 2; the join kernel 4 besides 0.4
-// for each MB of parts; a third launch 2.
+// with 16, taken as 1.6 for all); a block of rows 7 besides 0.9 (1.2) for each chunk of every
+// warp, and beside tiles they get done 0.7 of what they would alone; a join in place 2; the join
+// kernel 4 besides 0.4 for each MB of parts; a third launch 2.
 constexpr float kTileUs = 9.0f, kTileStepUs = 1.2f, kTileStepWideUs = 1.6f, kRowsUs = 7.0f, kRowsStepUs = 0.9f,
                 kRowsStepWideUs = 1.2f, kBeside = 0.7f, kInPlaceUs = 2.0f, kJoinUs = 4.0f, kJoinMbUs = 0.4f,
                 kThirdUs = 2.0f;

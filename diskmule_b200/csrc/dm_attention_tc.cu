@@ -34,12 +34,12 @@
 // many have.
 //
 // Measured, causal 16384 tokens, 16 heads of dim 128: 807 us, 1.36 PFLOP/s; without a mask 8192
-// keys, dim 256 1.47, dim 64 0.74. What bounds it: dim 128, 1750 cycles a
-// tile of both units, where the tensor pipe needs 1280 (1460 counting what S reads from shared
-// memory: 6.5 KB for 40 cycles of 16 values) and the exponential unit as many (each busy 60% of
-// a run over 6144 tokens, the issue slots 41%), and power in long runs; dim 64, the exponentials, 2048 of 2600 cycles for 128 keys;
-// short prompts, 5000 cycles an item for the last product, the output's stores and the first
-// tile.
+// keys, dim 256 1.47, dim 64 0.74. What bounds it: at dim 128, 1750 cycles a tile of both units,
+// where the tensor pipe needs 1280 (1460 counting what S reads from shared memory: 6.5 KB for 40
+// cycles of 16 values) and the exponential unit as many (each busy 60% of a run over 6144 tokens,
+// the issue slots 41%), and power in long runs; at dim 64 the exponentials, 2048 of 2600 cycles
+// for 128 keys; in short prompts 5000 cycles an item for the last product, the output's stores
+// and the first tile.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
