@@ -122,6 +122,58 @@ class DecodeDesc(C.Structure):
     ]
 
 
+class ChunkDesc(C.Structure):
+    """dm_attention_chunk_desc."""
+    _fields_ = [
+        ("layer", I32), ("heads", I32), ("sequences", I32), ("window", I32), ("sinks", I32),
+        ("max_length", I32), ("scale", C.c_float), ("tokens", C.c_int64),
+        ("q", P), ("out", P), ("lse", P),
+        ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("rows", P), ("offsets", P),
+        ("workspace", P), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class RopeDesc(C.Structure):
+    """dm_rope_desc."""
+    _fields_ = [
+        ("rotary_dim", I32), ("interleaved", I32), ("axes", I32), ("scale", C.c_float),
+        ("theta", C.c_double), ("frequencies", C.POINTER(C.c_double)), ("pair_axes", C.POINTER(I32)),
+    ]
+
+
+class RotateDesc(C.Structure):
+    """dm_attention_rotate_desc."""
+    _fields_ = [
+        ("type", I32), ("heads", I32), ("kv_heads", I32), ("head_dim", I32), ("norms", I32),
+        ("epsilon", C.c_float), ("layer", I32), ("sequences", I32), ("tokens", C.c_int64),
+        ("q", P), ("k", P), ("v", P), ("q_out", P), ("k_out", P), ("v_out", P),
+        ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+        ("q_out_stride", C.c_int64 * 2), ("k_out_stride", C.c_int64 * 2),
+        ("v_out_stride", C.c_int64 * 2), ("q_weight", P), ("k_weight", P),
+        ("positions", P), ("rows", P), ("offsets", P),
+    ]
+
+
+class WeightsDesc(C.Structure):
+    """dm_attention_weights_desc."""
+    _fields_ = [
+        ("layer", I32), ("heads", I32), ("sequences", I32), ("window", I32), ("sinks", I32),
+        ("max_length", I32), ("scale", C.c_float), ("tokens", C.c_int64), ("q", P), ("lse", P),
+        ("q_stride", C.c_int64 * 2), ("rows", P), ("offsets", P),
+        ("weights", P), ("weights_stride", C.c_int64),
+    ]
+
+
+class EvictDesc(C.Structure):
+    """dm_kv_cache_evict_desc."""
+    _fields_ = [
+        ("sequences", I32), ("budget", I32), ("sinks", I32), ("recent", I32), ("rows", P),
+        ("weights", P), ("weights_stride", C.c_int64), ("keep_offsets", P), ("keep", P),
+    ]
+
+
+# DM_NORM_* bits of dm_attention_rotate
+NORM_Q, NORM_K, NORM_V = 1, 2, 4
 # DM_KV_* status bits
 KV_OUT_OF_PAGES, KV_BAD_SEQUENCE, KV_TOO_LONG, KV_BAD_TOKEN = 1, 2, 4, 8
 
@@ -238,6 +290,13 @@ SIGNATURES = {
     "dm_kv_cache_copy_pages": ([P, P, P, I32, P], I32),
     "dm_attention_decode_workspace": ([P, I32, I32, I32, I32, C.POINTER(C.c_uint64)], I32),
     "dm_attention_decode": ([P, C.POINTER(DecodeDesc), P], I32),
+    "dm_attention_chunk_workspace": ([P, C.POINTER(ChunkDesc), C.POINTER(C.c_uint64)], I32),
+    "dm_attention_chunk": ([P, C.POINTER(ChunkDesc), P], I32),
+    "dm_rope_create": ([P, C.POINTER(RopeDesc), C.POINTER(P)], I32),
+    "dm_rope_destroy": ([P], None),
+    "dm_attention_rotate": ([P, P, P, C.POINTER(RotateDesc), P], I32),
+    "dm_attention_weights": ([P, C.POINTER(WeightsDesc), P], I32),
+    "dm_kv_cache_evict": ([P, C.POINTER(EvictDesc), P], I32),
     "dm_synth_fill_host": ([I32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_float,
                             C.c_float, P], I32),
     "dm_synth_fill_device": ([I32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_float,

@@ -1,9 +1,12 @@
 """Attention and its paged key/value cache over the C ABI (include/diskmule_attention.h).
 
 `prompt_attention` runs whole prompts, `KvCache` holds the pages of many sequences and
-`KvCache.decode_attention` runs one query token per sequence against them. Every tensor and
-list is a device pointer (an int); strides are in elements. Calls are ordered on `stream`
-(0: the default stream) and allocate nothing.
+`KvCache.decode_attention` runs one query token per sequence against them,
+`KvCache.chunk_attention` any number of new tokens. `rotate` norms and rotates queries and keys
+on their way there, `KvCache.token_weights` sums the attention that tokens receive and
+`KvCache.evict` keeps those that received most. Every tensor and list is a device pointer (an
+int); strides are in elements. Calls are ordered on `stream` (0: the default stream) and
+allocate nothing.
 """
 from __future__ import annotations
 
@@ -40,6 +43,74 @@ def prompt_attention(ctx: CudaContext, *, type: int, heads: int, kv_heads: int, 
 def attention_status(ctx: CudaContext, stream: int = 0):
     """Wait for `stream`; raises if a bounded wait inside an attention kernel ran out."""
     check(N.lib().dm_attention_status(ctx.handle, stream or None))
+
+
+class Rope:
+    """Which values of a head turn with the position, and how fast (dm_rope). `frequencies`
+    (radians per position, one per pair) default to theta^(-2 i / rotary_dim); `pair_axes`
+    names the axis of positions that each pair turns with (all 0)."""
+
+    def __init__(self, ctx: CudaContext, rotary_dim: int, *, theta: float = 10000.0, frequencies=None,
+                 pair_axes=None, axes: int = 0, interleaved: bool = False, scale: float = 1.0):
+        self._h = None
+        self._ctx = ctx
+        self._lib = N.lib()
+        half = rotary_dim // 2
+        f = a = None
+        if frequencies is not None:
+            f = np.ascontiguousarray(frequencies, np.float64)
+        if pair_axes is not None:
+            a = np.ascontiguousarray(pair_axes, np.int32)
+        for given in (f, a):
+            if given is not None and given.shape != (half,):
+                raise ValueError(f"{half} pairs, and values of shape {given.shape}")
+        self.axes = axes or (1 if a is None else int(a.max(initial=0)) + 1)
+        d = N.RopeDesc(rotary_dim, int(interleaved), self.axes, scale, theta)
+        if f is not None:
+            d.frequencies = f.ctypes.data_as(C.POINTER(C.c_double))
+        if a is not None:
+            d.pair_axes = a.ctypes.data_as(C.POINTER(C.c_int32))
+        h = C.c_void_p()
+        check(self._lib.dm_rope_create(ctx.handle, C.byref(d), C.byref(h)))
+        self._h = h
+
+    @property
+    def handle(self):
+        return self._h
+
+    def close(self):
+        if self._h:
+            self._lib.dm_rope_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rotate(ctx: CudaContext, rope: Rope | None, *, type: int, head_dim: int, tokens: int, heads: int = 0,
+           kv_heads: int = 0, q: int = 0, k: int = 0, v: int = 0, q_out: int = 0, k_out: int = 0,
+           v_out: int = 0, cache: KvCache | None = None, layer: int = 0, sequences: int = 0,
+           offsets: int = 0, n: int = 0, positions: int = 0, norm_q: bool = False, norm_k: bool = False,
+           norm_v: bool = False, q_weight: int = 0, k_weight: int = 0, epsilon: float = 1e-6,
+           q_stride=None, k_stride=None, v_stride=None, q_out_stride=None, k_out_stride=None,
+           v_out_stride=None, stream: int = 0):
+    """Norm each head and rotate queries and keys, into `*_out` and, with a cache, keys and values
+    into its pages as the last tokens of `sequences` (dm_attention_rotate)."""
+    norms = norm_q * N.NORM_Q | norm_k * N.NORM_K | norm_v * N.NORM_V
+    d = N.RotateDesc(type, heads, kv_heads, head_dim, norms, epsilon, layer, n, tokens, q or None, k or None,
+                     v or None, q_out or None, k_out or None, v_out or None)
+    for name, pair in (("q_stride", q_stride), ("k_stride", k_stride), ("v_stride", v_stride),
+                       ("q_out_stride", q_out_stride), ("k_out_stride", k_out_stride),
+                       ("v_out_stride", v_out_stride)):
+        if pair:
+            setattr(d, name, _strides(pair))
+    d.q_weight, d.k_weight = q_weight or None, k_weight or None
+    d.positions, d.rows, d.offsets = positions or None, sequences or None, offsets or None
+    check(N.lib().dm_attention_rotate(ctx.handle, rope.handle if rope else None,
+                                      cache.handle if cache else None, C.byref(d), stream or None))
 
 
 class KvCache:
@@ -119,6 +190,46 @@ class KvCache:
         if q_stride or out_stride:
             d.q_stride, d.out_stride = _strides(q_stride), _strides(out_stride)
         check(self._lib.dm_attention_decode(self._h, C.byref(d), stream or None))
+
+    def chunk_workspace(self, heads: int, n: int, tokens: int, max_length: int, window: int = 0,
+                        sinks: int = 0) -> int:
+        """Bytes of workspace that chunk_attention needs for these numbers."""
+        d = N.ChunkDesc(0, heads, n, window, sinks, max_length, 0.0, tokens)
+        size = C.c_uint64(0)
+        check(self._lib.dm_attention_chunk_workspace(self._h, C.byref(d), C.byref(size)))
+        return size.value
+
+    def chunk_attention(self, *, layer: int, heads: int, q: int, out: int, offsets: int, n: int,
+                        tokens: int, max_length: int, sequences: int = 0, lse: int = 0, window: int = 0,
+                        sinks: int = 0, scale: float = 0.0, q_stride=None, out_stride=None,
+                        workspace: int = 0, workspace_bytes: int = 0, stream: int = 0):
+        """The last offsets[i + 1] - offsets[i] tokens of each of `n` sequences over the cache
+        (dm_attention_chunk)."""
+        d = N.ChunkDesc(layer, heads, n, window, sinks, max_length, scale, tokens, q, out, lse or None)
+        d.rows, d.offsets = sequences or None, offsets
+        d.workspace, d.workspace_bytes = workspace or None, workspace_bytes
+        if q_stride or out_stride:
+            d.q_stride, d.out_stride = _strides(q_stride), _strides(out_stride)
+        check(self._lib.dm_attention_chunk(self._h, C.byref(d), stream or None))
+
+    def token_weights(self, *, layer: int, heads: int, q: int, lse: int, offsets: int, n: int, tokens: int,
+                      max_length: int, weights: int, weights_stride: int, sequences: int = 0, window: int = 0,
+                      sinks: int = 0, scale: float = 0.0, q_stride=None, stream: int = 0):
+        """Add the attention that cached tokens get from these queries to `weights`, f32
+        [max_sequences, weights_stride] (dm_attention_weights)."""
+        d = N.WeightsDesc(layer, heads, n, window, sinks, max_length, scale, tokens, q, lse)
+        if q_stride:
+            d.q_stride = _strides(q_stride)
+        d.rows, d.offsets = sequences or None, offsets
+        d.weights, d.weights_stride = weights, weights_stride
+        check(self._lib.dm_attention_weights(self._h, C.byref(d), stream or None))
+
+    def evict(self, *, sequences: int, n: int, budget: int, weights: int, weights_stride: int,
+              keep_offsets: int, keep: int, sinks: int = 0, recent: int = 0, stream: int = 0):
+        """Keep `budget` tokens of each sequence: the first `sinks`, the last `recent` and the
+        heaviest between (dm_kv_cache_evict)."""
+        d = N.EvictDesc(n, budget, sinks, recent, sequences, weights, weights_stride, keep_offsets, keep)
+        check(self._lib.dm_kv_cache_evict(self._h, C.byref(d), stream or None))
 
     def close(self):
         if self._h:

@@ -8,6 +8,7 @@
 
 #include "dm_attention.cuh"
 #include "dm_attention_tc.cuh"
+#include "dm_mma.cuh"
 #include "dm_tcgen05.cuh"
 
 using dmi::fail;
@@ -37,7 +38,7 @@ constexpr int kJoinThreads = 128;
 constexpr int kMostJoined = 8;     // shared parts that a block of the own part joins itself
 constexpr int kMostParts = 512;
 
-enum Mode { kPrompt, kOwn, kShared };
+enum Mode { kPrompt, kOwn, kShared, kChunks };
 
 template <int DP, int WARPS>
 struct RowsCfg {
@@ -51,51 +52,6 @@ struct RowsCfg {
   static_assert(kJoin <= WARPS * kRing, "the states fit the rings");
   static constexpr int kBlocks = kSmem <= 112 * 1024 ? 2 : 1;  // per SM
 };
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
-  const int bytes = valid ? 16 : 0;  // 0: zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes));
-}
-__device__ __forceinline__ void ldm4(uint32_t addr, uint32_t *r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ldm4t(uint32_t addr, uint32_t *r) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
-  if (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Wait for a copy; false after `limit` clocks (looked at before the warp goes to sleep).
-__device__ __forceinline__ bool copy_landed(uint32_t bar, uint32_t parity, int64_t limit) {
-  const long long start = clock64();
-  while (true) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if (clock64() - start >= limit) return false;
-    if (mbar_try(bar, parity)) return true;
-  }
-}
 
 // Add a state (ml, o) to the sums that refer to z.
 __device__ __forceinline__ void add_state(float &l, float4 &v, float2 ml, float4 o, float z) {
@@ -123,6 +79,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             const __grid_constant__ KvView c) {
   using Cfg = RowsCfg<DP, WARPS>;
   constexpr int kWarps = WARPS, kThreads = Cfg::kThreads;
+  constexpr bool kPacked = MODE == kPrompt || MODE == kChunks;  // query rows by offsets
   extern __shared__ uint8_t raw[];
   uint8_t *smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
   __shared__ RowsSmem<WARPS> sh;
@@ -130,7 +87,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   if (MODE != kPrompt && tid < WARPS * kStages) mbar_init(smem_u32(&sh.full[tid / kStages][tid % kStages]), 1);
   if (MODE != kPrompt) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   const int dim = MODE == kPrompt ? p.dim : c.head_dim;
-  const int group = MODE == kPrompt ? p.group : d.group;
+  const int group = kPacked ? p.group : d.group;
 
   // The own part of a decode call reads nothing that the shared part's kernel before it
   // writes, and that one has waited for what both read: they run side by side.
@@ -141,17 +98,19 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   // ---- the block's rows, its keys and where they lie
   int kv_head, first = 0, last, table_row = 0;
   int64_t k0 = 0;  // prompt: first key row
-  if (MODE == kPrompt) {
-    kv_head = blockIdx.y;
+  if (kPacked) {
+    kv_head = MODE == kPrompt ? blockIdx.y : blockIdx.x % c.kv_heads;
     if (warp == 0) {
-      const TileOf t = find_tile(p, group, kRows, blockIdx.x);
+      const TileOf t = find_tile(p, group, kRows, MODE == kPrompt ? blockIdx.x : blockIdx.x / c.kv_heads);
       if (lane == 0) sh.tile = t;
     }
     __syncthreads();
     const TileOf t = sh.tile;
     if (t.seq < 0) return;
     k0 = t.k0;
-    const int lq = t.q1 - t.q0, lk = t.k1 - t.k0;
+    const int lq = t.q1 - t.q0;
+    int lk = t.k1 - t.k0;
+    if (MODE == kChunks) table_row = sequence_of(c, d, t.seq, &lk);
     if (tid < kRows) {
       const int64_t r = (int64_t)t.tile * kRows + tid;
       const int token = (int)(r / group), head = kv_head * group + (int)(r % group);
@@ -191,10 +150,15 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 #pragma unroll
   for (int r = 0; r < kRows; r++)
     if (sh.q[r] >= 0) {
-      if (MODE != kPrompt && sh.high[r] > high) table_row = sh.table[r];
+      if (!kPacked && sh.high[r] > high) table_row = sh.table[r];
       low = min(low, sh.low[r]), high = max(high, sh.high[r]);
     }
   low = low / kChunk * kChunk;
+  Range range{};  // chunks: keys go by their number among those that are seen
+  if (MODE == kChunks) {
+    range = range_of(p, low, high, kChunk);
+    low = 0, high = range.keys;
+  }
   first = low, last = high;
   if (MODE != kPrompt && high > low) {
     // this block's part: whole chunks for every warp, and no fewer than 128 keys
@@ -209,7 +173,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   // a row that is not there sees everything: its results are dropped
   const int low_a = qa < 0 ? 0 : sh.low[ra], high_a = qa < 0 ? INT32_MAX : sh.high[ra];
   const int low_b = qb < 0 ? 0 : sh.low[rb8], high_b = qb < 0 ? INT32_MAX : sh.high[rb8];
-  const uint16_t *qp = MODE == kPrompt ? p.q : d.q;
+  const uint16_t *qp = kPacked ? p.q : d.q;
   uint32_t qf[DP / 16][4];
 #pragma unroll
   for (int k = 0; k < DP / 16; k++)
@@ -229,8 +193,9 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   // As the table has it: a number outside the pool is outside the map, too, and reads as zeros.
   // It is looked at when it is used, so that nothing waits for it here, and reported at the end.
   uint32_t largest = 0;
+  auto key_of = [&](int number) -> int { return MODE == kChunks ? range.key(number) : number; };
   auto page_of = [&](int key) -> int {
-    return MODE == kPrompt || key >= last ? -1 : c.table[(int64_t)table_row * c.max_pages + (key >> page_bits)];
+    return MODE == kPrompt || key >= last ? -1 : c.table[(int64_t)table_row * c.max_pages + (key_of(key) >> page_bits)];
   };
   auto load = [&](int key, int page, int stage) {
     const uint32_t kd = ring + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;
@@ -253,7 +218,7 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         const bool is_v = lane >= DP / 64;
         const int slab = lane % (DP / 64);
         tma_load_4d((is_v ? vd : kd) + slab * Cfg::kSlab, is_v ? &v_map : &k_map, slab * 64,
-                    key & (c.page_tokens - 1), kv_head, page, bar);
+                    key_of(key) & (c.page_tokens - 1), kv_head, page, bar);
       }
     }
   };
@@ -262,7 +227,8 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 #pragma unroll
   for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
   float ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
-  const float scale = MODE == kPrompt ? p.scale : d.scale;
+  const float scale = kPacked ? p.scale : d.scale;
+  const int sinks = MODE == kChunks && p.window ? p.sinks : 0;
   constexpr float kRoom = kRowsHeadroom<BF16>;
 
   constexpr int kStep = kWarps * kChunk;
@@ -317,9 +283,10 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int j = key + t * 8 + (lane & 3) * 2 + e;
-        s[t][e] = j >= low_a && j < high_a ? s[t][e] * scale : -INFINITY;
-        s[t][2 + e] = j >= low_b && j < high_b ? s[t][2 + e] * scale : -INFINITY;
+        const int j = key_of(key) + t * 8 + (lane & 3) * 2 + e;
+        const bool sink = MODE == kChunks && j < sinks;
+        s[t][e] = (j >= low_a || sink) && j < high_a ? s[t][e] * scale : -INFINITY;
+        s[t][2 + e] = (j >= low_b || sink) && j < high_b ? s[t][2 + e] * scale : -INFINITY;
         na = fmaxf(na, s[t][e]);
         nb = fmaxf(nb, s[t][2 + e]);
       }
@@ -354,8 +321,9 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     // Where a key is hidden from one row and seen by another, 0 * v must stay 0 for the
     // first: values that are not finite are left out of the product and added for the rows
     // that see them.
-    const bool mixed = __any_sync(0xffffffffu, low_a > key || high_a < key + kChunk ||
-                                                   low_b > key || high_b < key + kChunk);
+    const int at_key = key_of(key);
+    const bool mixed = __any_sync(0xffffffffu, low_a > at_key || high_a < at_key + kChunk ||
+                                                   low_b > at_key || high_b < at_key + kChunk);
     bool wild = false;
     {
       const int r = (lane & 7) + (((lane >> 3) & 1) << 3);
@@ -373,8 +341,9 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
     if (mixed && __any_sync(0xffffffffu, wild)) {
       for (int r = 0; r < kChunk; r++) {
-        const bool sees_a = key + r >= low_a && key + r < high_a;
-        const bool sees_b = key + r >= low_b && key + r < high_b;
+        const bool sink = MODE == kChunks && at_key + r < sinks;
+        const bool sees_a = (at_key + r >= low_a || sink) && at_key + r < high_a;
+        const bool sees_b = (at_key + r >= low_b || sink) && at_key + r < high_b;
 #pragma unroll
         for (int n = 0; n < DP / 8; n++) {
           uint32_t w;
@@ -455,10 +424,10 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
       for (int i = 0; i < kMostJoined; i++)
         if (ml[i].y != 0.0f) add_state(l, v, ml[i], u[i], z);  // else nothing was written
     if (final) {
-      float *lse = MODE == kPrompt ? p.lse : d.lse;
+      float *lse = kPacked ? p.lse : d.lse;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (col < dim) {
-        uint16_t *out = (MODE == kPrompt ? p.out : d.out) + sh.out[r] + col;
+        uint16_t *out = (kPacked ? p.out : d.out) + sh.out[r] + col;
         *reinterpret_cast<uint2 *>(out) =
             make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
       }
@@ -476,8 +445,10 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 // and, with many parts, by their bytes.
 // ---------------------------------------------------------------------------
 
+// Chunks: a row that no entry owns has no parts.
 template <bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeArgs d, int dim) {
+__global__ void __launch_bounds__(kJoinThreads)
+join_kernel(const __grid_constant__ DecodeArgs d, const int32_t *offsets, int entries, int dim) {
   constexpr int kWarps = kJoinThreads / 32;
   __shared__ float top[kWarps], sum[kWarps], factor[kMostParts];
   __shared__ float4 acc[kWarps][64];
@@ -485,6 +456,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = d.part.parts;
   wait_for_previous();
   let_next_start();
+  if (offsets && (row / d.heads < offsets[0] || row / d.heads >= offsets[entries])) return;
   float2 ml[kMostParts / kJoinThreads];
   float m = -INFINITY;
 #pragma unroll
@@ -701,6 +673,29 @@ uint64_t decode_workspace(const DecodePlan &plan, int64_t rows, int dim) {
   return plan.parts() > 1 ? (uint64_t)plan.parts() * rows * (dim * 4 + 8) : 0;
 }
 
+// How a call on chunks of new tokens is cut.
+struct ChunkPlan {
+  bool wide = false;  // eight warps a block
+  int splits = 1;     // of each block's keys
+};
+
+ChunkPlan chunk_plan(int kv_heads, int heads, int dim, int entries, int64_t tokens, int max_length, int window,
+                     int sinks) {
+  ChunkPlan plan;
+  const int group = heads / kv_heads;
+  const int64_t keys = std::max<int64_t>(1, window ? std::min<int64_t>(max_length, (int64_t)window + sinks) : max_length);
+  // blocks: half of each entry's last one is empty on average
+  const int64_t rows = tokens <= entries ? tokens * ((group + kRows - 1) / kRows) : tokens * group / kRows + (entries + 1) / 2;
+  const int64_t items = std::max<int64_t>(1, rows * kv_heads);
+  plan.wide = dim <= 128 && items <= kSms;
+  plan.splits = splits_of(items, (int)keys, kSms * (plan.wide || dim > 128 ? 1 : 2));
+  return plan;
+}
+
+uint64_t chunk_workspace(const ChunkPlan &plan, int64_t rows, int dim) {
+  return plan.splits > 1 ? (uint64_t)plan.splits * rows * (dim * 4 + 8) : 0;
+}
+
 }  // namespace dma
 
 using namespace dma;
@@ -713,7 +708,7 @@ static int32_t bounded_length(const dm_kv_cache_desc &d, int32_t max_length) {
 // Every tile looks for its sequence among all, 32 at a time: half a microsecond for each.
 constexpr int32_t kMostSequences = 1 << 20;
 
-static int32_t check_strides(const int64_t *given, int64_t heads, int dim, int64_t *use, const char *what) {
+int32_t dma::check_strides(const int64_t *given, int64_t heads, int dim, int64_t *use, const char *what) {
   const bool none = given[0] == 0 && given[1] == 0;
   use[0] = none ? heads * dim : given[0];
   use[1] = none ? dim : given[1];
@@ -723,7 +718,7 @@ static int32_t check_strides(const int64_t *given, int64_t heads, int dim, int64
   return DM_OK;
 }
 
-static int32_t check_scale(float given, int dim, float *use) {
+int32_t dma::check_scale(float given, int dim, float *use) {
   if (!std::isfinite(given) || given < 0.0f)
     return fail(DM_ERR_POSITIVE_PARAMETER, "attention needs a finite scale that is not negative");
   *use = (given == 0.0f ? 1.0f / std::sqrt((float)dim) : given) * kLog2e;
@@ -865,7 +860,99 @@ int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *
   }
   if (plan.parts() > 1 && !a.joins)
     return launch_chained("attention join launch", kd.type == DM_BF16 ? join_kernel<true> : join_kernel<false>,
-                          dim3((unsigned)a.part.rows), kJoinThreads, 0, s, a, kd.head_dim);
+                          dim3((unsigned)a.part.rows), kJoinThreads, 0, s, a, (const int32_t *)nullptr, 0, kd.head_dim);
+  return DM_OK;
+}
+
+// What both chunk calls look at.
+static int32_t check_chunk(const dm_kv_cache *cache, const dm_attention_chunk_desc *in, dma::ChunkPlan *plan,
+                           uint64_t *bytes) {
+  if (!cache || !in) return fail(DM_ERR_INVALID_ARGUMENT, "null argument");
+  const dm_kv_cache_desc &d = cache->desc;
+  if (in->heads <= 0 || in->heads % d.kv_heads || in->heads / d.kv_heads > 128)
+    return fail(DM_ERR_ELEMENT_COUNT, "%d query heads over %d key/value heads", in->heads, d.kv_heads);
+  if (in->sequences < 0 || in->sequences > kMostSequences)
+    return fail(DM_ERR_ELEMENT_COUNT, "%d sequences", in->sequences);
+  if (in->window < 0 || in->sinks < 0)
+    return fail(DM_ERR_ELEMENT_COUNT, "window %d, %d sinks", in->window, in->sinks);
+  if (in->max_length < 0) return fail(DM_ERR_ELEMENT_COUNT, "max_length %d", in->max_length);
+  if (in->tokens < 0 || in->tokens > kMostTokens) return fail(DM_ERR_ELEMENT_COUNT, "a bad number of tokens");
+  const int64_t rows = in->tokens * in->heads;
+  const int64_t tiles = in->tokens * (in->heads / d.kv_heads) / kRows + in->sequences;
+  if (rows > INT32_MAX || tiles > INT32_MAX / d.kv_heads) return fail(DM_ERR_OVERFLOW, "too many query rows");
+  *plan = chunk_plan(d.kv_heads, in->heads, d.head_dim, in->sequences, in->tokens,
+                     bounded_length(d, in->max_length), in->window, in->sinks);
+  *bytes = chunk_workspace(*plan, rows, d.head_dim);
+  return DM_OK;
+}
+
+int32_t dm_attention_chunk_workspace(const dm_kv_cache *cache, const dm_attention_chunk_desc *in, uint64_t *bytes) {
+  if (!bytes) return fail(DM_ERR_INVALID_ARGUMENT, "null argument");
+  ChunkPlan plan;
+  return check_chunk(cache, in, &plan, bytes);
+}
+
+int32_t dm_attention_chunk(dm_kv_cache *cache, const dm_attention_chunk_desc *in, void *stream) {
+  ChunkPlan plan;
+  uint64_t need = 0;
+  if (int32_t rc = check_chunk(cache, in, &plan, &need)) return rc;
+  const dm_kv_cache_desc &kd = cache->desc;
+  if (in->layer < 0 || in->layer >= kd.layers)
+    return fail(DM_ERR_INVALID_LAYER, "layer %d of %d", in->layer, kd.layers);
+  if (in->tokens == 0 || in->sequences == 0) return DM_OK;
+  if (!in->q || !in->out || !in->offsets) return fail(DM_ERR_INVALID_ARGUMENT, "null tensor");
+  if (((uintptr_t)in->q | (uintptr_t)in->out) & 15)
+    return fail(DM_ERR_INVALID_ARGUMENT, "attention tensors must be 16-byte aligned");
+  if (need && (!in->workspace || ((uintptr_t)in->workspace & 15)))
+    return fail(DM_ERR_INVALID_ARGUMENT, "chunks need a 16-byte aligned workspace");
+  if (in->workspace_bytes < need)
+    return fail(DM_ERR_BYTE_LENGTH, "a workspace of %llu bytes, %llu are needed",
+                (unsigned long long)in->workspace_bytes, (unsigned long long)need);
+  PromptArgs p{};
+  p.q = (const uint16_t *)in->q;
+  p.out = (uint16_t *)in->out;
+  p.lse = in->lse;
+  if (int32_t rc = check_strides(in->q_stride, in->heads, kd.head_dim, p.q_stride, "query")) return rc;
+  if (int32_t rc = check_strides(in->out_stride, in->heads, kd.head_dim, p.out_stride, "output")) return rc;
+  if (int32_t rc = check_scale(in->scale, kd.head_dim, &p.scale)) return rc;
+  p.q_offsets = p.k_offsets = in->offsets;
+  p.q_tokens = p.k_tokens = in->tokens;
+  p.heads = in->heads;
+  p.kv_heads = kd.kv_heads;
+  p.group = in->heads / kd.kv_heads;
+  p.dim = kd.head_dim;
+  p.sequences = in->sequences;
+  p.causal = 1;
+  p.window = in->window;
+  p.sinks = in->sinks;
+  DecodeArgs a{};
+  a.out = p.out;
+  a.lse = p.lse;
+  a.out_stride[0] = p.out_stride[0];
+  a.out_stride[1] = p.out_stride[1];
+  a.sequences = in->rows;
+  a.heads = in->heads;
+  a.layer = in->layer;
+  a.max_length = bounded_length(kd, in->max_length);
+  a.splits = a.part.parts = plan.splits;
+  a.part.rows = in->tokens * in->heads;
+  a.part.o = (float *)in->workspace;
+  a.part.ml = (float2 *)(a.part.o + (int64_t)a.part.parts * a.part.rows * kd.head_dim);
+  a.timeout = cache->ctx->status + kStatusWord;
+  a.wait_limit = wait_limit(cache->ctx);
+  cudaSetDevice(cache->ctx->device);
+  cudaStream_t s = (cudaStream_t)stream;
+  CUtensorMap maps[2];
+  if (!describe_chunks(kd.type, cache->view, in->layer, kChunk, maps))
+    return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
+  const int64_t tiles = in->tokens * p.group / kRows + in->sequences;
+  const dim3 grid((unsigned)(tiles * kd.kv_heads), plan.splits);
+  if (int32_t rc = plan.wide ? launch_rows<kChunks, 8>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s)
+                             : launch_rows<kChunks, 4>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s))
+    return rc;
+  if (plan.splits > 1)
+    return launch_chained("attention join launch", kd.type == DM_BF16 ? join_kernel<true> : join_kernel<false>,
+                          dim3((unsigned)a.part.rows), kJoinThreads, 0, s, a, in->offsets, in->sequences, kd.head_dim);
   return DM_OK;
 }
 

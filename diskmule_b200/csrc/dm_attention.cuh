@@ -29,7 +29,8 @@ struct PromptArgs {
   const int32_t *q_offsets, *k_offsets;
   int64_t q_tokens, k_tokens;
   int32_t heads, kv_heads, group, dim, sequences, causal, window;
-  float scale;  // times log2 e
+  int32_t sinks;  // chunks: with a window, keys below this are seen all the same
+  float scale;    // times log2 e
 };
 
 // States of parts of the keys: o [part][row][dim], ml [part][row] = (m, l), with row =
@@ -51,6 +52,7 @@ __device__ __forceinline__ int high_of(const PromptArgs &p, int lq, int lk, int 
   return p.causal ? max(0, min(lk, place_of(lq, lk, i) + 1)) : lk;
 }
 
+// Decode; of chunks the parts, the cache's side and the waits.
 struct DecodeArgs {
   const uint16_t *q;
   uint16_t *out;
@@ -170,6 +172,23 @@ __device__ __forceinline__ TileOf find_tile(const PromptArgs &p, int per_token, 
   return r;
 }
 
+// Chunks: the keys that an item's rows see, [0, end) where the window reaches back to the sinks, else
+// [0, sinks) and [low, end). Numbered without the gap they are [0, keys). sinks is a multiple of
+// `unit`, so a run of `unit` numbers from a multiple of it on is a run of keys, and low is one of
+// the power of two in `unit`, so that boxes of that size lie in one page.
+struct Range {
+  int sinks, low, keys;
+  __device__ __forceinline__ int key(int number) const { return number < sinks ? number : number - sinks + low; }
+};
+__device__ __forceinline__ Range range_of(const PromptArgs &p, int low, int end, int unit) {
+  Range r{0, 0, end};
+  // no end is near 2^31, and sinks beyond it are all there are
+  const int sinks = p.window ? (min(p.sinks, end) + unit - 1) / unit * unit : 0;
+  low = low / (unit & -unit) * (unit & -unit);
+  if (low > sinks) r = Range{sinks, low, sinks + max(0, end - low)};
+  return r;
+}
+
 // Row of the page table and tokens of batch entry b; an entry that is out of range is empty.
 __device__ __forceinline__ int sequence_of(const KvView &c, const DecodeArgs &a, int b, int *length) {
   const int row = a.sequences ? a.sequences[b] : b;
@@ -180,5 +199,9 @@ __device__ __forceinline__ int sequence_of(const KvView &c, const DecodeArgs &a,
   *length = min(max(c.lengths[row], 0), min(a.max_length, c.max_pages * c.page_tokens));
   return row;
 }
+
+// Strides of a call, {token, head} (both 0: contiguous), and the scale of its scores.
+int32_t check_strides(const int64_t *given, int64_t heads, int dim, int64_t *use, const char *what);
+int32_t check_scale(float given, int dim, float *use);
 
 }  // namespace dma

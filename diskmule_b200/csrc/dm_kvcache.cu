@@ -5,6 +5,7 @@
 // asked for is the i-th lowest free one whatever the number of threads. Many blocks then
 // move rows. All of it is bound by latency (the plan: a few dependent passes over a list
 // and over `references`) or by memory (the rows), and nothing waits for the host.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -15,6 +16,7 @@
 
 using dma::KvView;
 using dmi::fail;
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -426,6 +428,168 @@ gather_kernel(KvView c, Plan p, PlanArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Eviction: choose the tokens that stay, compact by the list, move their weights.
+//
+// The budget-th largest weight is found digit by digit (11, 11 and 10 bits of the weights'
+// patterns in their order): each step counts the next digit of those that share the digits found so
+// far. The blocks of a cluster have a part of the sequence each and add their counts through
+// distributed shared memory. Then one pass writes the positions above that weight, and the first
+// of those equal to it, in order. Bound by latency: five passes over weights that lie in L2.
+// ---------------------------------------------------------------------------
+
+constexpr int kMostRanks = 8;
+constexpr int kRankTokens = 4096;  // of a block before a sequence gets another
+constexpr int kDigits = 2048;
+
+struct EvictArgs {
+  const int32_t *rows;
+  float *weights;
+  int64_t stride;
+  int32_t *keep_offsets, *keep;
+  int32_t n, budget, sinks, recent;
+};
+
+// In the order of the values; NaN below all
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 + 0 = 0
+  return x != x ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ int tokens_of(const KvView &c, int row) {
+  if (row < 0 || row >= c.max_sequences) return 0;
+  return (int)min((int64_t)max(c.lengths[row], 0), c.max_pages * (int64_t)c.page_tokens);
+}
+
+// Cluster (all x, i) chooses for entry i.
+__global__ void __launch_bounds__(kPlanThreads) choose_kernel(KvView c, EvictArgs a) {
+  __shared__ int count[3][kDigits];
+  __shared__ int shared[4], found[2];
+  auto cluster = cg::this_cluster();
+  const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x;
+  chain();
+  for (int i = tid; i < 3 * kDigits; i += kPlanThreads) (&count[0][0])[i] = 0;
+  const int entry = blockIdx.y, row = a.rows[entry];
+  const int length = tokens_of(c, row), budget = a.budget;
+  // where the entry's list begins
+  int before = 0, sum;
+  for (int i = tid; i < entry; i += kPlanThreads) before += min(tokens_of(c, a.rows[i]), budget);
+  block_scan(before, &sum);
+  const int begin = sum;
+  const bool fits = length <= a.stride;
+  if (rank == 0 && tid == 0) {
+    if (entry == 0) a.keep_offsets[0] = 0;
+    // a count below zero is refused with the rest of the call
+    a.keep_offsets[entry + 1] = fits ? begin + min(length, budget) : -1;
+  }
+  if (!fits) return;
+  int32_t *keep = a.keep + begin;
+  if (length <= budget) {
+    for (int j = rank * kPlanThreads + tid; j < length; j += ranks * kPlanThreads) keep[j] = j;
+    return;
+  }
+  const float *weights = a.weights + row * a.stride;
+  const int low = a.sinks, high = length - a.recent;  // tokens that are weighed
+  int need = budget - a.sinks - a.recent;             // of them
+  // this block's tokens: a multiple of four for every thread
+  const int share = ((length + ranks - 1) / ranks + 3) / 4 * 4;
+  const int from = min(length, rank * share), to = min(length, from + share);
+  uint32_t digits = 0;  // of the last weight that stays, from above
+  cluster.sync();  // the counts are zero
+#pragma unroll 1
+  for (int step = 0; step < 3; step++) {
+    const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, above = step == 0 ? 32 : step == 1 ? 21 : 10;
+    const uint32_t mask = step == 2 ? 1023 : 2047;
+    for (int j = max(low, from) + tid; j < min(high, to); j += kPlanThreads) {
+      const uint32_t u = ordered(weights[j]);
+      if (step == 0 || u >> above == digits) atomicAdd(&count[step][u >> shift & mask], 1);
+    }
+    cluster.sync();
+    // two digits a thread, the largest first
+    int mine[2] = {0, 0};
+    for (int r = 0; r < ranks; r++) {
+      const int *there = ranks == 1 ? count[step] : cluster.map_shared_rank(&count[step][0], r);
+      for (int k = 0; k < 2; k++) mine[k] += there[kDigits - 1 - (2 * tid + k)];
+    }
+    const int upto = block_scan(mine[0] + mine[1], &sum), first = upto - mine[0] - mine[1];
+    if (need > 0 && first < need && need <= upto) {
+      const int second = need > first + mine[0];
+      found[0] = kDigits - 1 - (2 * tid + second);
+      found[1] = need - first - (second ? mine[0] : 0);
+    }
+    __syncthreads();
+    if (need > 0) {
+      digits = digits << (step == 0 ? 0 : step == 1 ? 11 : 10) | found[0];
+      need = found[1];  // of those that share the digits
+    }
+    __syncthreads();
+  }
+  // What stays: whatever the weight, above the last one, or among the first `need` equal to it
+  auto class_of = [&](int j) -> uint32_t {
+    if (j >= to) return 0;
+    if (j < low || j >= high) return 1;
+    if (budget == a.sinks + a.recent) return 0;
+    const uint32_t u = ordered(weights[j]);
+    return u > digits ? 1 : u == digits ? 1u << 16 : 0;
+  };
+  // Both counts of a round of 4 tokens a thread fit 16 bits; those of a block do not.
+  int sure = 0, ties = 0;
+  for (int j0 = from; j0 < to; j0 += 4 * kPlanThreads)
+    for (int k = 0; k < 4; k++) {
+      const uint32_t x = class_of(j0 + k * kPlanThreads + tid);
+      sure += x & 0xffff, ties += x >> 16;
+    }
+  block_scan(sure, &sum);
+  if (tid == 0) shared[0] = sum;
+  block_scan(ties, &sum);
+  if (tid == 0) shared[1] = sum;
+  cluster.sync();
+  int at = 0, left = need;  // places before this block's; ties that may still stay
+  for (int r = 0; r < rank; r++) {
+    const int *there = cluster.map_shared_rank(&shared[0], r);
+    const int some = min(there[1], left);
+    at += there[0] + some, left -= some;
+  }
+  for (int j0 = from; j0 < to; j0 += 4 * kPlanThreads) {
+    uint32_t x[4], all = 0;
+    for (int k = 0; k < 4; k++) x[k] = class_of(j0 + 4 * tid + k), all += x[k];
+    uint32_t b = (uint32_t)block_scan((int)all, &sum) - all;
+    for (int k = 0; k < 4; k++, b += x[k - 1]) {
+      const int tie = b >> 16;
+      if (x[k] == 1 || (x[k] && tie < left)) keep[at + (b & 0xffff) + min(tie, left)] = j0 + 4 * tid + k;
+    }
+    at += (sum & 0xffff) + min(sum >> 16, left);
+    left -= min(sum >> 16, left);
+  }
+  cluster.sync();  // nobody reads this block's shared memory any more
+}
+
+// Weights of entry i go with their tokens, whose places only fall: a round's sources lie at its
+// own places or behind them. Before the lengths change.
+__global__ void __launch_bounds__(kPlanThreads) move_weights_kernel(KvView c, Plan p, EvictArgs a) {
+  chain();
+  if (!*p.ok) return;
+  const int i = blockIdx.x, row = a.rows[i], tid = threadIdx.x;
+  const int begin = a.keep_offsets[i], count = a.keep_offsets[i + 1] - begin, length = tokens_of(c, row);
+  const int32_t *keep = a.keep + begin;
+  float *weights = a.weights + row * a.stride;
+  if (count == length) return;
+  for (int j0 = 0; j0 < length; j0 += 4 * kPlanThreads) {
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int j = j0 + k * kPlanThreads + tid;
+      x[k] = j < count ? weights[keep[j]] : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int j = j0 + k * kPlanThreads + tid;
+      if (j < length) weights[j] = x[k];
+    }
+  }
+}
+
 // Free: block i takes the length of its sequence (a repeat finds zero) and lets go.
 __global__ void __launch_bounds__(kCopyThreads) free_kernel(KvView c, const int32_t *rows) {
   __shared__ int held;
@@ -525,6 +689,14 @@ constexpr int64_t kSmallCopy = 512 * 1024, kSmallRows = 16384;  // bytes of page
 template <typename... Params, typename... Args>
 int32_t launch(void (*kernel)(Params...), dim3 grid, int threads, void *stream, const Args &...args) {
   return dma::launch_chained("cache launch", kernel, grid, threads, 0, (cudaStream_t)stream, args...);
+}
+
+int32_t launch_gather(const dm_kv_cache *c, const PlanArgs &a, int64_t kept, void *stream) {
+  // at most this many fresh pages
+  const int64_t fresh = std::min<int64_t>(c->desc.pages, kept / c->desc.page_tokens + a.n);
+  const dim3 grid(blocks_along(c->view.page_bytes / 16, fresh, kGridBlocks),
+                  (unsigned)std::min<int64_t>(fresh + a.n, 65535));
+  return launch(gather_kernel, grid, kCopyThreads, stream, c->view, plan_of(c), a);
 }
 
 int32_t check_list(const dm_kv_cache *cache, const void *list, int32_t n) {
@@ -724,11 +896,7 @@ int32_t dm_kv_cache_compact(dm_kv_cache *c, const int32_t *sequences, const int3
   const PlanArgs a{sequences, keep_offsets, keep, kept, n};
   if (int32_t rc = launch(plan_kernel<kCompact>, 1, kPlanThreads, stream, c->view, plan_of(c), a))
     return rc;
-  // at most this many fresh pages
-  const int64_t fresh = std::min<int64_t>(c->desc.pages, kept / c->desc.page_tokens + n);
-  const dim3 grid(blocks_along(c->view.page_bytes / 16, fresh, kGridBlocks),
-                  (unsigned)std::min<int64_t>(fresh + n, 65535));
-  return launch(gather_kernel, grid, kCopyThreads, stream, c->view, plan_of(c), a);
+  return launch_gather(c, a, kept, stream);
 }
 
 int32_t dm_kv_cache_free(dm_kv_cache *c, const int32_t *sequences, int32_t n, void *stream) {
@@ -748,6 +916,36 @@ int32_t dm_kv_cache_copy_pages(dm_kv_cache *c, const int32_t *source, const int3
   cudaSetDevice(c->ctx->device);
   const dim3 grid(blocks_along(c->view.page_bytes / 16, n, kGridBlocks), n);
   return launch(copy_pages_kernel, grid, kCopyThreads, stream, c->view, source, target);
+}
+
+int32_t dm_kv_cache_evict(dm_kv_cache *c, const dm_kv_cache_evict_desc *in, void *stream) {
+  if (!in) return fail(DM_ERR_INVALID_ARGUMENT, "null argument");
+  if (int32_t rc = check_list(c, in->rows, in->sequences)) return rc;
+  if (in->sinks < 0 || in->recent < 0 || in->budget < 0 || (int64_t)in->sinks + in->recent > in->budget)
+    return fail(DM_ERR_ELEMENT_COUNT, "%d first and %d last tokens of %d", in->sinks, in->recent, in->budget);
+  if ((int64_t)in->budget * in->sequences > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many kept tokens");
+  if (in->weights_stride < 0) return fail(DM_ERR_INVALID_ARGUMENT, "a negative stride of weights");
+  if (in->sequences == 0) return DM_OK;
+  if (in->sequences > 65535) return fail(DM_ERR_ELEMENT_COUNT, "%d sequences in one call", in->sequences);
+  if (!in->weights || !in->keep_offsets || (!in->keep && in->budget))
+    return fail(DM_ERR_INVALID_ARGUMENT, "null weights or keep list");
+  if (((uintptr_t)in->weights | (uintptr_t)in->keep_offsets | (uintptr_t)in->keep) & 3)
+    return fail(DM_ERR_INVALID_ARGUMENT, "weights and lists must be 4-byte aligned");
+  cudaSetDevice(c->ctx->device);
+  const int32_t n = in->sequences;
+  const EvictArgs e{in->rows, in->weights, in->weights_stride, in->keep_offsets, in->keep, n, in->budget, in->sinks,
+                    in->recent};
+  const int64_t most = std::min<int64_t>((int64_t)c->desc.max_pages * c->desc.page_tokens, in->weights_stride);
+  int ranks = 1;
+  while (ranks < kMostRanks && most > (int64_t)ranks * kRankTokens) ranks *= 2;
+  if (int32_t rc = dma::launch_clusters("cache launch", choose_kernel, dim3(ranks, n), ranks, kPlanThreads, 0,
+                                        (cudaStream_t)stream, c->view, e))
+    return rc;
+  const int64_t kept = (int64_t)in->budget * n;
+  const PlanArgs a{in->rows, in->keep_offsets, in->keep, kept, n};
+  if (int32_t rc = launch(plan_kernel<kCompact>, 1, kPlanThreads, stream, c->view, plan_of(c), a)) return rc;
+  if (int32_t rc = launch(move_weights_kernel, n, kPlanThreads, stream, c->view, plan_of(c), e)) return rc;
+  return launch_gather(c, a, kept, stream);
 }
 
 }  // extern "C"

@@ -35,21 +35,30 @@ __device__ __forceinline__ void wait_for_previous() {
 
 // A launch that may be scheduled while the kernel before it still runs; the kernel calls
 // wait_for_previous before it touches what that one or its predecessors wrote.
+// launch_clusters: `ranks` blocks along x make a cluster.
 template <typename... Params, typename... Args>
-int32_t launch_chained(const char *what, void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
-                       cudaStream_t stream, const Args &...args) {
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
+int32_t launch_clusters(const char *what, void (*kernel)(Params...), dim3 grid, int ranks, int threads, size_t smem,
+                        cudaStream_t stream, const Args &...args) {
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = ranks;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = threads;
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = ranks > 1 ? 2 : 1;
   DM_CUDA(cudaLaunchKernelEx(&config, kernel, args...), what);
   return DM_OK;
+}
+template <typename... Params, typename... Args>
+int32_t launch_chained(const char *what, void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                       cudaStream_t stream, const Args &...args) {
+  return launch_clusters(what, kernel, grid, 1, threads, smem, stream, args...);
 }
 
 }  // namespace dma

@@ -7,6 +7,12 @@
  *   dm_kv_cache_*         a paged cache: extend, write, fork, compact, free, copy pages
  *   dm_attention_decode   one query token per sequence against the cache; tokens that all
  *                         sequences share are read once for the whole batch
+ *   dm_attention_chunk    the new tokens of each sequence, one or thousands, against the cache,
+ *                         with a sliding window and first tokens that stay visible (sinks)
+ *   dm_attention_rotate   norms of each head and position rotation on the way from the
+ *                         projections to the queries and into the cache
+ *   dm_attention_weights  the attention that each cached token has received
+ *   dm_kv_cache_evict     cut sequences down to the tokens that have received most
  *
  * Conventions:
  *   - tensors are DM_BF16 or DM_F16, the same type on input and output; scores, softmax
@@ -163,6 +169,133 @@ DM_API int32_t dm_attention_decode_workspace(const dm_kv_cache *cache, int32_t h
                                              uint64_t *bytes);
 DM_API int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode_desc *desc,
                                    void *stream);
+
+/* ---- chunks of new tokens ------------------------------------------------------------- */
+
+/* Attention of new tokens, which lie in the cache already, over all that their sequences hold.
+ * q and out [tokens, heads, head_dim] (strides as above), lse [tokens, heads]. Entry i owns the
+ * rows [offsets[i], offsets[i + 1]) (device int32, [sequences + 1], ascending from >= 0); they
+ * are the last tokens of cache row rows[i] (NULL = row i), in order: row j of L stands at
+ * position p = j + length - L and sees the keys k <= p; with window > 0 only k > p - window and
+ * k < sinks (without a window sinks has no meaning). A row that sees no key (more rows than
+ * tokens, an entry outside the table) gives zeros and -infinity. Rows of q that no entry owns
+ * are not read and their output is left as it was, so tokens and sequences may be bounds (a
+ * captured graph): entries without rows are passed over. Entries may name a row twice.
+ * max_length bounds the lengths as in decode, and so do workspace and bad page numbers; at most
+ * 128 query heads per key/value head and 2^20 sequences. */
+typedef struct {
+  int32_t layer, heads, sequences, window, sinks, max_length;
+  float scale;
+  int64_t tokens;
+  const void *q;
+  void *out;
+  float *lse;
+  int64_t q_stride[2], out_stride[2];
+  const int32_t *rows, *offsets;
+  void *workspace;
+  uint64_t workspace_bytes;
+} dm_attention_chunk_desc;
+
+/* Bytes for a call with these numbers; the other members of desc are not looked at. */
+DM_API int32_t dm_attention_chunk_workspace(const dm_kv_cache *cache,
+                                            const dm_attention_chunk_desc *desc, uint64_t *bytes);
+DM_API int32_t dm_attention_chunk(dm_kv_cache *cache, const dm_attention_chunk_desc *desc,
+                                  void *stream);
+
+/* ---- norms and position rotation ------------------------------------------------------- */
+
+/* What turns with the position: the first rotary_dim values of a head (a multiple of 16 up to
+ * 256), in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved. Pair i turns by
+ * positions[pair_axes[i]] * frequencies[i] radians. frequencies (host, rotary_dim / 2 of them;
+ * NULL = theta^(-2 i / rotary_dim)) are taken in 64 bits and angles are exact to 2^-32 of a
+ * turn wherever the position. pair_axes (host, NULL = all 0) are below axes, 1 to 4. scale
+ * multiplies cosine and sine (0 = 1). The arrays are copied. */
+typedef struct dm_rope dm_rope;
+typedef struct {
+  int32_t rotary_dim, interleaved, axes;
+  float scale;
+  double theta;
+  const double *frequencies;
+  const int32_t *pair_axes;
+} dm_rope_desc;
+
+DM_API int32_t dm_rope_create(dm_cuda_context *ctx, const dm_rope_desc *desc, dm_rope **out);
+DM_API void dm_rope_destroy(dm_rope *rope);
+
+/* Each head of q, k and v [tokens, heads or kv_heads, head_dim] is divided by its root mean
+ * square (if norms has its bit: x / sqrt(mean x^2 + epsilon), times q_weight or k_weight, f32
+ * [head_dim], NULL = ones), queries and keys are then rotated (rope NULL: not), in f32 and
+ * rounded once. Results go to q_out, k_out and v_out (each may be its input, with the same
+ * strides) and, with a cache, keys and values into layer `layer` of it: entry i owns the rows
+ * [offsets[i], offsets[i + 1]), which are the last tokens of cache row rows[i] (NULL = row i;
+ * lengths count them already). NULL inputs are left out (k and v go together where there is a
+ * cache), and so are NULL outputs.
+ * positions: device int32 [axes][tokens]; NULL (with a cache) = the token's place in its
+ * sequence along every axis. With a cache, rows that no entry owns are not read and their
+ * outputs are left as they were; one whose place is not in the table is not cached and sets
+ * DM_KV_BAD_TOKEN, and stands at position 0 where positions is NULL. No cache row is named
+ * twice. Without a cache the call does all tokens and reads neither rows nor offsets.
+ * Pointers are 16-byte aligned, weights 4; strides as above. */
+enum { DM_NORM_Q = 1, DM_NORM_K = 2, DM_NORM_V = 4 };
+typedef struct {
+  int32_t type, heads, kv_heads, head_dim, norms;
+  float epsilon;
+  int32_t layer, sequences;
+  int64_t tokens;
+  const void *q, *k, *v;
+  void *q_out, *k_out, *v_out;
+  int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2], k_out_stride[2], v_out_stride[2];
+  const float *q_weight, *k_weight;
+  const int32_t *positions, *rows, *offsets;
+} dm_attention_rotate_desc;
+
+/* cache may be NULL; it and rope belong to ctx. */
+DM_API int32_t dm_attention_rotate(dm_cuda_context *ctx, const dm_rope *rope, dm_kv_cache *cache,
+                                   const dm_attention_rotate_desc *desc, void *stream);
+
+/* ---- received attention, and eviction by it --------------------------------------------- */
+
+/* weights[rows[i]][k] += the attention that token k of the sequence gets from the rows of q of
+ * entry i, over all heads: sum exp(scale q k - lse), with q, lse, entries, window and sinks as in
+ * dm_attention_chunk (decode: one row each) and lse what it returned; a row whose lse is
+ * -infinity gives nothing. weights: device f32, one row of weights_stride for every row of the
+ * table; tokens from weights_stride on are passed over. Calls that are alike add in the same order. A cache row
+ * that is named twice counts for its first entry and sets DM_KV_BAD_SEQUENCE; entries outside
+ * the table are passed over. */
+typedef struct {
+  int32_t layer, heads, sequences, window, sinks, max_length;
+  float scale;
+  int64_t tokens;
+  const void *q;
+  const float *lse;
+  int64_t q_stride[2];
+  const int32_t *rows, *offsets;
+  float *weights;
+  int64_t weights_stride;
+} dm_attention_weights_desc;
+
+DM_API int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_weights_desc *desc,
+                                    void *stream);
+
+/* Cuts the sequences rows[i] (device int32) down to `budget` tokens: the first `sinks`, the last
+ * `recent` (together at most budget) and, of those between, the ones with the largest weights
+ * (of equal ones the earlier; -0 equals 0; NaN is below all), in their order. A sequence of at
+ * most budget tokens keeps all. keep_offsets [sequences + 1] and keep [sequences * budget]
+ * (device int32) receive the positions that stay, packed as dm_kv_cache_compact takes them, and
+ * the cache is compacted by them under its rules; the kept tokens' weights move along, and those
+ * of the places behind them, up to the old length, become 0. weights_stride must hold every
+ * token of a row of the table, or of the longest sequence (DM_KV_BAD_TOKEN otherwise). What is
+ * refused leaves cache and weights unchanged; keep and keep_offsets are then undefined. */
+typedef struct {
+  int32_t sequences, budget, sinks, recent;
+  const int32_t *rows;
+  float *weights;
+  int64_t weights_stride;
+  int32_t *keep_offsets, *keep;
+} dm_kv_cache_evict_desc;
+
+DM_API int32_t dm_kv_cache_evict(dm_kv_cache *cache, const dm_kv_cache_evict_desc *desc,
+                                 void *stream);
 
 #ifdef __cplusplus
 }
