@@ -561,6 +561,7 @@ constexpr int kSms = 148;
 // tokens take 48 and 52.
 constexpr int64_t kMostRowsBytes = 12 << 20;
 constexpr int kSplitKeys = 128;  // a block's keys at least, where there are several
+constexpr int kTileRows = 128;   // of a unit on tcgen05 tiles
 
 // Blocks that cut `items` rows of blocks along `keys`: as many as run at once, no more (a
 // second round costs more than shorter blocks save).
@@ -675,21 +676,61 @@ uint64_t decode_workspace(const DecodePlan &plan, int64_t rows, int dim) {
 
 // How a call on chunks of new tokens is cut.
 struct ChunkPlan {
-  bool wide = false;  // eight warps a block
-  int splits = 1;     // of each block's keys
+  bool tiles = false;  // on tcgen05 tiles, else on blocks of 16 rows
+  bool wide = false;   // these: eight warps a block
+  int splits = 1;      // of each item's keys
 };
 
+// Microseconds on one B200, as measured, for a tile of one unit's rows and of two (80 keys of dim
+// 128, 128 of the others; pages of 16 tokens at dim 256, where wider ones take half), and for what
+// an item of a block has besides. The rest is as in decode.
+constexpr float kChunkStepUs[3][2] = {{1.2f, 1.5f}, {0.9f, 1.05f}, {2.0f, 2.0f}}, kChunkItemUs = 2.0f;
+
+// The host knows bounds only: entries, their rows together, the longest one's keys. Entries are
+// taken to be alike.
 ChunkPlan chunk_plan(int kv_heads, int heads, int dim, int entries, int64_t tokens, int max_length, int window,
                      int sinks) {
-  ChunkPlan plan;
+  ChunkPlan best;
+  if (tokens == 0 || entries == 0) return best;
   const int group = heads / kv_heads;
-  const int64_t keys = std::max<int64_t>(1, window ? std::min<int64_t>(max_length, (int64_t)window + sinks) : max_length);
-  // blocks: half of each entry's last one is empty on average
-  const int64_t rows = tokens <= entries ? tokens * ((group + kRows - 1) / kRows) : tokens * group / kRows + (entries + 1) / 2;
-  const int64_t items = std::max<int64_t>(1, rows * kv_heads);
-  plan.wide = dim <= 128 && items <= kSms;
-  plan.splits = splits_of(items, (int)keys, kSms * (plan.wide || dim > 128 ? 1 : 2));
-  return plan;
+  const int64_t busy = std::min<int64_t>(entries, tokens), each = (tokens + busy - 1) / busy;
+  // what the rows of a block or unit see
+  auto keys_of = [&](int64_t rows) {
+    return (int)std::max<int64_t>(1, window ? std::min<int64_t>(max_length, (int64_t)window + sinks + rows) : max_length);
+  };
+  auto join_us = [&](int parts) { return parts > 1 ? kJoinUs + kJoinMbUs * parts * ((float)tokens * heads * dim * 4e-6f) : 0.0f; };
+  float best_us = 0.0f;
+  auto offer = [&](const ChunkPlan &plan, float us) {
+    if (best_us == 0.0f || us < best_us) best = plan, best_us = us;
+  };
+  {
+    const int64_t blocks = busy * ((each * group + kRows - 1) / kRows) * kv_heads;
+    const int keys = keys_of(kRows / group);
+    ChunkPlan plan;
+    plan.wide = dim <= 128 && blocks <= kSms;
+    const int at_once = kSms * (plan.wide || dim > 128 ? 1 : 2), warps = plan.wide ? 8 : 4;
+    const float step = dim > 128 ? kRowsStepWideUs : kRowsStepUs;
+    const int most = splits_of(blocks, keys, at_once);
+    for (int splits : {1, most}) {
+      plan.splits = splits;
+      offer(plan, std::max(1.0f, (float)blocks * splits / at_once) *
+                      (kRowsUs + step * ((keys + 16 * warps * splits - 1) / (16 * warps * splits))) + join_us(splits));
+    }
+  }
+  const int64_t per = tile_chunk_tokens(dim, group);
+  const int64_t items = busy * ((each + per - 1) / per) * kv_heads;
+  const bool two = each > kTileRows / group;
+  const int tiles = (keys_of(std::min(each, per)) + tile_keys(dim) - 1) / tile_keys(dim);
+  const float step = kChunkStepUs[dim <= 64 ? 0 : dim <= 128 ? 1 : 2][two];
+  ChunkPlan plan;
+  plan.tiles = true;
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(2 * kSms / items, std::min(tiles / 2, kMostParts)));
+  for (plan.splits = 1; plan.splits <= most; plan.splits++) {
+    const int64_t rounds = (items * plan.splits + kSms - 1) / kSms;
+    offer(plan, kTileUs + rounds * step * ((tiles + plan.splits - 1) / plan.splits) + (rounds - 1) * kChunkItemUs +
+                    join_us(plan.splits));
+  }
+  return best;
 }
 
 uint64_t chunk_workspace(const ChunkPlan &plan, int64_t rows, int dim) {
@@ -943,11 +984,13 @@ int32_t dm_attention_chunk(dm_kv_cache *cache, const dm_attention_chunk_desc *in
   cudaSetDevice(cache->ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   CUtensorMap maps[2];
-  if (!describe_chunks(kd.type, cache->view, in->layer, kChunk, maps))
+  const bool on_tiles = plan.tiles && tile_chunks_fit(p);
+  if (!on_tiles && !describe_chunks(kd.type, cache->view, in->layer, kChunk, maps))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
   const int64_t tiles = in->tokens * p.group / kRows + in->sequences;
   const dim3 grid((unsigned)(tiles * kd.kv_heads), plan.splits);
-  if (int32_t rc = plan.wide ? launch_rows<kChunks, 8>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s)
+  if (int32_t rc = on_tiles  ? launch_tile_chunks(kd.type, p, a, cache->view, s)
+                   : plan.wide ? launch_rows<kChunks, 8>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s)
                              : launch_rows<kChunks, 4>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s))
     return rc;
   if (plan.splits > 1)

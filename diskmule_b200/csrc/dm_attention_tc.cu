@@ -101,7 +101,8 @@ struct Item {
   int n[2];                         // tiles of each unit
   int max_low, min_high;            // every row sees the keys [max_low, min_high)
   int token0, lq, lk, q0, k0;       // first token of the item and of its sequence
-  int table_row, end;               // shared: where its pages are looked up; no row sees keys from `end` on
+  int table_row, end;               // paged: where its pages are looked up; no row sees keys from `end` on
+  int split, sinks, gap;            // chunks: its part of the keys; numbers from `sinks` on are keys `gap` further
   int wild;                         // values that are not finite were found
 };
 
@@ -181,16 +182,16 @@ constexpr uint32_t idesc(bool bf16, int n, bool b_n_major) {
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-enum TcMode { kTcPrompt, kTcShared };
+enum TcMode { kTcPrompt, kTcShared, kTcChunks };
 
 struct TcArgs {
   PromptArgs p;
   DecodeArgs d;
   KvView c;
   int tokens;     // of a unit: 128 / group
-  int tiles;      // prompt: upper bound of the number of items per key/value head
+  int tiles;      // prompt, chunks: upper bound of the number of items per key/value head
   int alternate;  // shared: one unit's rows hold them all; the units take tiles in turn
-  int k_box, v_box;  // shared: rows of a TMA box
+  int k_box, v_box;  // paged: rows of a TMA box
   int wide;          // rows of the result (or of the parts) lie on 32-byte boundaries
   int32_t *timeout;
   int64_t wait_limit;
@@ -287,10 +288,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// First key of tile t of an item; chunks number the keys without the gap behind the sinks.
+template <int MODE, int KEYS>
+__device__ __forceinline__ int key_of(const Item &w, int t) {
+  const int number = w.first + t * KEYS;
+  return MODE == kTcChunks && number >= w.sinks ? number + w.gap : number;
+}
 // Whether some row does not see some key of tile t.
-template <int KEYS>
+template <int MODE, int KEYS>
 __device__ __forceinline__ bool mixed(const Item &w, int t) {
-  const int key = w.first + t * KEYS;
+  const int key = key_of<MODE, KEYS>(w, t);
   return key < w.max_low || key + KEYS > w.min_high;
 }
 
@@ -319,6 +326,47 @@ struct Place {
   }
 };
 
+// Chunks: the items of `tokens` tokens in order of their sequences' lengths, in four steps of the
+// longest, so that no long item begins when the others are done, and from a sequence's last on.
+// One warp; as find_tile.
+__device__ __forceinline__ TileOf find_chunk(const PromptArgs &p, const DecodeArgs &d, const KvView &c, int tokens,
+                                             int64_t tile) {
+  const int lane = threadIdx.x & 31;
+  TileOf r{-1, 0, 0, 0, 0, 0, 0};
+  const int step = d.max_length / 4 + 1;
+  for (int turn = 3; turn >= 0; turn--)
+    for (int s0 = 0; s0 < p.sequences; s0 += 32) {
+      const int s = s0 + lane;
+      int q0 = 0, q1 = 0;
+      if (s < p.sequences) {
+        int length;
+        sequence_of(c, d, s, &length);
+        q0 = p.q_offsets[s], q1 = p.q_offsets[s + 1];
+        q0 = (int)min((int64_t)max(q0, 0), p.q_tokens), q1 = max(q0, (int)min((int64_t)q1, p.q_tokens));
+        if (length / step != turn) q1 = q0;
+      }
+      const int64_t n = ((int64_t)(q1 - q0) + tokens - 1) / tokens;
+      int64_t upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, tile < upto);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        r.seq = s0 + src;
+        r.tile = (int)__shfl_sync(0xffffffffu, upto - 1 - tile, src);
+        r.q0 = __shfl_sync(0xffffffffu, q0, src);
+        r.q1 = __shfl_sync(0xffffffffu, q1, src);
+        return r;
+      }
+      tile -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+  r.behind = tile;
+  return r;
+}
+
 // Load the K or V tiles of an item into the ring, chunk by chunk.
 template <int MODE, int DP, bool V>
 __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles, const TcArgs &a,
@@ -329,10 +377,10 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   constexpr int kSlabs = V ? DP / 64 : Cfg::kKSlabs;      // its slabs of 64 values
   const int lane = threadIdx.x & 31;
   const int kv_head = w.kv_head, k0 = w.k0, table_row = w.table_row, end = w.end;
-  int key = w.first;
-  // shared: a box lies in one page; lane i looks the tile's i-th up, a tile ahead. Boxes and
+  constexpr bool kPaged = MODE != kTcPrompt;
+  // paged: a box lies in one page; lane i looks the tile's i-th up, a tile ahead. Boxes and
   // pages are powers of two or whole chunks.
-  const int box = MODE == kTcPrompt ? kRows : V ? a.v_box : a.k_box;
+  const int box = !kPaged ? kRows : V ? a.v_box : a.k_box;
   const int most = kRows / box, page_bits = 31 - __clz(a.c.page_tokens);
   auto looks = [&](int at) -> bool { return lane * box < Cfg::kKeys && at + lane * box < end; };
   // As the table has it: a number outside the pool is outside the map, too, and reads as zeros.
@@ -341,11 +389,13 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   auto page_at = [&](int at) -> int {
     return looks(at) ? a.c.table[(int64_t)table_row * a.c.max_pages + ((at + lane * box) >> page_bits)] : -1;
   };
-  int next_pages = MODE == kTcShared && tiles > 0 ? page_at(key) : 0;
-  for (int t = 0; t < tiles; t++, key += Cfg::kKeys) {
-    const int pages = next_pages;
-    if (MODE == kTcShared && !V && looks(key)) largest = max(largest, (uint32_t)pages);
-    if (MODE == kTcShared && t + 1 < tiles) next_pages = page_at(key + Cfg::kKeys);
+  // shared: all of the shared pages are there; else up to the last key
+  const int most_keys = MODE == kTcShared ? a.d.shared : end;
+  int next_pages = kPaged && tiles > 0 ? page_at(key_of<MODE, Cfg::kKeys>(w, 0)) : 0;
+  for (int t = 0; t < tiles; t++) {
+    const int pages = next_pages, key = key_of<MODE, Cfg::kKeys>(w, t);
+    if (kPaged && !V && looks(key)) largest = max(largest, (uint32_t)pages);
+    if (kPaged && t + 1 < tiles) next_pages = page_at(key_of<MODE, Cfg::kKeys>(w, t + 1));
     // No sooner than it is needed: blocks that have not started are for whoever is done first.
     if (!V && t == max(0, tiles - kWantTiles) && lead) mbar_arrive(smem_u32(&sh.want));
     if (!V && lead) sh.loaded = place.round * TcCfg<DP>::kSlots + place.slot;
@@ -356,8 +406,8 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
       const uint32_t dst = ring + place.slot * Cfg::kChunkBytes;
       // shared: the chunk's boxes, each in kSlabs slabs; one lane for each
       const int slab = lane % kSlabs, mine = lane / kSlabs;
-      const int boxes = MODE == kTcPrompt ? 1 : from + kRows <= a.d.shared ? most : max(0, a.d.shared - from) / box;
-      const int page = MODE == kTcShared ? __shfl_sync(0xffffffffu, pages, (V ? c * most : 0) + mine) : 0;
+      const int boxes = !kPaged ? 1 : from + kRows <= most_keys ? most : max(0, most_keys - from + box - 1) / box;
+      const int page = kPaged ? __shfl_sync(0xffffffffu, pages, (V ? c * most : 0) + mine) : 0;
       uint64_t &empty = V ? sh.v_empty[place.slot] : sh.k_empty[place.slot];
       if (place.round > 0 && !wait(sh, a.wait_limit, empty, place.parity() ^ 1)) return false;
       if (lead) mbar_expect_tx(bar, kSlabs * boxes * box * 128);
@@ -371,7 +421,7 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
       __syncwarp();
     }
   }
-  if (MODE == kTcShared && !V && largest >= (uint32_t)a.c.pages) atomicOr(a.c.status, DM_KV_BAD_TOKEN);
+  if (kPaged && !V && largest >= (uint32_t)a.c.pages) atomicOr(a.c.status, DM_KV_BAD_TOKEN);
   return true;
 }
 
@@ -387,7 +437,8 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
   const uint32_t k_ring = base + kUnits * Cfg::kQBytes, v_ring = k_ring + kSlots * Cfg::kChunkBytes;
-  const int group = MODE == kTcPrompt ? a.p.group : a.d.group;
+  constexpr bool kPacked = MODE != kTcShared;  // query rows by offsets
+  const int group = kPacked ? a.p.group : a.d.group;
   const int per_unit = a.tokens * group;  // rows in use of a unit's 128
   const int alternate = MODE == kTcShared && a.alternate;
   const int split = MODE == kTcShared ? blockIdx.y : 0;
@@ -443,16 +494,20 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       int64_t all = INT64_MAX;  // tiles of the batch, once a block has been behind them
       while (ok) {
       Item w{};
-      if (MODE == kTcPrompt) {
+      if (kPacked) {
         if (block < 0) {
           w.stop = 1;
         } else {
-          // key/value heads side by side, the last (longest, if causal) tiles of the batch first
+          // key/value heads side by side, the last (longest, if causal) tiles of the batch first,
+          // chunks the longest sequences
           w.kv_head = block % a.p.kv_heads;
-          const int tile = a.tiles - 1 - block / a.p.kv_heads;
+          const int splits = MODE == kTcChunks ? a.d.splits : 1, rest = block / a.p.kv_heads;
+          w.split = rest % splits;
+          const int tile = MODE == kTcChunks ? rest / splits : a.tiles - 1 - rest;
           TileOf t{-1};
           if (tile < all) {
-            t = find_tile(a.p, 1, kUnits * a.tokens, tile);
+            t = MODE == kTcChunks ? find_chunk(a.p, a.d, a.c, kUnits * a.tokens, tile)
+                                  : find_tile(a.p, 1, kUnits * a.tokens, tile);
             if (t.seq < 0) all = tile - t.behind;
           }
           if (t.seq < 0) {
@@ -460,16 +515,33 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           } else {
             w.q0 = t.q0;
             w.k0 = t.k0;
-            const int lq = w.lq = t.q1 - t.q0, lk = w.lk = t.k1 - t.k0;
+            if (MODE == kTcChunks) w.table_row = sequence_of(a.c, a.d, t.seq, &w.lk);
+            else w.lk = t.k1 - t.k0;
+            const int lq = w.lq = t.q1 - t.q0, lk = w.lk;
             w.token0 = t.tile * kUnits * a.tokens;
             const int last = min(lq, w.token0 + kUnits * a.tokens) - 1;
             // limits of the first and last token bound the others'
             w.max_low = low_of(a.p, lq, lk, last);
             w.min_high = high_of(a.p, lq, lk, w.token0);
-            w.first = low_of(a.p, lq, lk, w.token0) / 16 * 16;
-            auto tiles_to = [&](int end) { return max(0, (end - w.first + kKeys - 1) / kKeys); };
-            w.tiles = tiles_to(high_of(a.p, lq, lk, last));
-            w.n[0] = tiles_to(high_of(a.p, lq, lk, min(last, w.token0 + a.tokens - 1)));
+            const int low = low_of(a.p, lq, lk, w.token0), end = high_of(a.p, lq, lk, last);
+            const int end0 = high_of(a.p, lq, lk, min(last, w.token0 + a.tokens - 1));  // of the first unit
+            if (MODE == kTcChunks) {
+              const Range r = range_of(a.p, low, end, kKeys);
+              const int all = (r.keys + kKeys - 1) / kKeys, per = (all + splits - 1) / splits;
+              const int t0 = min(all, w.split * per);
+              w.end = end;
+              w.sinks = r.sinks;
+              w.gap = r.low - r.sinks;
+              w.first = t0 * kKeys;
+              w.tiles = min(all, t0 + per) - t0;
+              const int upto = min(end0, r.sinks) + max(0, end0 - r.low);  // numbers below end0
+              w.n[0] = min(w.tiles, max(0, (upto + kKeys - 1) / kKeys - t0));
+            } else {
+              w.first = low / 16 * 16;
+              auto tiles_to = [&](int end) { return max(0, (end - w.first + kKeys - 1) / kKeys); };
+              w.tiles = tiles_to(end);
+              w.n[0] = tiles_to(end0);
+            }
             w.n[1] = kUnits == 2 && w.token0 + a.tokens < lq ? w.tiles : 0;
           }
         }
@@ -514,7 +586,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         items++;
         if (w.stop) break;
       }
-      if (MODE == kTcPrompt) {
+      if (kPacked) {
         if (w.stop == 0 && !(ok = wait_item(sh, a.wait_limit, sh.want, (items - 1) & 1))) break;
         if (lane == 0) {
           fence_async_smem();  // the last answer has been read
@@ -566,10 +638,10 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         } else if (warp == Cfg::kScrubWarp || warp >= Cfg::kOWarp + kUnits) {
           // ---- values that are not finite leave mixed tiles; the others are passed on
           // rows behind the last key are no one's: other sequences, or what the ring held before
-          const int keys = MODE == kTcPrompt ? w.lk : a.d.shared;
+          const int keys = MODE == kTcPrompt ? w.lk : MODE == kTcShared ? a.d.shared : w.end;
           bool found = false;
           for (int t = 0; t < tiles && ok; t++) {
-            const bool mix = mixed<kKeys>(w, t);
+            const bool mix = mixed<MODE, kKeys>(w, t);
             for (int c = 0; c < kChunks; c++, place.next()) {
               if (!(ok = wait(sh, a.wait_limit, sh.v_full[place.slot], place.parity()))) break;
               if (mix) {
@@ -592,7 +664,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
                     uint32_t y[4] = {x.x, x.y, x.z, x.w};
                     for (int k = 0; k < 4; k++) y[k] = zero_not_finite<BF16>(y[k], bad);
                     if (!bad) continue;
-                    found |= w.first + t * kKeys + c * Cfg::kVKeys + j / 8 % Cfg::kVKeys < keys;
+                    found |= key_of<MODE, kKeys>(w, t) + c * Cfg::kVKeys + j / 8 % Cfg::kVKeys < keys;
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(v + j * 16), "r"(y[0]),
                                  "r"(y[1]), "r"(y[2]), "r"(y[3])
                                  : "memory");
@@ -693,7 +765,8 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     const int unit = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
     const uint32_t o_at = tmem + lanes + Cfg::kOCol + unit * DP;
-    const float c = MODE == kTcPrompt ? a.p.scale : a.d.scale;
+    const float c = kPacked ? a.p.scale : a.d.scale;
+    const int sinks = MODE == kTcChunks && a.p.window ? a.p.sinks : 0;
     const uint64_t cc = pair(c, c);
     constexpr float kRoom = kTileHeadroom<BF16>;
     const int dim = MODE == kTcPrompt ? a.p.dim : a.c.head_dim;
@@ -708,10 +781,10 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       int64_t out_at = 0, index = 0;
       const int token = w.token0 + (alternate ? 0 : unit * a.tokens) + row / group;
       const int head = w.kv_head * group + row % group;
-      const bool valid = row < per_unit && token < (MODE == kTcPrompt ? w.lq : a.d.batch);
+      const bool valid = row < per_unit && token < (kPacked ? w.lq : a.d.batch);
       if (valid) {
         const int64_t r = w.q0 + (int64_t)token;
-        if (MODE == kTcPrompt) {
+        if (kPacked) {
           low = low_of(a.p, w.lq, w.lk, token), high = high_of(a.p, w.lq, w.lk, token);
           out_at = r * a.p.out_stride[0] + head * a.p.out_stride[1];
           index = r * a.p.heads + head;
@@ -729,7 +802,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (!(ok = wait(sh, a.wait_limit, sh.s_full[unit], number & 1))) break;
         fence_after();
         const uint32_t s_at = tmem + lanes + unit * Cfg::kUnitCols;
-        const int key = w.first + tile_of(unit, i) * kKeys;
+        const int key = key_of<MODE, kKeys>(w, tile_of(unit, i));
         float x[kKeys];
 #pragma unroll
         for (int j = 0; j + 32 <= kKeys; j += 32) tmem_ld32(s_at + j, x + j);
@@ -740,7 +813,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         const int from = low - key, to = high - key;  // columns [from, to) are visible
         if (__any_sync(0xffffffffu, from > 0 || to < kKeys)) {
 #pragma unroll
-          for (int j = 0; j < kKeys; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
+          for (int j = 0; j < kKeys; j++) x[j] = (j >= from || j < sinks - key) && j < to ? x[j] : -INFINITY;
         }
         float top[4] = {m, m, m, m};
 #pragma unroll
@@ -804,11 +877,10 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       fence_after();
       const bool wild = n > 0 && *(volatile int *)&sh.item[at].wild;
       const bool final = MODE == kTcPrompt || a.d.part.parts == 1;
+      const int part = MODE == kTcChunks ? w.split : a.d.first_part + (alternate ? 2 * split + unit : split);
       const float inv = !final ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t part_at =
-          MODE == kTcShared
-              ? (int64_t)(a.d.first_part + (alternate ? 2 * split + unit : split)) * a.d.part.rows + index
-              : 0;
+          MODE == kTcPrompt ? 0 : (int64_t)part * a.d.part.rows + index;
 #pragma unroll 1
       for (int j = 0; j < DP; j += 32) {
         float o[32];
@@ -822,9 +894,10 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         }
         if (wild && valid) {  // rare: what was left out of the products
           for (int i = 0; i < n; i++) {
-            const int t = tile_of(unit, i), key = w.first + t * kKeys;
-            if (!mixed<kKeys>(w, t)) continue;
-            for (int r = max(key, low); r < min(key + kKeys, high); r++) {
+            const int t = tile_of(unit, i), key = key_of<MODE, kKeys>(w, t);
+            if (!mixed<MODE, kKeys>(w, t)) continue;
+            for (int r = key < sinks ? key : max(key, low); r < min(key + kKeys, high); r++) {
+              if (r < low && r >= sinks) continue;
               const uint16_t *v;
               if (MODE == kTcPrompt) {
                 v = a.p.v + (w.k0 + (int64_t)r) * a.p.v_stride[0] + w.kv_head * a.p.v_stride[1];
@@ -851,7 +924,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           }
         }
         if (valid && final) {
-          uint16_t *out = (MODE == kTcPrompt ? a.p.out : a.d.out) + out_at + j;
+          uint16_t *out = (kPacked ? a.p.out : a.d.out) + out_at + j;
           uint32_t h[16];
 #pragma unroll
           for (int k = 0; k < 16; k++) h[k] = pack2<BF16>(o[2 * k] * inv, o[2 * k + 1] * inv);
@@ -869,7 +942,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         }
       }
       if (valid && final) {
-        float *lse = MODE == kTcPrompt ? a.p.lse : a.d.lse;
+        float *lse = kPacked ? a.p.lse : a.d.lse;
         if (lse) lse[index] = l == 0.0f ? -INFINITY : (m * c - kRoom + log2_fast(l)) * kLn2;
       } else if (valid) {
         a.d.part.ml[part_at] = make_float2(m * c - kRoom, l);
@@ -962,6 +1035,13 @@ int units_of(int dim) { return dim > 128 ? 1 : 2; }
 int keys_of(int dim) { return dim > 64 && dim <= 128 ? TcCfg<128>::kKeys : TcCfg<64>::kKeys; }
 int v_keys_of(int dim) { return dim > 128 ? TcCfg<256>::kVKeys : keys_of(dim); }
 
+// a box lies in one page and divides a chunk: pages are powers of two from 16
+void boxes(const KvView &c, TcArgs *a) {
+  auto rows = [&](int keys) { return std::min(c.page_tokens, keys & -keys); };
+  a->k_box = rows(keys_of(c.head_dim));
+  a->v_box = rows(v_keys_of(c.head_dim));
+}
+
 bool aligned32(const uint16_t *p, const int64_t *stride) {
   return ((uintptr_t)p & 31) == 0 && stride[0] % 16 == 0 && stride[1] % 16 == 0;
 }
@@ -998,6 +1078,35 @@ int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, dm_cuda_context *c
   return launch<kTcPrompt>(bf16, p.dim, dim3((unsigned)(tiles * p.kv_heads)), maps, a, stream);
 }
 
+bool tile_chunks_fit(const PromptArgs &p) {  // as above: the cache has no strides of its own
+  return p.q_stride[0] > 0 && p.q_stride[1] > 0 && p.q_stride[0] < (int64_t)1 << 37 &&
+         p.q_stride[1] * p.group < (int64_t)1 << 37;
+}
+
+int tile_chunk_tokens(int dim, int group) { return units_of(dim) * (kUnitRows / group); }
+
+int32_t launch_tile_chunks(int32_t type, const PromptArgs &p, const DecodeArgs &d, const KvView &c,
+                           cudaStream_t stream) {
+  TcArgs a{};
+  a.p = p;
+  a.d = d;
+  a.c = c;
+  a.tokens = kUnitRows / p.group;
+  a.timeout = d.timeout;
+  a.wait_limit = d.wait_limit;
+  const int64_t tiles = p.q_tokens / tile_chunk_tokens(p.dim, p.group) + p.sequences;
+  if (tiles * p.kv_heads * d.splits > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
+  a.tiles = (int)tiles;
+  a.wide = d.part.parts > 1 ? ((uintptr_t)d.part.o & 31) == 0 : aligned32(p.out, p.out_stride);
+  const bool bf16 = type == DM_BF16;
+  CUtensorMap maps[3];
+  boxes(c, &a);
+  if (!encode_q(&maps[0], bf16, p.q, p.q_stride, p.dim, p.group, p.kv_heads, p.q_tokens, a.tokens) ||
+      !encode_cache(&maps[1], bf16, c, d.layer, 0, a.k_box) || !encode_cache(&maps[2], bf16, c, d.layer, 1, a.v_box))
+    return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
+  return launch<kTcChunks>(bf16, p.dim, dim3((unsigned)(tiles * p.kv_heads * d.splits)), maps, a, stream);
+}
+
 bool tile_shared_alternates(int dim, int group, int batch) {
   return units_of(dim) == 2 && batch <= kUnitRows / group;
 }
@@ -1026,10 +1135,7 @@ int32_t launch_tile_shared(int32_t type, const DecodeArgs &d, const KvView &c, c
   a.wide = d.part.parts > 1 ? ((uintptr_t)d.part.o & 31) == 0 : aligned32(d.out, d.out_stride);
   const bool bf16 = type == DM_BF16;
   CUtensorMap maps[3];
-  // a box lies in one page and divides a chunk: pages are powers of two from 16
-  auto rows = [&](int keys) { return std::min(c.page_tokens, keys & -keys); };
-  a.k_box = rows(keys_of(c.head_dim));
-  a.v_box = rows(v_keys_of(c.head_dim));
+  boxes(c, &a);
   if (!encode_q(&maps[0], bf16, d.q, d.q_stride, c.head_dim, d.group, c.kv_heads, d.batch, a.tokens) ||
       !encode_cache(&maps[1], bf16, c, d.layer, 0, a.k_box) || !encode_cache(&maps[2], bf16, c, d.layer, 1, a.v_box))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");

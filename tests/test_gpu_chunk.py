@@ -300,11 +300,12 @@ def test_two_streams(ctx):
 
 
 def test_empty_calls_and_refusals(ctx):
-    pool = Paged(ctx, torch.bfloat16, 2, 64, 16, [500])
+    # a bound on the lengths that no block walks alone, so that there is a workspace
+    pool = Paged(ctx, torch.bfloat16, 2, 64, 16, [500], max_pages=4000)
     q = normal(generator(2), (4, 4, 64), torch.bfloat16)
     o = ints([0, 4])
-    good = dict(layer=0, heads=4, q=q.data_ptr(), out=q.data_ptr(), offsets=o.data_ptr(), n=1, tokens=4, max_length=500)
-    size = pool.cache.chunk_workspace(4, 1, 4, 500)
+    good = dict(layer=0, heads=4, q=q.data_ptr(), out=q.data_ptr(), offsets=o.data_ptr(), n=1, tokens=4, max_length=60000)
+    size = pool.cache.chunk_workspace(4, 1, 4, 60000)
     work = torch.empty(max(16, size), dtype=torch.uint8, device="cuda")
     good.update(workspace=work.data_ptr(), workspace_bytes=size)
     pool.cache.chunk_attention(**dict(good, n=0))
