@@ -984,7 +984,7 @@ int32_t dm_attention_chunk(dm_kv_cache *cache, const dm_attention_chunk_desc *in
   cudaSetDevice(cache->ctx->device);
   cudaStream_t s = (cudaStream_t)stream;
   CUtensorMap maps[2];
-  const bool on_tiles = plan.tiles && tile_chunks_fit(p);
+  const bool on_tiles = plan.tiles && tile_queries_fit(p.q_stride, p.group);
   if (!on_tiles && !describe_chunks(kd.type, cache->view, in->layer, kChunk, maps))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
   const int64_t tiles = in->tokens * p.group / kRows + in->sequences;

@@ -197,57 +197,9 @@ struct TcArgs {
   int64_t wait_limit;
 };
 
-// One lane of a converged warp. What it decides is uniform, so the operands of the
-// instructions under it can stay in uniform registers.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t yes;
-  asm volatile(
-      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(yes));
-  return yes != 0;
-}
-
-// The products with the issuing lane as a predicate: no branch around them, so the addresses
-// are computed for the whole warp, in uniform registers, where the instruction wants them.
-__device__ __forceinline__ void mma_ss_if(uint32_t lead, uint32_t d, uint64_t adesc, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts_if(uint32_t lead, uint32_t d, uint32_t a, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
-      : "memory");
-}
-__device__ __forceinline__ void commit_if(uint32_t lead, uint32_t bar) {
-  asm volatile(
-      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
-      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
-      "r"(lead)
-      : "memory");
-}
-// A value that is the same in all lanes, in a uniform register.
-__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
-
 // Bounded wait that also ends when another role has given up; one answer for the warp. A
 // warp that waits sleeps in try_wait: one that polls takes issue slots from the softmax warps
 // beside it (measured: a third of the prompt rate).
-__device__ __forceinline__ bool mbar_look(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
 __device__ __forceinline__ bool wait(TcSmem &sh, int64_t limit, uint64_t &bar, uint32_t parity) {
   constexpr unsigned kAll = 0xffffffffu;
   const uint32_t b = smem_u32(&bar);
@@ -1078,9 +1030,8 @@ int32_t launch_tile_prompt(int32_t type, const PromptArgs &p, dm_cuda_context *c
   return launch<kTcPrompt>(bf16, p.dim, dim3((unsigned)(tiles * p.kv_heads)), maps, a, stream);
 }
 
-bool tile_chunks_fit(const PromptArgs &p) {  // as above: the cache has no strides of its own
-  return p.q_stride[0] > 0 && p.q_stride[1] > 0 && p.q_stride[0] < (int64_t)1 << 37 &&
-         p.q_stride[1] * p.group < (int64_t)1 << 37;
+bool tile_queries_fit(const int64_t *q_stride, int group) {  // as above: the cache has no strides of its own
+  return q_stride[0] > 0 && q_stride[1] > 0 && q_stride[0] < (int64_t)1 << 37 && q_stride[1] * group < (int64_t)1 << 37;
 }
 
 int tile_chunk_tokens(int dim, int group) { return units_of(dim) * (kUnitRows / group); }
@@ -1114,6 +1065,15 @@ bool tile_shared_alternates(int dim, int group, int batch) {
 bool describe_chunks(int32_t type, const KvView &c, int layer, int rows, CUtensorMap *maps) {
   return encode_cache(&maps[0], type == DM_BF16, c, layer, 0, rows) &&
          encode_cache(&maps[1], type == DM_BF16, c, layer, 1, rows);
+}
+
+bool describe_queries(int32_t type, const void *q, const int64_t *stride, int dim, int group, int kv_heads,
+                      int64_t tokens, int box_tokens, CUtensorMap *map) {
+  return encode_q(map, type == DM_BF16, q, stride, dim, group, kv_heads, tokens, box_tokens);
+}
+
+bool describe_keys(int32_t type, const KvView &c, int layer, int rows, CUtensorMap *map) {
+  return encode_cache(map, type == DM_BF16, c, layer, 0, rows);
 }
 
 int tile_keys(int dim) { return keys_of(dim); }
