@@ -7,9 +7,9 @@
 // per position as fractions of 2^64, the product with the position wraps around exactly where
 // whole turns do, and its upper 32 bits are the angle.
 //
-// A group of 8, 16 or 32 lanes holds one head, 16 bytes a lane: the sum of squares is a few
-// shuffles, and a pair's other half is another lane's vector. A block computes the sines of its
-// tokens once, for all their heads.
+// A warp takes a token. 8, 16 or 32 lanes hold a head, 16 bytes a lane: the sum of squares is a
+// few shuffles, and a pair's other half is another lane's vector. Sines and weights are multiplied
+// once for all heads of a token.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -18,6 +18,7 @@
 #include <new>
 
 #include "dm_attention.cuh"
+#include "dm_tcgen05.cuh"
 
 using dmi::fail;
 
@@ -32,10 +33,10 @@ struct dm_rope {
 namespace dma {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kBlockTokens = 8;  // of a block at most: a warp looks after each
-constexpr int kPairs = 128;
-constexpr int kFlight = 4;      // loads of a thread in flight
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kBlocks = 4;   // of an SM
+constexpr int kPairs = 128;  // at most
+constexpr int kFlight = 4;   // 16-byte loads of a thread in flight
 
 enum Kind { kQ, kK, kV };
 
@@ -49,7 +50,7 @@ struct RotateArgs {
   const int32_t *pair_axes;
   int64_t tokens;
   int32_t first[3], heads;  // first row of each kind among a token's; rows of a token
-  int32_t dim, rotary, interleaved, norms, sequences, layer, cached, block_tokens;
+  int32_t dim, rotary, interleaved, norms, sequences, layer, cached;
   float scale, epsilon;
 };
 
@@ -71,144 +72,199 @@ __device__ __forceinline__ int entry_of(const int32_t *offsets, int n, int64_t t
   return n > 0 && t < offsets[low + 1] ? low : -1;
 }
 
+// Two 16-bit values as f32
+template <bool BF16>
+__device__ __forceinline__ uint64_t both(uint32_t x) {
+  if (BF16) return dm::tc::pair(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+  return dm::tc::pair(f.x, f.y);
+}
+
+__device__ __forceinline__ float rsqrt_fast(float x) {  // within two units of the last place
+  float y;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Values of a head that one lane has, as pairs of f32
+struct Eight {
+  uint64_t v[4];
+};
+template <bool BF16>
+__device__ __forceinline__ Eight unpack(const uint32_t *r) {
+  return Eight{{both<BF16>(r[0]), both<BF16>(r[1]), both<BF16>(r[2]), both<BF16>(r[3])}};
+}
+
+// Warp (x, warp) does part y of a token's heads.
 template <int LANES, bool BF16>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(const __grid_constant__ KvView c,
-                                                          const __grid_constant__ RotateArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_constant__ KvView c,
+                                                                   const __grid_constant__ RotateArgs a) {
+  using namespace dm::tc;
   constexpr unsigned kAll = 0xffffffffu;
-  constexpr int kGroups = kThreads / LANES;
-  __shared__ float cosine[kBlockTokens][kPairs], sine[kBlockTokens][kPairs];
-  __shared__ float weight[2][LANES * 8];
-  __shared__ int64_t place_at[kBlockTokens];  // byte offset of the token's place in part 0 of its page; -1: none
-  __shared__ int owned[kBlockTokens];
+  constexpr int kSide = 32 / LANES;  // heads side by side
+  __shared__ alignas(16) float cosine[kWarps][LANES * 8], sine[kWarps][LANES * 8];  // of each value of the token's heads
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int vec = lane % LANES, side = lane / LANES, col = vec * 8;
+  const int64_t t = (int64_t)blockIdx.x * kWarps + warp;
+  if (t >= a.tokens) return;
+  const bool in = col < a.dim;
+  const int begin = (int)((int64_t)a.heads * blockIdx.y / gridDim.y);
+  const int end = (int)((int64_t)a.heads * (blockIdx.y + 1) / gridDim.y);
   wait_for_previous();
   let_next_start();
 
-  for (int i = tid; i < 2 * LANES * 8; i += kThreads) {
-    const int which = i / (LANES * 8), col = i % (LANES * 8);
-    weight[which][col] = a.weight[which] && col < a.dim ? a.weight[which][col] : 1.0f;
-  }
-  const int64_t token0 = (int64_t)blockIdx.x * a.block_tokens;
-  const int tokens = (int)min((int64_t)a.block_tokens, a.tokens - token0);
-  if (warp < tokens) {
-    const int64_t t = token0 + warp;
-    int64_t place = 0;
-    bool mine = true;
-    if (a.cached) {
-      const int i = entry_of(a.offsets, a.sequences, t);
-      mine = i >= 0;
-      if (mine) {
-        const int row = a.rows ? a.rows[i] : i;
-        int page = -1;
-        if (row >= 0 && row < c.max_sequences) {
-          const int length = c.lengths[row];
-          place = length - ((int64_t)a.offsets[i + 1] - t);
-          if (place >= 0 && place < length && place / c.page_tokens < c.max_pages)
-            page = c.table[(int64_t)row * c.max_pages + place / c.page_tokens];
-        }
-        const bool fits = (unsigned)page < (unsigned)c.pages;
-        if (lane == 0) {
-          place_at[warp] = fits ? page * c.page_bytes + a.layer * c.layer_bytes +
-                                      (place % c.page_tokens) * c.head_dim * 2 : -1;
-          if (!fits && blockIdx.y == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
-        }
-        if (!fits) place = 0;
-      }
+  // Heads of a kind go kSide at a time, kFlight times as many to a batch; the next batch is on its
+  // way while one is done.
+  auto low_of = [&](int kind) { return max(begin, a.first[kind]); };
+  auto high_of = [&](int kind) { return min(end, kind == kQ ? a.first[kK] : kind == kK ? a.first[kV] : a.heads); };
+  int ahead = -1, left = -side;  // of the loads: kind, and heads from this lane's on
+  const uint8_t *from = nullptr;
+  int64_t from_step = 0;
+  uint4 x[kFlight] = {};
+  auto load = [&]() {
+    while (left <= -side && ahead < kV) {
+      ahead++;
+      const int low = low_of(ahead);
+      left = max(high_of(ahead) - low, 0) - side;
+      from = a.in[ahead] + t * a.in_stride[ahead][0] + (low + side - a.first[ahead]) * a.in_stride[ahead][1] + col * 2;
+      from_step = kSide * a.in_stride[ahead][1];
     }
-    if (lane == 0) owned[warp] = mine;
-    if (mine)
-      for (int i = lane; i < a.rotary / 2; i += 32) {
-        const int64_t p = a.positions ? a.positions[a.pair_axes[i] * a.tokens + t] : place;
-        const uint64_t turns = (uint64_t)p * a.turns[i];
-        // half turns, -1 to 1; their f32 is off by at most 2^-25
-        const float half = (float)(int32_t)(turns >> 32) * 0x1p-31f;
-        float s, k;
-        sincospif(half, &s, &k);
-        cosine[warp][i] = k * a.scale;
-        sine[warp][i] = s * a.scale;
-      }
-  }
-  __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kFlight; k++, from += from_step)
+      if (in && left > k * kSide) x[k] = *reinterpret_cast<const uint4 *>(from);
+    left -= kFlight * kSide;
+  };
+  load();
 
-  const int group = tid / LANES, vec = tid % LANES, col = vec * 8;
-  const int half = a.rotary / 2;
-  const float share = 1.0f / a.dim;
-  // where the other halves of this lane's pairs are
-  const bool turns = col < a.rotary, upper = !a.interleaved && col >= half;
-  const int other = turns && !a.interleaved ? (upper ? vec - half / 8 : vec + half / 8) : vec;
-  const int pair0 = a.interleaved ? col / 2 : upper ? col - half : col;
-  const int all = tokens * a.heads, stride = kGroups * gridDim.y;
-  int at = blockIdx.y * kGroups + group;
-  int token = at / a.heads, head = at % a.heads;
-  // rounds are the same for all lanes of a warp
-  for (int from = blockIdx.y * kGroups; from < all; from += kFlight * stride) {
-    uint4 x[kFlight];
-    int token_of[kFlight], head_of[kFlight];
-    bool valid[kFlight];
-#pragma unroll
-    for (int k = 0; k < kFlight; k++) {
-      token_of[k] = token, head_of[k] = head;
-      valid[k] = at < all && col < a.dim && owned[min(token, kBlockTokens - 1)];
-      x[k] = make_uint4(0, 0, 0, 0);
-      if (valid[k]) {
-        const int kind = head >= a.first[kV] ? kV : head >= a.first[kK] ? kK : kQ;
-        x[k] = *reinterpret_cast<const uint4 *>(a.in[kind] + (token0 + token) * a.in_stride[kind][0] +
-                                                (head - a.first[kind]) * a.in_stride[kind][1] + col * 2);
-      }
-      at += stride, head += stride;
-      while (head >= a.heads) head -= a.heads, token++;
+  // ---- the token's place and its sines, while the first heads come in
+  int64_t place = 0, cached_at = -1;
+  const int page_bits = 31 - __clz(c.page_tokens);  // pages are powers of two
+  if (a.cached) {
+    const int i = entry_of(a.offsets, a.sequences, t);
+    if (i < 0) return;
+    const int row = a.rows ? a.rows[i] : i;
+    int page = -1;
+    if (row >= 0 && row < c.max_sequences) {
+      const int length = c.lengths[row];
+      place = length - ((int64_t)a.offsets[i + 1] - t);
+      if (place >= 0 && place < length && (place >> page_bits) < c.max_pages)
+        page = c.table[(int64_t)row * c.max_pages + (place >> page_bits)];
     }
+    if ((unsigned)page < (unsigned)c.pages) {
+      cached_at = page * c.page_bytes + a.layer * c.layer_bytes + (place & (c.page_tokens - 1)) * c.head_dim * 2 + col * 2;
+    } else {
+      place = 0;
+      if (lane == 0 && blockIdx.y == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
+    }
+  }
+  const int half = a.rotary / 2;
+  for (int i = lane; i < half; i += 32) {
+    const int64_t p = a.positions ? a.positions[a.pair_axes[i] * a.tokens + t] : place;
+    const uint64_t turns = (uint64_t)p * a.turns[i];
+    float s, k;
+    // half turns, -1 to 1; their f32 is off by at most 2^-25
+    sincospif((float)(int32_t)(turns >> 32) * 0x1p-31f, &s, &k);
+    const int first = a.interleaved ? 2 * i : i, second = a.interleaved ? first + 1 : i + half;
+    cosine[warp][first] = cosine[warp][second] = k * a.scale;
+    sine[warp][first] = -s * a.scale;
+    sine[warp][second] = s * a.scale;
+  }
+  for (int i = a.rotary + lane; i < a.dim; i += 32) cosine[warp][i] = 1.0f, sine[warp][i] = 0.0f;
+  __syncwarp();
+
+  // where the other halves of this lane's pairs are; pairs side by side are exchanged in place
+  const int other = a.interleaved || col >= a.rotary ? vec : col >= half ? vec - half / 8 : vec + half / 8;
+  const float share = 1.0f / a.dim;
+  Eight own{}, across{};  // a value is own times it plus across times the other of its pair, over the root
+#pragma unroll 1
+  for (int kind = kQ; kind <= kV; kind++) {
+    const int n = high_of(kind) - low_of(kind), head = low_of(kind) + side - a.first[kind];
+    if (n <= 0) continue;
+    const bool normed = (a.norms >> kind) & 1, rotated = kind != kV && a.rotary > 0;
+    if (kind != kV && in)
 #pragma unroll
-    for (int k = 0; k < kFlight; k++) {
-      if (from + k * stride >= all) break;
-      const int kind = head_of[k] >= a.first[kV] ? kV : head_of[k] >= a.first[kK] ? kK : kQ;
-      const int slot = min(token_of[k], kBlockTokens - 1);
-      const bool normed = (a.norms >> kind) & 1, rotated = kind != kV && a.rotary > 0;
-      const uint32_t raw[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-      uint32_t across[4];
-      float v[8], sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        v[e] = to_float<BF16>((uint16_t)(raw[e / 2] >> (16 * (e & 1))));
-        sum += v[e] * v[e];
-      }
-#pragma unroll
-      for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(kAll, sum, o);
-#pragma unroll
-      for (int e = 0; e < 4; e++) across[e] = __shfl_sync(kAll, raw[e], other, LANES);
-      if (!valid[k]) continue;
-      uint4 y = x[k];
-      if (normed || rotated) {
-        const float r = normed ? rsqrtf(sum * share + a.epsilon) : 1.0f;
-        const float *w = normed && kind != kV ? weight[kind] : nullptr;
-        float out[8];
-        if (rotated && turns) {
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const int from_col = a.interleaved ? col + (e ^ 1) : other * 8 + e;
-            const int pair = a.interleaved ? pair0 + e / 2 : pair0 + e;
-            const float mine = w ? v[e] * w[col + e] : v[e];
-            const uint16_t h = a.interleaved ? (uint16_t)(raw[e / 2] >> (16 * ((e ^ 1) & 1)))
-                                             : (uint16_t)(across[e / 2] >> (16 * (e & 1)));
-            const float theirs = w ? to_float<BF16>(h) * w[from_col] : to_float<BF16>(h);
-            const bool second = a.interleaved ? e & 1 : upper;
-            const float s = sine[slot][pair];
-            out[e] = (mine * cosine[slot][pair] + theirs * (second ? s : -s)) * r;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e++) out[e] = (w ? v[e] * w[col + e] : v[e]) * r;
+      for (int e = 0; e < 4; e++) {
+        float2 k = *reinterpret_cast<const float2 *>(&cosine[warp][col + 2 * e]);
+        float2 s = *reinterpret_cast<const float2 *>(&sine[warp][col + 2 * e]);
+        if (normed && a.weight[kind]) {
+          const float *w = a.weight[kind] + 2 * e, *here = w + col, *there = w + other * 8;
+          const bool swap = a.interleaved && col < a.rotary;
+          k.x *= here[0], k.y *= here[1];
+          s.x *= there[swap], s.y *= there[!swap];
         }
-        y = make_uint4(pack2<BF16>(out[0], out[1]), pack2<BF16>(out[2], out[3]), pack2<BF16>(out[4], out[5]),
-                       pack2<BF16>(out[6], out[7]));
+        own.v[e] = pair(k.x, k.y), across.v[e] = pair(s.x, s.y);
       }
-      const int own = head_of[k] - a.first[kind];
-      if (a.out[kind])
-        *reinterpret_cast<uint4 *>(a.out[kind] + (token0 + token_of[k]) * a.out_stride[kind][0] +
-                                   own * a.out_stride[kind][1] + col * 2) = y;
-      if (a.cached && kind != kQ && place_at[slot] >= 0)
-        *reinterpret_cast<uint4 *>(c.memory + place_at[slot] +
-                                   ((kind == kV ? c.kv_heads : 0) + own) * c.head_bytes + col * 2) = y;
+    const int64_t out_step = kSide * a.out_stride[kind][1], cache_step = kSide * c.head_bytes;
+    const bool out_too = in && a.out[kind], cache_too = in && kind != kQ && cached_at >= 0;
+    uint8_t *out = a.out[kind] + t * a.out_stride[kind][0] + head * a.out_stride[kind][1] + col * 2;
+    uint8_t *cache = c.memory + cached_at + ((kind == kV ? c.kv_heads : 0) + head) * c.head_bytes;
+    const bool turns = rotated && col < a.rotary;
+#pragma unroll 1
+    for (int i = 0; i < n; i += kFlight * kSide) {
+      uint32_t r[kFlight][4];
+#pragma unroll
+      for (int k = 0; k < kFlight; k++) r[k][0] = x[k].x, r[k][1] = x[k].y, r[k][2] = x[k].z, r[k][3] = x[k].w;
+      load();
+      if (normed || rotated) {
+        Eight v[kFlight];
+        float root[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; k++) {
+          v[k] = unpack<BF16>(r[k]);
+          root[k] = 1.0f;
+        }
+        if (normed) {
+#pragma unroll
+          for (int k = 0; k < kFlight; k++) {
+            uint64_t sum = mul2(v[k].v[0], v[k].v[0]);
+#pragma unroll
+            for (int e = 1; e < 4; e++) sum = fma2(v[k].v[e], v[k].v[e], sum);
+            root[k] = in ? __uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)) : 0.0f;
+          }
+#pragma unroll
+          for (int o = 1; o < LANES; o <<= 1)
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) root[k] += __shfl_xor_sync(kAll, root[k], o);
+#pragma unroll
+          for (int k = 0; k < kFlight; k++) root[k] = rsqrt_fast(root[k] * share + a.epsilon);
+        }
+        if (kind != kV) {
+          if (rotated)
+#pragma unroll
+            for (int k = 0; k < kFlight; k++)
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                r[k][e] = a.interleaved ? __funnelshift_l(r[k][e], r[k][e], 16) : __shfl_sync(kAll, r[k][e], other, LANES);
+#pragma unroll
+          for (int k = 0; k < kFlight; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[k].v[e] = mul2(v[k].v[e], own.v[e]);
+          // what does not turn stays apart from the rest of its head: 0 times infinity is no zero
+          if (turns)
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) {
+              const Eight u = unpack<BF16>(r[k]);
+#pragma unroll
+              for (int e = 0; e < 4; e++) v[k].v[e] = fma2(u.v[e], across.v[e], v[k].v[e]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kFlight; k++) {
+          const uint64_t scale = pair(root[k], root[k]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            v[k].v[e] = mul2(v[k].v[e], scale);
+            r[k][e] = pack2<BF16>(__uint_as_float((uint32_t)v[k].v[e]), __uint_as_float((uint32_t)(v[k].v[e] >> 32)));
+          }
+        }
+      }
+      if (out_too)
+#pragma unroll
+        for (int k = 0; k < kFlight; k++, out += out_step)
+          if (i + k * kSide + side < n) *reinterpret_cast<uint4 *>(out) = make_uint4(r[k][0], r[k][1], r[k][2], r[k][3]);
+      if (cache_too)
+#pragma unroll
+        for (int k = 0; k < kFlight; k++, cache += cache_step)
+          if (i + k * kSide + side < n) *reinterpret_cast<uint4 *>(cache) = make_uint4(r[k][0], r[k][1], r[k][2], r[k][3]);
     }
   }
 }
@@ -369,20 +425,12 @@ int32_t dm_attention_rotate(dm_cuda_context *ctx, const dm_rope *rope, dm_kv_cac
     a.scale = rope->scale;
   }
   cudaSetDevice(ctx->device);
-  const int groups = kThreads / (a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32);
-  // Few tokens: their heads over several blocks, so that no thread has two; many: blocks of
-  // several tokens with kFlight loads a thread at least.
-  int64_t blocks = in->tokens;
-  unsigned along = 1;
-  a.block_tokens = 1;
-  if (in->tokens * ((a.heads + groups - 1) / groups) <= 148 * 4) {
-    along = (a.heads + groups - 1) / groups;
-  } else {
-    a.block_tokens = (int)std::min<int64_t>(kBlockTokens, std::max<int64_t>(1, in->tokens / (148 * 8)));
-    blocks = (in->tokens + a.block_tokens - 1) / a.block_tokens;
-  }
+  // A warp to a token; few tokens: their heads over several, down to two rounds each.
+  const int side = a.dim <= 64 ? 4 : a.dim <= 128 ? 2 : 1;
+  const int64_t blocks = (in->tokens + kWarps - 1) / kWarps;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(148 * kBlocks / blocks, (a.heads + 2 * side - 1) / (2 * side)));
   const KvView view = cache ? cache->view : KvView{};
-  const dim3 grid((unsigned)blocks, along);
+  const dim3 grid((unsigned)blocks, (unsigned)parts);
   return in->type == DM_BF16 ? launch_rotate<true>(grid, (cudaStream_t)stream, view, a)
                              : launch_rotate<false>(grid, (cudaStream_t)stream, view, a);
 }

@@ -179,7 +179,7 @@ DM_API int32_t dm_attention_decode(dm_kv_cache *cache, const dm_attention_decode
  * position p = j + length - L and sees the keys k <= p; with window > 0 only k > p - window and
  * k < sinks (without a window sinks has no meaning). A row that sees no key (more rows than
  * tokens, an entry outside the table) gives zeros and -infinity. Rows of q that no entry owns
- * are not read and their output is left as it was, so tokens and sequences may be bounds (a
+ * have no influence and their output is left as it was, so tokens and sequences may be bounds (a
  * captured graph): entries without rows are passed over. Entries may name a row twice.
  * max_length bounds the lengths as in decode, and so do workspace and bad page numbers; at most
  * 128 query heads per key/value head and 2^20 sequences. */
@@ -231,7 +231,7 @@ DM_API void dm_rope_destroy(dm_rope *rope);
  * lengths count them already). NULL inputs are left out (k and v go together where there is a
  * cache), and so are NULL outputs.
  * positions: device int32 [axes][tokens]; NULL (with a cache) = the token's place in its
- * sequence along every axis. With a cache, rows that no entry owns are not read and their
+ * sequence along every axis. With a cache, rows that no entry owns have no influence and their
  * outputs are left as they were; one whose place is not in the table is not cached and sets
  * DM_KV_BAD_TOKEN, and stands at position 0 where positions is NULL. No cache row is named
  * twice. Without a cache the call does all tokens and reads neither rows nor offsets.
