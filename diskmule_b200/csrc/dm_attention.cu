@@ -515,6 +515,53 @@ join_kernel(const __grid_constant__ DecodeArgs d, const int32_t *offsets, int en
   if (tid == 0 && d.lse) d.lse[row] = l == 0.0f ? -INFINITY : (m + log2_fast(l)) * kLn2;
 }
 
+// The same with a warp to a row, for many rows of few parts: bound by memory, where a block to a
+// row is bound by the blocks (48000 rows of dim 128 in 2 parts 54 us longer than this one's 17).
+constexpr int kFewParts = 8, kRowWarps = 8, kFewRows = 1024;
+
+template <bool BF16>
+__global__ void __launch_bounds__(kRowWarps * 32)
+join_few_kernel(const __grid_constant__ DecodeArgs d, const int32_t *offsets, int entries, int dim) {
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, parts = d.part.parts;
+  wait_for_previous();
+  let_next_start();
+  if (row >= d.part.rows || row / d.heads < offsets[0] || row / d.heads >= offsets[entries]) return;
+  const float2 ml = lane < parts ? d.part.ml[lane * d.part.rows + row] : make_float2(-INFINITY, 0.0f);
+  float m = ml.x;
+#pragma unroll
+  for (int x = 1; x < kFewParts; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  m = __shfl_sync(0xffffffffu, m, 0);
+  // a part that has seen nothing was not written
+  const float mine = ml.y == 0.0f ? 0.0f : exp2_fast(ml.x - (m == -INFINITY ? 0.0f : m));
+  float l = ml.y * mine;
+#pragma unroll
+  for (int x = 1; x < kFewParts; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  l = __shfl_sync(0xffffffffu, l, 0);
+  float4 v[2] = {};
+  const float *part = d.part.o + row * dim + lane * 4;
+#pragma unroll
+  for (int i = 0; i < kFewParts; i++) {
+    const float f = __shfl_sync(0xffffffffu, mine, i);
+    if (i >= parts || f == 0.0f) continue;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      if (h * 128 + lane * 4 < dim) {
+        const float4 u = *reinterpret_cast<const float4 *>(part + i * d.part.rows * dim + h * 128);
+        v[h].x += u.x * f, v[h].y += u.y * f, v[h].z += u.z * f, v[h].w += u.w * f;
+      }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t token = row / d.heads, head = row % d.heads;
+  uint16_t *out = d.out + token * d.out_stride[0] + head * d.out_stride[1] + lane * 4;
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+    if (h * 128 + lane * 4 < dim)
+      *reinterpret_cast<uint2 *>(out + h * 128) =
+          make_uint2(pack2<BF16>(v[h].x * inv, v[h].y * inv), pack2<BF16>(v[h].z * inv, v[h].w * inv));
+  if (lane == 0 && d.lse) d.lse[row] = l == 0.0f ? -INFINITY : (m + log2_fast(l)) * kLn2;
+}
+
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
@@ -682,29 +729,33 @@ struct ChunkPlan {
 };
 
 // Microseconds on one B200, as measured, for a tile of one unit's rows and of two (80 keys of dim
-// 128, 128 of the others; pages of 16 tokens at dim 256, where wider ones take half), and for what
-// an item of a block has besides. The rest is as in decode.
-constexpr float kChunkStepUs[3][2] = {{1.2f, 1.5f}, {0.9f, 1.05f}, {2.0f, 2.0f}}, kChunkItemUs = 2.0f;
+// 128, 128 of the others; dim 256 with pages of 64 tokens and of 16), and for what an item of a
+// block has besides. The rest is as in decode.
+constexpr float kChunkStepUs[3][2] = {{1.2f, 1.6f}, {0.9f, 1.05f}, {1.6f, 2.05f}}, kChunkItemUs = 2.0f;
+constexpr float kGain = 0.95f;  // more parts have to be worth their workspace
+constexpr int64_t kMostPartBytes = 128 << 20;
 
 // The host knows bounds only: entries, their rows together, the longest one's keys. Entries are
 // taken to be alike.
-ChunkPlan chunk_plan(int kv_heads, int heads, int dim, int entries, int64_t tokens, int max_length, int window,
+ChunkPlan chunk_plan(const dm_kv_cache_desc &c, int heads, int entries, int64_t tokens, int max_length, int window,
                      int sinks) {
   ChunkPlan best;
   if (tokens == 0 || entries == 0) return best;
-  const int group = heads / kv_heads;
+  const int dim = c.head_dim, group = heads / c.kv_heads;
   const int64_t busy = std::min<int64_t>(entries, tokens), each = (tokens + busy - 1) / busy;
+  const int64_t part_bytes = tokens * heads * dim * 4;
   // what the rows of a block or unit see
   auto keys_of = [&](int64_t rows) {
     return (int)std::max<int64_t>(1, window ? std::min<int64_t>(max_length, (int64_t)window + sinks + rows) : max_length);
   };
-  auto join_us = [&](int parts) { return parts > 1 ? kJoinUs + kJoinMbUs * parts * ((float)tokens * heads * dim * 4e-6f) : 0.0f; };
+  auto join_us = [&](int parts) { return parts > 1 ? kJoinUs + kJoinMbUs * 1e-6f * parts * part_bytes : 0.0f; };
   float best_us = 0.0f;
   auto offer = [&](const ChunkPlan &plan, float us) {
-    if (best_us == 0.0f || us < best_us) best = plan, best_us = us;
+    if (plan.splits > 1 && plan.splits * part_bytes > kMostPartBytes) return;
+    if (best_us == 0.0f || us < best_us * (plan.splits > best.splits ? kGain : 1.0f)) best = plan, best_us = us;
   };
   {
-    const int64_t blocks = busy * ((each * group + kRows - 1) / kRows) * kv_heads;
+    const int64_t blocks = busy * ((each * group + kRows - 1) / kRows) * c.kv_heads;
     const int keys = keys_of(kRows / group);
     ChunkPlan plan;
     plan.wide = dim <= 128 && blocks <= kSms;
@@ -713,18 +764,18 @@ ChunkPlan chunk_plan(int kv_heads, int heads, int dim, int entries, int64_t toke
     const int most = splits_of(blocks, keys, at_once);
     for (int splits : {1, most}) {
       plan.splits = splits;
-      offer(plan, std::max(1.0f, (float)blocks * splits / at_once) *
-                      (kRowsUs + step * ((keys + 16 * warps * splits - 1) / (16 * warps * splits))) + join_us(splits));
+      const int64_t rounds = (blocks * splits + at_once - 1) / at_once;
+      offer(plan, rounds * (kRowsUs + step * ((keys + 16 * warps * splits - 1) / (16 * warps * splits))) + join_us(splits));
     }
   }
   const int64_t per = tile_chunk_tokens(dim, group);
-  const int64_t items = busy * ((each + per - 1) / per) * kv_heads;
-  const bool two = each > kTileRows / group;
+  const int64_t items = busy * ((each + per - 1) / per) * c.kv_heads;
   const int tiles = (keys_of(std::min(each, per)) + tile_keys(dim) - 1) / tile_keys(dim);
-  const float step = kChunkStepUs[dim <= 64 ? 0 : dim <= 128 ? 1 : 2][two];
+  const bool second = dim > 128 ? c.page_tokens < 64 : each > kTileRows / group;
+  const float step = kChunkStepUs[dim <= 64 ? 0 : dim <= 128 ? 1 : 2][second];
   ChunkPlan plan;
   plan.tiles = true;
-  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(2 * kSms / items, std::min(tiles / 2, kMostParts)));
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(std::max<int64_t>(2 * kSms / items, 4), std::min(tiles / 2, kMostParts)));
   for (plan.splits = 1; plan.splits <= most; plan.splits++) {
     const int64_t rounds = (items * plan.splits + kSms - 1) / kSms;
     offer(plan, kTileUs + rounds * step * ((tiles + plan.splits - 1) / plan.splits) + (rounds - 1) * kChunkItemUs +
@@ -921,7 +972,7 @@ static int32_t check_chunk(const dm_kv_cache *cache, const dm_attention_chunk_de
   const int64_t rows = in->tokens * in->heads;
   const int64_t tiles = in->tokens * (in->heads / d.kv_heads) / kRows + in->sequences;
   if (rows > INT32_MAX || tiles > INT32_MAX / d.kv_heads) return fail(DM_ERR_OVERFLOW, "too many query rows");
-  *plan = chunk_plan(d.kv_heads, in->heads, d.head_dim, in->sequences, in->tokens,
+  *plan = chunk_plan(d, in->heads, in->sequences, in->tokens,
                      bounded_length(d, in->max_length), in->window, in->sinks);
   *bytes = chunk_workspace(*plan, rows, d.head_dim);
   return DM_OK;
@@ -993,6 +1044,10 @@ int32_t dm_attention_chunk(dm_kv_cache *cache, const dm_attention_chunk_desc *in
                    : plan.wide ? launch_rows<kChunks, 8>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s)
                              : launch_rows<kChunks, 4>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s))
     return rc;
+  if (plan.splits > 1 && plan.splits <= kFewParts && a.part.rows > kFewRows)
+    return launch_chained("attention join launch", kd.type == DM_BF16 ? join_few_kernel<true> : join_few_kernel<false>,
+                          dim3((unsigned)((a.part.rows + kRowWarps - 1) / kRowWarps)), kRowWarps * 32, 0, s, a,
+                          in->offsets, in->sequences, kd.head_dim);
   if (plan.splits > 1)
     return launch_chained("attention join launch", kd.type == DM_BF16 ? join_kernel<true> : join_kernel<false>,
                           dim3((unsigned)a.part.rows), kJoinThreads, 0, s, a, in->offsets, in->sequences, kd.head_dim);

@@ -333,7 +333,7 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   // paged: a box lies in one page; lane i looks the tile's i-th up, a tile ahead. Boxes and
   // pages are powers of two or whole chunks.
   const int box = !kPaged ? kRows : V ? a.v_box : a.k_box;
-  const int most = kRows / box, page_bits = 31 - __clz(a.c.page_tokens);
+  const int box_bits = 31 - __clz(box), most = kPaged ? kRows >> box_bits : 1, page_bits = 31 - __clz(a.c.page_tokens);
   auto looks = [&](int at) -> bool { return lane * box < Cfg::kKeys && at + lane * box < end; };
   // As the table has it: a number outside the pool is outside the map, too, and reads as zeros.
   // It is looked at a tile later, so that nothing waits for it, and reported at the end.
@@ -343,32 +343,45 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   };
   // shared: all of the shared pages are there; else up to the last key
   const int most_keys = MODE == kTcShared ? a.d.shared : end;
-  int next_pages = kPaged && tiles > 0 ? page_at(key_of<MODE, Cfg::kKeys>(w, 0)) : 0;
+  const int number0 = w.first, sinks = MODE == kTcChunks ? w.sinks : 0, gap = MODE == kTcChunks ? w.gap : 0;
+  auto key_at = [&](int t) -> int {
+    const int number = number0 + t * Cfg::kKeys;
+    return MODE == kTcChunks && number >= sinks ? number + gap : number;
+  };
+  // the chunk's boxes, each in kSlabs slabs; one lane for each
+  const int slab = lane % kSlabs, mine = lane / kSlabs;
+  const uint32_t place_in = slab * kRows * 128 + mine * box * 128;
+  int next_pages = kPaged && tiles > 0 ? page_at(key_at(0)) : 0;
   for (int t = 0; t < tiles; t++) {
-    const int pages = next_pages, key = key_of<MODE, Cfg::kKeys>(w, t);
+    const int pages = next_pages, key = key_at(t);
     if (kPaged && !V && looks(key)) largest = max(largest, (uint32_t)pages);
-    if (kPaged && t + 1 < tiles) next_pages = page_at(key_of<MODE, Cfg::kKeys>(w, t + 1));
+    if (kPaged && t + 1 < tiles) next_pages = page_at(key_at(t + 1));
     // No sooner than it is needed: blocks that have not started are for whoever is done first.
     if (!V && t == max(0, tiles - kWantTiles) && lead) mbar_arrive(smem_u32(&sh.want));
     if (!V && lead) sh.loaded = place.round * TcCfg<DP>::kSlots + place.slot;
+    // the same for all chunks of a tile of K
+    int boxes = !kPaged ? 1 : min(most, max(0, most_keys - key + box - 1) >> box_bits);
+    int page = kPaged ? __shfl_sync(0xffffffffu, pages, mine) : 0, row = (key + mine * box) & (a.c.page_tokens - 1);
 #pragma unroll 1
     for (int c = 0; c < Cfg::kChunks; c++, place.next()) {
-      const int from = V ? key + c * kRows : key, x0 = V ? 0 : c * kSlabs * 64;
+      const int x0 = V ? 0 : c * kSlabs * 64;
+      if (V && kPaged && c > 0) {
+        const int from = key + c * kRows;
+        boxes = min(most, max(0, most_keys - from + box - 1) >> box_bits);
+        page = __shfl_sync(0xffffffffu, pages, c * most + mine);
+        row = (from + mine * box) & (a.c.page_tokens - 1);
+      }
       const uint32_t bar = smem_u32(V ? &sh.v_full[place.slot] : &sh.k_full[place.slot]);
       const uint32_t dst = ring + place.slot * Cfg::kChunkBytes;
-      // shared: the chunk's boxes, each in kSlabs slabs; one lane for each
-      const int slab = lane % kSlabs, mine = lane / kSlabs;
-      const int boxes = !kPaged ? 1 : from + kRows <= most_keys ? most : max(0, most_keys - from + box - 1) / box;
-      const int page = kPaged ? __shfl_sync(0xffffffffu, pages, (V ? c * most : 0) + mine) : 0;
       uint64_t &empty = V ? sh.v_empty[place.slot] : sh.k_empty[place.slot];
       if (place.round > 0 && !wait(sh, a.wait_limit, empty, place.parity() ^ 1)) return false;
       if (lead) mbar_expect_tx(bar, kSlabs * boxes * box * 128);
       __syncwarp();
       if (MODE == kTcPrompt) {
-        if (lane < kSlabs) tma_load_3d(dst + slab * kRows * 128, map, x0 + slab * 64, kv_head, k0 + from, bar);
+        if (lane < kSlabs)
+          tma_load_3d(dst + slab * kRows * 128, map, x0 + slab * 64, kv_head, k0 + key + (V ? c * kRows : 0), bar);
       } else if (mine < boxes) {
-        tma_load_4d(dst + slab * kRows * 128 + mine * box * 128, map, x0 + slab * 64,
-                    (from + mine * box) & (a.c.page_tokens - 1), kv_head, page, bar);
+        tma_load_4d(dst + place_in, map, x0 + slab * 64, row, kv_head, page, bar);
       }
       __syncwarp();
     }

@@ -30,15 +30,16 @@ constexpr int kFreeBatch = 8;  // pages per thread and step of the search for fr
 //   first  [max_sequences]   rank of an entry's first fresh page
 //   stay   [max_sequences]   compact: leading pages that an entry keeps
 //   moved  [max_sequences]   compact: blocks that have moved their rows of an entry
+//   old    [max_sequences]   compact: length of an entry before
 //   fresh  [pages]           page numbers by rank
 //   owner  [pages]           list entry that a fresh page goes to
 struct Plan {
-  int32_t *ok, *total, *marks, *first, *stay, *moved, *fresh, *owner;
+  int32_t *ok, *total, *marks, *first, *stay, *moved, *old, *fresh, *owner;
 };
 constexpr int kPlanHeader = 4;
 
 size_t plan_ints(const dm_kv_cache_desc &d) {
-  return kPlanHeader + 4 * (size_t)d.max_sequences + 2 * (size_t)d.pages;
+  return kPlanHeader + 5 * (size_t)d.max_sequences + 2 * (size_t)d.pages;
 }
 
 Plan plan_of(const dm_kv_cache *c) {
@@ -49,7 +50,8 @@ Plan plan_of(const dm_kv_cache *c) {
   p.first = p.marks + c->desc.max_sequences;
   p.stay = p.first + c->desc.max_sequences;
   p.moved = p.stay + c->desc.max_sequences;
-  p.fresh = p.moved + c->desc.max_sequences;
+  p.old = p.moved + c->desc.max_sequences;
+  p.fresh = p.old + c->desc.max_sequences;
   p.owner = p.fresh + c->desc.pages;
   return p;
 }
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(KvView c, Plan p, Pl
             if ((unsigned)last < (unsigned)c.pages && c.references[last] > 1) stay--;
           }
         }
-        if ((tid & 31) == 0) p.stay[i] = stay, p.moved[i] = 0;
+        if ((tid & 31) == 0) p.stay[i] = stay, p.moved[i] = 0, p.old[i] = c.lengths[row];
       }
       // Between its first and last token, which are in range, an entry's list ascends. All
       // lists in one pass, kSteps loads of a thread in flight: a step down is rare where no new
@@ -385,16 +387,45 @@ __device__ void settle_entry(const KvView &c, const Plan &p, const PlanArgs &a, 
   if (threadIdx.x == 0) c.lengths[row] = count;
 }
 
+// Weights go with their tokens, whose places only fall: a round's sources lie at its own places or
+// behind them. The places behind the last one become 0.
+__device__ void move_weights(float *weights, const int32_t *keep, int count, int length) {
+  if (count == length) return;
+  for (int j0 = 0; j0 < length; j0 += 8 * kCopyThreads) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int j = j0 + k * kCopyThreads + threadIdx.x;
+      x[k] = j < count ? weights[keep[j]] : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int j = j0 + k * kCopyThreads + threadIdx.x;
+      if (j < length) weights[j] = x[k];
+    }
+  }
+}
+
 // Compact: jobs (along y) are the plan's fresh pages, then the entries without one. Block
-// (x, f) gathers its part of page f; the last block of an entry's pages settles it.
+// (x, f) gathers its part of page f; the last block of an entry's pages settles it. The weights of
+// an eviction go along in the last jobs' first blocks.
+template <bool EVICT>
 __global__ void __launch_bounds__(kCopyThreads)
-gather_kernel(KvView c, Plan p, PlanArgs a) {
+gather_kernel(KvView c, Plan p, PlanArgs a, float *weights, int64_t weights_stride) {
   chain();
   if (!*p.ok) return;
   const int total = *p.total;
   __shared__ int64_t source[256];  // of each row of the page, -1 where it has none
   __shared__ int last;
-  for (int f = blockIdx.y; f < total + a.n; f += gridDim.y) {
+  const int jobs = total + (EVICT ? 2 : 1) * a.n;
+  for (int f = blockIdx.y; f < jobs; f += gridDim.y) {
+    if (EVICT && f >= total + a.n) {
+      const int i = f - total - a.n;
+      if (blockIdx.x == 0)
+        move_weights(weights + a.rows[i] * weights_stride, a.keep + a.other[i], a.other[i + 1] - a.other[i], p.old[i]);
+      continue;
+    }
     if (f >= total) {
       const int i = f - total;
       if (blockIdx.x == 0 && pages_for(c, a.other[i + 1] - a.other[i]) == p.stay[i]) settle_entry(c, p, a, i);
@@ -431,16 +462,19 @@ gather_kernel(KvView c, Plan p, PlanArgs a) {
 // ---------------------------------------------------------------------------
 // Eviction: choose the tokens that stay, compact by the list, move their weights.
 //
-// The budget-th largest weight is found digit by digit (11, 11 and 10 bits of the weights'
-// patterns in their order): each step counts the next digit of those that share the digits found so
-// far. The blocks of a cluster have a part of the sequence each and add their counts through
-// distributed shared memory. Then one pass writes the positions above that weight, and the first
-// of those equal to it, in order. Bound by latency: five passes over weights that lie in L2.
+// The budget-th largest weight is found by narrowing the range of bit patterns (in the order of
+// their values) that it lies in, from the smallest and largest weight on: each step counts the
+// patterns of 2048 equal parts of the range. Patterns go by the logarithm, so weights spread over
+// the parts whatever their scale, and two steps do for most. The blocks of a cluster have a part
+// of the sequence each and add their counts through distributed shared memory. One pass then
+// writes the positions of the weights above that one, and of the first equal to it, in order.
+// Bound by latency: a few passes over weights that lie in L2, and about 15 barriers (with 3 steps of
+// 11 bits, a pass to count and barriers of clusters throughout 11 us for 300 tokens, 21 for 8191).
 // ---------------------------------------------------------------------------
 
 constexpr int kMostRanks = 8;
-constexpr int kRankTokens = 4096;  // of a block before a sequence gets another
-constexpr int kDigits = 2048;
+constexpr int kRankTokens = 16384;  // of a block before a sequence gets another
+constexpr int kParts = 2 * kPlanThreads;
 
 struct EvictArgs {
   const int32_t *rows;
@@ -462,18 +496,24 @@ __device__ __forceinline__ int tokens_of(const KvView &c, int row) {
 }
 
 // Cluster (all x, i) chooses for entry i.
-__global__ void __launch_bounds__(kPlanThreads) choose_kernel(KvView c, EvictArgs a) {
-  __shared__ int count[3][kDigits];
-  __shared__ int shared[4], found[2];
+__global__ void __launch_bounds__(kPlanThreads, 1) choose_kernel(KvView c, EvictArgs a) {
+  __shared__ int count[2][kParts];
+  __shared__ int found[3], share_of[2];          // a step's answer; this block's places: above, and equal
+  __shared__ uint32_t bounds[2][kPlanThreads / 32], range[2];
   auto cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank(), tid = threadIdx.x;
+  const int lane = tid & 31, warp = tid >> 5;
+  auto sync = [&]() {
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+  };
   chain();
-  for (int i = tid; i < 3 * kDigits; i += kPlanThreads) (&count[0][0])[i] = 0;
   const int entry = blockIdx.y, row = a.rows[entry];
   const int length = tokens_of(c, row), budget = a.budget;
+  for (int i = tid; i < kParts; i += kPlanThreads) count[0][i] = 0;
   // where the entry's list begins
   int before = 0, sum;
-  for (int i = tid; i < entry; i += kPlanThreads) before += min(tokens_of(c, a.rows[i]), budget);
+  for (int i = tid; i < entry; i += kPlanThreads) before = add_upto(before, min(tokens_of(c, a.rows[i]), budget));
   block_scan(before, &sum);
   const int begin = sum;
   const bool fits = length <= a.stride;
@@ -494,61 +534,83 @@ __global__ void __launch_bounds__(kPlanThreads) choose_kernel(KvView c, EvictArg
   // this block's tokens: a multiple of four for every thread
   const int share = ((length + ranks - 1) / ranks + 3) / 4 * 4;
   const int from = min(length, rank * share), to = min(length, from + share);
-  uint32_t digits = 0;  // of the last weight that stays, from above
-  cluster.sync();  // the counts are zero
+  const int first = max(low, from), behind = min(high, to);
+  uint32_t bottom = 0xffffffffu, top = 0;  // patterns that the last weight to stay lies between
+  for (int j = first + tid; j < behind; j += kPlanThreads) {
+    const uint32_t u = ordered(weights[j]);
+    bottom = min(bottom, u), top = max(top, u);
+  }
+  bottom = __reduce_min_sync(0xffffffffu, bottom), top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) bounds[0][warp] = bottom, bounds[1][warp] = top;
+  __syncthreads();
+  if (warp == 0) {
+    bottom = __reduce_min_sync(0xffffffffu, bounds[0][lane]), top = __reduce_max_sync(0xffffffffu, bounds[1][lane]);
+    if (lane == 0) range[0] = bottom, range[1] = top;
+  }
+  sync();
+  bottom = range[0], top = range[1];
+  for (int r = 0; r < ranks && ranks > 1; r++) {
+    const uint32_t *there = cluster.map_shared_rank(&range[0], r);
+    bottom = min(bottom, there[0]), top = max(top, there[1]);
+  }
+  // Until the range is one pattern, or all weights left in it stay
+  bool open = need > 0;
 #pragma unroll 1
-  for (int step = 0; step < 3; step++) {
-    const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, above = step == 0 ? 32 : step == 1 ? 21 : 10;
-    const uint32_t mask = step == 2 ? 1023 : 2047;
-    for (int j = max(low, from) + tid; j < min(high, to); j += kPlanThreads) {
+  for (int step = 0; open && bottom < top; step ^= 1) {
+    const int shift = max(0, 32 - __clz(top - bottom) - 11);
+    for (int j = first + tid; j < behind; j += kPlanThreads) {
       const uint32_t u = ordered(weights[j]);
-      if (step == 0 || u >> above == digits) atomicAdd(&count[step][u >> shift & mask], 1);
+      if (u >= bottom && u <= top) atomicAdd(&count[step][(u - bottom) >> shift], 1);
     }
-    cluster.sync();
-    // two digits a thread, the largest first
+    sync();
+    for (int i = tid; i < kParts; i += kPlanThreads) count[step ^ 1][i] = 0;  // the next step's, read by all before this one
+    // two parts a thread, the largest first
     int mine[2] = {0, 0};
     for (int r = 0; r < ranks; r++) {
       const int *there = ranks == 1 ? count[step] : cluster.map_shared_rank(&count[step][0], r);
-      for (int k = 0; k < 2; k++) mine[k] += there[kDigits - 1 - (2 * tid + k)];
+      for (int k = 0; k < 2; k++) mine[k] += there[kParts - 1 - (2 * tid + k)];
     }
-    const int upto = block_scan(mine[0] + mine[1], &sum), first = upto - mine[0] - mine[1];
-    if (need > 0 && first < need && need <= upto) {
-      const int second = need > first + mine[0];
-      found[0] = kDigits - 1 - (2 * tid + second);
-      found[1] = need - first - (second ? mine[0] : 0);
-    }
-    __syncthreads();
-    if (need > 0) {
-      digits = digits << (step == 0 ? 0 : step == 1 ? 11 : 10) | found[0];
-      need = found[1];  // of those that share the digits
+    const int upto = block_scan(mine[0] + mine[1], &sum), above = upto - mine[0] - mine[1];
+    if (above < need && need <= upto) {
+      const int second = need > above + mine[0];
+      found[0] = kParts - 1 - (2 * tid + second);
+      found[1] = need - above - (second ? mine[0] : 0);  // of those in the part
+      found[2] = mine[second];
     }
     __syncthreads();
+    const uint32_t part = bottom + ((uint32_t)found[0] << shift);
+    need = found[1];
+    open = found[1] < found[2];
+    top = min(top, part + ((1u << shift) - 1)), bottom = part;
+    sync();  // the zeros are there, and found has been read
   }
-  // What stays: whatever the weight, above the last one, or among the first `need` equal to it
+  // What stays: whatever the weight, from the range's end on, or among the first `need` in it. (If
+  // the range has several patterns, all in it stay; if none is needed, none does.)
   auto class_of = [&](int j) -> uint32_t {
     if (j >= to) return 0;
     if (j < low || j >= high) return 1;
-    if (budget == a.sinks + a.recent) return 0;
     const uint32_t u = ordered(weights[j]);
-    return u > digits ? 1 : u == digits ? 1u << 16 : 0;
+    return need == 0 || u < bottom ? 0 : u > top ? 1 : 1u << 16;
   };
-  // Both counts of a round of 4 tokens a thread fit 16 bits; those of a block do not.
-  int sure = 0, ties = 0;
-  for (int j0 = from; j0 < to; j0 += 4 * kPlanThreads)
-    for (int k = 0; k < 4; k++) {
-      const uint32_t x = class_of(j0 + k * kPlanThreads + tid);
-      sure += x & 0xffff, ties += x >> 16;
+  int at = 0, left = need;  // places before this block's; in the range that may still stay
+  if (ranks > 1) {
+    // both counts of a round of 4 tokens a thread fit 16 bits; those of a block do not
+    int sure = 0, ties = 0;
+    for (int j0 = from; j0 < to; j0 += 4 * kPlanThreads)
+      for (int k = 0; k < 4; k++) {
+        const uint32_t x = class_of(j0 + k * kPlanThreads + tid);
+        sure += x & 0xffff, ties += x >> 16;
+      }
+    block_scan(sure, &sum);
+    if (tid == 0) share_of[0] = sum;
+    block_scan(ties, &sum);
+    if (tid == 0) share_of[1] = sum;
+    cluster.sync();
+    for (int r = 0; r < rank; r++) {
+      const int *there = cluster.map_shared_rank(&share_of[0], r);
+      const int some = min(there[1], left);
+      at += there[0] + some, left -= some;
     }
-  block_scan(sure, &sum);
-  if (tid == 0) shared[0] = sum;
-  block_scan(ties, &sum);
-  if (tid == 0) shared[1] = sum;
-  cluster.sync();
-  int at = 0, left = need;  // places before this block's; ties that may still stay
-  for (int r = 0; r < rank; r++) {
-    const int *there = cluster.map_shared_rank(&shared[0], r);
-    const int some = min(there[1], left);
-    at += there[0] + some, left -= some;
   }
   for (int j0 = from; j0 < to; j0 += 4 * kPlanThreads) {
     uint32_t x[4], all = 0;
@@ -561,33 +623,7 @@ __global__ void __launch_bounds__(kPlanThreads) choose_kernel(KvView c, EvictArg
     at += (sum & 0xffff) + min(sum >> 16, left);
     left -= min(sum >> 16, left);
   }
-  cluster.sync();  // nobody reads this block's shared memory any more
-}
-
-// Weights of entry i go with their tokens, whose places only fall: a round's sources lie at its
-// own places or behind them. Before the lengths change.
-__global__ void __launch_bounds__(kPlanThreads) move_weights_kernel(KvView c, Plan p, EvictArgs a) {
-  chain();
-  if (!*p.ok) return;
-  const int i = blockIdx.x, row = a.rows[i], tid = threadIdx.x;
-  const int begin = a.keep_offsets[i], count = a.keep_offsets[i + 1] - begin, length = tokens_of(c, row);
-  const int32_t *keep = a.keep + begin;
-  float *weights = a.weights + row * a.stride;
-  if (count == length) return;
-  for (int j0 = 0; j0 < length; j0 += 4 * kPlanThreads) {
-    float x[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int j = j0 + k * kPlanThreads + tid;
-      x[k] = j < count ? weights[keep[j]] : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int j = j0 + k * kPlanThreads + tid;
-      if (j < length) weights[j] = x[k];
-    }
-  }
+  if (ranks > 1) cluster.sync();  // nobody reads this block's shared memory any more
 }
 
 // Free: block i takes the length of its sequence (a repeat finds zero) and lets go.
@@ -691,12 +727,13 @@ int32_t launch(void (*kernel)(Params...), dim3 grid, int threads, void *stream, 
   return dma::launch_chained("cache launch", kernel, grid, threads, 0, (cudaStream_t)stream, args...);
 }
 
-int32_t launch_gather(const dm_kv_cache *c, const PlanArgs &a, int64_t kept, void *stream) {
+int32_t launch_gather(const dm_kv_cache *c, const PlanArgs &a, int64_t kept, float *weights, int64_t stride, void *stream) {
   // at most this many fresh pages
   const int64_t fresh = std::min<int64_t>(c->desc.pages, kept / c->desc.page_tokens + a.n);
   const dim3 grid(blocks_along(c->view.page_bytes / 16, fresh, kGridBlocks),
-                  (unsigned)std::min<int64_t>(fresh + a.n, 65535));
-  return launch(gather_kernel, grid, kCopyThreads, stream, c->view, plan_of(c), a);
+                  (unsigned)std::min<int64_t>(fresh + (weights ? 2 : 1) * a.n, 65535));
+  return launch(weights ? gather_kernel<true> : gather_kernel<false>, grid, kCopyThreads, stream, c->view, plan_of(c), a,
+                weights, stride);
 }
 
 int32_t check_list(const dm_kv_cache *cache, const void *list, int32_t n) {
@@ -896,7 +933,7 @@ int32_t dm_kv_cache_compact(dm_kv_cache *c, const int32_t *sequences, const int3
   const PlanArgs a{sequences, keep_offsets, keep, kept, n};
   if (int32_t rc = launch(plan_kernel<kCompact>, 1, kPlanThreads, stream, c->view, plan_of(c), a))
     return rc;
-  return launch_gather(c, a, kept, stream);
+  return launch_gather(c, a, kept, nullptr, 0, stream);
 }
 
 int32_t dm_kv_cache_free(dm_kv_cache *c, const int32_t *sequences, int32_t n, void *stream) {
@@ -944,8 +981,7 @@ int32_t dm_kv_cache_evict(dm_kv_cache *c, const dm_kv_cache_evict_desc *in, void
   const int64_t kept = (int64_t)in->budget * n;
   const PlanArgs a{in->rows, in->keep_offsets, in->keep, kept, n};
   if (int32_t rc = launch(plan_kernel<kCompact>, 1, kPlanThreads, stream, c->view, plan_of(c), a)) return rc;
-  if (int32_t rc = launch(move_weights_kernel, n, kPlanThreads, stream, c->view, plan_of(c), e)) return rc;
-  return launch_gather(c, a, kept, stream);
+  return launch_gather(c, a, kept, in->weights, in->weights_stride, stream);
 }
 
 }  // extern "C"

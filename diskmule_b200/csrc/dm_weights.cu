@@ -324,7 +324,7 @@ struct Turn {  // a place in a ring
   __device__ void next() {
     if (++slot == SLOTS) slot = 0, round++;
   }
-  // What has been loaded lands before the block ends.
+  // What has been loaded lands before the block ends, whether or not somebody waits for it.
   __device__ void drain(uint64_t *full) {
     for (int n = min(SLOTS, (int)(round * SLOTS + slot)); n > 0; n--) {
       if (--slot < 0) slot = SLOTS - 1, round--;
@@ -421,7 +421,7 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
             tma_load_4d(base + k.slot * kSlab + lane * t.k_box * 128, &k_map, slab * 64, place, h, page, bar);
         }
       if (rank == 0 && lane < used && (unsigned)page >= (unsigned)c.pages) atomicOr(c.status, DM_KV_BAD_TOKEN);
-      if (!ok) k.drain(sh.k_full);
+      k.drain(sh.k_full);
     } else if (warp == kSoft + 1) {
       // ---- queries
       Turn<Cfg::kQuerySlots> q;
@@ -434,7 +434,7 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
           tma_load_4d(q_ring + q.slot * Cfg::kQBytes + lane * COLS * 128, &q_map, lane * 64, 0, at.head,
                       (int)(e.q0 + (int64_t)at.tile * per), bar);
       }
-      if (!ok) q.drain(sh.q_full);
+      q.drain(sh.q_full);
     } else if (warp == kSoft + 2) {
       // ---- products
       constexpr uint32_t kIdesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(COLS >> 3) << 17) |
@@ -469,11 +469,9 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
         fresh = ends;
         if (ends) k = slab;
       }
-      if (!ok) {  // products in flight end before tensor memory is let go
-        if (lead) mma_commit(smem_u32(&sh.drain));
-        __syncwarp();
-        mbar_wait(smem_u32(&sh.drain), 0);
-      }
+      // products in flight end before tensor memory is let go, whoever has given up
+      commit_if(one, smem_u32(&sh.drain));
+      mbar_wait(smem_u32(&sh.drain), 0);
     } else {
       // ---- statistics: a lane's rows of several tiles at once, a batch ahead
       constexpr int kRowsOf = (COLS + 31) / 32;

@@ -261,7 +261,8 @@ DM_API int32_t dm_attention_rotate(dm_cuda_context *ctx, const dm_rope *rope, dm
  * -infinity gives nothing. weights: device f32, one row of weights_stride for every row of the
  * table; tokens from weights_stride on are passed over. Calls that are alike add in the same order. A cache row
  * that is named twice counts for its first entry and sets DM_KV_BAD_SEQUENCE; entries outside
- * the table are passed over. */
+ * the table are passed over. At most 65535 entries. After a wait that ran out
+ * (dm_attention_status) the sums are undefined. */
 typedef struct {
   int32_t layer, heads, sequences, window, sinks, max_length;
   float scale;
@@ -285,7 +286,8 @@ DM_API int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_weigh
  * the cache is compacted by them under its rules; the kept tokens' weights move along, and those
  * of the places behind them, up to the old length, become 0. weights_stride must hold every
  * token of a row of the table, or of the longest sequence (DM_KV_BAD_TOKEN otherwise). What is
- * refused leaves cache and weights unchanged; keep and keep_offsets are then undefined. */
+ * refused leaves cache and weights unchanged; keep and keep_offsets are then undefined. At most
+ * 65535 entries. */
 typedef struct {
   int32_t sequences, budget, sinks, recent;
   const int32_t *rows;
