@@ -358,6 +358,10 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u, q_ring = base + Cfg::kKeySlots * kSlab;
   auto cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map));
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map));
+  }
   if (tid < kMostSlabs) mbar_init(smem_u32(&sh.k_full[tid]), 1), mbar_init(smem_u32(&sh.k_empty[tid]), 1);
   if (tid < kMostQueries) mbar_init(smem_u32(&sh.q_full[tid]), 1), mbar_init(smem_u32(&sh.q_empty[tid]), 1);
   if (tid < kStatSlots) mbar_init(smem_u32(&sh.z_full[tid]), 1), mbar_init(smem_u32(&sh.z_empty[tid]), 4 * HALVES);
@@ -387,12 +391,19 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     if (last < e.lq) t1 = last < 0 ? 0 : (int)(last / per) + 1;
   }
   if (t1 <= t0) return;
-  if (warp == kSoft) tmem_alloc(smem_u32(&sh.tmem), Cfg::kTmem);
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const uint32_t tmem = sh.tmem;
-  if (ranks > 1) cluster.sync();  // the others' shared memory is there
+  // Loads begin at once. Tensor memory is for the warps that weigh and the one of the products; the
+  // others' shared memory (the barrier's other half) is needed at the end.
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  constexpr int kProducts = kSoft + 2;
+  if (warp < kSoft || warp == kProducts) {
+    if (warp == kProducts) tmem_alloc(smem_u32(&sh.tmem), Cfg::kTmem);
+    fence_before();
+    asm volatile("bar.sync 1, %0;" ::"n"((kSoft + 1) * 32) : "memory");
+    fence_after();
+  }
+  const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+  const bool adds = rank == 0 && tid < kKeys && first + tid < e.end;
+  const float old = adds ? a.weights[e.row * a.weights_stride + first + tid] : 0.0f;
 
   // this block's share of heads x tiles
   const int64_t all = (int64_t)(t1 - t0) * c.kv_heads;
@@ -581,11 +592,12 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   fence_before();
   __syncthreads();
   if (tid == 0 && sh.abort) atomicExch(a.d.timeout, 1);
-  if (warp == kSoft) {
+  if (warp == kProducts) {
     fence_after();
     tmem_dealloc(tmem, Cfg::kTmem);
   }
   // ---- the sums of the ranks, and of the two groups of each, in order
+  if (ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (ranks * kGroups > 1) {
     if (warp < kSoft) {
       float *there = ranks > 1 ? cluster.map_shared_rank(&sums[0][0], 0) : &sums[0][0];
@@ -593,11 +605,11 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
     }
     if (ranks > 1) cluster.sync();
     else __syncthreads();
-    if (rank > 0 || tid >= kKeys) return;
+    if (!adds) return;
     total = 0.0f;
     for (int i = 0; i < ranks * kGroups; i++) total += sums[i][tid];
   }
-  if (tid < kKeys && first + tid < e.end) a.weights[e.row * a.weights_stride + first + tid] += total;
+  if (adds) a.weights[e.row * a.weights_stride + first + tid] = old + total;
 }
 
 template <int DP, int COLS, int HALVES>
