@@ -136,6 +136,15 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_
   load();
 
   // ---- the token's place and its sines, while the first heads come in
+  const int half = a.rotary / 2;
+  uint64_t turns[kPairs / 32] = {};
+  int64_t position[kPairs / 32] = {};
+#pragma unroll
+  for (int j = 0; j < kPairs / 32; j++)
+    if (lane + 32 * j < half) {
+      turns[j] = a.turns[lane + 32 * j];
+      if (a.positions) position[j] = a.positions[a.pair_axes[lane + 32 * j] * a.tokens + t];
+    }
   int64_t place = 0, cached_at = -1;
   const int page_bits = 31 - __clz(c.page_tokens);  // pages are powers of two
   if (a.cached) {
@@ -156,19 +165,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_
       if (lane == 0 && blockIdx.y == 0) atomicOr(c.status, DM_KV_BAD_TOKEN);
     }
   }
-  const int half = a.rotary / 2;
-  for (int i = lane; i < half; i += 32) {
-    const int64_t p = a.positions ? a.positions[a.pair_axes[i] * a.tokens + t] : place;
-    const uint64_t turns = (uint64_t)p * a.turns[i];
+#pragma unroll
+  for (int j = 0; j < kPairs / 32; j++) {
+    const int i = lane + 32 * j;
+    if (i >= half) break;
+    const uint64_t angle = (uint64_t)(a.positions ? position[j] : place) * turns[j];
     float s, k;
     // half turns, -1 to 1; their f32 is off by at most 2^-25
-    sincospif((float)(int32_t)(turns >> 32) * 0x1p-31f, &s, &k);
+    sincospif((float)(int32_t)(angle >> 32) * 0x1p-31f, &s, &k);
     const int first = a.interleaved ? 2 * i : i, second = a.interleaved ? first + 1 : i + half;
     cosine[warp][first] = cosine[warp][second] = k * a.scale;
     sine[warp][first] = -s * a.scale;
     sine[warp][second] = s * a.scale;
   }
-  for (int i = a.rotary + lane; i < a.dim; i += 32) cosine[warp][i] = 1.0f, sine[warp][i] = 0.0f;
   __syncwarp();
 
   // where the other halves of this lane's pairs are; pairs side by side are exchanged in place
@@ -180,24 +189,28 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_
     const int n = high_of(kind) - low_of(kind), head = low_of(kind) + side - a.first[kind];
     if (n <= 0) continue;
     const bool normed = (a.norms >> kind) & 1, rotated = kind != kV && a.rotary > 0;
-    if (kind != kV && in)
+    const bool turning = rotated && col < a.rotary;
+    if (kind != kV && in) {
+      float k[8], s[8], here[8], there[8];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float2 k = *reinterpret_cast<const float2 *>(&cosine[warp][col + 2 * e]);
-        float2 s = *reinterpret_cast<const float2 *>(&sine[warp][col + 2 * e]);
-        if (normed && a.weight[kind]) {
-          const float *w = a.weight[kind] + 2 * e, *here = w + col, *there = w + other * 8;
-          const bool swap = a.interleaved && col < a.rotary;
-          k.x *= here[0], k.y *= here[1];
-          s.x *= there[swap], s.y *= there[!swap];
-        }
-        own.v[e] = pair(k.x, k.y), across.v[e] = pair(s.x, s.y);
+      for (int e = 0; e < 8; e++) k[e] = here[e] = there[e] = 1.0f, s[e] = 0.0f;
+      auto fetch8 = [](const float *p, float *to) {
+        const float4 u = reinterpret_cast<const float4 *>(p)[0], v = reinterpret_cast<const float4 *>(p)[1];
+        to[0] = u.x, to[1] = u.y, to[2] = u.z, to[3] = u.w, to[4] = v.x, to[5] = v.y, to[6] = v.z, to[7] = v.w;
+      };
+      if (turning) fetch8(&cosine[warp][col], k), fetch8(&sine[warp][col], s);
+      if (normed && a.weight[kind]) fetch8(a.weight[kind] + col, here), fetch8(a.weight[kind] + other * 8, there);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float x = a.interleaved ? there[e + 1] : there[e], y = a.interleaved ? there[e] : there[e + 1];
+        own.v[e / 2] = pair(k[e] * here[e], k[e + 1] * here[e + 1]);
+        across.v[e / 2] = pair(s[e] * x, s[e + 1] * y);
       }
+    }
     const int64_t out_step = kSide * a.out_stride[kind][1], cache_step = kSide * c.head_bytes;
     const bool out_too = in && a.out[kind], cache_too = in && kind != kQ && cached_at >= 0;
     uint8_t *out = a.out[kind] + t * a.out_stride[kind][0] + head * a.out_stride[kind][1] + col * 2;
     uint8_t *cache = c.memory + cached_at + ((kind == kV ? c.kv_heads : 0) + head) * c.head_bytes;
-    const bool turns = rotated && col < a.rotary;
 #pragma unroll 1
     for (int i = 0; i < n; i += kFlight * kSide) {
       uint32_t r[kFlight][4];
@@ -239,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_
 #pragma unroll
             for (int e = 0; e < 4; e++) v[k].v[e] = mul2(v[k].v[e], own.v[e]);
           // what does not turn stays apart from the rest of its head: 0 times infinity is no zero
-          if (turns)
+          if (turning)
 #pragma unroll
             for (int k = 0; k < kFlight; k++) {
               const Eight u = unpack<BF16>(r[k]);
@@ -403,8 +416,8 @@ int32_t dm_attention_rotate(dm_cuda_context *ctx, const dm_rope *rope, dm_kv_cac
     a.heads += heads;
   }
   if (a.heads == 0) return DM_OK;
-  if (((uintptr_t)in->q_weight | (uintptr_t)in->k_weight) & 3)
-    return fail(DM_ERR_INVALID_ARGUMENT, "norm weights must be 4-byte aligned");
+  if (((uintptr_t)in->q_weight | (uintptr_t)in->k_weight) & 15)
+    return fail(DM_ERR_INVALID_ARGUMENT, "norm weights must be 16-byte aligned");
   a.weight[0] = in->q_weight;
   a.weight[1] = in->k_weight;
   a.positions = in->positions;

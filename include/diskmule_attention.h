@@ -235,7 +235,7 @@ DM_API void dm_rope_destroy(dm_rope *rope);
  * outputs are left as they were; one whose place is not in the table is not cached and sets
  * DM_KV_BAD_TOKEN, and stands at position 0 where positions is NULL. No cache row is named
  * twice. Without a cache the call does all tokens and reads neither rows nor offsets.
- * Pointers are 16-byte aligned, weights 4; strides as above. */
+ * Tensors and weights are 16-byte aligned; strides as above. */
 enum { DM_NORM_Q = 1, DM_NORM_K = 2, DM_NORM_V = 4 };
 typedef struct {
   int32_t type, heads, kv_heads, head_dim, norms;
