@@ -18,7 +18,6 @@
 #include <new>
 
 #include "dm_attention.cuh"
-#include "dm_tcgen05.cuh"
 
 using dmi::fail;
 
@@ -34,9 +33,9 @@ namespace dma {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kBlocks = 4;   // of an SM
+constexpr int kBlocks = 7;   // of an SM
 constexpr int kPairs = 128;  // at most
-constexpr int kFlight = 4;   // 16-byte loads of a thread in flight
+constexpr int kFlight = 2;   // 16-byte loads of a thread in flight
 
 enum Kind { kQ, kK, kV };
 
@@ -74,10 +73,9 @@ __device__ __forceinline__ int entry_of(const int32_t *offsets, int n, int64_t t
 
 // Two 16-bit values as f32
 template <bool BF16>
-__device__ __forceinline__ uint64_t both(uint32_t x) {
-  if (BF16) return dm::tc::pair(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x));
-  return dm::tc::pair(f.x, f.y);
+__device__ __forceinline__ float2 both(uint32_t x) {
+  if (BF16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&x));
 }
 
 __device__ __forceinline__ float rsqrt_fast(float x) {  // within two units of the last place
@@ -87,7 +85,7 @@ __device__ __forceinline__ float rsqrt_fast(float x) {  // within two units of t
 }
 // Values of a head that one lane has, as pairs of f32
 struct Eight {
-  uint64_t v[4];
+  float2 v[4];
 };
 template <bool BF16>
 __device__ __forceinline__ Eight unpack(const uint32_t *r) {
@@ -98,7 +96,6 @@ __device__ __forceinline__ Eight unpack(const uint32_t *r) {
 template <int LANES, bool BF16>
 __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_constant__ KvView c,
                                                                    const __grid_constant__ RotateArgs a) {
-  using namespace dm::tc;
   constexpr unsigned kAll = 0xffffffffu;
   constexpr int kSide = 32 / LANES;  // heads side by side
   __shared__ alignas(16) float cosine[kWarps][LANES * 8], sine[kWarps][LANES * 8];  // of each value of the token's heads
@@ -203,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const float x = a.interleaved ? there[e + 1] : there[e], y = a.interleaved ? there[e] : there[e + 1];
-        own.v[e / 2] = pair(k[e] * here[e], k[e + 1] * here[e + 1]);
-        across.v[e / 2] = pair(s[e] * x, s[e + 1] * y);
+        own.v[e / 2] = make_float2(k[e] * here[e], k[e + 1] * here[e + 1]);
+        across.v[e / 2] = make_float2(s[e] * x, s[e + 1] * y);
       }
     }
     const int64_t out_step = kSide * a.out_stride[kind][1], cache_step = kSide * c.head_bytes;
@@ -228,10 +225,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_
         if (normed) {
 #pragma unroll
           for (int k = 0; k < kFlight; k++) {
-            uint64_t sum = mul2(v[k].v[0], v[k].v[0]);
+            float2 sum = __fmul2_rn(v[k].v[0], v[k].v[0]);
 #pragma unroll
-            for (int e = 1; e < 4; e++) sum = fma2(v[k].v[e], v[k].v[e], sum);
-            root[k] = in ? __uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32)) : 0.0f;
+            for (int e = 1; e < 4; e++) sum = __ffma2_rn(v[k].v[e], v[k].v[e], sum);
+            root[k] = in ? sum.x + sum.y : 0.0f;
           }
 #pragma unroll
           for (int o = 1; o < LANES; o <<= 1)
@@ -250,23 +247,23 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_kernel(const __grid_
 #pragma unroll
           for (int k = 0; k < kFlight; k++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[k].v[e] = mul2(v[k].v[e], own.v[e]);
+            for (int e = 0; e < 4; e++) v[k].v[e] = __fmul2_rn(v[k].v[e], own.v[e]);
           // what does not turn stays apart from the rest of its head: 0 times infinity is no zero
           if (turning)
 #pragma unroll
             for (int k = 0; k < kFlight; k++) {
               const Eight u = unpack<BF16>(r[k]);
 #pragma unroll
-              for (int e = 0; e < 4; e++) v[k].v[e] = fma2(u.v[e], across.v[e], v[k].v[e]);
+              for (int e = 0; e < 4; e++) v[k].v[e] = __ffma2_rn(u.v[e], across.v[e], v[k].v[e]);
             }
         }
 #pragma unroll
         for (int k = 0; k < kFlight; k++) {
-          const uint64_t scale = pair(root[k], root[k]);
+          const float2 scale = make_float2(root[k], root[k]);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            v[k].v[e] = mul2(v[k].v[e], scale);
-            r[k][e] = pack2<BF16>(__uint_as_float((uint32_t)v[k].v[e]), __uint_as_float((uint32_t)(v[k].v[e] >> 32)));
+            const float2 y = __fmul2_rn(v[k].v[e], scale);
+            r[k][e] = pack2<BF16>(y.x, y.y);
           }
         }
       }
