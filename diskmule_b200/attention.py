@@ -19,8 +19,11 @@ from ._native import check
 from .moe import CudaContext
 
 
+_Pair = C.c_int64 * 2
+
+
 def _strides(pair):  # zeros: contiguous
-    return (C.c_int64 * 2)() if pair is None else (C.c_int64 * 2)(*pair)
+    return _Pair() if pair is None else _Pair(*pair)
 
 
 def prompt_attention(ctx: CudaContext, *, type: int, heads: int, kv_heads: int, head_dim: int,
@@ -102,15 +105,30 @@ def rotate(ctx: CudaContext, rope: Rope | None, *, type: int, head_dim: int, tok
     norms = norm_q * N.NORM_Q | norm_k * N.NORM_K | norm_v * N.NORM_V
     d = N.RotateDesc(type, heads, kv_heads, head_dim, norms, epsilon, layer, n, tokens, q or None, k or None,
                      v or None, q_out or None, k_out or None, v_out or None)
-    for name, pair in (("q_stride", q_stride), ("k_stride", k_stride), ("v_stride", v_stride),
-                       ("q_out_stride", q_out_stride), ("k_out_stride", k_out_stride),
-                       ("v_out_stride", v_out_stride)):
-        if pair:
-            setattr(d, name, _strides(pair))
-    d.q_weight, d.k_weight = q_weight or None, k_weight or None
-    d.positions, d.rows, d.offsets = positions or None, sequences or None, offsets or None
-    check(N.lib().dm_attention_rotate(ctx.handle, rope.handle if rope else None,
-                                      cache.handle if cache else None, C.byref(d), stream or None))
+    if q_stride:
+        d.q_stride = _Pair(*q_stride)
+    if k_stride:
+        d.k_stride = _Pair(*k_stride)
+    if v_stride:
+        d.v_stride = _Pair(*v_stride)
+    if q_out_stride:
+        d.q_out_stride = _Pair(*q_out_stride)
+    if k_out_stride:
+        d.k_out_stride = _Pair(*k_out_stride)
+    if v_out_stride:
+        d.v_out_stride = _Pair(*v_out_stride)
+    if q_weight:
+        d.q_weight = q_weight
+    if k_weight:
+        d.k_weight = k_weight
+    if positions:
+        d.positions = positions
+    if sequences:
+        d.rows = sequences
+    if offsets:
+        d.offsets = offsets
+    check(N.lib().dm_attention_rotate(ctx.handle, rope._h if rope else None, cache._h if cache else None, C.byref(d),
+                                      stream or None))
 
 
 class KvCache:
