@@ -5,6 +5,12 @@
 // the products here (mma.sync tiles of 16 keys x 8 query rows): a key's sum stays in the threads
 // that hold its row, over all queries and heads, and one block owns a key, so nothing is added
 // atomically and the order of the sums is fixed.
+//
+// scale q k and lse may be in the tens where their difference is near 0, so neither may be rounded
+// before it is taken. With c the f32 next to scale log2 e, the weight is 2^(c (q k - lse / scale)) to
+// one part in 2^24 of the exponent; c lse / scale is kept as hi + lo, the exponent is one fused
+// c q k - hi, and the factor 2^-lo goes into the sum's multiplication. (With lse rounded, sums of
+// tokens far down a sequence were off by 1.2e-6 instead of 4e-7.)
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -52,7 +58,8 @@ struct WeightsArgs {
   float *weights;
   int64_t weights_stride, tokens;
   int32_t heads, group, window, sinks;
-  float scale;  // times log2 e
+  float scale;          // c
+  float ratio, ratio2;  // c / scale as a sum
   DecodeArgs d;  // rows, max_length, waits
 };
 
@@ -85,6 +92,14 @@ __device__ __forceinline__ Entry open_entry(const WeightsArgs &a, const KvView &
            (!a.window || first + keys > max(e.p0, 0) - (a.window - 1) || first < a.sinks);
   e.report = twice && first == 0 && length > 0;
   return e;
+}
+
+// The exponent's second term of a row, and the factor for what it leaves out. A row without
+// statistics gives nothing.
+__device__ __forceinline__ void exponent_of(const WeightsArgs &a, float lse, float *z, float *factor) {
+  const float hi = lse * a.ratio, lo = fmaf(lse, a.ratio2, fmaf(lse, a.ratio, -hi));
+  *z = lse == -INFINITY ? -INFINITY : -hi;
+  *factor = isfinite(hi) ? fmaf(lo, -kLn2, 1.0f) : 1.0f;
 }
 
 template <int DP, bool BF16>
@@ -206,11 +221,11 @@ weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
         mma16816<BF16>(s2, kf[2 * k + 1], b[2], b[3]);
       }
       const float2 lse = *reinterpret_cast<const float2 *>(&lse_of[buffer][t * kTileRows + (lane & 3) * 2]);
-      const float z[2] = {lse.x == -INFINITY ? -INFINITY : -lse.x * kLog2e,
-                          lse.y == -INFINITY ? -INFINITY : -lse.y * kLog2e};
-      float w[4];
+      float z[2], factor[2], w[4];
+      exponent_of(a, lse.x, &z[0], &factor[0]);
+      exponent_of(a, lse.y, &z[1], &factor[1]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = exp2_fast(fmaf(s[i] + s2[i], a.scale, z[i & 1]));
+      for (int i = 0; i < 4; i++) w[i] = exp2_fast(fmaf(s[i] + s2[i], a.scale, z[i & 1])) * factor[i & 1];
       // some key is hidden from some row
       if (key + kWarpKeys - 1 > from || (a.window && to - key >= a.window && key + kWarpKeys > a.sinks)) {
 #pragma unroll
@@ -270,7 +285,8 @@ struct TileCfg {
   static constexpr int kBlocks = HALVES == 2 ? 1 : COLS <= 32 && DP <= 128 ? 3 : 2;
   static constexpr int kKeys = HALVES * kHalf;
   static constexpr int kSlab = kKeys * 128;  // bytes: 64 values of the keys
-  static constexpr int kRoom = (kBlocks == 3 ? 67 : kBlocks == 2 ? 100 : 200) * 1024;
+  // for rings, beside 8 (15 with 64 columns, 29 with 128) KB of the rest and 1 KB that a block costs
+  static constexpr int kRoom = (kBlocks == 3 ? 66 : kBlocks == 1 ? 196 : COLS == 64 ? 97 : 104) * 1024;
   static constexpr int kQBytes = COLS * DP * 2;
   static constexpr int kSlabs = DP / 64;  // of a head
   // warps that weigh: with many query rows a second four, which take every other tile
@@ -286,11 +302,13 @@ struct TileCfg {
   static_assert(kKeySlots >= kSlabs && kQuerySlots >= 2, "a head's keys and two query tiles fit");
 };
 
+template <int COLS>
 struct TileSmem {
+  static constexpr int kRowsOf = COLS < 32 ? 32 : COLS;  // a lane's at least
   uint64_t k_full[kMostSlabs], k_empty[kMostSlabs], q_full[kMostQueries], q_empty[kMostQueries];
   uint64_t z_full[kStatSlots], z_empty[kStatSlots], s_full[kMostBuffers], s_free[kMostBuffers], drain;
-  alignas(16) float z[kStatSlots][kMostColumns];    // of a tile's query rows: -lse log2 e
-  alignas(16) int place[kStatSlots][kMostColumns];  // -1: no row
+  alignas(16) float z[kStatSlots][kRowsOf], factor[kStatSlots][kRowsOf];  // of a tile's query rows
+  alignas(16) int place[kStatSlots][kRowsOf];  // -1: no row
   uint32_t tmem;
   volatile int abort;
 };
@@ -351,7 +369,7 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   constexpr int kSoft = Cfg::kSoft, kGroups = Cfg::kGroups, kKeys = Cfg::kKeys, kSlab = Cfg::kSlab,
                 kBuffers = Cfg::kBuffers;
   extern __shared__ uint8_t raw[];
-  __shared__ TileSmem sh;
+  __shared__ TileSmem<COLS> sh;
   __shared__ float sums[kMostRanks * kGroups][kKeys];
   const WeightsArgs &a = t.w;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -507,11 +525,11 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       fetch();
       Turn<kStatSlots> s;
       while (at.left > 0 && ok) {
-        float z[kStatBatch][kRowsOf];
+        float z[kStatBatch][kRowsOf], factor[kStatBatch][kRowsOf];
 #pragma unroll
         for (int b = 0; b < kStatBatch; b++)
 #pragma unroll
-          for (int k = 0; k < kRowsOf; k++) z[b][k] = lse[b][k] == -INFINITY ? -INFINITY : -lse[b][k] * kLog2e;
+          for (int k = 0; k < kRowsOf; k++) exponent_of(a, lse[b][k], &z[b][k], &factor[b][k]);
         fetch();
 #pragma unroll
         for (int b = 0; b < kStatBatch; b++) {
@@ -521,6 +539,7 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
           for (int k = 0; k < kRowsOf; k++) {
             const int64_t i = (int64_t)at.tile * per + token[k];
             sh.z[s.slot][lane + k * 32] = z[b][k];
+            sh.factor[s.slot][lane + k * 32] = factor[b][k];
             sh.place[s.slot][lane + k * 32] = i < e.lq ? e.p0 + (int)i : -1;
           }
           __syncwarp();
@@ -581,7 +600,11 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
           }
         }
 #pragma unroll
-        for (int j = 0; j < kStep; j += 2) sum[j / 2 & 1] = add2(sum[j / 2 & 1], pair(x[j], x[j + 1]));
+        for (int j = 0; j < kStep; j += 4) {
+          const float4 f = *reinterpret_cast<const float4 *>(&sh.factor[z.slot][j0 + j]);
+          sum[0] = fma2(pair(x[j], x[j + 1]), pair(f.x, f.y), sum[0]);
+          sum[1] = fma2(pair(x[j + 2], x[j + 3]), pair(f.z, f.w), sum[1]);
+        }
       }
       __syncwarp();
       if (lane == 0) arrive(sh.z_empty[z.slot]);
@@ -641,6 +664,19 @@ int32_t launch_weights(dim3 grid, int ranks, const CUtensorMap &map, const Weigh
 
 constexpr int kSms = 148;
 
+// Tensor cores cut a partial sum off where they add the next 16 products to it, so scores come out
+// small: measured on scores of one key, by 1.0 to 1.2 times 2^-26 of themselves a step for bf16 and
+// 1.9 to 2.4 times that for f16, whose products have more bits; where the products' signs vary, as they
+// do in attention, by 1.0 and 1.5 times. That is as much as all other errors of a sum together, and
+// the only one of them with a sign. The scale takes it back on average (a step and a piece of 128
+// queries, dim 128 and 256: 5 to 12 times 10^-7 of the sums before, 1 to 7 with it).
+void set_scale(WeightsArgs *a, double given, int steps, bool bf16) {
+  const double scale = given * (1.0 + steps * (bf16 ? 0x1p-26 : 0x1.8p-26));
+  a->scale = (float)(scale * 1.4426950408889634);
+  a->ratio = (float)(a->scale / scale);
+  a->ratio2 = (float)(a->scale / scale - a->ratio);
+}
+
 // How many blocks share the queries of their keys. Microseconds on one B200, as measured: a block
 // has 6 besides (8 in a cluster) its keys at its part of an SM's 44 KB each, or its query tiles:
 // 1.8 for 128 rows and 256 keys, 0.8 for 64 and 128, 0.4 and 0.3 for 32 and 16.
@@ -685,6 +721,7 @@ extern "C" int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_w
   WeightsArgs a{};
   if (int32_t rc = check_strides(in->q_stride, in->heads, d.head_dim, a.q_stride, "query")) return rc;
   if (int32_t rc = check_scale(in->scale, d.head_dim, &a.scale)) return rc;
+  const double given = in->scale == 0.0f ? 1.0 / std::sqrt((double)d.head_dim) : in->scale;
   a.q = (const uint16_t *)in->q;
   a.lse = in->lse;
   a.offsets = in->offsets;
@@ -708,6 +745,7 @@ extern "C" int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_w
     int columns = d.head_dim > 128 ? 64 : kMostColumns;
     while (columns > 16 && columns / 2 >= each * a.group) columns /= 2;
     TileArgs t{};
+    set_scale(&a, given, (d.head_dim + 15) / 16, bf);
     t.w = a;
     t.tokens = columns / a.group;
     t.k_box = std::min<int>(d.page_tokens, kHalf);
@@ -727,6 +765,7 @@ extern "C" int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_w
   if (!describe_chunks(d.type, cache->view, in->layer, kWarpKeys, maps))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
   const int64_t tiles = (keys + kKeys - 1) / kKeys;
+  set_scale(&a, given, (d.head_dim + 31) / 32, bf);  // two chains of products
   // few blocks: several share the queries of their keys
   const int64_t steps = (each * a.group + kTileRows - 1) / kTileRows * d.kv_heads;
   int ranks = 1;
