@@ -28,7 +28,8 @@ using namespace dm::tc;
 // heads of dim 128, 67 us, 5.9 TB/s; 256 of them 236 us, 6.7. Small calls are latency (table,
 // queries, keys, join of the warps): 2 sequences of 200 tokens 5 us. Weights are rounded to 16
 // bits before the product (its operands have one type), the sums are not. Prompts whose tensors
-// are broadcast (a stride of zero) take this kernel, too.
+// are broadcast (a stride of zero) take this kernel, too, and chunks of few query rows: one token
+// over 98304 (32 and 8 heads of dim 128, 403 MB) 66 us besides the join's 6, 6.1 TB/s.
 // ---------------------------------------------------------------------------
 
 constexpr int kRows = 16;    // query rows of a block: one mma tile

@@ -94,6 +94,13 @@ __device__ __forceinline__ Entry open_entry(const WeightsArgs &a, const KvView &
   return e;
 }
 
+// ---------------------------------------------------------------------------
+// On mma.sync tiles: for queries that no tensor map holds (broadcast ones) and groups of more than 64
+// heads. Every block of 64 keys reads all of its entry's queries through shared memory; that and two
+// blocks of four warps an SM bound it (last 128 queries of prompts of 3000 to 12000 tokens, 32 and 8
+// heads of dim 128, 870 us, where the other kernel takes 69).
+// ---------------------------------------------------------------------------
+
 // The exponent's second term of a row, and the factor for what it leaves out. A row without
 // statistics gives nothing.
 __device__ __forceinline__ void exponent_of(const WeightsArgs &a, float lse, float *z, float *factor) {
@@ -271,6 +278,15 @@ weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
 // give). A thread has one key: it reads its row of the product, weighs and sums it along
 // the columns, and keeps the sum over all of the block's queries and heads. One warp each loads keys
 // (in slabs of 64 values) and queries, issues products and fetches statistics.
+//
+// Bound, with many query rows, by the exponentials: a tile of 128 rows and 256 keys takes 2400 cycles,
+// 2048 of them the exponential unit's (products of 128 columns and two halves: 64 columns took 1500
+// for a quarter of that, most of it issue and waits); a block's first loads and its end cost 9000
+// more, and a ragged batch does not fill the last round: last 128 queries of prompts of 3000 to 12000
+// tokens 69 us, 39% of the exponential unit over all. With few rows by memory: one query of each of 16
+// chats of 1186 to 3901 tokens, 32 and 8 heads of dim 128 (83 MB) 19 us, 4.3 TB/s, of which a block's
+// chain of look-ups and the first keys' latency are a third. A quarter of the exponentials as a
+// polynomial gained 7%, more lost; it is not here.
 // ---------------------------------------------------------------------------
 
 constexpr int kHalf = 128;  // keys of a product
