@@ -221,3 +221,42 @@ def test_a_long_chat(ctx):
     pool.lens = [0, budget + 8, 0]
     check_chunk(pool, q, [8], out, lse, layer=0, rows=[1])
     assert pool.cache.status() == 0
+
+
+def test_captured_weights_and_eviction(ctx):
+    """Clusters in a graph: replayed after lengths, offsets and sums have changed, as direct calls."""
+    lens = [3000, 20000]
+    pool = Paged(ctx, torch.bfloat16, 2, 64, 16, lens, layers=1, spare=1400, max_pages=1300)
+    q = normal(generator(2), (40, 8, 64), torch.bfloat16, 2.0)
+    lse = torch.full((40, 8), 12.0, device="cuda")
+    weights = torch.zeros(2, 1300 * 16, device="cuda")
+    o, rows, side = ints([0, 1, 40]), ints([0, 1]), torch.cuda.Stream()
+    keep, off = ints([0] * 2 * 2500), ints([0] * 3)
+
+    def calls(stream):
+        pool.cache.token_weights(layer=0, heads=8, q=q.data_ptr(), lse=lse.data_ptr(), offsets=o.data_ptr(), n=2, tokens=40,
+                                 max_length=20800, weights=weights.data_ptr(), weights_stride=weights.stride(0), stream=stream)
+        pool.cache.evict(sequences=rows.data_ptr(), n=2, budget=2500, sinks=4, recent=64, weights=weights.data_ptr(),
+                         weights_stride=weights.stride(0), keep_offsets=off.data_ptr(), keep=keep.data_ptr(), stream=stream)
+
+    start = [t.clone() for t in (pool.memory, pool.table, pool.lengths, pool.references)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        calls(side.cuda_stream)
+    for new, shorter in (([1, 39], 0), ([0, 3], 11), ([40, 0], 700)):
+        got = []
+        for run in (g.replay, lambda: calls(0)):
+            for t, s in zip((pool.memory, pool.table, pool.lengths, pool.references), start):
+                t.copy_(s)
+            pool.lengths.sub_(shorter)
+            o.copy_(ints(offsets(new)))
+            weights.copy_(torch.rand(weights.shape, generator=generator(5), device="cuda"))
+            keep.zero_()
+            run()
+            torch.cuda.synchronize()
+            got.append([t.clone().view(torch.int16) if t.dtype == torch.bfloat16 else t.clone()
+                        for t in (pool.memory, pool.table, pool.lengths, pool.references, weights, keep, off)])
+        assert pool.cache.status() == 0
+        for a, b in zip(*got):
+            assert torch.equal(a, b)
+        assert got[0][2].tolist() == [min(2500, n - shorter) for n in lens]
