@@ -100,6 +100,7 @@ struct TcCfg {
   // Registers: the launch's share (128 or 168 a thread) split anew, so that a row's scores and
   // the weights made from them stay in registers: 256 x 192 + 256 x 64 = 512 x 128, and
   // 128 x 216 + 256 x 144 = 384 x 168.
+  static constexpr int kScaled = DP == 64 ? 32 : 64;         // columns of O rescaled at once
   static constexpr int kSoftRegs = DP == 256 ? 216 : 192, kOtherRegs = DP == 256 ? 144 : 64;
 };
 
@@ -742,6 +743,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     const int sinks = MODE == kTcChunks && a.p.window ? a.p.sinks : 0;
     const uint64_t cc = pair(c, c);
     constexpr float kRoom = kTileHeadroom<BF16>;
+    constexpr int kScaled = Cfg::kScaled;
     const int dim = MODE == kTcPrompt ? a.p.dim : a.c.head_dim;
     int number = 0;  // tiles of this unit so far
     for (int items = 0; ok; items++) {
@@ -785,8 +787,14 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[unit]));
         const int from = low - key, to = high - key;  // columns [from, to) are visible
         if (__any_sync(0xffffffffu, from > 0 || to < kKeys)) {
+          if (MODE == kTcChunks && key < sinks) {
+            const int first = sinks - key;
 #pragma unroll
-          for (int j = 0; j < kKeys; j++) x[j] = (j >= from || j < sinks - key) && j < to ? x[j] : -INFINITY;
+            for (int j = 0; j < kKeys; j++) x[j] = (j >= from || j < first) && j < to ? x[j] : -INFINITY;
+          } else {
+#pragma unroll
+            for (int j = 0; j < kKeys; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
+          }
         }
         float top[4] = {m, m, m, m};
 #pragma unroll
@@ -802,13 +810,15 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             if (!(ok = wait(sh, a.wait_limit, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
             fence_after();
 #pragma unroll 1
-            for (int j = 0; j < DP; j += 16) {
-              uint32_t o[16];
-              tmem_ld16(o_at + j, o);
+            for (int j = 0; j < DP; j += kScaled) {  // bound by the latency of its reads
+              uint32_t o[kScaled];
+#pragma unroll
+              for (int k = 0; k < kScaled; k += 16) tmem_ld16(o_at + j + k, o + k);
               tmem_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st16(o_at + j, o);
+              for (int k = 0; k < kScaled; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+#pragma unroll
+              for (int k = 0; k < kScaled; k += 16) tmem_st16(o_at + j + k, o + k);
             }
           }
           l *= f;
