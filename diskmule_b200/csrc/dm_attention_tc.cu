@@ -4,7 +4,7 @@
 // one key/value head: row = token * group + head) with its own scores S [128 x keys f32],
 // weights P (16-bit) and output sum O [128 x dim f32], all in tensor memory. Per tile:
 //   S = Q K^T       tcgen05.mma, both operands in shared memory (128-byte swizzle, TMA)
-//   P = 2^(S - m)   one thread per row: maximum, exponentials, sum, all f32
+//   P = 2^(S - m)   one thread per row (chunks of dim 256: two): maximum, exponentials, sum, all f32
 //   O += P V        tcgen05.mma, P in tensor memory, V as it lies (keys down, dim across)
 // m is the running maximum with slack: O and l are rescaled only where the maximum has grown
 // by more than 2^8 since m was taken; until then the weights of newer keys may reach 2^8 (f16:
@@ -39,7 +39,8 @@
 // cut in parts, which a kernel of its own joins. 4096 tokens over 28672, 16 heads of dim 128: 846 us
 // by themselves, 1.22 PFLOP/s (two rounds of 256 equal items on 148 SMs), 960 at the power limit; 2001
 // tokens over 6000 beside 30 single ones over 190 to 7643: 286 and 330; 1500 tokens, window 1024 and
-// 4 sinks, dim 256, with others 45 (one round, 11 tiles of 2.9 us: one unit waits for its own steps).
+// 4 sinks, dim 256, with others 38 (one round: 11 tiles of 1.5 us, of which four hide keys from some
+// rows, between a first tile after 5 us and a last product and output of 4).
 //
 // Measured, causal 16384 tokens, 16 heads of dim 128: 807 us, 1.36 PFLOP/s; without a mask 8192
 // keys, dim 256 1.47, dim 64 0.74. What bounds it: at dim 128, 1750 cycles a tile of both units,
@@ -70,17 +71,18 @@ constexpr int kItems = 4;        // items between the first role and the last
 constexpr int kMostSlots = 5;
 constexpr int kWantTiles = 6;    // tiles left to load when the next item is chosen; at least 1
 
-template <int DP>
+// SIDES: threads of a row, each with its part of a tile's keys and of the dims.
+template <int DP, int SIDES = 1>
 struct TcCfg {
   static constexpr int kUnits = DP == 256 ? 1 : 2;
   static constexpr int kKeys = DP == 128 ? 80 : 128;         // of a tile
   // warps
-  static constexpr int kSoftWarps = 4 * kUnits;
+  static constexpr int kSoftWarps = 4 * kUnits * SIDES;
   static constexpr int kItemWarp = kSoftWarps, kKWarp = kItemWarp + 1, kVWarp = kItemWarp + 2;
   static constexpr int kScrubWarp = kItemWarp + 3;
   static constexpr int kSWarp = kItemWarp + 4;               // products S, one warp per unit
   static constexpr int kOWarp = kSWarp + kUnits;             // products O
-  static constexpr int kThreads = DP == 256 ? 384 : 512;     // whole groups of four warps
+  static constexpr int kThreads = kSoftWarps == 4 ? 384 : 512;  // whole groups of four warps
   // the warps behind the last one scrub too
   static constexpr int kScrubWarps = 1 + kThreads / 32 - (kOWarp + kUnits);
   static constexpr int kConsumers = kThreads / 32 - 1;       // of an item
@@ -92,16 +94,18 @@ struct TcCfg {
   static constexpr int kKSlabs = DP / 64 / kChunks;          // 64-value slabs of a K chunk
   static constexpr int kSlots = DP == 128 ? 4 : 5;           // of a ring
   static constexpr int kQBytes = kUnitRows * DP * 2;
-  static constexpr int kSmem = 1024 + kUnits * kQBytes + 2 * kSlots * kChunkBytes;
+  static constexpr int kSmem = 1024 + kUnits * kQBytes + 2 * kSlots * kChunkBytes;  // beside TcSmem
   // columns of tensor memory
   static constexpr int kUnitCols = DP == 64 ? 192 : 128;     // S from unit to unit
   static constexpr int kPCol = kKeys;                        // P from S
   static constexpr int kOCol = DP == 64 ? 384 : 256;
   // Registers: the launch's share (128 or 168 a thread) split anew, so that a row's scores and
   // the weights made from them stay in registers: 256 x 192 + 256 x 64 = 512 x 128, and
-  // 128 x 216 + 256 x 144 = 384 x 168.
+  // 128 x 216 + 256 x 144 = 384 x 168. Two threads to a row have half the scores each: 256 x 160 +
+  // 256 x 96 (192 and 64 spill in the other roles, and take 5% longer).
   static constexpr int kScaled = DP == 64 ? 32 : 64;         // columns of O rescaled at once
-  static constexpr int kSoftRegs = DP == 256 ? 216 : 192, kOtherRegs = DP == 256 ? 144 : 64;
+  static constexpr int kSoftRegs = kSoftWarps == 4 ? 216 : SIDES == 2 ? 160 : 192;
+  static constexpr int kOtherRegs = kSoftWarps == 4 ? 144 : SIDES == 2 ? 96 : 64;
 };
 
 // What the roles know of an item.
@@ -123,12 +127,17 @@ struct TcSmem {
   // chunks: loaded; fit to use (V, by the scrub warp); all products done
   uint64_t k_full[kMostSlots], k_empty[kMostSlots];
   uint64_t v_full[kMostSlots], v_clean[kMostSlots], v_empty[kMostSlots], drain[4];
+  uint64_t told[4], heard[4];  // both sides of a quarter of the rows have left word, and read the other's
+  float word[2][kUnitRows];
   uint4 answer;  // which block was taken over
   Item item[kItems];
   uint32_t tmem;
   volatile int abort;
   volatile uint32_t loaded, asked;  // signs of life: chunks of K, and blocks, asked for
 };
+
+static_assert(TcCfg<256>::kSmem + sizeof(TcSmem) <= 227 * 1024 && TcCfg<128>::kSmem + sizeof(TcSmem) <= 227 * 1024,
+              "a block's shared memory");
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -399,11 +408,19 @@ __device__ __forceinline__ bool load_tiles(TcSmem &sh, const Item &w, int tiles,
   return true;
 }
 
+// A row's sides. One unit has four softmax warps, one a scheduler, and nothing beside them while they
+// wait. Pages and sinks leave chunks of dim 256 with tiles of 3200 cycles then, where the products
+// need 2050; with two threads to a row 2800 (1500 tokens, windows 1024 and 4096: 40 and 89 us, now 36
+// and 77). A prompt's tile takes 2450 with one.
+template <int MODE, int DP>
+constexpr int kSidesOf = MODE == kTcChunks && DP == 256 ? 2 : 1;
+
 template <int MODE, int DP, bool BF16>
-__global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
+__global__ void __launch_bounds__((TcCfg<DP, kSidesOf<MODE, DP>>::kThreads), 1)
 tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
             const __grid_constant__ CUtensorMap v_map, const __grid_constant__ TcArgs a) {
-  using Cfg = TcCfg<DP>;
+  constexpr int kSides = kSidesOf<MODE, DP>;
+  using Cfg = TcCfg<DP, kSides>;
   constexpr int kUnits = Cfg::kUnits, kKeys = Cfg::kKeys, kChunks = Cfg::kChunks, kSlots = Cfg::kSlots;
   using Ring = Place<kSlots>;
   extern __shared__ uint8_t raw[];
@@ -432,8 +449,8 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(smem_u32(&sh.s_full[i]), 1);
-      mbar_init(smem_u32(&sh.s_free[i]), 4);
-      mbar_init(smem_u32(&sh.p_full[i]), 4);
+      mbar_init(smem_u32(&sh.s_free[i]), 4 * kSides);
+      mbar_init(smem_u32(&sh.p_full[i]), 4 * kSides);
       mbar_init(smem_u32(&sh.pv_done[i]), 1);
     }
     for (int i = 0; i < kSlots; i++) {
@@ -447,7 +464,11 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     mbar_init(smem_u32(&sh.q_empty), kUnits);
     mbar_init(smem_u32(&sh.next_block), 1);
     mbar_init(smem_u32(&sh.want), 1);
-    for (int i = 0; i < 4; i++) mbar_init(smem_u32(&sh.drain[i]), 1);
+    for (int i = 0; i < 4; i++) {
+      mbar_init(smem_u32(&sh.drain[i]), 1);
+      mbar_init(smem_u32(&sh.told[i]), 2);
+      mbar_init(smem_u32(&sh.heard[i]), 2);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == Cfg::kItemWarp) tmem_alloc(smem_u32(&sh.tmem), 512);
@@ -734,9 +755,25 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
     }
   } else {
-    // ---- softmax: one thread per row
+    // ---- softmax: one thread per row and side
     take_registers<Cfg::kSoftRegs>();
-    const int unit = warp >> 2, row = tid & 127;
+    const int unit = kSides == 1 ? warp >> 2 : 0, side = kSides == 1 ? 0 : warp >> 2, row = tid & 127;
+    constexpr int kCols = kKeys / kSides, kDims = DP / kSides;  // of a thread
+    // What the other thread of the row says; false where it has given up.
+    uint32_t talks = 0;
+    auto swap_words = [&](float mine, float *theirs) -> bool {
+      uint64_t &told = sh.told[warp & 3], &heard = sh.heard[warp & 3];
+      if (talks > 0 && !wait(sh, a.wait_limit, heard, (talks - 1) & 1)) return false;
+      sh.word[side][row] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&told));
+      if (!wait(sh, a.wait_limit, told, talks & 1)) return false;
+      *theirs = sh.word[side ^ 1][row];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&heard));
+      talks++;
+      return true;
+    };
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
     const uint32_t o_at = tmem + lanes + Cfg::kOCol + unit * DP;
     const float c = kPacked ? a.p.scale : a.d.scale;
@@ -777,31 +814,36 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (!(ok = wait(sh, a.wait_limit, sh.s_full[unit], number & 1))) break;
         fence_after();
         const uint32_t s_at = tmem + lanes + unit * Cfg::kUnitCols;
-        const int key = key_of<MODE, kKeys>(w, tile_of(unit, i));
-        float x[kKeys];
+        const int key = key_of<MODE, kKeys>(w, tile_of(unit, i)) + side * kCols;
+        float x[kCols];
 #pragma unroll
-        for (int j = 0; j + 32 <= kKeys; j += 32) tmem_ld32(s_at + j, x + j);
-        if (kKeys % 32) tmem_ld16(s_at + kKeys / 32 * 32, reinterpret_cast<uint32_t *>(x + kKeys / 32 * 32));
+        for (int j = 0; j + 32 <= kCols; j += 32) tmem_ld32(s_at + side * kCols + j, x + j);
+        if (kCols % 32) tmem_ld16(s_at + kCols / 32 * 32, reinterpret_cast<uint32_t *>(x + kCols / 32 * 32));
         tmem_wait_ld();
         fence_before();
         if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[unit]));
         const int from = low - key, to = high - key;  // columns [from, to) are visible
-        if (__any_sync(0xffffffffu, from > 0 || to < kKeys)) {
+        if (__any_sync(0xffffffffu, from > 0 || to < kCols)) {
           if (MODE == kTcChunks && key < sinks) {
             const int first = sinks - key;
 #pragma unroll
-            for (int j = 0; j < kKeys; j++) x[j] = (j >= from || j < first) && j < to ? x[j] : -INFINITY;
+            for (int j = 0; j < kCols; j++) x[j] = (j >= from || j < first) && j < to ? x[j] : -INFINITY;
           } else {
 #pragma unroll
-            for (int j = 0; j < kKeys; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
+            for (int j = 0; j < kCols; j++) x[j] = j >= from && j < to ? x[j] : -INFINITY;
           }
         }
         float top[4] = {m, m, m, m};
 #pragma unroll
-        for (int j = 0; j < kKeys; j += 8)
+        for (int j = 0; j < kCols; j += 8)
 #pragma unroll
           for (int k = 0; k < 4; k++) top[k] = max3(top[k], x[j + 2 * k], x[j + 2 * k + 1]);
-        const float now = max3(top[0], top[1], fmaxf(top[2], top[3]));
+        float now = max3(top[0], top[1], fmaxf(top[2], top[3]));
+        if (kSides == 2) {
+          float other;
+          if (!(ok = swap_words(now, &other))) break;
+          now = fmaxf(now, other);
+        }
         // 2^8: the slack of the running maximum. Each row goes by its own scores alone.
         const bool grows = (now - m) * c > 8.0f;
         if (__any_sync(0xffffffffu, grows)) {
@@ -810,7 +852,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             if (!(ok = wait(sh, a.wait_limit, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
             fence_after();
 #pragma unroll 1
-            for (int j = 0; j < DP; j += kScaled) {  // bound by the latency of its reads
+            for (int j = side * kDims; j < (side + 1) * kDims; j += kScaled) {  // bound by the latency of its reads
               uint32_t o[kScaled];
 #pragma unroll
               for (int k = 0; k < kScaled; k += 16) tmem_ld16(o_at + j + k, o + k);
@@ -835,7 +877,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         }
         uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < kKeys; j += 16) {
+        for (int j = 0; j < kCols; j += 16) {
           uint32_t p[8];
 #pragma unroll
           for (int k = 0; k < 8; k++) {
@@ -845,7 +887,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             sum[k & 1] = add2(sum[k & 1], pair(e0, e1));
             p[k] = pack2<BF16>(e0, e1);
           }
-          tmem_st8(p_at + j / 2, p);
+          tmem_st8(p_at + (side * kCols + j) / 2, p);
         }
         sum[0] = add2(sum[0], sum[1]);
         l += __uint_as_float((uint32_t)sum[0]) + __uint_as_float((uint32_t)(sum[0] >> 32));
@@ -856,6 +898,11 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       }
       if (!ok) break;
       // ---- result
+      if (kSides == 2) {
+        float other;
+        if (!(ok = swap_words(l, &other))) break;
+        l += other;
+      }
       if (n > 0 && !(ok = wait(sh, a.wait_limit, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
       fence_after();
       const bool wild = n > 0 && *(volatile int *)&sh.item[at].wild;
@@ -865,7 +912,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       const int64_t part_at =
           MODE == kTcPrompt ? 0 : (int64_t)part * a.d.part.rows + index;
 #pragma unroll 1
-      for (int j = 0; j < DP; j += 32) {
+      for (int j = side * kDims; j < (side + 1) * kDims; j += 32) {
         float o[32];
         __syncwarp();
         if (n > 0) {
@@ -924,10 +971,10 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             if (j + k < dim) store32(out + k, reinterpret_cast<const uint32_t *>(o + k), a.wide);
         }
       }
-      if (valid && final) {
+      if (valid && final && side == 0) {
         float *lse = kPacked ? a.p.lse : a.d.lse;
         if (lse) lse[index] = l == 0.0f ? -INFINITY : (m * c - kRoom + log2_fast(l)) * kLn2;
-      } else if (valid) {
+      } else if (valid && side == 0) {
         a.d.part.ml[part_at] = make_float2(m * c - kRoom, l);
       }
       fence_before();  // O has been read before the next item's weights are announced
@@ -1000,7 +1047,8 @@ template <int MODE, int DP, bool BF16>
 int32_t launch(dim3 grid, const CUtensorMap *maps, const TcArgs &a, cudaStream_t s) {
   auto fn = tile_kernel<MODE, DP, BF16>;
   DM_CUDA(dm::ensure_smem_limit((const void *)fn), "attention shared memory");
-  return launch_chained("attention launch", fn, grid, TcCfg<DP>::kThreads, TcCfg<DP>::kSmem, s, maps[0],
+  using Cfg = TcCfg<DP, kSidesOf<MODE, DP>>;
+  return launch_chained("attention launch", fn, grid, Cfg::kThreads, Cfg::kSmem, s, maps[0],
                         maps[1], maps[2], a);
 }
 
