@@ -260,3 +260,49 @@ def test_captured_weights_and_eviction(ctx):
         for a, b in zip(*got):
             assert torch.equal(a, b)
         assert got[0][2].tolist() == [min(2500, n - shorter) for n in lens]
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [31, 33, 2500])
+def test_many_entries(ctx, dim, n):
+    """Entries without rows between a few with many: items and tokens are found behind all of them."""
+    some = {0: 1, 7: 150, n // 2: 3, n - 2: 70, n - 1: 1}
+    new, lens = [some.get(i, 0) for i in range(n)], [some.get(i, 0) + 90 if i in some or i < 20 else 0 for i in range(n)]
+    pool = Paged(ctx, torch.bfloat16, 2, dim, 16, lens)
+    q = normal(generator(n), (sum(new), 4, dim), torch.bfloat16, 2.0)
+    for window, sinks in ((0, 0), (40, 3)):
+        out, lse = run_chunk(pool, q, new, window=window, sinks=sinks)
+        check_chunk(pool, q, new, out, lse, window=window, sinks=sinks)
+    out, lse = run_chunk(pool, q, new)
+    weights = torch.zeros(n, max(lens), device="cuda")
+    run_weights(pool, q, lse, new, weights)
+    want, bound = received(pool, q, lse, new, 1, 0, 0, dim ** -0.5, None)
+    assert np.all(np.abs(to64(weights) - want) <= bound)
+
+
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, float("inf")), (torch.float16, float("nan"))])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 4)])
+def test_hidden_values_of_wide_heads(ctx, dtype, value, dim, window, sinks):
+    """Tokens that are not finite, hidden from some rows by the order of tokens or by the window: rows
+    that do not see them are what they are without, also where several hundred rows do see them."""
+    n, a = 1500, 700
+    pool = Paged(ctx, dtype, 1, dim, 64, [n])
+    q = normal(generator(2), (a, 4, dim), dtype, 2.0)
+    before, lse0 = run_chunk(pool, q, [a], window=window, sinks=sinks)
+    check_chunk(pool, q, [a], before, lse0, window=window, sinks=sinks)
+    hit = 1150  # of position 350 among the rows
+    page, r = pool.at(0, hit)
+    pool.memory[page, 1, :, :, r] = value
+    out, lse = run_chunk(pool, q, [a], window=window, sinks=sinks)
+    sees = np.zeros(a, bool)
+    sees[hit - (n - a):(hit - (n - a) + window if window else a)] = True
+    free = torch.tensor(~sees, device="cuda")
+    assert torch.equal(out[free], before[free]) and torch.equal(lse[free], lse0[free])
+    pool.memory[page, 1, 0, :, r] = 0
+    pool.memory[page, 1, 1, :, r] = 0
+    pool.memory[page, 1, 1, 0, r, dim - 3] = value
+    out, _ = run_chunk(pool, q, [a], window=window, sinks=sinks)
+    assert not torch.isfinite(out[~free, :, dim - 3]).any()
+    out[~free, :, dim - 3] = 0
+    assert torch.isfinite(out).all()
