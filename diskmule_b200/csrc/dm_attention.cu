@@ -729,10 +729,11 @@ struct ChunkPlan {
   int splits = 1;      // of each item's keys
 };
 
-// Microseconds on one B200, as measured, for a tile of one unit's rows and of two (80 keys of dim
-// 128, 128 of the others; dim 256 with pages of 64 tokens and of 16), and for what an item of a
-// block has besides. The rest is as in decode.
-constexpr float kChunkStepUs[3][2] = {{1.2f, 1.6f}, {0.9f, 1.05f}, {1.6f, 2.05f}}, kChunkItemUs = 2.0f;
+// Microseconds on one B200, as measured, for a tile of one unit's rows (where memory does not set the
+// rate, which it does whatever the cut) and of two (80 keys of dim 128, 128 of the others; dim 256
+// with pages of 64 tokens and of 16), and for what an item of a block has besides. The rest is as in
+// decode.
+constexpr float kChunkStepUs[3][2] = {{0.8f, 1.6f}, {0.8f, 1.05f}, {1.6f, 2.05f}}, kChunkItemUs = 2.0f;
 constexpr float kGain = 0.95f;  // more parts have to be worth their workspace
 constexpr int64_t kMostPartBytes = 128 << 20;
 

@@ -36,9 +36,14 @@
 // Chunks of new tokens over the cache (kTcChunks) are prompts whose keys lie in pages: boxes of whole
 // pages or parts of them, looked up a tile ahead. Keys that no row of an item sees, between the sinks
 // and its window, are left out of the numbering of its keys. Where there are few items their keys are
-// cut in parts, which a kernel of its own joins. 4096 tokens over 28672, 16 heads of dim 128: 846 us
-// by themselves, 1.22 PFLOP/s (two rounds of 256 equal items on 148 SMs), 960 at the power limit; 2001
-// tokens over 6000 beside 30 single ones over 190 to 7643: 286 and 330; 1500 tokens, window 1024 and
+// cut in parts, which a kernel of its own joins. An item of one unit's rows at most (a single token, a
+// draft, the end of a prompt) goes through both units, which take its tiles in turn, since one unit
+// alone waits for each of its steps. Each unit then joins half of the dims from both sums, which it
+// can read, as a row has the same lane of tensor memory in both (16 tokens over 20000, not cut: dim
+// 128 231 us on one unit, 197 on two; dim 64 195 and 131).
+// 4096 tokens over 28672, 16 heads of dim 128: 846 us by themselves, 1.22 PFLOP/s (two rounds of 256
+// equal items on 148 SMs), 950 at the power limit; 2001 tokens over 6000 beside 30 single ones over
+// 190 to 7643: 269 and 316 (295 and 334 with single tokens on one unit); 1500 tokens, window 1024 and
 // 4 sinks, dim 256, with others 38 (one round: 11 tiles of 1.5 us, of which four hide keys from some
 // rows, between a first tile after 5 us and a last product and output of 4).
 //
@@ -69,6 +74,7 @@ namespace {
 constexpr int kUnitRows = 128;
 constexpr int kItems = 4;        // items between the first role and the last
 constexpr int kMostSlots = 5;
+constexpr int kJoinTiles = 2;    // of an item for two units to take in turn (64 items of two: 35 us, now 33)
 constexpr int kWantTiles = 6;    // tiles left to load when the next item is chosen; at least 1
 
 // SIDES: threads of a row, each with its part of a tile's keys and of the dims.
@@ -112,6 +118,7 @@ struct TcCfg {
 struct Item {
   int stop, kv_head, first, tiles;  // first key, number of key tiles
   int n[2];                         // tiles of each unit
+  int alternate;                    // one unit's rows are all there are: both have them, and take tiles in turn
   int max_low, min_high;            // every row sees the keys [max_low, min_high)
   int token0, lq, lk, q0, k0;       // first token of the item and of its sequence
   int table_row, end;               // paged: where its pages are looked up; no row sees keys from `end` on
@@ -420,6 +427,7 @@ __global__ void __launch_bounds__((TcCfg<DP, kSidesOf<MODE, DP>>::kThreads), 1)
 tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
             const __grid_constant__ CUtensorMap v_map, const __grid_constant__ TcArgs a) {
   constexpr int kSides = kSidesOf<MODE, DP>;
+  constexpr bool kJoins = MODE == kTcChunks && DP <= 128;  // units join what they have of one item
   using Cfg = TcCfg<DP, kSides>;
   constexpr int kUnits = Cfg::kUnits, kKeys = Cfg::kKeys, kChunks = Cfg::kChunks, kSlots = Cfg::kSlots;
   using Ring = Place<kSlots>;
@@ -431,14 +439,13 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
   constexpr bool kPacked = MODE != kTcShared;  // query rows by offsets
   const int group = kPacked ? a.p.group : a.d.group;
   const int per_unit = a.tokens * group;  // rows in use of a unit's 128
-  const int alternate = MODE == kTcShared && a.alternate;
   const int split = MODE == kTcShared ? blockIdx.y : 0;
   // P of a unit's product `number`: which, and how often it has been used before
   auto p_of = [&](int u, int number) -> int { return kUnits == 2 ? u : number & 1; };
   auto p_round = [&](int number) -> int { return kUnits == 2 ? number : number >> 1; };
-  auto tile_of = [&](int u, int i) -> int { return alternate ? 2 * i + u : i; };
+  auto tile_of = [&](int alternate, int u, int i) -> int { return alternate ? 2 * i + u : i; };
   // whether tile t of an item is one of the n of unit u
-  auto is_mine = [&](int u, int t, int n) -> bool { return alternate ? (t & 1) == u : t < n; };
+  auto is_mine = [&](int alternate, int u, int t, int n) -> bool { return alternate ? (t & 1) == u : t < n; };
 
   if (tid == 0) {
     sh.abort = 0;
@@ -538,12 +545,17 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
               w.n[0] = tiles_to(end0);
             }
             w.n[1] = kUnits == 2 && w.token0 + a.tokens < lq ? w.tiles : 0;
+            if (kJoins && w.n[1] == 0 && w.tiles >= kJoinTiles) {
+              w.alternate = 1;
+              w.n[0] = (w.tiles + 1) / 2;
+              w.n[1] = w.tiles / 2;
+            }
           }
         }
       } else if (items > 0) {
         w.stop = 1;
       } else {
-        const int units = alternate ? 1 : kUnits;
+        const int alternate = w.alternate = a.alternate, units = alternate ? 1 : kUnits;
         const int blocks = (a.d.batch + units * a.tokens - 1) / (units * a.tokens);
         w.kv_head = block / blocks;
         w.token0 = block % blocks * units * a.tokens;
@@ -608,7 +620,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (!(ok = wait_item(sh, a.wait_limit, sh.item_full[at], (items / kItems) & 1))) break;
         const Item &w = sh.item[at];
         if (uniform(w.stop)) break;
-        const int tiles = uniform(w.tiles);
+        const int tiles = uniform(w.tiles), alternate = MODE == kTcPrompt ? 0 : uniform(w.alternate);
         if (warp == Cfg::kKWarp) {
           // ---- queries and keys
           if (tiles > 0) {
@@ -681,7 +693,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           if (tiles > 0 && !(ok = wait(sh, a.wait_limit, sh.q_full, q_uses++ & 1))) break;
           if (tiles > 0 && n == 0 && lead) mbar_arrive(smem_u32(&sh.q_empty));
           for (int t = 0, left = n; t < tiles && ok; t++) {
-            const bool mine = is_mine(unit, t, n);
+            const bool mine = is_mine(alternate, unit, t, n);
             if (mine && number > 0 && !(ok = wait(sh, a.wait_limit, sh.s_free[unit], (number - 1) & 1)))
               break;  // S has been read
 #pragma unroll
@@ -713,7 +725,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           const int n = uniform(w.n[unit]);
           const uint32_t d = columns + Cfg::kOCol + unit * DP;
           for (int t = 0, own = 0; t < tiles && ok; t++) {
-            const bool mine = is_mine(unit, t, n);
+            const bool mine = is_mine(alternate, unit, t, n);
             const int which = p_of(unit, number);
             const uint32_t p = columns + unit * Cfg::kUnitCols + Cfg::kPCol + (which - unit) * kKeys / 2;
             if (mine && !(ok = wait(sh, a.wait_limit, sh.p_full[which], p_round(number) & 1))) break;
@@ -760,15 +772,16 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     const int unit = kSides == 1 ? warp >> 2 : 0, side = kSides == 1 ? 0 : warp >> 2, row = tid & 127;
     constexpr int kCols = kKeys / kSides, kDims = DP / kSides;  // of a thread
     // What the other thread of the row says; false where it has given up.
+    const int voice = kSides == 2 ? side : unit;
     uint32_t talks = 0;
     auto swap_words = [&](float mine, float *theirs) -> bool {
       uint64_t &told = sh.told[warp & 3], &heard = sh.heard[warp & 3];
       if (talks > 0 && !wait(sh, a.wait_limit, heard, (talks - 1) & 1)) return false;
-      sh.word[side][row] = mine;
+      sh.word[voice][row] = mine;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&told));
       if (!wait(sh, a.wait_limit, told, talks & 1)) return false;
-      *theirs = sh.word[side ^ 1][row];
+      *theirs = sh.word[voice ^ 1][row];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&heard));
       talks++;
@@ -782,13 +795,13 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
     constexpr float kRoom = kTileHeadroom<BF16>;
     constexpr int kScaled = Cfg::kScaled;
     const int dim = MODE == kTcPrompt ? a.p.dim : a.c.head_dim;
-    int number = 0;  // tiles of this unit so far
+    int number = 0, others = 0;  // tiles of this unit so far, and of the other one
     for (int items = 0; ok; items++) {
       const int at = items % kItems;
       if (!(ok = wait_item(sh, a.wait_limit, sh.item_full[at], (items / kItems) & 1))) break;
       const Item &w = sh.item[at];
       if (w.stop) break;
-      const int n = w.n[unit];
+      const int n = w.n[unit], alternate = MODE == kTcPrompt ? 0 : w.alternate;
       int low = 0, high = INT32_MAX;  // the keys that the row sees; all, if it is not in use
       int64_t out_at = 0, index = 0;
       const int token = w.token0 + (alternate ? 0 : unit * a.tokens) + row / group;
@@ -814,7 +827,7 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         if (!(ok = wait(sh, a.wait_limit, sh.s_full[unit], number & 1))) break;
         fence_after();
         const uint32_t s_at = tmem + lanes + unit * Cfg::kUnitCols;
-        const int key = key_of<MODE, kKeys>(w, tile_of(unit, i)) + side * kCols;
+        const int key = key_of<MODE, kKeys>(w, tile_of(alternate, unit, i)) + side * kCols;
         float x[kCols];
 #pragma unroll
         for (int j = 0; j + 32 <= kCols; j += 32) tmem_ld32(s_at + side * kCols + j, x + j);
@@ -904,6 +917,21 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
         l += other;
       }
       if (n > 0 && !(ok = wait(sh, a.wait_limit, sh.pv_done[p_of(unit, number - 1)], p_round(number - 1) & 1))) break;
+      // Items whose tiles the units have taken in turn: each gives half of the dims, from both sums.
+      const bool joins = kJoins && alternate;
+      float f = 1.0f, f1 = 0.0f;  // of this unit's sum, and of the other's
+      if (kJoins) others += w.n[unit ^ 1];
+      if (joins) {
+        float m1, l1;
+        if (!(ok = swap_words(m, &m1)) || !(ok = swap_words(l, &l1))) break;
+        // with its word the other has announced its last weights, so that one product is open at most
+        if (!(ok = wait(sh, a.wait_limit, sh.pv_done[unit ^ 1], (others - 1) & 1))) break;
+        const float top = fmaxf(m, m1);
+        f = m == -INFINITY ? 0.0f : exp2_fast((m - top) * c);
+        f1 = m1 == -INFINITY ? 0.0f : exp2_fast((m1 - top) * c);
+        m = top;
+        l = unit == 0 ? l * f + l1 * f1 : l1 * f1 + l * f;
+      }
       fence_after();
       const bool wild = n > 0 && *(volatile int *)&sh.item[at].wild;
       const bool final = MODE == kTcPrompt || a.d.part.parts == 1;
@@ -912,10 +940,18 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
       const int64_t part_at =
           MODE == kTcPrompt ? 0 : (int64_t)part * a.d.part.rows + index;
 #pragma unroll 1
-      for (int j = side * kDims; j < (side + 1) * kDims; j += 32) {
+      for (int j = side * kDims + (joins ? unit * DP / 2 : 0); j < (joins ? (unit + 1) * DP / 2 : (side + 1) * kDims);
+           j += 32) {
         float o[32];
         __syncwarp();
-        if (n > 0) {
+        if (joins) {
+          float o1[32];
+          tmem_ld32(o_at + j, o);
+          tmem_ld32(tmem + lanes + Cfg::kOCol + (unit ^ 1) * DP + j, o1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; k++) o[k] = o[k] * f + o1[k] * f1;
+        } else if (n > 0) {
           tmem_ld32(o_at + j, o);
           tmem_wait_ld();
         } else {
@@ -923,8 +959,8 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
           for (int k = 0; k < 32; k++) o[k] = 0.0f;
         }
         if (wild && valid) {  // rare: what was left out of the products
-          for (int i = 0; i < n; i++) {
-            const int t = tile_of(unit, i), key = key_of<MODE, kKeys>(w, t);
+          for (int i = 0; i < (joins ? w.tiles : n); i++) {
+            const int t = joins ? i : tile_of(alternate, unit, i), key = key_of<MODE, kKeys>(w, t);
             if (!mixed<MODE, kKeys>(w, t)) continue;
             for (int r = key < sinks ? key : max(key, low); r < min(key + kKeys, high); r++) {
               if (r < low && r >= sinks) continue;
@@ -971,13 +1007,18 @@ tile_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ C
             if (j + k < dim) store32(out + k, reinterpret_cast<const uint32_t *>(o + k), a.wide);
         }
       }
-      if (valid && final && side == 0) {
+      const bool speaks = side == 0 && !(joins && unit);
+      if (valid && final && speaks) {
         float *lse = kPacked ? a.p.lse : a.d.lse;
         if (lse) lse[index] = l == 0.0f ? -INFINITY : (m * c - kRoom + log2_fast(l)) * kLn2;
-      } else if (valid && side == 0) {
+      } else if (valid && speaks) {
         a.d.part.ml[part_at] = make_float2(m * c - kRoom, l);
       }
       fence_before();  // O has been read before the next item's weights are announced
+      if (joins) {     // by both units
+        float none;
+        if (!(ok = swap_words(0.0f, &none))) break;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.item_empty[at]));
     }
