@@ -306,3 +306,53 @@ def test_hidden_values_of_wide_heads(ctx, dtype, value, dim, window, sinks):
     assert not torch.isfinite(out[~free, :, dim - 3]).any()
     out[~free, :, dim - 3] = 0
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, float("nan")), (torch.float16, float("inf"))])
+@pytest.mark.parametrize("dim,kv,heads", [(64, 8, 32), (128, 8, 32), (96, 4, 20)])
+@pytest.mark.parametrize("n,window,sinks", [(700, 0, 0), (700, 200, 6), (91, 0, 0), (1501, 1000, 0)])
+def test_hidden_values_of_many_short_entries(ctx, dtype, value, dim, kv, heads, n, window, sinks):
+    """The same for entries of few rows, in the first and the last tiles that some of them see."""
+    a, count, which = 30, 12, 5
+    pool = Paged(ctx, dtype, kv, dim, 16, [n] * count)
+    q = normal(generator(2), (a * count, heads, dim), dtype, 2.0)
+    before, lse0 = run_chunk(pool, q, [a] * count, window=window, sinks=sinks)
+    check_chunk(pool, q, [a] * count, before, lse0, window=window, sinks=sinks, some=4)
+    first = n - a  # position of the entry's first row
+    for hit in (n - 10, first - window + 12 if window else n - 1):
+        page, r = pool.at(which, hit)
+        kept = pool.memory[page, 1, :, :, r].clone()
+        pool.memory[page, 1, :, :, r] = value
+        out, lse = run_chunk(pool, q, [a] * count, window=window, sinks=sinks)
+        sees = np.zeros((count, a), bool)
+        for t in range(a):
+            sees[which, t] = hit <= first + t and (not window or hit > first + t - window or hit < sinks)
+        assert 0 < sees.sum() < a
+        sees = torch.tensor(sees.reshape(-1), device="cuda")
+        assert torch.equal(out[~sees], before[~sees]) and torch.equal(lse[~sees], lse0[~sees])
+        pool.memory[page, 1, 0, :, r] = 0
+        pool.memory[page, 1, 1, :, r] = 0
+        pool.memory[page, 1, 1, 0, r, dim - 3] = value
+        out, _ = run_chunk(pool, q, [a] * count, window=window, sinks=sinks)
+        group = heads // kv
+        assert not torch.isfinite(out[sees, :group, dim - 3]).any()
+        out[sees, :group, dim - 3] = 0
+        assert torch.isfinite(out).all()
+        pool.memory[page, 1, :, :, r] = kept
+
+
+def test_rising_and_falling_scores_of_short_entries(ctx):
+    """Scores that rise or fall from key to key, so that halves of a row's tiles differ by powers of two."""
+    n, a, count = 1000, 20, 16
+    for dim in (64, 128):
+        pool = Paged(ctx, torch.bfloat16, 4, dim, 16, [n] * count)
+        for s in range(count):
+            ids = pool.table[s, :-(-n // 16)].long()
+            x = torch.zeros(len(ids) * 16, device="cuda")
+            x[:n] = torch.arange(n, device="cuda") / 8
+            pool.memory[ids, 1, 0] = 0
+            pool.memory[ids, 1, 0, :, :, 0] = x.view(-1, 1, 16).to(torch.bfloat16).expand(-1, 4, 16)
+        q = torch.zeros(a * count, 16, dim, dtype=torch.bfloat16, device="cuda")
+        q[:, 0::2, 0], q[:, 1::2, 0] = 8.0, -8.0
+        out, lse = run_chunk(pool, q, [a] * count)
+        check_chunk(pool, q, [a] * count, out, lse, some=3)
