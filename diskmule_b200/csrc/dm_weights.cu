@@ -101,11 +101,12 @@ __device__ __forceinline__ Entry open_entry(const WeightsArgs &a, const KvView &
 // heads of dim 128, 870 us, where the other kernel takes 69).
 // ---------------------------------------------------------------------------
 
-// The exponent's second term of a row, and the factor for what it leaves out. A row without
-// statistics gives nothing.
+// The exponent's second term of a row, and the factor for what it leaves out. (A row without
+// statistics gives nothing whatever its query holds, so its weights are not left to -infinity here:
+// with a score that is not finite that is NaN.)
 __device__ __forceinline__ void exponent_of(const WeightsArgs &a, float lse, float *z, float *factor) {
   const float hi = lse * a.ratio, lo = fmaf(lse, a.ratio2, fmaf(lse, a.ratio, -hi));
-  *z = lse == -INFINITY ? -INFINITY : -hi;
+  *z = -hi;
   *factor = isfinite(hi) ? fmaf(lo, -kLn2, 1.0f) : 1.0f;
 }
 
@@ -232,7 +233,8 @@ weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
       exponent_of(a, lse.x, &z[0], &factor[0]);
       exponent_of(a, lse.y, &z[1], &factor[1]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = exp2_fast(fmaf(s[i] + s2[i], a.scale, z[i & 1])) * factor[i & 1];
+      for (int i = 0; i < 4; i++)
+        w[i] = (i & 1 ? lse.y : lse.x) == -INFINITY ? 0.0f : exp2_fast(fmaf(s[i] + s2[i], a.scale, z[i & 1])) * factor[i & 1];
       // some key is hidden from some row
       if (key + kWarpKeys - 1 > from || (a.window && to - key >= a.window && key + kWarpKeys > a.sinks)) {
 #pragma unroll
@@ -324,7 +326,8 @@ struct TileSmem {
   uint64_t k_full[kMostSlabs], k_empty[kMostSlabs], q_full[kMostQueries], q_empty[kMostQueries];
   uint64_t z_full[kStatSlots], z_empty[kStatSlots], s_full[kMostBuffers], s_free[kMostBuffers], drain;
   alignas(16) float z[kStatSlots][kRowsOf], factor[kStatSlots][kRowsOf];  // of a tile's query rows
-  alignas(16) int place[kStatSlots][kRowsOf];  // -1: no row
+  alignas(16) int place[kStatSlots][kRowsOf];  // -1: no row, or one without statistics
+  int holes[kStatSlots];                       // a row of the tile has no statistics
   uint32_t tmem;
   volatile int abort;
 };
@@ -542,22 +545,30 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       Turn<kStatSlots> s;
       while (at.left > 0 && ok) {
         float z[kStatBatch][kRowsOf], factor[kStatBatch][kRowsOf];
+        bool none[kStatBatch][kRowsOf];
 #pragma unroll
         for (int b = 0; b < kStatBatch; b++)
 #pragma unroll
-          for (int k = 0; k < kRowsOf; k++) exponent_of(a, lse[b][k], &z[b][k], &factor[b][k]);
+          for (int k = 0; k < kRowsOf; k++) {
+            exponent_of(a, lse[b][k], &z[b][k], &factor[b][k]);
+            none[b][k] = lse[b][k] == -INFINITY;
+          }
         fetch();
 #pragma unroll
         for (int b = 0; b < kStatBatch; b++) {
           if (at.left <= 0) break;
           if (s.round > 0 && !(ok = wait(sh.abort, limit, sh.z_empty[s.slot], (s.round - 1) & 1))) break;
+          bool hole = false;
 #pragma unroll
           for (int k = 0; k < kRowsOf; k++) {
             const int64_t i = (int64_t)at.tile * per + token[k];
             sh.z[s.slot][lane + k * 32] = z[b][k];
             sh.factor[s.slot][lane + k * 32] = factor[b][k];
-            sh.place[s.slot][lane + k * 32] = i < e.lq ? e.p0 + (int)i : -1;
+            sh.place[s.slot][lane + k * 32] = i < e.lq && !none[b][k] ? e.p0 + (int)i : -1;
+            hole |= i < e.lq && none[b][k];
           }
+          hole = __any_sync(0xffffffffu, hole);
+          if (lead) sh.holes[s.slot] = hole;
           __syncwarp();
           if (lead) arrive(sh.z_full[s.slot]);
           at.next(), s.next();
@@ -580,9 +591,9 @@ tile_weights_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
       if (!(ok = wait(sh.abort, limit, sh.s_full[s.slot], s.round & 1))) break;
       fence_after();
       const int from = e.p0 + at.tile * per, count = min(per, e.lq - at.tile * per), to = from + count - 1;
-      // every key is seen by every row, and there are as many rows as columns
+      // every key is seen by every row, all have statistics, and there are as many as columns
       const bool clear = count * group == COLS && far <= from &&
-                         (!a.window || to - near < a.window || far < a.sinks);
+                         (!a.window || to - near < a.window || far < a.sinks) && !sh.holes[z.slot];
       constexpr int kStep = COLS < 32 ? COLS : 32;
       uint64_t sum[2] = {0, 0};
 #pragma unroll

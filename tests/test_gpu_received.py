@@ -1,0 +1,60 @@
+"""Received weight where a row or an entry gives nothing, and how near its sums come."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from attention_plain import to64
+from diskmule_b200 import CudaContext, _native as N
+from diskmule_b200.attention import attention_status
+from paged import Paged, generator, normal
+from test_gpu_evict import received, run_weights, statistics
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = CudaContext(0)
+    yield c
+    c.close()
+
+
+def sums(pool, q, lse, new, rows=None, layer=1, **more):
+    w = torch.zeros(pool.table.shape[0], max(pool.lens), device="cuda")
+    run_weights(pool, q, lse, new, w, layer=layer, rows=rows, **more)
+    attention_status(pool.cache._ctx)
+    return w
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("new,lens,heads,dim,window,sinks", [
+    ([6], [400], 4, 64, 0, 0), ([1, 2], [300, 900], 8, 128, 0, 0), ([128, 40], [700, 500], 8, 64, 0, 0),
+    ([128], [700], 8, 128, 200, 4), ([70], [900], 4, 256, 0, 0), ([9, 3], [200, 90], 192, 64, 0, 0)])
+def test_rows_without_statistics(ctx, new, lens, heads, dim, window, sinks, value, dtype):
+    """A row whose lse is -infinity gives nothing whatever its query holds: padding, say. (192
+    heads over 2 are a group that tiles do not take.)"""
+    pool = Paged(ctx, dtype, 2, dim, 16, lens)
+    q = normal(generator(2), (sum(new), heads, dim), dtype)
+    lse = torch.full(q.shape[:2], 6.0, device="cuda")
+    lse[::3] = -math.inf
+    lse[1:, 1] = -math.inf
+    want = sums(pool, q, lse, new, window=window, sinks=sinks)
+    assert torch.isfinite(want).all() and want.sum() > 0
+    q[lse == -math.inf] = value
+    assert torch.equal(sums(pool, q, lse, new, window=window, sinks=sinks), want)
+
+
+def test_broadcast_rows_without_statistics(ctx):
+    """The same on the tiles of queries that no tensor map holds."""
+    pool = Paged(ctx, torch.bfloat16, 2, 64, 16, [400])
+    q = torch.full((1, 8, 64), math.nan, dtype=torch.bfloat16, device="cuda")
+    q[:, :5] = normal(generator(2), (1, 5, 64), torch.bfloat16)
+    q = q.expand(50, 8, 64)
+    lse = torch.full((50, 8), 6.0, device="cuda")
+    lse[:, 5:] = -math.inf
+    got = sums(pool, q, lse, [50])
+    want, bound = received(pool, q.nan_to_num(0.0), lse, [50], 1, 0, 0, 0.125, None)
+    assert np.all(np.abs(to64(got) - want) <= bound)
