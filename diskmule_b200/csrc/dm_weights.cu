@@ -69,21 +69,31 @@ struct Entry {
   int lq, row, end, p0;  // query rows; table row; keys that count; place of the first query
   bool seen, report;     // some row may see some key; the sequence is named twice
 };
+// First row of entry i, and one behind its last.
+__device__ __forceinline__ int2 rows_of(const WeightsArgs &a, int i) {
+  const int q0 = (int)min((int64_t)max(a.offsets[i], 0), a.tokens);
+  return make_int2(q0, max(q0, (int)min((int64_t)a.offsets[i + 1], a.tokens)));
+}
 // also(row) runs beside the loads, for a row of the table.
 template <typename Also>
 __device__ __forceinline__ Entry open_entry(const WeightsArgs &a, const KvView &c, int first, int keys, int threads,
                                             Also also) {
   Entry e;
-  const int i = blockIdx.y, q0 = a.offsets[i], q1 = a.offsets[i + 1];
+  const int i = blockIdx.y;
+  const int2 rows = rows_of(a, i);
   e.row = a.d.sequences ? a.d.sequences[i] : i;
   int twice = 0;
   if (a.d.sequences)
-    for (int j = threadIdx.x; j < i; j += threads) twice |= a.d.sequences[j] == e.row;
+    for (int j = threadIdx.x; j < i; j += threads)  // entries without rows take nobody's place
+      if (a.d.sequences[j] == e.row) {
+        const int2 others = rows_of(a, j);
+        twice |= others.y > others.x;
+      }
   int length = 0;
   if (e.row >= 0 && e.row < c.max_sequences) also(e.row);
   e.row = sequence_of(c, a.d, i, &length);
-  e.q0 = min((int64_t)max(q0, 0), a.tokens);
-  e.lq = (int)(max(e.q0, min((int64_t)q1, a.tokens)) - e.q0);
+  e.q0 = rows.x;
+  e.lq = rows.y - rows.x;
   e.end = (int)min((int64_t)length, a.weights_stride);
   e.p0 = length - e.lq;
   twice = __syncthreads_or(twice) && e.lq > 0;

@@ -259,10 +259,10 @@ DM_API int32_t dm_attention_rotate(dm_cuda_context *ctx, const dm_rope *rope, dm
  * entry i, over all heads: sum exp(scale q k - lse), with q, lse, entries, window and sinks as in
  * dm_attention_chunk (decode: one row each) and lse what it returned; a row whose lse is
  * -infinity gives nothing. weights: device f32, one row of weights_stride for every row of the
- * table; tokens from weights_stride on are passed over. Calls that are alike add in the same order. A cache row
- * that is named twice counts for its first entry and sets DM_KV_BAD_SEQUENCE; entries outside
- * the table are passed over. At most 65535 entries. After a wait that ran out
- * (dm_attention_status) the sums are undefined. */
+ * table; tokens from weights_stride on are passed over. Calls that are alike add in the same order.
+ * A cache row that is named twice counts for its first entry with rows and sets
+ * DM_KV_BAD_SEQUENCE; entries outside the table and those without rows are passed over. At most
+ * 65535 entries. After a wait that ran out (dm_attention_status) the sums are undefined. */
 typedef struct {
   int32_t layer, heads, sequences, window, sinks, max_length;
   float scale;

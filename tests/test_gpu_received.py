@@ -58,3 +58,23 @@ def test_broadcast_rows_without_statistics(ctx):
     got = sums(pool, q, lse, [50])
     want, bound = received(pool, q.nan_to_num(0.0), lse, [50], 1, 0, 0, 0.125, None)
     assert np.all(np.abs(to64(got) - want) <= bound)
+
+
+@pytest.mark.parametrize("heads", [4, 130])
+@pytest.mark.parametrize("new,rows,counted,status", [
+    ([0, 5, 0, 3], [0, 0, 0, 1], {0: (0, 5), 1: (5, 3)}, 0),       # idle places that name a busy row
+    ([0, 5, 3], [1, 1, 1], {1: (0, 5)}, N.KV_BAD_SEQUENCE),        # the first one with rows counts
+    ([4, 0, 2], [7, 0, 0], {0: (4, 2)}, 0)])
+def test_entries_without_rows_take_nobodys_place(ctx, new, rows, counted, status, heads):
+    pool = Paged(ctx, torch.bfloat16, 2, 64, 16, [300, 200])
+    q = normal(generator(3), (sum(new), heads, 64), torch.bfloat16, 2.0)
+    lse = statistics(pool, q, new, 1, 0, 0, 0.125, rows)
+    got = to64(sums(pool, q, lse, new, rows=rows))
+    assert pool.cache.status() == status
+    for row in range(2):
+        if row not in counted:
+            assert np.all(got[row] == 0)
+            continue
+        at, n = counted[row]
+        want, bound = received(pool, q[at:at + n], lse[at:at + n], [n], 1, 0, 0, 0.125, [row])
+        assert np.all(np.abs(got[row] - want[row]) <= bound[row])
