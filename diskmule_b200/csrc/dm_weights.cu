@@ -701,14 +701,13 @@ int32_t launch_weights(dim3 grid, int ranks, const CUtensorMap &map, const Weigh
 
 constexpr int kSms = 148;
 
-// Tensor cores cut a partial sum off where they add the next 16 products to it, so scores come out
-// small: measured on scores of one key, by 1.0 to 1.2 times 2^-26 of themselves a step for bf16 and
-// 1.9 to 2.4 times that for f16, whose products have more bits; where the products' signs vary, as they
-// do in attention, by 1.0 and 1.5 times. That is as much as all other errors of a sum together, and
-// the only one of them with a sign. The scale takes it back on average (a step and a piece of 128
-// queries, dim 128 and 256: 5 to 12 times 10^-7 of the sums before, 1 to 7 with it).
-void set_scale(WeightsArgs *a, double given, int steps, bool bf16) {
-  const double scale = given * (1.0 + steps * (bf16 ? 0x1p-26 : 0x1.8p-26));
+// c and c / scale. Scores are the tensor cores' sums as they are, which cut a partial sum off where the
+// next 16 products are added to it: they come out small by up to 1.2 times 2^-26 of themselves a step
+// (f16: 2.4), and products that leave nothing to cut off are exact. Attention's own statistics are made
+// from such scores, too, so with them a row's weights come to one: 160 rows with scores of 8 times
+// normal, dim 64 to 256, to 2 10^-6 (a scale that gives the cut back on average 1 to 9 10^-6, and exact
+// products up to 1.5 10^-5 too large, though with a lse from exact scores sums are 2 to 4 times nearer).
+void set_scale(WeightsArgs *a, double scale) {
   a->scale = (float)(scale * 1.4426950408889634);
   a->ratio = (float)(a->scale / scale);
   a->ratio2 = (float)(a->scale / scale - a->ratio);
@@ -758,7 +757,7 @@ extern "C" int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_w
   WeightsArgs a{};
   if (int32_t rc = check_strides(in->q_stride, in->heads, d.head_dim, a.q_stride, "query")) return rc;
   if (int32_t rc = check_scale(in->scale, d.head_dim, &a.scale)) return rc;
-  const double given = in->scale == 0.0f ? 1.0 / std::sqrt((double)d.head_dim) : in->scale;
+  set_scale(&a, in->scale == 0.0f ? 1.0 / std::sqrt((double)d.head_dim) : in->scale);
   a.q = (const uint16_t *)in->q;
   a.lse = in->lse;
   a.offsets = in->offsets;
@@ -782,7 +781,6 @@ extern "C" int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_w
     int columns = d.head_dim > 128 ? 64 : kMostColumns;
     while (columns > 16 && columns / 2 >= each * a.group) columns /= 2;
     TileArgs t{};
-    set_scale(&a, given, (d.head_dim + 15) / 16, bf);
     t.w = a;
     t.tokens = columns / a.group;
     t.k_box = std::min<int>(d.page_tokens, kHalf);
@@ -802,7 +800,6 @@ extern "C" int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_w
   if (!describe_chunks(d.type, cache->view, in->layer, kWarpKeys, maps))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
   const int64_t tiles = (keys + kKeys - 1) / kKeys;
-  set_scale(&a, given, (d.head_dim + 31) / 32, bf);  // two chains of products
   // few blocks: several share the queries of their keys
   const int64_t steps = (each * a.group + kTileRows - 1) / kTileRows * d.kv_heads;
   int ranks = 1;

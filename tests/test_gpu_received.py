@@ -9,6 +9,7 @@ from attention_plain import to64
 from diskmule_b200 import CudaContext, _native as N
 from diskmule_b200.attention import attention_status
 from paged import Paged, generator, normal
+from test_gpu_chunk import run_chunk
 from test_gpu_evict import received, run_weights, statistics
 
 pytestmark = pytest.mark.gpu
@@ -78,3 +79,45 @@ def test_entries_without_rows_take_nobodys_place(ctx, new, rows, counted, status
         at, n = counted[row]
         want, bound = received(pool, q[at:at + n], lse[at:at + n], [n], 1, 0, 0, 0.125, [row])
         assert np.all(np.abs(got[row] - want[row]) <= bound[row])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,heads", [(1, 4), (70, 4), (5, 72)])
+def test_exact_products(ctx, rows, heads, dim, dtype):
+    """Queries and keys of small integers, whose products and partial sums are exact: what is left
+    is the exponent's one rounding (2^-24 of it), the exponential's two units of 2^-23 and four of
+    2^-24 for the factors, and the sum's. Nothing in it grows with the score alone."""
+    n = 200
+    pool = Paged(ctx, dtype, 1, dim, 64, [n], layers=1, seed=1)
+    g = generator(3)
+    shape = tuple(pool.memory[pool.table[0, :4].long(), 0, 0].shape)
+    pool.memory[pool.table[0, :4].long(), 0, 0] = torch.randint(-4, 5, shape, generator=g, device="cuda").to(dtype)
+    q = torch.randint(-8, 9, (rows, heads, dim), generator=g, device="cuda").to(dtype)
+    lse = statistics(pool, q, [rows], 0, 0, 0, dim ** -0.5, None)
+    got = to64(sums(pool, q, lse, [rows], layer=0))[0]
+    K, Q, E = pool.tokens(0, 0)[0, 0], to64(q), to64(lse)
+    want, bound, terms = np.zeros(n), np.zeros(n), np.zeros(n)
+    for t in range(rows):
+        seen = n - rows + t + 1
+        x = K[:seen] @ Q[t].T * dim ** -0.5 - E[t]
+        want[:seen] += np.exp(x).sum(1)
+        bound[:seen] += (np.exp(x) * (2.0 ** -22 + (np.abs(x) + 4) * 2.0 ** -24)).sum(1)
+        terms[:seen] += heads
+    # weights below the smallest normal number are gone
+    assert np.all(np.abs(got - want) <= bound + want * terms * 2.0 ** -24 + terms * 2.0 ** -126)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_weights_with_the_statistics_of_chunks(ctx, dim, dtype):
+    """With the lse that chunks return a row's weights come to one: both have the same scores. What
+    is left is lse's three roundings (sum, logarithm, to nats), 2^-24 of it each at most, and a few
+    units (2^-21) of exponentials and sums."""
+    new, lens = [300, 200], [700, 900]
+    pool = Paged(ctx, dtype, 2, dim, 64, lens, layers=1, seed=dim)
+    q = normal(generator(5), (sum(new), 8, dim), dtype, 8.0)
+    lse = run_chunk(pool, q, new, layer=0)[1]
+    total = to64(sums(pool, q, lse, new, layer=0)).sum()
+    each = total / (sum(new) * 8)
+    assert abs(each - 1) <= 3 * 2.0 ** -24 * float(lse.abs().mean()) + 2.0 ** -21
