@@ -102,6 +102,9 @@ def rotate(ctx: CudaContext, rope: Rope | None, *, type: int, head_dim: int, tok
            v_out_stride=None, stream: int = 0):
     """Norm each head and rotate queries and keys, into `*_out` and, with a cache, keys and values
     into its pages as the last tokens of `sequences` (dm_attention_rotate)."""
+    # null would mean that none is wanted
+    if rope is not None and not rope._h or cache is not None and not cache._h:
+        raise N.DmError(N.ERR_INVALID_ARGUMENT, "a closed rotation or cache")
     norms = norm_q * N.NORM_Q | norm_k * N.NORM_K | norm_v * N.NORM_V
     d = N.RotateDesc(type, heads, kv_heads, head_dim, norms, epsilon, layer, n, tokens, q or None, k or None,
                      v or None, q_out or None, k_out or None, v_out or None)

@@ -41,3 +41,21 @@ def test_descriptors_match_the_header(tmp_path):
     lines = subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split("\n")
     for (t, m, s), line in zip(pairs, lines):
         assert [int(x) for x in line.split()] == [C.sizeof(s), getattr(s, m).offset], t
+
+
+@pytest.mark.parametrize("which", ["rope", "cache"])
+def test_rotate_refuses_what_is_closed(which):
+    """A closed rotation is not "no rotation", a closed cache not "no cache"."""
+    from diskmule_b200 import DmError
+    from diskmule_b200.attention import KvCache, Rope, rotate
+
+    class Context:
+        handle = None
+
+    closed = (Rope if which == "rope" else KvCache).__new__(Rope if which == "rope" else KvCache)
+    closed._h = None
+    given = dict(rope=None, cache=None)
+    given[which] = closed
+    with pytest.raises(DmError) as e:
+        rotate(Context(), type=N.BF16, head_dim=64, tokens=0, **given)
+    assert e.value.status == N.ERR_INVALID_ARGUMENT and "closed" in str(e.value)
