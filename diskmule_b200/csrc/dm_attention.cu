@@ -102,7 +102,8 @@ rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
   if (kPacked) {
     kv_head = MODE == kPrompt ? blockIdx.y : blockIdx.x % c.kv_heads;
     if (warp == 0) {
-      const TileOf t = find_tile(p, group, kRows, MODE == kPrompt ? blockIdx.x : blockIdx.x / c.kv_heads);
+      const TileOf t = MODE == kPrompt ? find_tile(p, group, kRows, blockIdx.x)
+                                       : find_sparse_tile(p, group, kRows, blockIdx.x / c.kv_heads);
       if (lane == 0) sh.tile = t;
     }
     __syncthreads();
@@ -799,7 +800,7 @@ static int32_t bounded_length(const dm_kv_cache_desc &d, int32_t max_length) {
   return (int32_t)std::min<int64_t>(max_length, (int64_t)d.max_pages * d.page_tokens);
 }
 
-// Every tile looks for its sequence among all, 32 at a time: half a microsecond for each.
+// Every tile of a prompt looks for its sequence among all, 32 at a time: half a microsecond for each.
 constexpr int32_t kMostSequences = 1 << 20;
 
 int32_t dma::check_strides(const int64_t *given, int64_t heads, int dim, int64_t *use, const char *what) {
@@ -972,7 +973,7 @@ static int32_t check_chunk(const dm_kv_cache *cache, const dm_attention_chunk_de
   if (in->max_length < 0) return fail(DM_ERR_ELEMENT_COUNT, "max_length %d", in->max_length);
   if (in->tokens < 0 || in->tokens > kMostTokens) return fail(DM_ERR_ELEMENT_COUNT, "a bad number of tokens");
   const int64_t rows = in->tokens * in->heads;
-  const int64_t tiles = in->tokens * (in->heads / d.kv_heads) / kRows + in->sequences;
+  const int64_t tiles = chunk_tiles(in->tokens, in->sequences, in->heads / d.kv_heads, kRows);
   if (rows > INT32_MAX || tiles > INT32_MAX / d.kv_heads) return fail(DM_ERR_OVERFLOW, "too many query rows");
   *plan = chunk_plan(d, in->heads, in->sequences, in->tokens,
                      bounded_length(d, in->max_length), in->window, in->sinks);
@@ -1040,7 +1041,7 @@ int32_t dm_attention_chunk(dm_kv_cache *cache, const dm_attention_chunk_desc *in
   const bool on_tiles = plan.tiles && tile_queries_fit(p.q_stride, p.group);
   if (!on_tiles && !describe_chunks(kd.type, cache->view, in->layer, kChunk, maps))
     return fail(DM_ERR_COMMAND, "could not describe the cache for TMA");
-  const int64_t tiles = in->tokens * p.group / kRows + in->sequences;
+  const int64_t tiles = chunk_tiles(in->tokens, in->sequences, p.group, kRows);
   const dim3 grid((unsigned)(tiles * kd.kv_heads), plan.splits);
   if (int32_t rc = on_tiles  ? launch_tile_chunks(kd.type, p, a, cache->view, s)
                    : plan.wide ? launch_rows<kChunks, 8>(kd.type, kd.head_dim, grid, maps, p, a, cache->view, s)
