@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from diskmule_b200 import CudaContext
+from diskmule_b200 import CudaContext, _native as N
 from diskmule_b200.attention import attention_status
 from paged import Paged, generator, normal
 from test_gpu_chunk import check_chunk, run_chunk
@@ -51,3 +51,34 @@ def test_few_rows_among_idle_entries(ctx, n, dim):
         took = milliseconds(lambda: run_chunk(pool, q, new, rows=rows))
         # lists are made and copied within it; a search through all entries takes every block ms: 1450 in all
         assert took < 25, took
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1000, 1 << 18])
+def test_pieces_of_prompts_among_idle_entries(ctx, n, dim):
+    """Tiles: looking through the entries takes longer than a wait may last, and is no reason to
+    give up."""
+    lens = [700, 900, 90]
+    pool = Paged(ctx, torch.bfloat16, 2, dim, 16, lens)
+    new, rows = idle(n, {0: (1, 300), n // 3: (0, 260), n - 2: (2, 2)})
+    q = normal(generator(n), (562, 8, dim), torch.bfloat16, 2.0)
+    try:
+        N.check(N.lib().dm_selftest_attention_wait(ctx.handle, 2000000))  # 1 ms; 2^18 entries take ten times that
+        out, lse = run_chunk(pool, q, new, rows=rows)
+        attention_status(ctx)
+    finally:
+        N.check(N.lib().dm_selftest_attention_wait(ctx.handle, 0))
+    check_chunk(pool, q, [300, 260, 2], out, lse, rows=[1, 0, 2], some=4)
+
+
+@pytest.mark.parametrize("dim,heads,kv", [(64, 8, 2), (256, 4, 1)])
+def test_hundreds_of_drafts(ctx, dim, heads, kv):
+    """Items are found whatever the order in which a block takes them, in all steps of the lengths."""
+    r = np.random.RandomState(dim)
+    new = [int(x) for x in r.choice([0, 1, 5, 40, 70, 200], 300)]
+    lens = [n + int(x) for n, x in zip(new, r.choice([0, 10, 300, 900], 300))]
+    pool = Paged(ctx, torch.bfloat16, kv, dim, 16, lens)
+    q = normal(generator(4), (sum(new), heads, dim), torch.bfloat16, 2.0)
+    for max_length in (max(lens), 5000):
+        out, lse = run_chunk(pool, q, new, max_length=max_length)
+        check_chunk(pool, q, new, out, lse, some=1)
