@@ -151,7 +151,7 @@ weights_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant_
   if (ranks > 1) cluster.sync();  // the others' shared memory is there
 
   // ---- tiles of query rows, of all key/value heads one after the other; this block's share
-  const int rows = lq * group;  // at most 2^31 by the call's check
+  const int rows = lq * group;  // a tile more is still below 2^31 by the call's check
   const int per_head = (rows + kTileRows - 1) / kTileRows;
   const int64_t all = (int64_t)per_head * c.kv_heads;
   const int u0 = (int)(all * rank / ranks), u1 = (int)(all * (rank + 1) / ranks);
@@ -746,7 +746,8 @@ extern "C" int32_t dm_attention_weights(dm_kv_cache *cache, const dm_attention_w
     return fail(DM_ERR_ELEMENT_COUNT, "window %d, %d sinks", in->window, in->sinks);
   if (in->max_length < 0) return fail(DM_ERR_ELEMENT_COUNT, "max_length %d", in->max_length);
   if (in->tokens < 0 || in->tokens > kMostTokens) return fail(DM_ERR_ELEMENT_COUNT, "a bad number of tokens");
-  if (in->tokens * in->heads > INT32_MAX) return fail(DM_ERR_OVERFLOW, "too many query rows");
+  // the rows of a head are counted in 32 bits up to a whole tile
+  if (in->tokens * in->heads > INT32_MAX - kTileRows) return fail(DM_ERR_OVERFLOW, "too many query rows");
   if (in->weights_stride < 0) return fail(DM_ERR_INVALID_ARGUMENT, "a negative stride of weights");
   const int64_t keys = std::min(std::min<int64_t>(in->max_length, (int64_t)d.max_pages * d.page_tokens), in->weights_stride);
   if (in->tokens == 0 || in->sequences == 0 || keys == 0) return DM_OK;

@@ -6,9 +6,9 @@ import pytest
 import torch
 
 from attention_plain import to64
-from diskmule_b200 import CudaContext, _native as N
+from diskmule_b200 import CudaContext, DmError, _native as N
 from diskmule_b200.attention import attention_status
-from paged import Paged, generator, normal
+from paged import Paged, generator, ints, normal
 from test_gpu_chunk import run_chunk
 from test_gpu_evict import received, run_weights, statistics
 
@@ -121,3 +121,17 @@ def test_weights_with_the_statistics_of_chunks(ctx, dim, dtype):
     total = to64(sums(pool, q, lse, new, layer=0)).sum()
     each = total / (sum(new) * 8)
     assert abs(each - 1) <= 3 * 2.0 ** -24 * float(lse.abs().mean()) + 2.0 ** -21
+
+
+def test_too_many_rows(ctx):
+    """Rows are counted in 32 bits, up to a whole tile of them: refused before anything is read."""
+    pool = Paged(ctx, torch.bfloat16, 1, 64, 16, [300])
+    q = normal(generator(1), (1, 1, 64), torch.bfloat16)
+    lse, o = torch.zeros(1, device="cuda"), ints([0, 1])
+    weights = torch.zeros(1, 304, device="cuda")
+    for heads, tokens in ((127, 16909320), (126, 17043521), (72, 1 << 25), (2, 1073741823)):
+        with pytest.raises(DmError) as e:
+            pool.cache.token_weights(layer=0, heads=heads, q=q.data_ptr(), lse=lse.data_ptr(), offsets=o.data_ptr(),
+                                     n=1, tokens=tokens, max_length=300, weights=weights.data_ptr(), weights_stride=304)
+        assert e.value.status == N.ERR_OVERFLOW
+    assert weights.sum() == 0
