@@ -207,9 +207,9 @@ DM_API int32_t dm_attention_chunk(dm_kv_cache *cache, const dm_attention_chunk_d
 /* What turns with the position: the first rotary_dim values of a head (a multiple of 16 up to
  * 256), in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved. Pair i turns by
  * positions[pair_axes[i]] * frequencies[i] radians. frequencies (host, rotary_dim / 2 of them;
- * NULL = theta^(-2 i / rotary_dim)) are taken in 64 bits and angles are exact to 2^-32 of a
- * turn wherever the position. pair_axes (host, NULL = all 0) are below axes, 1 to 4. scale
- * multiplies cosine and sine (0 = 1). The arrays are copied. */
+ * NULL = theta^(-2 i / rotary_dim)) are taken in 64 bits, and an angle is off by at most 2^-25 of
+ * a turn wherever the position (frequencies up to 256). pair_axes (host, NULL = all 0) are below
+ * axes, 1 to 4. scale multiplies cosine and sine (0 = 1). The arrays are copied. */
 typedef struct dm_rope dm_rope;
 typedef struct {
   int32_t rotary_dim, interleaved, axes;
