@@ -306,11 +306,25 @@ struct Place {
 // Where a block's search for items stands: at 32 entries in a step of the lengths, with `before` items
 // before them. A block's items mostly ascend, so it looks at every entry four times in all (0.7 us for
 // 32 of them), not for every item: 1024 entries of 8 tokens, 32 and 8 heads of dim 128, 2007 us, now
-// 784; of 40 tokens, 16 and 2 heads of dim 256, 1698 and 993.
+// 784; of 40 tokens, 16 and 2 heads of dim 256, 1698 and 993. Runs of entries without rows are passed
+// over by a search (3 entries of up to 300 rows among 4096: 475 us with a look at each for every item,
+// 375 at each four times, now 24).
 struct ChunkSearch {
   int turn = 3, s0 = 0;
   int64_t before = 0;
 };
+
+// The last of offsets[low .. high], which ascend, that is at most q; offsets[low] is. One warp.
+__device__ __forceinline__ int last_upto(const int32_t *offsets, int low, int high, int q) {
+  const int lane = threadIdx.x & 31;
+  for (int count = high - low + 1; count > 1;) {
+    const int step = (count + 31) / 32, end = low + count;
+    const int64_t at = low + (int64_t)lane * step;
+    low += (__popc(__ballot_sync(0xffffffffu, at < end && offsets[at] <= q)) - 1) * step;
+    count = min(step, end - low);
+  }
+  return low;
+}
 
 // Chunks: the items of `tokens` tokens in order of their sequences' lengths, in four steps of the
 // longest, so that no long item begins when the others are done, and from a sequence's last on.
@@ -324,14 +338,19 @@ __device__ __forceinline__ TileOf find_chunk(const PromptArgs &p, const DecodeAr
   for (; at.turn >= 0; at.turn--, at.s0 = 0)
     for (; at.s0 < p.sequences; at.s0 += 32) {
       const int s = at.s0 + lane;
-      int q0 = 0, q1 = 0;
+      int q0 = 0, q1 = 0, length = 0;
       if (s < p.sequences) {
-        int length;
         sequence_of(c, d, s, &length);
         q0 = p.q_offsets[s], q1 = p.q_offsets[s + 1];
         q0 = (int)min((int64_t)max(q0, 0), p.q_tokens), q1 = max(q0, (int)min((int64_t)q1, p.q_tokens));
-        if (length / step != at.turn) q1 = q0;
       }
+      if (lane == 0) looked = looked + 1;
+      if (!__any_sync(0xffffffffu, q1 > q0)) {  // on with the next entry that has rows, if there is one
+        const int q = __shfl_sync(0xffffffffu, q0, 0);
+        at.s0 = (q < p.q_tokens ? last_upto(p.q_offsets, at.s0, p.sequences, q) : p.sequences) - 32;
+        continue;
+      }
+      if (length / step != at.turn) q1 = q0;
       const int64_t n = ((int64_t)(q1 - q0) + tokens - 1) / tokens;
       int64_t upto = at.before + n;
       if (lane > 0) upto = n;
@@ -350,7 +369,6 @@ __device__ __forceinline__ TileOf find_chunk(const PromptArgs &p, const DecodeAr
         return r;
       }
       at.before = __shfl_sync(0xffffffffu, upto, 31);
-      if (lane == 0) looked = looked + 1;
     }
   r.behind = tile - at.before;
   return r;

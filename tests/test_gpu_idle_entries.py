@@ -4,8 +4,8 @@ import pytest
 import torch
 
 from diskmule_b200 import CudaContext, _native as N
-from diskmule_b200.attention import attention_status
-from paged import Paged, generator, normal
+from diskmule_b200.attention import attention_status, offsets
+from paged import Paged, generator, ints, normal
 from test_gpu_chunk import check_chunk, run_chunk
 
 pytestmark = pytest.mark.gpu
@@ -56,14 +56,14 @@ def test_few_rows_among_idle_entries(ctx, n, dim):
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("n", [1000, 1 << 18])
 def test_pieces_of_prompts_among_idle_entries(ctx, n, dim):
-    """Tiles: looking through the entries takes longer than a wait may last, and is no reason to
-    give up."""
+    """Tiles: looking through the entries is no reason to give up, however long (a look at each of
+    2^18 four times takes 20 ms)."""
     lens = [700, 900, 90]
     pool = Paged(ctx, torch.bfloat16, 2, dim, 16, lens)
     new, rows = idle(n, {0: (1, 300), n // 3: (0, 260), n - 2: (2, 2)})
     q = normal(generator(n), (562, 8, dim), torch.bfloat16, 2.0)
     try:
-        N.check(N.lib().dm_selftest_attention_wait(ctx.handle, 2000000))  # 1 ms; 2^18 entries take ten times that
+        N.check(N.lib().dm_selftest_attention_wait(ctx.handle, 2000000))  # 1 ms
         out, lse = run_chunk(pool, q, new, rows=rows)
         attention_status(ctx)
     finally:
@@ -82,3 +82,29 @@ def test_hundreds_of_drafts(ctx, dim, heads, kv):
     for max_length in (max(lens), 5000):
         out, lse = run_chunk(pool, q, new, max_length=max_length)
         check_chunk(pool, q, new, out, lse, some=1)
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_idle_entries_are_passed_over_at_once(ctx, dim):
+    """Pieces of prompts on tiles; offsets beyond the bound of tokens, too."""
+    n, lens = 1 << 20, [700, 900, 90]
+    pool = Paged(ctx, torch.bfloat16, 2, dim, 16, lens)
+    new, rows = idle(n, {5: (1, 300), n // 3: (0, 260), n - 40: (2, 2)})
+    q = normal(generator(n), (562, 8, dim), torch.bfloat16, 2.0)
+    o, r, out = ints(offsets(new)), ints(rows), torch.zeros_like(q)
+
+    def run(tokens=562):
+        need = pool.cache.chunk_workspace(8, n, tokens, 900)
+        work = torch.empty(max(16, need), dtype=torch.uint8, device="cuda")
+        pool.cache.chunk_attention(layer=1, heads=8, q=q.data_ptr(), out=out.data_ptr(), sequences=r.data_ptr(),
+                                   offsets=o.data_ptr(), n=n, tokens=tokens, max_length=900, workspace=work.data_ptr(),
+                                   workspace_bytes=need)
+
+    # a look at each of 2^20 entries takes a block some 20 ms
+    assert milliseconds(run) < 5
+    want = out.clone()
+    out.zero_()
+    run(tokens=560)  # the last entry's rows are not there
+    torch.cuda.synchronize()
+    attention_status(ctx)
+    assert torch.equal(out[:560], want[:560]) and (out[560:] == 0).all()
