@@ -417,6 +417,10 @@ int32_t dm_attention_rotate(dm_cuda_context *ctx, const dm_rope *rope, dm_kv_cac
     a.out[i] = (uint8_t *)to[i];
     if (int32_t rc = check_strides(from_stride[i], heads, in->head_dim, a.in_stride[i], names[i])) return rc;
     if (int32_t rc = check_strides(to_stride[i], heads, in->head_dim, a.out_stride[i], names[i])) return rc;
+    // in place: else a token's result would lie where another warp is yet to read
+    if (from[i] == to[i] && ((in->tokens > 1 && a.in_stride[i][0] != a.out_stride[i][0]) ||
+                             (heads > 1 && a.in_stride[i][1] != a.out_stride[i][1])))
+      return fail(DM_ERR_INVALID_ARGUMENT, "a %s rotated in place needs the same strides for its output", names[i]);
     for (int j = 0; j < 2; j++) a.in_stride[i][j] *= 2, a.out_stride[i][j] *= 2;
     a.heads += heads;
   }

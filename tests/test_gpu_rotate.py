@@ -331,3 +331,25 @@ def test_refusals(ctx):
         Rope(ctx, 32, frequencies=[1.0] * 15)
     torch.cuda.synchronize()
     assert torch.equal(before, call.qkv) and call.pool.cache.status() == 0
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+def test_in_place_with_other_strides_is_refused(ctx, which):
+    """A result over its input under other strides would overwrite what other warps have yet to
+    read. What is alike, or has one token and one head only, is done."""
+    fused = normal(generator(1), (9, 12, 64), torch.bfloat16)
+    before, at = fused.clone(), ints([[3] * 9])
+    given = {which: fused.data_ptr(), f"{which}_out": fused.data_ptr(), "heads" if which == "q" else "kv_heads": 4}
+    call = lambda tokens=9, **more: rotate(ctx, None, type=N.BF16, head_dim=64, tokens=tokens, positions=at.data_ptr(),
+                                           norm_q=True, norm_k=True, norm_v=True, **{**given, **more})
+    for strides in ({f"{which}_stride": (768, 64)}, {f"{which}_out_stride": (768, 64)},
+                    {f"{which}_stride": (768, 64), f"{which}_out_stride": (768, 128)}):
+        with pytest.raises(DmError) as e:
+            call(**strides)
+        assert e.value.status == N.ERR_INVALID_ARGUMENT
+    torch.cuda.synchronize()
+    assert torch.equal(fused, before)
+    call(**{f"{which}_stride": (768, 64), f"{which}_out_stride": (768, 64)})
+    call(tokens=1, **{f"{which}_stride": (64, 64)})  # one token: its place is the same whatever the stride
+    torch.cuda.synchronize()
+    assert not torch.equal(fused[:, :4], before[:, :4]) and torch.equal(fused[:, 4:], before[:, 4:])
