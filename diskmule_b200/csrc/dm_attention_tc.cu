@@ -44,8 +44,12 @@
 // 4096 tokens over 28672, 16 heads of dim 128: 846 us by themselves, 1.22 PFLOP/s (two rounds of 256
 // equal items on 148 SMs), 950 at the power limit; 2001 tokens over 6000 beside 30 single ones over
 // 190 to 7643: 269 and 316 (295 and 334 with single tokens on one unit); 1500 tokens, window 1024 and
-// 4 sinks, dim 256, with others 38 (one round: 11 tiles of 1.5 us, of which four hide keys from some
-// rows, between a first tile after 5 us and a last product and output of 4).
+// 4 sinks, dim 256, with others 38. That is one round of items of 11 tiles, whose 62,500 cycles (1.67
+// GHz) are 4300 until the item is found, 5000 until its first scores are there, 43,700 for the tiles
+// (3800 for one that hides nothing and rescales nothing, 2150 of the threads and 1650 waiting for
+// scores; 3300 to 4600 with hidden keys or rows whose maximum grows, which wait for the product before),
+// 5000 for the last product and 4600 for the output; 5000 more from cold caches. Pages of 16, 64 or 256
+// tokens make no difference; without sinks it is 33 us.
 //
 // Measured, causal 16384 tokens, 16 heads of dim 128: 807 us, 1.36 PFLOP/s; without a mask 8192
 // keys, dim 256 1.47, dim 64 0.74. What bounds it: at dim 128, 1750 cycles a tile of both units,

@@ -12,10 +12,11 @@
 // few shuffles, and a pair's other half is another lane's vector. Sines and weights are multiplied
 // once for all heads of a token, and the next heads are on their way while some are done.
 //
-// Bound by memory where there is much to do: 8191 tokens of 32 + 8 + 8 heads of dim 128 (201 MB) take
-// 42 us, 4.8 TB/s of a copy's 6.5; the same loads and stores alone take 33. A token's look-ups (entry,
-// length, page, positions) and sines are a chain of 2 to 3 us, which 28 warps an SM hide: 3802 tokens
-// of 16 + 2 + 2 heads of dim 256 (78 MB) 19 us. (One block for eight tokens with the sines in shared
+// 8191 tokens of 32 + 8 + 8 heads of dim 128 (201 MB) take 42 us, 4.8 TB/s of a copy's 6.5; the same
+// loads and stores alone take 33. No unit is near its limit (DRAM 46% busy, issue 58%): it is the
+// latency of a token's look-ups (entry, length, page, positions) and sines, a chain of 2 to 3 us, and
+// of its heads behind them, which 28 warps an SM hide in part: 3802 tokens of 16 + 2 + 2 heads of dim
+// 256 (78 MB) 19 us. (One block for eight tokens with the sines in shared
 // memory 94 and 51 us; loads through a ring in shared memory 51 and 33, four at a time in registers
 // and 16 warps 49 and 29.) Few tokens are latency: 5 us.
 #include <cuda_runtime.h>

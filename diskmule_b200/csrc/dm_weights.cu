@@ -9,8 +9,8 @@
 // scale q k and lse may be in the tens where their difference is near 0, so neither may be rounded
 // before it is taken. With c the f32 next to scale log2 e, the weight is 2^(c (q k - lse / scale)) to
 // one part in 2^24 of the exponent; c lse / scale is kept as hi + lo, the exponent is one fused
-// c q k - hi, and the factor 2^-lo goes into the sum's multiplication. (With lse rounded, sums of
-// tokens far down a sequence were off by 1.2e-6 instead of 4e-7.)
+// c q k - hi, and the factor 2^-lo goes into the sum's multiplication. (c lse / scale rounded to f32
+// would be off by up to 2^-24 of itself, one part in a million of a weight where it is 24.)
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
